@@ -30,6 +30,8 @@
  *   nt_embedding           NeuraTensorModel.embedding  neuratensor/core/model.py:258
  *   nt_lm_head             NeuraTensorModel.norm + lm_head neuratensor/core/model.py:283-284
  *   nt_greedy_tokens       top-k = 1 sampling in NeuraTensorModel.generate model.py:344-359
+ *   nt_rotary              apply_rotary at given positions model.py:119-126
+ *   nt_logits_process      repetition penalty in NeuraTensorModel.generate model.py:336-342
  *   nt_lif_ssm_fused       LIF spikes driving the selective scan with given dt/B/C
  *                          (snn.py:167-182 feeding ssm.py:106-139,184-221)
  *
@@ -258,6 +260,92 @@ NT_API int nt_lif_ssm_fused(int64_t B, int64_t L, int64_t d, int64_t N,
 NT_API int nt_window_attention(int dtype, int64_t B, int64_t T, int64_t n_heads, int64_t head_dim,
                         int64_t window, const void* qkv, int64_t ld_qkv, const void* cos_t,
                         const void* sin_t, void* out, int64_t ld_out, void* stream);
+
+/* Rotary positions on any tensor of heads (the rotation of apply_rotary,
+ * model.py:119-126, at given positions).  x, y: [B,T,H,D] in `dtype` with
+ * element strides (sb, st, sh, 1); x == y rotates in place.  The first R
+ * dimensions of each head turn in R/2 pairs: (i, i + R/2) when interleaved == 0,
+ * (2i, 2i + 1) otherwise; dimensions past R are copied.  Pair i of the token
+ * at position p turns by the angle p * inv_freq[i], taken in float64:
+ *   y1 = m (x1 cos - x2 sin),  y2 = m (x2 cos + x1 sin),  m = mscale,
+ * in float32 with one rounding to `dtype`.  inverse != 0 turns backwards (the
+ * gradient of the forward call with the same arguments).  positions: int64,
+ * row b starts at positions + b*p_sb (p_sb = 0: shared by the batch);
+ * inv_freq: [R/2] float32. */
+NT_API int nt_rotary(int dtype, int64_t B, int64_t T, int64_t H, int64_t D, int64_t R, int interleaved,
+                     int inverse, float mscale, const void* x, int64_t x_sb, int64_t x_st, int64_t x_sh,
+                     const int64_t* positions, int64_t p_sb, const float* inv_freq,
+                     void* y, int64_t y_sb, int64_t y_st, int64_t y_sh, void* stream);
+
+/* The 8-bit attention cache (no counterpart in the reference, whose attention
+ * is stateless across calls).  Codes are e4m3 bytes in pages of `page` tokens
+ * (16, 32 or 64), [n_pages, Hkv, page, D] contiguous, D 64 or 128; every page
+ * and head has one float32 scale, a power of two >= 2^-126, in
+ * [n_pages, Hkv]; keys and values have their own.  Position p of sequence b
+ * is slot p % page of page table[b, p / page] (int32, row stride table_sb,
+ * n_blocks entries).  lengths[b] (int32) counts the tokens of sequence b with
+ * the new ones; its counts[b] (int32, NULL: T) new tokens are rows 0..counts-1
+ * of k, v and q and the last counts[b] positions.
+ *
+ * nt_kv_append writes rows t < counts[b] of k and v ([B,T,Hkv,D] in `dtype`,
+ * element strides, unit stride in D).  Block scale: the smallest power of two
+ * s with max|x| <= 448 s over the block's finite new values, and not below the
+ * block's scale when the block holds older tokens; older codes are re-encoded
+ * when it grows.  Codes: x / s rounded to nearest even, saturating; NaN stays
+ * NaN.  Slots behind the new tokens are left as they are.  A page that is
+ * written must belong to one sequence.  A sequence with counts outside [0, T],
+ * lengths < counts or lengths past the table, and a page outside
+ * [0, n_pages), is skipped and sets the bad-argument bit of the device error
+ * word. */
+NT_API int nt_kv_append(int dtype, int64_t B, int64_t T, int64_t Hkv, int64_t D, int64_t page, int64_t n_pages,
+                        int64_t n_blocks, const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh,
+                        const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                        void* k_codes, float* k_scale, void* v_codes, float* v_scale,
+                        const int32_t* table, int64_t table_sb, const int32_t* lengths, const int32_t* counts,
+                        void* stream);
+
+/* Attention of the new tokens over the cache.  q: [B,T,Hq,D] in `dtype`
+ * (strides as above), Hq a multiple of Hkv; query head h reads cached head
+ * h / (Hq / Hkv).  Row t < counts[b] stands at p = lengths[b] - counts[b] + t
+ * and sees keys j <= p, and j >= p - window when window >= 0 (-1: no window).
+ * out: [B,T,Hq,D] contiguous in `dtype`, softmax(scale q.k) v; rows
+ * t >= counts[b], rows that see no key and sequences with bad counts or lengths
+ * are zero.  Keys in a page outside [0, n_pages) are not seen and set the
+ * bad-argument bit.  Scores and sums in float32.  Meant for one to a few new
+ * tokens per sequence; any T is right.
+ * Workspace: nt_kv_attention_workspace_bytes() (0 when no split is taken). */
+NT_API int64_t nt_kv_attention_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                               int64_t page, int64_t n_blocks, int64_t window);
+NT_API int nt_kv_attention(int dtype, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t page,
+                           int64_t n_pages, int64_t n_blocks, int64_t window, float scale,
+                           const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                           const void* k_codes, const float* k_scale, const void* v_codes, const float* v_scale,
+                           const int32_t* table, int64_t table_sb, const int32_t* lengths, const int32_t* counts,
+                           void* out, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Penalties, biases and masks on logits (NeuraTensorModel.generate's
+ * repetition penalty, model.py:336-342, and what callers add to it), one pass
+ * over [B, V] rows in `dtype` (row strides ld, ldo; out == logits allowed).
+ * With c the count of v among tokens[b, 0..lengths[b]) (int64, row stride
+ * tok_ld, lengths NULL: L) and g the count from prompt_lengths[b] (NULL: 0) on:
+ *   x = repetition penalty r, where c > 0: x > 0 ? x/r : x*r, once, or c times
+ *       with a rounding to `dtype` after each when each != 0 (generate's loop)
+ *   x = x - frequency*g - presence*[g > 0]
+ *   x = x + bias[b, j] for the last j with bias_ids[b, j] == v (int64, ids
+ *       outside [0, V) are skipped)
+ *   x = -inf where bit v % 32 of allowed[b, v / 32] is 0
+ * in float32, one rounding to `dtype`; x/r is the product with float32 1/r.
+ * Tokens outside [0, V) are skipped.  A penalty is a [B] float32 array, or the
+ * scalar beside it when the pointer is NULL (1, 0, 0: none).  tokens, bias and
+ * allowed may be NULL (L, NB 0).  allowed: uint32 words, row stride
+ * allowed_ld (0: one row for the batch). */
+NT_API int nt_logits_process(int dtype, int64_t B, int64_t V, const void* logits, int64_t ld,
+                             const int64_t* tokens, int64_t tok_ld, int64_t L, const int32_t* lengths,
+                             const int32_t* prompt_lengths, int each,
+                             const float* repetition, float repetition_all, const float* frequency,
+                             float frequency_all, const float* presence, float presence_all,
+                             const int64_t* bias_ids, int64_t ids_ld, const float* bias, int64_t bias_ld, int64_t NB,
+                             const uint32_t* allowed, int64_t allowed_ld, void* out, int64_t ldo, void* stream);
 
 #ifdef __cplusplus
 }

@@ -7,10 +7,12 @@ missing or the tensors are not on an sm_100 GPU, the call raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import math
 import os
 import threading
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor
@@ -33,7 +35,7 @@ class NativeError(RuntimeError):
 
 _lib = None
 _lock = threading.Lock()
-_I64, _I32, _P = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p
+_I64, _I32, _F32, _P = ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p
 
 _SIGS = {
     "nt_abi_version": ([], _I32),
@@ -62,6 +64,14 @@ _SIGS = {
     "nt_attention_forward": ([_I32, _I64, _I64, _I64, _I64, _I64] + [_P] * 8 + [_I64, _P], _I32),
     "nt_lm_head_workspace_bytes": ([_I32, _I64, _I64, _I64], _I64),
     "nt_lm_head": ([_I32, _I64, _I64, _I64, _P, _P, _P, _P, _P, _I64, _P], _I32),
+    "nt_rotary": ([_I32, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _F32, _P, _I64, _I64, _I64, _P, _I64, _P, _P, _I64,
+                   _I64, _I64, _P], _I32),
+    "nt_kv_append": ([_I32] + [_I64] * 7 + [_P, _I64, _I64, _I64] * 2 + [_P] * 5 + [_I64, _P, _P, _P], _I32),
+    "nt_kv_attention_workspace_bytes": ([_I64] * 8, _I64),
+    "nt_kv_attention": ([_I32] + [_I64] * 9 + [_F32, _P, _I64, _I64, _I64] + [_P] * 5 + [_I64, _P, _P, _P, _P, _I64, _P],
+                        _I32),
+    "nt_logits_process": ([_I32, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P, _I32] + [_P, _F32] * 3 +
+                          [_P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P], _I32),
 }
 
 EXPORTED = tuple(_SIGS)
@@ -443,6 +453,318 @@ def lm_head(x: Tensor, gamma: Tensor, W: Tensor, workspace: Optional[Tensor] = N
     rc = L.nt_lm_head(_DT[a], M, dm, vocab, _p(x2), _p(g2), _p(W2), _p(logits), _p(ws), ws.numel(), _stream(dev))
     _check("nt_lm_head", rc)
     return logits
+
+
+# --------------------------------------------------------------------------- #
+#  A generation step with an attention memory: rotary positions, the 8-bit     #
+#  cache, attention over it, penalties on logits                               #
+# --------------------------------------------------------------------------- #
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _guard(dev: torch.device):
+    """Makes `dev` current for a launch when it is not."""
+    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _refuse_grad(fn: str, *ts: Optional[Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError(f"{fn} has no backward; detach the inputs or run under torch.no_grad()")
+
+
+def _ints(t: Tensor, dtype: torch.dtype, what: str) -> Tensor:
+    if t.dtype == dtype:
+        return t
+    if t.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
+    return t.to(dtype)
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, inv_freq, layout, mscale, inverse):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.how = (layout, mscale, inverse)
+        return _rotary(x, positions, inv_freq, layout, mscale, inverse, None)
+
+    @staticmethod
+    def backward(ctx, g):
+        positions, inv_freq = ctx.saved_tensors
+        layout, mscale, inverse = ctx.how
+        return rotary(g, positions, inv_freq, layout, mscale, not inverse), None, None, None, None, None
+
+
+def rotary(x: Tensor, positions: Tensor, inv_freq: Tensor, layout: str = "half", mscale: float = 1.0,
+           inverse: bool = False, out: Optional[Tensor] = None) -> Tensor:
+    """Rotary positions (the rotation of apply_rotary, model.py:119-126, at any positions).
+
+    x: [B, T, H, D] float32 or bfloat16, any strides with unit stride in D (q|k of a qkv
+    projection can be rotated where they lie); positions: int64 [B, T], or [T] for all
+    rows; inv_freq: [R/2] float32, the first R <= D dimensions turn and the rest are
+    copied.  layout "half" pairs (i, i + R/2), "interleaved" (2i, 2i + 1).  Pair i turns
+    by positions * inv_freq[i], taken in float64, and is multiplied by mscale; one
+    rounding.  inverse turns backwards.  out may be x (in place).  Differentiable in x
+    (not with out)."""
+    if torch.is_grad_enabled() and (x.requires_grad or inv_freq.requires_grad):
+        if inv_freq.requires_grad:
+            raise RuntimeError("rotary has no gradient for inv_freq; detach it")
+        if out is not None:
+            raise RuntimeError("rotary with out= has no backward; detach x or leave out away")
+        return _Rotary.apply(x, positions, inv_freq, layout, mscale, inverse)
+    return _rotary(x, positions, inv_freq, layout, mscale, inverse, out)
+
+
+def _rotary(x, positions, inv_freq, layout, mscale, inverse, out):
+    dev = _require_cuda(x, positions, inv_freq, out)
+    code = _dtype_code(x)
+    if x.dim() != 4:
+        raise ValueError(f"x must be [B, T, H, D], got {tuple(x.shape)}")
+    B, T, H, D = x.shape
+    if layout not in ("half", "interleaved"):
+        raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1:
+        raise ValueError("inv_freq must be a float32 vector of R/2 frequencies")
+    R = 2 * inv_freq.numel()
+    if not 2 <= R <= D:
+        raise ValueError(f"{R} rotated dimensions do not fit a head of {D}")
+    positions = _ints(positions, torch.int64, "positions")
+    if positions.shape != (B, T):
+        if positions.dim() not in (1, 2) or positions.shape[-1] != T:
+            raise ValueError(f"positions must be [T] or [B, T] = {(B, T)}, got {tuple(positions.shape)}")
+        positions = positions.expand(B, T)
+    if T > 1 and positions.stride(1) != 1:
+        positions = positions.contiguous()
+    if x.stride(3) != 1 and D > 1:
+        x = x.contiguous()
+    if out is None:
+        out = torch.empty((B, T, H, D), dtype=x.dtype, device=dev)
+    else:
+        if out.shape != x.shape or out.dtype != x.dtype or out.stride(3) != 1:
+            raise ValueError("out must have x's shape and dtype and unit stride in D")
+        if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+            raise ValueError("out must not overlap itself")
+    inv_freq = inv_freq.contiguous()
+    with _guard(dev):
+        rc = load().nt_rotary(code, B, T, H, D, R, int(layout == "interleaved"), int(inverse), float(mscale),
+                              x.data_ptr(), x.stride(0), x.stride(1), x.stride(2), positions.data_ptr(),
+                              positions.stride(0), inv_freq.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
+                              out.stride(2), torch.cuda.current_stream(dev).cuda_stream)
+    _check("nt_rotary", rc)
+    return out
+
+
+def _cache_args(fn, B, D, k_codes, k_scale, v_codes, v_scale, table, lengths, counts):
+    """Checks the tensors of a cache; returns (heads, page, pages, blocks, table, lengths, counts)."""
+    if k_codes.dim() != 4 or k_codes.shape != v_codes.shape or k_codes.shape[3] != D:
+        raise ValueError(f"{fn}: codes must be [pages, heads, page, {D}], got {tuple(k_codes.shape)} and "
+                         f"{tuple(v_codes.shape)}")
+    for t in (k_codes, v_codes):
+        if t.dtype not in (torch.float8_e4m3fn, torch.uint8) or not t.is_contiguous():
+            raise ValueError(f"{fn}: codes must be contiguous float8_e4m3fn (or its bytes as uint8)")
+    n, H, P, _ = k_codes.shape
+    for t in (k_scale, v_scale):
+        if t.dtype != torch.float32 or t.shape != (n, H) or not t.is_contiguous():
+            raise ValueError(f"{fn}: scales must be contiguous float32 [pages, heads] = {(n, H)}")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != B or (table.shape[1] > 1 and
+                                                                               table.stride(1) != 1):
+        raise ValueError(f"{fn}: table must be int32 [{B}, blocks] with unit stride")
+    lengths = _ints(lengths, torch.int32, "lengths").contiguous()
+    if lengths.shape != (B,):
+        raise ValueError(f"{fn}: lengths must be [{B}], got {tuple(lengths.shape)}")
+    if counts is not None:
+        counts = _ints(counts, torch.int32, "counts").contiguous()
+        if counts.shape != (B,):
+            raise ValueError(f"{fn}: counts must be [{B}], got {tuple(counts.shape)}")
+    return H, P, n, table.shape[1], lengths, counts
+
+
+def kv_append(k: Tensor, v: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: Tensor, v_scale: Tensor, table: Tensor,
+              lengths: Tensor, counts: Optional[Tensor] = None) -> None:
+    """Writes new keys and values into the paged 8-bit cache, in place.
+
+    k, v: [B, T, H, D] float32 or bfloat16 (unit stride in D, D 64 or 128); codes:
+    [pages, H, page, D] float8_e4m3fn, page 16, 32 or 64; scales: [pages, H] float32, one
+    power of two per page and head; table: int32 [B, blocks], position p of sequence b
+    lies in page table[b, p // page].  lengths [B]: tokens of each sequence with the new
+    ones; counts [B] (None: T): how many of the T rows are new, rows 0..counts-1, which
+    become the last counts positions.  A page's scale grows with its largest value, and
+    its older codes are re-encoded then.  A page that is written must belong to one
+    sequence; a bad length, count or page is skipped and flagged (device_error_flags)."""
+    _refuse_grad("kv_append", k, v)
+    dev = _require_cuda(k, v, k_codes, k_scale, v_codes, v_scale, table, lengths, counts)
+    code = _dtype_code(k)
+    if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError(f"k and v must be [B, T, H, D] of one dtype, got {tuple(k.shape)} {k.dtype} and "
+                         f"{tuple(v.shape)} {v.dtype}")
+    B, T, H, D = k.shape
+    heads, P, n, blocks, lengths, counts = _cache_args("kv_append", B, D, k_codes, k_scale, v_codes, v_scale, table,
+                                                       lengths, counts)
+    if heads != H:
+        raise ValueError(f"kv_append: the cache has {heads} heads, k and v have {H}")
+    if k_codes.data_ptr() == v_codes.data_ptr() and n:
+        raise ValueError("kv_append: keys and values need a cache each")
+    if k.stride(3) != 1:
+        k = k.contiguous()
+    if v.stride(3) != 1:
+        v = v.contiguous()
+    with _guard(dev):
+        rc = load().nt_kv_append(code, B, T, H, D, P, n, blocks, k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
+                                 v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), k_codes.data_ptr(),
+                                 k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
+                                 table.stride(0), lengths.data_ptr(), None if counts is None else counts.data_ptr(),
+                                 torch.cuda.current_stream(dev).cuda_stream)
+    _check("nt_kv_append", rc)
+
+
+def kv_attention(q: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: Tensor, v_scale: Tensor, table: Tensor,
+                 lengths: Tensor, counts: Optional[Tensor] = None, window: Optional[int] = None,
+                 scale: Optional[float] = None) -> Tensor:
+    """Attention of the new tokens over the paged 8-bit cache (kv_append) -> [B, T, Hq, D].
+
+    q: [B, T, Hq, D] float32 or bfloat16, Hq a multiple of the cache's heads; row
+    t < counts[b] stands at lengths[b] - counts[b] + t and sees the keys up to it, with a
+    window only those from position - window on.  Other rows are zero.  scale: of the
+    scores, 1/sqrt(D) by default."""
+    _refuse_grad("kv_attention", q)
+    dev = _require_cuda(q, k_codes, k_scale, v_codes, v_scale, table, lengths, counts)
+    code = _dtype_code(q)
+    if q.dim() != 4:
+        raise ValueError(f"q must be [B, T, H, D], got {tuple(q.shape)}")
+    B, T, Hq, D = q.shape
+    H, P, n, blocks, lengths, counts = _cache_args("kv_attention", B, D, k_codes, k_scale, v_codes, v_scale, table,
+                                                   lengths, counts)
+    if H < 1 or Hq < H or Hq % H:
+        raise ValueError(f"kv_attention: {Hq} query heads over {H} cached heads")
+    if window is not None and window < 0:
+        raise ValueError(f"kv_attention: window must be None or >= 0, got {window}")
+    win = -1 if window is None else int(window)
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=dev)
+    L = load()
+    nbytes = L.nt_kv_attention_workspace_bytes(B, T, Hq, H, D, P, blocks, win)
+    ws = _workspace(nbytes, dev) if nbytes else None
+    with _guard(dev):
+        rc = L.nt_kv_attention(code, B, T, Hq, H, D, P, n, blocks, win, 1.0 / math.sqrt(D) if scale is None else scale,
+                               q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), k_codes.data_ptr(),
+                               k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
+                               table.stride(0), lengths.data_ptr(), None if counts is None else counts.data_ptr(),
+                               out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
+                               torch.cuda.current_stream(dev).cuda_stream)
+    _check("nt_kv_attention", rc)
+    return out
+
+
+def _per_row(name: str, v, B: int, none: float) -> Tuple[Optional[Tensor], float]:
+    """A penalty as ([B] float32, unused) or (None, scalar)."""
+    if v is None:
+        return None, none
+    if isinstance(v, Tensor):
+        if v.shape != (B,):
+            raise ValueError(f"{name} must be a number or [{B}], got {tuple(v.shape)}")
+        return _c(v, torch.float32), none
+    return None, float(v)
+
+
+def logits_process(logits: Tensor, tokens: Optional[Tensor] = None, lengths: Optional[Tensor] = None,
+                   prompt_lengths: Optional[Tensor] = None, repetition: Union[None, float, Tensor] = None,
+                   frequency: Union[None, float, Tensor] = None, presence: Union[None, float, Tensor] = None,
+                   each: bool = False, bias_ids: Optional[Tensor] = None, bias: Optional[Tensor] = None,
+                   allowed: Optional[Tensor] = None, out: Optional[Tensor] = None) -> Tensor:
+    """Penalties for repeated tokens, biases and masks on logits [B, V], one pass (model.py:336-342 and more).
+
+    tokens: [B, L] int64 history, of which row b counts the first lengths[b] (None: L); ids
+    outside the vocabulary are skipped.  repetition r (a number or [B]): a logit x whose
+    token is in the history becomes x / r if positive, else x * r; with each=True once per
+    occurrence, rounded each time, as generate does.  frequency and presence: what is
+    taken off per occurrence and for any, counted from prompt_lengths[b] (None: 0) on.
+    bias_ids [B, N] int64 and bias [B, N]: added to the logits of the ids (-1: none; of
+    equal ids the last holds).  allowed: int32 words [B or 1, ceil(V / 32)]; a zero bit v % 32 of
+    word v // 32 makes the logit -inf (pack_allowed).  float32 arithmetic, one rounding;
+    out may be logits."""
+    _refuse_grad("logits_process", logits, bias)
+    dev = _require_cuda(logits, tokens, lengths, prompt_lengths, bias_ids, bias, allowed, out,
+                        *(t for t in (repetition, frequency, presence) if isinstance(t, Tensor)))
+    code = _dtype_code(logits)
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [B, V], got {tuple(logits.shape)}")
+    B, V = logits.shape
+    if logits.stride(1) != 1 and V > 1:
+        logits = logits.contiguous()
+    L = tok_ld = 0
+    if tokens is not None:
+        tokens = _ints(tokens, torch.int64, "tokens")
+        if tokens.dim() != 2 or tokens.shape[0] != B:
+            raise ValueError(f"tokens must be [{B}, L], got {tuple(tokens.shape)}")
+        L = tokens.shape[1]
+        if L > 1 and tokens.stride(1) != 1:
+            tokens = tokens.contiguous()
+        tok_ld = tokens.stride(0)
+    elif lengths is not None or prompt_lengths is not None:
+        raise ValueError("lengths of a history that is not given")
+    rows = []
+    for name, t in (("lengths", lengths), ("prompt_lengths", prompt_lengths)):
+        if t is not None:
+            t = _ints(t, torch.int32, name).contiguous()
+            if t.shape != (B,):
+                raise ValueError(f"{name} must be [{B}], got {tuple(t.shape)}")
+        rows.append(t)
+    lengths, prompt_lengths = rows
+    if each and prompt_lengths is not None:
+        raise ValueError("a repetition penalty per occurrence takes no prompt_lengths")
+    rep, rep_all = _per_row("repetition", repetition, B, 1.0)
+    fq, fq_all = _per_row("frequency", frequency, B, 0.0)
+    ps, ps_all = _per_row("presence", presence, B, 0.0)
+    if rep is None and not (rep_all > 0.0 and math.isfinite(rep_all)):
+        raise ValueError(f"repetition must be above 0, got {rep_all}")
+    NB = ids_ld = bias_ld = 0
+    if (bias_ids is None) != (bias is None):
+        raise ValueError("bias_ids and bias go together")
+    if bias_ids is not None:
+        if bias_ids.dim() != 2 or bias_ids.shape[0] != B or bias.shape != bias_ids.shape:
+            raise ValueError(f"bias_ids and bias must be [{B}, N], got {tuple(bias_ids.shape)} and {tuple(bias.shape)}")
+        bias_ids = _ints(bias_ids, torch.int64, "bias_ids")
+        bias = bias if bias.dtype == torch.float32 else bias.float()
+        NB = bias.shape[1]
+        if NB > 1 and bias_ids.stride(1) != 1:
+            bias_ids = bias_ids.contiguous()
+        if NB > 1 and bias.stride(1) != 1:
+            bias = bias.contiguous()
+        ids_ld, bias_ld = bias_ids.stride(0), bias.stride(0)
+    allowed_ld = 0
+    if allowed is not None:
+        words = (V + 31) // 32
+        if allowed.dtype not in (torch.int32, torch.uint32) or allowed.dim() != 2 or allowed.shape[0] not in (1, B) or \
+                allowed.shape[1] < words:
+            raise ValueError(f"allowed must be int32 [{B} or 1, {words}], got {allowed.dtype} {tuple(allowed.shape)}")
+        if allowed.shape[1] > 1 and allowed.stride(1) != 1:
+            allowed = allowed.contiguous()
+        allowed_ld = allowed.stride(0) if allowed.shape[0] == B else 0
+    if out is None:
+        out = torch.empty((B, V), dtype=logits.dtype, device=dev)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or (V > 1 and out.stride(1) != 1) or \
+            (B > 1 and out.stride(0) < V):
+        raise ValueError("out must be [B, V] in the logits' dtype with unit column stride")
+    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    with _guard(dev):
+        rc = load().nt_logits_process(code, B, V, logits.data_ptr(), logits.stride(0), p(tokens), tok_ld, L, p(lengths),
+                                      p(prompt_lengths), int(each), p(rep), rep_all, p(fq), fq_all, p(ps), ps_all,
+                                      p(bias_ids), ids_ld, p(bias), bias_ld, NB, p(allowed), allowed_ld, out.data_ptr(),
+                                      out.stride(0), torch.cuda.current_stream(dev).cuda_stream)
+    _check("nt_logits_process", rc)
+    return out
+
+
+def pack_allowed(mask: Tensor) -> Tensor:
+    """A boolean mask [B, V] of allowed tokens as the int32 words that logits_process takes."""
+    if mask.dtype != torch.bool or mask.dim() != 2:
+        raise ValueError("mask must be a boolean [B, V]")
+    B, V = mask.shape
+    bits = torch.zeros((B, (V + 31) // 32 * 32), dtype=torch.int64, device=mask.device)
+    bits[:, :V] = mask
+    words = (bits.view(B, -1, 32) << torch.arange(32, device=mask.device)).sum(-1)
+    return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
 
 
 def launch_count() -> int:

@@ -1,0 +1,116 @@
+"""Refusals of the generation-step entry points that need no GPU: a status and a message, never an abort."""
+import ctypes
+
+import pytest
+import torch
+
+FAKE = ctypes.c_void_p(4096)
+
+
+@pytest.fixture(scope="module")
+def nat():
+    from neuratensor_b200 import build, native
+    build.build()
+    native.load()
+    return native
+
+
+def rotary(L, dtype=0, B=1, T=2, H=3, D=64, R=64, x=FAKE, y=FAKE, pos=FAKE, freq=FAKE, ys=(384, 192, 64)):
+    return L.nt_rotary(dtype, B, T, H, D, R, 0, 0, 1.0, x, 384, 192, 64, pos, 2, freq, y, *ys, None)
+
+
+@pytest.mark.parametrize("bad,status,text", [
+    (dict(dtype=2), 2, "dtype"), (dict(R=63), 1, "even"), (dict(R=66), 1, "even"), (dict(R=0), 1, "even"), (dict(B=-1), 1, "sizes"),
+    (dict(D=0), 1, "sizes"), (dict(x=None), 1, "null"), (dict(pos=None), 1, "null"), (dict(freq=None), 1, "null"),
+    (dict(y=None), 1, "null"), (dict(ys=(1, 2, 3)), 1, "in place")])
+def test_rotary_status(nat, bad, status, text):
+    L = nat.load()
+    assert rotary(L, **bad) == status
+    assert text in L.nt_last_error().decode()
+
+
+def test_empty_calls_succeed(nat):
+    L = nat.load()
+    assert rotary(L, B=0, x=None) == 0 and rotary(L, T=0, x=None) == 0
+    assert append(L, T=0, k=None) == 0
+    assert attention(L, B=0, q=None) == 0
+    assert logits(L, B=0, x=None) == 0
+
+
+def append(L, dtype=1, B=1, T=1, H=2, D=64, page=16, n=4, blocks=2, k=FAKE, codes=FAKE, lengths=FAKE):
+    return L.nt_kv_append(dtype, B, T, H, D, page, n, blocks, k, 0, 0, 0, FAKE, 0, 0, 0, codes, FAKE, FAKE, FAKE, FAKE, 2, lengths,
+                          None, None)
+
+
+@pytest.mark.parametrize("bad,status,text", [
+    (dict(dtype=2), 2, "dtype"), (dict(D=72), 1, "head_dim"), (dict(page=8), 1, "page"), (dict(page=48), 1, "page"),
+    (dict(B=65536), 1, "sizes"), (dict(H=0), 1, "sizes"), (dict(k=None), 1, "null"), (dict(lengths=None), 1, "null"),
+    (dict(codes=ctypes.c_void_p(4104)), 1, "alignment")])
+def test_append_status(nat, bad, status, text):
+    L = nat.load()
+    assert append(L, **bad) == status
+    assert text in L.nt_last_error().decode()
+
+
+def attention(L, dtype=1, B=1, T=1, Hq=2, H=2, D=64, page=16, blocks=2, window=-1, q=FAKE, codes=FAKE, ws=None, nbytes=0):
+    return L.nt_kv_attention(dtype, B, T, Hq, H, D, page, 4, blocks, window, 1.0, q, 0, 0, 0, codes, FAKE, FAKE, FAKE, FAKE, 2, FAKE,
+                             None, FAKE, ws, nbytes, None)
+
+
+@pytest.mark.parametrize("bad,status,text", [
+    (dict(dtype=0x7), 2, "dtype"), (dict(D=256), 1, "head_dim"), (dict(page=128), 1, "page"), (dict(Hq=3), 1, "sizes"),
+    (dict(Hq=1), 1, "sizes"), (dict(H=0), 1, "sizes"), (dict(blocks=1 << 28), 1, "sizes"), (dict(q=None), 1, "null"),
+    (dict(codes=ctypes.c_void_p(4104)), 1, "alignment"), (dict(blocks=4096), 6, "workspace")])
+def test_attention_status(nat, bad, status, text):
+    L = nat.load()
+    assert attention(L, **bad) == status
+    assert text in L.nt_last_error().decode()
+
+
+def test_attention_workspace_covers_long_caches(nat):
+    L = nat.load()
+    need = L.nt_kv_attention_workspace_bytes(1, 1, 32, 8, 128, 64, 2048, -1)
+    assert need > 0
+    assert attention(L, Hq=32, H=8, D=128, page=64, blocks=2048, ws=FAKE, nbytes=need - 1) == 6
+    assert L.nt_kv_attention_workspace_bytes(1, 1, 10, 10, 64, 16, 4, -1) == 0        # one CTA per head sees all of it
+    assert L.nt_kv_attention_workspace_bytes(0, 1, 1, 1, 64, 16, 4, -1) == 0
+
+
+def logits(L, dtype=0, B=1, V=100, x=FAKE, tokens=FAKE, n=5, prompts=None, each=0, rep=1.0, ids=None, nb=0, out=FAKE, ldo=100):
+    return L.nt_logits_process(dtype, B, V, x, 100, tokens, 5, n, None, prompts, each, None, rep, None, 0.0, None, 0.0, ids, 0, None, 0,
+                               nb, None, 0, out, ldo, None)
+
+
+@pytest.mark.parametrize("bad,status,text", [
+    (dict(dtype=2), 2, "dtype"), (dict(V=0), 1, "sizes"), (dict(B=-1), 1, "sizes"), (dict(x=None), 1, "null"),
+    (dict(tokens=None), 1, "null"), (dict(nb=3), 1, "null"), (dict(ldo=101), 1, "in place"), (dict(each=1, prompts=FAKE), 1, "occurrence"),
+    (dict(rep=0.0), 1, "above 0"), (dict(rep=float("nan")), 1, "above 0")])
+def test_logits_status(nat, bad, status, text):
+    L = nat.load()
+    assert logits(L, **bad) == status
+    assert text in L.nt_last_error().decode()
+
+
+def test_cpu_tensors_are_refused(nat):
+    x = torch.zeros(1, 1, 2, 64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        nat.rotary(x, torch.zeros(1, 1, dtype=torch.int64), torch.ones(32))
+    c, s = torch.zeros(2, 2, 16, 64, dtype=torch.uint8), torch.ones(2, 2)
+    args = (c, s, c.clone(), s.clone(), torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        nat.kv_append(x, x, *args)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        nat.kv_attention(x, *args)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        nat.logits_process(torch.zeros(1, 10))
+
+
+def test_pack_allowed_words():
+    from neuratensor_b200 import native
+    mask = torch.zeros(2, 70, dtype=torch.bool)
+    mask[0, [0, 31, 32, 69]] = True
+    mask[1] = True
+    words = native.pack_allowed(mask)
+    assert words.dtype == torch.int32 and words.tolist() == [[-2 ** 31 + 1, 1, 32], [-1, -1, 63]]
+    with pytest.raises(ValueError):
+        native.pack_allowed(mask.int())
