@@ -5,21 +5,21 @@
 // a window, j >= p - window.
 //
 // Bound by HBM: a step reads every visible code once (one byte per element)
-// and does two flops per query row with it.  So nothing is staged: the codes
-// go from global memory to registers in the shape the matrix instruction
-// takes, one tile of 16 keys ahead of the arithmetic, and the tensor cores
-// (mma m16n8k16, f16 in, float32 sums) do the products that would cost the
-// CUDA cores a conversion and an FMA per element.  The 16-row operand is the
-// query rows of one cached head: eight of them (a step of eight shared heads,
-// or a draft of a few tokens), and in the other eight rows what f16 leaves of
-// them, which makes the product exact to float32 for float32 queries and costs
-// nothing; e4m3 codes and bf16 queries are exact in f16 as they are.
+// and does two flops per query row with it.  Each warp streams its own tiles of
+// 16 keys through a ring in shared memory (16-byte cp.async, two tiles ahead of
+// the arithmetic, no barrier between warps), and the tensor cores (mma m16n8k16,
+// f16 in, float32 sums) do the products that would cost the CUDA cores a
+// conversion and an FMA per element.  The cached operand is the 16-row one of
+// each product (keys of K, then dimensions of V^T), the query rows of one cached
+// head the 8 columns: up to eight shared heads of a step, or a draft of a few
+// tokens.  e4m3 codes and bf16 queries are exact in f16; float32 queries and
+// weights are split into two f16 and take each product twice.
 //
 // The k order of a product is free, so a lane takes 16 consecutive dimensions
-// of a key (one 16-byte load) as its part of four k-steps, with q in the same
-// order; likewise lane group g of V owns D/8 consecutive dimensions, one per
-// n-tile, of the four keys whose probabilities the lane holds after the first
-// product, so the probabilities never leave their registers either.
+// of a key (one 16-byte read) as its part of four k-steps, with q in the same
+// order; likewise lane group g of V owns D/8 consecutive dimensions of the four
+// keys whose probabilities the lane holds, which come from the first product by
+// one 8x8 transpose per eight keys.
 //
 // Softmax is online, in float32, base 2: a warp keeps its rows' running
 // maximum, sum and output over its tiles; four warps of a CTA join in shared
@@ -29,7 +29,7 @@
 // rounding is 2^-9, and as an f16 pair for float32.
 #include "nt_kernels.cuh"
 
-#include <cuda_fp8.h>
+#include <cuda_fp16.h>
 
 #include <algorithm>
 
@@ -50,7 +50,7 @@ struct KvAttnArgs {
     int chunk;                         // tiles per CTA
     int splits, row_tiles;
     float scale_log2;
-    const void* q; int64_t q_sb, q_st, q_sh;
+    const void* q; int64_t q_sb, q_st, q_sh; int q_vec;
     const uint8_t* kc; const float* ks; const uint8_t* vc; const float* vs;
     const int32_t* table; int64_t table_sb;
     const int32_t* lengths; const int32_t* counts;
@@ -83,15 +83,27 @@ __device__ __forceinline__ Span span_of(const KvAttnArgs& a, int64_t b, int row_
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1, float c0, float c1, float c2, float c3) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
-                 "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
-// two e4m3 codes (low 16 bits) to two f16 values, exactly
-__device__ __forceinline__ uint32_t cvt2(uint32_t w) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-    return (uint32_t)h.x | ((uint32_t)h.y << 16);
+// two e4m3 codes (the low or the high half of w) to two f16 values, exactly
+__device__ __forceinline__ uint32_t cvt_lo(uint32_t w) {
+    uint32_t r;
+    asm("{.reg .b16 a, b; mov.b32 {a, b}, %1; cvt.rn.f16x2.e4m3x2 %0, a;}" : "=r"(r) : "r"(w));
+    return r;
+}
+__device__ __forceinline__ uint32_t cvt_hi(uint32_t w) {
+    uint32_t r;
+    asm("{.reg .b16 a, b; mov.b32 {a, b}, %1; cvt.rn.f16x2.e4m3x2 %0, b;}" : "=r"(r) : "r"(w));
+    return r;
+}
+// an 8x8 matrix of f16, one row of two columns per lane, transposed
+__device__ __forceinline__ uint32_t transpose(uint32_t w) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+    return r;
 }
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -99,64 +111,26 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
 }
 __device__ __forceinline__ float2 unpack_h2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-// One tile of codes in registers: for K, rows g and g+8 of the tile, 16 bytes
-// per 64 dimensions; for V, rows 2c, 2c+1, 2c+8, 2c+9, the lane group's D/8 bytes.
-template <int D> struct TileRegs {
-    uint32_t k[2][D / 64][4];
-    uint32_t v[4][D / 32];
-    float ks, vs;
-    bool live;
-};
+// A warp's ring: kStages tiles of 16 keys, K then V, rows of D bytes.  16-byte
+// chunk c of a row is stored at chunk c ^ swizzle(row), so that the eight lanes
+// that read together (K: two rows, four chunks; V: four even or four odd rows,
+// two chunks) meet different banks.
+constexpr int kStages = 3;
+template <int D> constexpr int kTileBytes = kTile * D;
+template <int D> constexpr size_t kRingBytes = (size_t)kWarps * kStages * 2 * kTileBytes<D>;
+template <int D> __device__ __forceinline__ int k_swz(int row) { return D == 128 ? (row & 1) * 4 : 0; }
+template <int D> __device__ __forceinline__ int v_swz(int row) { return D == 128 ? row & 6 : (row >> 1) & 3; }
 
-template <int D>
-__device__ __forceinline__ void load_tile(TileRegs<D>& r, const KvAttnArgs& a, int key0, int page, int h, int g, int c) {
-    r.live = page >= 0 && page < a.n_pages;
-    if (!r.live) {
-        r.ks = r.vs = 0.f;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int i = 0; i < D / 64; ++i) r.k[n][i][0] = r.k[n][i][1] = r.k[n][i][2] = r.k[n][i][3] = 0u;
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) r.v[n][i] = 0u;
-        return;
-    }
-    const int64_t head = (int64_t)page * a.H + h;
-    const int slot = key0 & ((1 << a.page_shift) - 1);
-    const int64_t off = ((head << a.page_shift) + slot) * D;
-    const uint8_t* kp = a.kc + off;
-    const uint8_t* vp = a.vc + off;
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(kp + (n * 8 + g) * D + 64 * i + 16 * c));
-            r.k[n][i][0] = w.x; r.k[n][i][1] = w.y; r.k[n][i][2] = w.z; r.k[n][i][3] = w.w;
-        }
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-        const uint8_t* p = vp + ((n >> 1) * 8 + 2 * c + (n & 1)) * D + g * (D / 8);
-        if constexpr (D == 128) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-            r.v[n][0] = w.x; r.v[n][1] = w.y; r.v[n][2] = w.z; r.v[n][3] = w.w;
-        } else {
-            const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
-            r.v[n][0] = w.x; r.v[n][1] = w.y;
-        }
-    }
-    r.ks = __ldg(a.ks + head);
-    r.vs = __ldg(a.vs + head);
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-
 template <int DT, int D>
-__global__ void __launch_bounds__(kAttnThreads, 3) kv_attention_kernel(const __grid_constant__ KvAttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, 4) kv_attention_kernel(const __grid_constant__ KvAttnArgs a) {
     using El = Elem<DT>;
     using T = typename El::T;
     constexpr int KS = D / 16;                 // k-steps of the first product
-    constexpr int NT = D / 8;                  // n-tiles of the second
-    constexpr bool kPair = DT == NT_F32;       // rows 8..15 hold what f16 leaves of rows 0..7
+    constexpr int MT = D / 16;                 // 16-dimension tiles of the second
+    constexpr bool kPair = DT == NT_F32;       // a second product with what f16 leaves of q and of the weights
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int split = blockIdx.x, h = blockIdx.y / a.row_tiles, row_tile = blockIdx.y % a.row_tiles;
     const int64_t b = blockIdx.z;
@@ -167,7 +141,9 @@ __global__ void __launch_bounds__(kAttnThreads, 3) kv_attention_kernel(const __g
 
     const int row = row_tile * kRows + g, t = row / a.G;
     const bool live = t < s.cnt;
-    const int p = live ? s.start + t : -1;
+    // in the products a lane holds rows 2c and 2c + 1: their positions
+    const int t0 = (row_tile * kRows + 2 * c) / a.G, t1 = (row_tile * kRows + 2 * c + 1) / a.G;
+    const int p0 = t0 < s.cnt ? s.start + t0 : -1, p1 = t1 < s.cnt ? s.start + t1 : -1;
     // every row of the CTA sees all of a tile when it lies in [all_lo, all_hi)
     const int all_hi = s.start + row_tile * kRows / a.G + 1, all_lo = a.window >= 0 ? s.hi - 1 - a.window : 0;
 
@@ -179,10 +155,28 @@ __global__ void __launch_bounds__(kAttnThreads, 3) kv_attention_kernel(const __g
         float amax = 0.f;
         const T* q = static_cast<const T*>(a.q) + b * a.q_sb + (int64_t)t * a.q_st + (int64_t)(h * a.G + row % a.G) * a.q_sh;
 #pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+            if (!live) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[i][e] = 0.f;
+            } else if (a.q_vec) {
+                constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll
+                for (int e = 0; e < 16; e += E) {
+                    const uint4 w = __ldg(reinterpret_cast<const uint4*>(q + 64 * i + 16 * c + e));
+                    const T* x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+                    for (int j = 0; j < E; ++j) v[i][e + j] = El::to_f(x[j]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[i][e] = El::load(q + 64 * i + 16 * c + e);
+            }
+        }
+#pragma unroll
         for (int i = 0; i < D / 64; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                v[i][e] = live ? El::load(q + 64 * i + 16 * c + e) : 0.f;
                 const float m = fabsf(v[i][e]);
                 if (m <= 3.402823466e38f) amax = fmaxf(amax, m);
             }
@@ -207,167 +201,262 @@ __global__ void __launch_bounds__(kAttnThreads, 3) kv_attention_kernel(const __g
             }
     }
 
-    float o[NT][2];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    const float qi0 = __shfl_sync(0xffffffffu, q_inv, 8 * c), qi1 = __shfl_sync(0xffffffffu, q_inv, 8 * c + 4);
 
+    // o[j]: dimensions g*D/8 + 2j (rows 2c, 2c+1) and g*D/8 + 2j + 1 (the same rows), in units of v_unit
+    float o[MT][4];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, v_unit = 0.f;
+
+    // This warp's tiles are first + warp + kWarps * i, i < mine.  Lane j holds the
+    // page and the scales of the j-th of 32 tiles: f_* for the tiles being
+    // fetched, c_* for those being computed, at most two behind.
+    const int mine = last - first > warp ? (last - first - warp + kWarps - 1) / kWarps : 0;
     const int32_t* table = a.table + b * a.table_sb;
-    auto page_of = [&](int tile) { return tile < last ? table[(s.lo16 + tile * kTile) >> a.page_shift] : -1; };
-    int tile = first + warp;
-    TileRegs<D> cur, nxt;
+    int f_page = -1, c_page = -1;
+    float f_ks = 0.f, f_vs = 0.f, c_ks = 0.f, c_vs = 0.f;
     bool bad_page = false;
-    int page = page_of(tile), page2 = page_of(tile + kWarps);
-    if (tile < last) {
-        load_tile<D>(cur, a, s.lo16 + tile * kTile, page, h, g, c);
-        bad_page |= !cur.live;
-    }
-    for (; tile < last; tile += kWarps) {
-        page = page2;
-        page2 = page_of(tile + 2 * kWarps);
-        if (tile + kWarps < last) {
-            load_tile<D>(nxt, a, s.lo16 + (tile + kWarps) * kTile, page, h, g, c);
-            bad_page |= !nxt.live;
-        }
-        if (cur.live) {
-            const int key0 = s.lo16 + tile * kTile;
-            // scores of 16 keys: n-tile n, keys 8n + 2c and + 1 of row g
-            float sc[2][2];
-            const float f = q_inv * cur.ks;
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    const uint32_t w = cur.k[n][k / 4][k % 4];
-                    mma_f16(d, qh[k][0], ql[k][0], qh[k][1], ql[k][1], cvt2(w), cvt2(w >> 16), d[0], d[1], d[2], d[3]);
+    extern __shared__ __align__(128) unsigned char smem[];
+    unsigned char* ring = smem + warp * (kStages * 2 * kTileBytes<D>);
+    const uint32_t ring_u32 = smem_u32(ring);
+    auto fetch = [&](int i) {
+        if ((i & 31) == 0) {
+            f_page = -1;
+            if (i + lane < mine) {
+                const int pg = table[(s.lo16 + (first + warp + kWarps * (i + lane)) * kTile) >> a.page_shift];
+                if (pg < 0 || pg >= a.n_pages) {
+                    bad_page = true;
+                } else {
+                    f_page = pg;
+                    f_ks = __ldg(a.ks + (int64_t)pg * a.H + h);
+                    f_vs = __ldg(a.vs + (int64_t)pg * a.H + h);
                 }
-                sc[n][0] = (kPair ? d[0] + d[2] : d[0]) * f;
-                sc[n][1] = (kPair ? d[1] + d[3] : d[1]) * f;
             }
+        }
+        const int pg = __shfl_sync(0xffffffffu, f_page, i & 31);
+        if (pg >= 0 && i < mine) {
+            const int slot = ((first + warp + kWarps * i) * kTile + s.lo16) & ((1 << a.page_shift) - 1);
+            const int64_t off = ((((int64_t)pg * a.H + h) << a.page_shift) + slot) * D + lane * 16;
+            const uint32_t dst = ring_u32 + (i % kStages) * (2 * kTileBytes<D>);
+            constexpr int CH = D / 16;                  // chunks of a row
+#pragma unroll
+            for (int j = 0; j < kTileBytes<D> / 512; ++j) {
+                const int row = j * (32 / CH) + lane / CH, ch = lane % CH;
+                cp16(dst + row * D + ((ch ^ k_swz<D>(row)) << 4), a.kc + off + j * 512);
+                cp16(dst + kTileBytes<D> + row * D + ((ch ^ v_swz<D>(row)) << 4), a.vc + off + j * 512);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    fetch(0);
+    fetch(1);
+    for (int i = 0; i < mine; ++i) {
+        if ((i & 31) == 0) {
+            c_page = f_page;
+            c_ks = f_ks;
+            c_vs = f_vs;
+        }
+        __syncwarp();                                   // the stage that fetch writes has been read by all lanes
+        fetch(i + 2);
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        __syncwarp();                                   // every lane's part of tile i has landed
+        if (__shfl_sync(0xffffffffu, c_page, i & 31) >= 0) {
+            const int key0 = s.lo16 + (first + warp + kWarps * i) * kTile;
+            const unsigned char* kt = ring + (i % kStages) * (2 * kTileBytes<D>);
+            const unsigned char* vt = kt + kTileBytes<D>;
+            const float ks = __shfl_sync(0xffffffffu, c_ks, i & 31), vs = __shfl_sync(0xffffffffu, c_vs, i & 31);
+            // scores: d[0], d[1] key g of the tile, d[2], d[3] key g + 8, for rows 2c and 2c + 1
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) {
+                const int at = g * D + (((4 * j + c) ^ k_swz<D>(g)) << 4);
+                const uint4 u = *reinterpret_cast<const uint4*>(kt + at), w = *reinterpret_cast<const uint4*>(kt + 8 * D + at);
+                const uint32_t ku[4] = {u.x, u.y, u.z, u.w}, kw[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t a0 = cvt_lo(ku[k]), a1 = cvt_lo(kw[k]), a2 = cvt_hi(ku[k]), a3 = cvt_hi(kw[k]);
+                    mma_f16(d, a0, a1, a2, a3, qh[4 * j + k][0], qh[4 * j + k][1], d[0], d[1], d[2], d[3]);
+                    if constexpr (kPair) mma_f16(d, a0, a1, a2, a3, ql[4 * j + k][0], ql[4 * j + k][1], d[0], d[1], d[2], d[3]);
+                }
+            }
+            float sc[2][2] = {{d[0] * (qi0 * ks), d[1] * (qi1 * ks)}, {d[2] * (qi0 * ks), d[3] * (qi1 * ks)}};
             const bool whole = key0 >= all_lo && key0 >= s.lo && key0 + kTile <= all_hi;
-            uint32_t ind0 = 0u, ind1 = 0u;              // which keys the row sees, as f16 ones
             if (!whole) {
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < 2; ++n) {
+                    const int key = key0 + 8 * n + g;
+                    if (key > p0 || (a.window >= 0 && key < p0 - a.window)) sc[n][0] = -INFINITY;
+                    if (key > p1 || (a.window >= 0 && key < p1 - a.window)) sc[n][1] = -INFINITY;
+                }
+            }
+            float x0 = fmaxf(sc[0][0], sc[1][0]), x1 = fmaxf(sc[0][1], sc[1][1]);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int key = key0 + 8 * n + 2 * c + e;
-                        const bool see = key <= p && (a.window < 0 || key >= p - a.window);
-                        if (!see) sc[n][e] = -INFINITY;
-                        const uint32_t one = see ? 0x3c00u << (16 * e) : 0u;
-                        if (n == 0) ind0 |= one; else ind1 |= one;
-                    }
-                // slots that no row sees may hold anything, NaN too
+            for (int k = 4; k < 32; k *= 2) {
+                x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, k));
+                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, k));
+            }
+            if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+                x0 = fmaxf(x0, m0);
+                x1 = fmaxf(x1, m1);
+                const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - x0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - x1);
+                m0 = x0;
+                m1 = x1;
+                l0 *= f0;
+                l1 *= f1;
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    o[j][0] *= f0; o[j][1] *= f1;
+                    o[j][2] *= f0; o[j][3] *= f1;
+                }
+            }
+            // The sums are kept in units of one block's scale, so that another block's is
+            // a factor of its weights.  A larger scale becomes the unit; one far below it
+            // would push the weights out of f16 and multiplies its product instead.
+            if (vs > 2.f * v_unit) {
+                const float f = v_unit / vs;
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    o[j][0] *= f; o[j][1] *= f;
+                    o[j][2] *= f; o[j][3] *= f;
+                }
+                v_unit = vs;
+            }
+            const float rel = v_unit > 0.f ? vs / v_unit : 0.f;
+            const bool plain = rel >= 0.00390625f;                 // 2^-8
+            const float fold = plain ? rel : 1.f, unfold = plain ? v_unit / vs : 1.f;
+            const float b0f = m0 == -INFINITY ? 0.f : m0 - kPShift, b1f = m1 == -INFINITY ? 0.f : m1 - kPShift;
+            const float w00 = ex2(sc[0][0] - b0f) * fold, w01 = ex2(sc[0][1] - b1f) * fold;
+            const float w10 = ex2(sc[1][0] - b0f) * fold, w11 = ex2(sc[1][1] - b1f) * fold;
+            uint32_t pk0 = pack_h2(w00, w01), pk1 = pack_h2(w10, w11);
+            uint32_t bl0 = 0u, bl1 = 0u;
+            {
+                const float2 r0 = unpack_h2(pk0), r1 = unpack_h2(pk1);
+                if constexpr (kPair) {
+                    bl0 = transpose(pack_h2(w00 - r0.x, w01 - r0.y));
+                    bl1 = transpose(pack_h2(w10 - r1.x, w11 - r1.y));
+                    l0 = fmaf(w00 + w10, unfold, l0);
+                    l1 = fmaf(w01 + w11, unfold, l1);
+                } else {                                           // the weights that are used sum to one
+                    l0 = fmaf(r0.x + r1.x, unfold, l0);
+                    l1 = fmaf(r0.y + r1.y, unfold, l1);
+                }
+            }
+            uint32_t bh0 = transpose(pk0), bh1 = transpose(pk1);  // row g, keys 2c, 2c+1 and 2c+8, 2c+9
+            uint32_t vw[4][D / 32];
+            auto load_v = [&]() {
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
-                    const int key = key0 + (n >> 1) * 8 + 2 * c + (n & 1);
-                    if (key < s.lo || key >= s.hi) {
+                    const int r = (n >> 1) * 8 + 2 * c + (n & 1);
+                    const unsigned char* row = vt + r * D;
+                    if constexpr (D == 128) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(row + ((g ^ v_swz<D>(2 * c)) << 4));
+                        vw[n][0] = w.x; vw[n][1] = w.y; vw[n][2] = w.z; vw[n][3] = w.w;
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2*>(row + (((g >> 1) ^ v_swz<D>(2 * c)) << 4) + (g & 1) * 8);
+                        vw[n][0] = w.x; vw[n][1] = w.y;
+                    }
+                    // slots that no row sees may hold anything, NaN too
+                    if (!whole && (key0 + r < s.lo || key0 + r >= s.hi)) {
 #pragma unroll
-                        for (int i = 0; i < D / 32; ++i) cur.v[n][i] = 0u;
+                        for (int k = 0; k < D / 32; ++k) vw[n][k] = 0u;
                     }
                 }
-            }
-            float mx = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            if (__any_sync(0xffffffffu, mx > m)) {
-                const float mn = fmaxf(m, mx);
-                const float corr = m == -INFINITY ? 0.f : ex2(m - mn);
-                m = mn;
-                l *= corr;
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    o[j][0] *= corr;
-                    o[j][1] *= corr;
-                }
-            }
-            const float base = m == -INFINITY ? 0.f : m - kPShift;
-            const float p00 = ex2(sc[0][0] - base), p01 = ex2(sc[0][1] - base);
-            const float p10 = ex2(sc[1][0] - base), p11 = ex2(sc[1][1] - base);
-            uint32_t a0 = pack_h2(p00, p01), a2 = pack_h2(p10, p11), a1 = 0u, a3 = 0u;
-            {
-                const float2 r0 = unpack_h2(a0), r1 = unpack_h2(a2);
-                if constexpr (kPair) {
-                    a1 = pack_h2(p00 - r0.x, p01 - r0.y);
-                    a3 = pack_h2(p10 - r1.x, p11 - r1.y);
-                    l += (p00 + p01) + (p10 + p11);
-                } else {
-                    l += (r0.x + r0.y) + (r1.x + r1.y);       // the weights that are used sum to one
-                }
-            }
+            };
+            auto nan_bytes = [](uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u; };
+            load_v();
             // A NaN value among keys that some row does not see: 0 * NaN would reach
             // that row.  Rare, so it takes a second product: the values without their
             // NaNs, then infinity where a row sees one, turned to NaN (inf * 0).
             bool extra = false;
-            float vscale = cur.vs;
-            uint32_t nan_at[4][D / 32];
             if (!whole && a.T > 1) {
                 uint32_t any = 0u;
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
 #pragma unroll
-                    for (int i = 0; i < D / 32; ++i) any |= (cur.v[n][i] & 0x7f7f7f7fu) + 0x01010101u;
-                if (__any_sync(0xffffffffu, (any & 0x80808080u) != 0u)) {
-                    extra = true;
+                    for (int k = 0; k < D / 32; ++k) any |= nan_bytes(vw[n][k]);
+                extra = __any_sync(0xffffffffu, any != 0u);
+            }
+            // 16 dimensions by 16 keys of V^T: rows g and g + 8 are dimensions g*D/8 + 2j and + 1
+            auto v_tile = [&](int j, uint32_t (&f)[4]) {
+                const int k = j / 2;
+                const uint32_t sel = j & 1 ? 0x7362 : 0x5140;
+                const uint32_t lo = __byte_perm(vw[0][k], vw[1][k], sel), hi = __byte_perm(vw[2][k], vw[3][k], sel);
+                f[0] = cvt_lo(lo); f[1] = cvt_hi(lo); f[2] = cvt_lo(hi); f[3] = cvt_hi(hi);
+            };
+            if (plain && !extra) {
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    uint32_t f[4];
+                    v_tile(j, f);
+                    mma_f16(o[j], f[0], f[1], f[2], f[3], bh0, bh1, o[j][0], o[j][1], o[j][2], o[j][3]);
+                    if constexpr (kPair) mma_f16(o[j], f[0], f[1], f[2], f[3], bl0, bl1, o[j][0], o[j][1], o[j][2], o[j][3]);
+                }
+            } else {
+                float f_out = plain ? 1.f : rel;
+                if (extra) {
 #pragma unroll
                     for (int n = 0; n < 4; ++n)
 #pragma unroll
-                        for (int i = 0; i < D / 32; ++i) {
-                            const uint32_t hit = (((cur.v[n][i] & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
-                            nan_at[n][i] = hit * 0x7eu;        // 448
-                            cur.v[n][i] &= ~(hit * 0xffu);
-                        }
+                        for (int k = 0; k < D / 32; ++k) vw[n][k] &= ~(nan_bytes(vw[n][k]) * 0xffu);
                 }
-            }
-            for (;;) {
+                for (;;) {
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                    const uint32_t lo01 = __byte_perm(cur.v[0][i], cur.v[1][i], 0x5140), lo23 = __byte_perm(cur.v[0][i], cur.v[1][i], 0x7362);
-                    const uint32_t hi01 = __byte_perm(cur.v[2][i], cur.v[3][i], 0x5140), hi23 = __byte_perm(cur.v[2][i], cur.v[3][i], 0x7362);
+                    for (int j = 0; j < MT; ++j) {
+                        uint32_t f[4];
+                        float e[4];
+                        v_tile(j, f);
+                        mma_f16(e, f[0], f[1], f[2], f[3], bh0, bh1, 0.f, 0.f, 0.f, 0.f);
+                        if constexpr (kPair) mma_f16(e, f[0], f[1], f[2], f[3], bl0, bl1, e[0], e[1], e[2], e[3]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t w0 = (e < 2 ? lo01 : lo23) >> (16 * (e & 1)), w1 = (e < 2 ? hi01 : hi23) >> (16 * (e & 1));
-                        float d[4];
-                        mma_f16(d, a0, a1, a2, a3, cvt2(w0), cvt2(w1), 0.f, 0.f, 0.f, 0.f);
-                        o[4 * i + e][0] = fmaf(vscale, kPair ? d[0] + d[2] : d[0], o[4 * i + e][0]);
-                        o[4 * i + e][1] = fmaf(vscale, kPair ? d[1] + d[3] : d[1], o[4 * i + e][1]);
+                        for (int k = 0; k < 4; ++k) {
+                            o[j][k] = fmaf(f_out, e[k], o[j][k]);
+                            if (f_out == kHuge) o[j][k] = fmaf(o[j][k], 0.f, o[j][k]);
+                        }
                     }
+                    if (!extra) break;
+                    extra = false;
+                    f_out = kHuge;
+                    // which keys the rows see, as f16 ones, and the NaNs as 448
+                    const int ka = key0 + g, kb = key0 + 8 + g;
+                    auto sees = [&](int key, int p) { return key <= p && (a.window < 0 || key >= p - a.window); };
+                    pk0 = (sees(ka, p0) ? 0x3c00u : 0u) | (sees(ka, p1) ? 0x3c000000u : 0u);
+                    pk1 = (sees(kb, p0) ? 0x3c00u : 0u) | (sees(kb, p1) ? 0x3c000000u : 0u);
+                    bh0 = transpose(pk0);
+                    bh1 = transpose(pk1);
+                    bl0 = bl1 = 0u;
+                    load_v();
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+#pragma unroll
+                        for (int k = 0; k < D / 32; ++k) vw[n][k] = nan_bytes(vw[n][k]) * 0x7eu;
                 }
-                if (!extra) {
-                    if (vscale == kHuge)
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            o[j][0] = fmaf(o[j][0], 0.f, o[j][0]);
-                            o[j][1] = fmaf(o[j][1], 0.f, o[j][1]);
-                        }
-                    break;
-                }
-                extra = false;
-                vscale = kHuge;
-                a0 = ind0; a2 = ind1; a1 = a3 = 0u;
-#pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                    for (int i = 0; i < D / 32; ++i) cur.v[n][i] = nan_at[n][i];
             }
         }
-        cur = nxt;
     }
-    if (bad_page && lane == 0) atomicOr(a.err, ERRF_BAD_ARG);
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (bad_page) atomicOr(a.err, ERRF_BAD_ARG);
+#pragma unroll
+    for (int k = 4; k < 32; k *= 2) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, k);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, k);
+    }
 
-    // join the four warps: lane (g, c) of a warp holds row g, dimensions [c*D/4, (c+1)*D/4)
-    __shared__ float so[kWarps][kRows][D];
-    __shared__ float sm[kWarps][kRows], sl[kWarps][kRows];
+    // join the four warps
+    __syncthreads();                                    // all rings are read: their memory takes the sums
+    float (*so)[kRows][D] = reinterpret_cast<float (*)[kRows][D]>(smem);
+    float (*sm)[kRows] = reinterpret_cast<float (*)[kRows]>(smem + sizeof(float) * kWarps * kRows * D);
+    float (*sl)[kRows] = sm + kWarps;
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) so[warp][g][(2 * c + half) * NT + j] = o[j][half];
-    if (c == 0) {
-        sm[warp][g] = m;
-        sl[warp][g] = l;
+    for (int j = 0; j < MT; ++j) {
+        const int d = g * (D / 8) + 2 * j;
+        *reinterpret_cast<float2*>(&so[warp][2 * c][d]) = make_float2(o[j][0] * v_unit, o[j][2] * v_unit);
+        *reinterpret_cast<float2*>(&so[warp][2 * c + 1][d]) = make_float2(o[j][1] * v_unit, o[j][3] * v_unit);
+    }
+    if (g == 0) {
+        sm[warp][2 * c] = m0;
+        sm[warp][2 * c + 1] = m1;
+        sl[warp][2 * c] = l0;
+        sl[warp][2 * c + 1] = l1;
     }
     __syncthreads();
     const int rows = min(kRows, a.T * a.G - row_tile * kRows);
@@ -448,7 +537,10 @@ Plan plan_of(int64_t B, int64_t T, int64_t G, int64_t H, int64_t D, int64_t page
 template <int DT, int D>
 int launch_kv_attention(const KvAttnArgs& a, int64_t B, cudaStream_t stream) {
     const dim3 grid((unsigned)a.splits, (unsigned)(a.H * a.row_tiles), (unsigned)B);
-    kv_attention_kernel<DT, D><<<grid, kAttnThreads, 0, stream>>>(a);
+    const size_t smem = std::max(kRingBytes<D>, sizeof(float) * kWarps * kRows * (D + 2));
+    const cudaError_t e = cudaFuncSetAttribute(kv_attention_kernel<DT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return fail(NT_ERR_CUDA, "nt_kv_attention: %s", cudaGetErrorString(e));
+    kv_attention_kernel<DT, D><<<grid, kAttnThreads, smem, stream>>>(a);
     const int rc = check_launch("kv_attention_kernel");
     if (rc != NT_OK || a.splits == 1) return rc;
     const dim3 jgrid((unsigned)(a.H * a.row_tiles * kRows), 1, (unsigned)B);
@@ -502,6 +594,8 @@ int nt_kv_attention(int dtype, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, in
     a.chunk = pl.chunk; a.splits = pl.splits; a.row_tiles = pl.row_tiles;
     a.scale_log2 = scale * kLog2e;
     a.q = q; a.q_sb = q_sb; a.q_st = q_st; a.q_sh = q_sh;
+    const int64_t es = dtype == NT_F32 ? 4 : 2;
+    a.q_vec = ((reinterpret_cast<uintptr_t>(q) | (uint64_t)((q_sb | q_st | q_sh) * es)) & 15) == 0;
     a.kc = static_cast<const uint8_t*>(k_codes); a.ks = k_scale;
     a.vc = static_cast<const uint8_t*>(v_codes); a.vs = v_scale;
     a.table = table; a.table_sb = table_sb; a.lengths = lengths; a.counts = counts;
