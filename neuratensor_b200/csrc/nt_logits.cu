@@ -4,26 +4,27 @@
 // history; frequency and presence penalties, biases and masks are what callers
 // add around it).
 //
-// Bound by HBM: logits in and out once, one mask bit per entry, and the
-// history once.  The history has to be counted per vocabulary entry before a
-// logit is final, so a cluster of CTAs owns a row: each CTA holds the counters
-// of its slice of the vocabulary in shared memory, reads its share of the
-// history and adds to whichever CTA of the cluster owns the token (distributed
-// shared memory), and after one cluster barrier streams its slice.  Integer
-// counters: their order of arrival changes nothing.
+// Bound by HBM: logits in and out once, one mask bit per entry, the history
+// once.  The history has to be counted per vocabulary entry before a logit is
+// final, so a CTA owns a slice of one row's vocabulary, with a counter per entry
+// in shared memory: it reads the row's whole history (from L2 for all slices
+// but the first), counts what falls into its slice, and then streams the slice.
+// Several CTAs share an SM, so one streams while another counts.  (A cluster of
+// CTAs per row that read the history once and counted into each other's shared
+// memory was slower: 131 us against 70 us for 250 x 131072 float32 with 4000 tokens of
+// history, 21.5 against 13.3 us for 64 x 32000 bf16 with 8704.)  Integer counters: the
+// order of arrival changes nothing.
 //
 // A counter holds the index (plus one) of the last bias entry of the token, the
 // number of occurrences after the prompt, and one bit for an occurrence at all:
 // 16 + 15 + 1 bits of one word while the history is below 2^15 tokens and the
-// biases below 2^16, else two words (the index in the second; not one of 64
-// bits, whose atomics in another CTA's shared memory lost updates when tried).
+// biases below 2^16, else two words.
+//
+// In place and without a mask nothing else changes, so only the entries with a
+// counter are read and written.
 #include "nt_kernels.cuh"
 
-#include <cooperative_groups.h>
-
 #include <algorithm>
-
-namespace cg = cooperative_groups;
 
 namespace nt {
 namespace {
@@ -40,7 +41,8 @@ struct LogArgs {
     const int64_t* ids; int64_t ids_ld; const float* bias; int64_t bias_ld; int NB;
     const uint32_t* allowed; int64_t allowed_ld;
     void* out; int64_t ldo;
-    int slice;                         // vocabulary entries per CTA and turn, a multiple of 128
+    int slice;                         // vocabulary entries per CTA, a multiple of 128
+    int slices;
 };
 
 // Where a counter's parts lie.  Narrow: bit 31 seen, bits 16..30 the
@@ -75,99 +77,141 @@ __global__ void __launch_bounds__(kLogThreads) logits_kernel(const __grid_consta
     using T = typename El::T;
     using K = Count<WIDE>;
     constexpr int E = 16 / (int)sizeof(T);
-    extern __shared__ __align__(16) uint32_t words[];       // [slice] counters, [slice] bias indices when wide
-    cg::cluster_group cluster = cg::this_cluster();
-    const int CS = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int64_t b = blockIdx.x / CS;
-    const T* x = static_cast<const T*>(a.x) + b * a.ld;
-    T* y = static_cast<T*>(a.out) + b * a.ldo;
+    extern __shared__ __align__(16) uint32_t smem[];
+    const int64_t b = blockIdx.x / a.slices;
+    const int64_t lo = (int64_t)(blockIdx.x % a.slices) * a.slice;
+    const int n = (int)(a.V - lo < a.slice ? a.V - lo : a.slice);
+    const T* x = static_cast<const T*>(a.x) + b * a.ld + lo;
+    T* y = static_cast<T*>(a.out) + b * a.ldo + lo;
+    // Entries before the first 16-byte boundary of x.  Entry i's counter is
+    // words[i], shifted so that those of a vector are 16-byte aligned too.
+    const int head_x = (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T);
+    const int head_y = (int)((16 - (reinterpret_cast<uintptr_t>(y) & 15)) & 15) / (int)sizeof(T);
+    const int pad = (E - head_x) & (E - 1);
+    uint32_t* words = smem + pad;
+    const int stride = a.slice + E;                     // from the counters to the bias indices when wide
     const float r = a.rep ? a.rep[b] : a.rep_all, fq = a.freq ? a.freq[b] : a.freq_all, ps = a.pres ? a.pres[b] : a.pres_all;
     const float r_inv = 1.f / r;
     const uint32_t* mask = a.allowed ? a.allowed + b * a.allowed_ld : nullptr;
-    const int64_t* ids = a.ids + b * a.ids_ld;
-    const float* bias = a.bias + b * a.bias_ld;
+    const float* bias = a.NB ? a.bias + b * a.bias_ld : nullptr;
     int len = a.tokens ? (a.lengths ? a.lengths[b] : a.L) : 0;
     len = len < 0 ? 0 : (len > a.L ? a.L : len);
-    const int prompt = a.prompts ? a.prompts[b] : 0;
-    const int64_t* tok = a.tokens + b * a.tok_ld;
-    const bool vec = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) == 0;
+    const bool counted = len > 0 || a.NB > 0;
 
-    for (int64_t base = 0; base < a.V; base += (int64_t)CS * a.slice) {
-        const int64_t lo = base + (int64_t)rank * a.slice;
-        const int n = lo < a.V ? (int)(a.V - lo < a.slice ? a.V - lo : a.slice) : 0;
-        for (int i = threadIdx.x; i < a.slice * K::kWords; i += kLogThreads) words[i] = 0;
-        cluster.sync();
-        for (int i = rank * kLogThreads + threadIdx.x; i < len; i += CS * kLogThreads) {
-            const int64_t v = tok[i];
-            if (v < base || v >= a.V) continue;
-            const int64_t rel = v - base;
-            if (rel >= (int64_t)CS * a.slice) continue;
-            const int owner = (int)((uint32_t)rel / (uint32_t)a.slice);
-            uint32_t* w = cluster.map_shared_rank(words, owner) + ((uint32_t)rel - (uint32_t)owner * a.slice);
-            if (i >= prompt) atomicAdd(w, K::kOne);
-            else atomicOr(w, K::kSeen);
-        }
-        cluster.sync();
-        for (int j = threadIdx.x; j < a.NB; j += kLogThreads) {
-            const int64_t v = ids[j];
-            if (v < lo || v >= lo + n) continue;
-            uint32_t* w = words + (v - lo) + (WIDE ? a.slice : 0);
-            // the upper bits no longer change, so the maximum is that of the index
-            atomicMax(w, WIDE ? (uint32_t)(j + 1) : (*w & 0xffff0000u) | (uint32_t)(j + 1));
+    if (counted) {
+        for (int i = threadIdx.x; i < stride * K::kWords / 4; i += kLogThreads)
+            reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        const int prompt = a.prompts ? a.prompts[b] : 0;
+        const int64_t* tok = a.tokens + b * a.tok_ld;
+        constexpr int R = 8;                            // tokens of a thread in flight
+        for (int i0 = threadIdx.x; i0 < len; i0 += R * kLogThreads) {
+            uint32_t v[R];
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                const int i = i0 + k * kLogThreads;
+                const int64_t t = i < len ? __ldg(tok + i) : -1;
+                v[k] = (uint64_t)t >> 32 ? ~0u : (uint32_t)t - (uint32_t)lo;
+            }
+#pragma unroll
+            for (int k = 0; k < R; ++k)
+                if (v[k] < (uint32_t)n) {
+                    if (i0 + k * kLogThreads >= prompt) atomicAdd(words + v[k], K::kOne);
+                    else atomicOr(words + v[k], K::kSeen);
+                }
         }
         __syncthreads();
-        auto idx = [&](int i) { return WIDE ? words[a.slice + i] : 0u; };
-        auto allowed = [&](int i) { return !mask || ((mask[(lo + i) >> 5] >> ((lo + i) & 31)) & 1u); };
-        const int nv = vec ? n / E : 0;
-        for (int i = threadIdx.x; i < nv; i += kLogThreads) {
-            const uint4 q = *reinterpret_cast<const uint4*>(x + lo + (int64_t)i * E);
-            const T* xv = reinterpret_cast<const T*>(&q);
-            uint4 o;
-            T* ov = reinterpret_cast<T*>(&o);
-            const int64_t at = lo + (int64_t)i * E;
-            const uint32_t bits = mask ? mask[at >> 5] >> (at & 31) : ~0u;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                float v = El::to_f(xv[e]);
-                v = process<DT, WIDE, EACH>(v, words[i * E + e], idx(i * E + e), r, r_inv, fq, ps, bias);
-                ov[e] = El::from_f((bits >> e) & 1u ? v : -INFINITY);
+        if (a.NB) {
+            const int64_t* ids = a.ids + b * a.ids_ld;
+            for (int j = threadIdx.x; j < a.NB; j += kLogThreads) {
+                const uint64_t v = (uint64_t)(__ldg(ids + j) - lo);
+                if (v < (uint64_t)n) {
+                    uint32_t* w = words + v + (WIDE ? stride : 0);
+                    // the upper bits no longer change, so the maximum is that of the index
+                    atomicMax(w, WIDE ? (uint32_t)(j + 1) : (*w & 0xffff0000u) | (uint32_t)(j + 1));
+                }
             }
-            *reinterpret_cast<uint4*>(y + at) = o;
+            __syncthreads();
         }
-        for (int i = nv * E + threadIdx.x; i < n; i += kLogThreads) {
-            const float v = process<DT, WIDE, EACH>(El::to_f(x[lo + i]), words[i], idx(i), r, r_inv, fq, ps, bias);
-            y[lo + i] = El::from_f(allowed(i) ? v : -INFINITY);
-        }
-        cluster.sync();                 // the next turn, or the end: nobody writes to a CTA that has left
     }
+    auto one = [&](int i) {                             // a single entry
+        const uint32_t w = counted ? words[i] : 0u, j = WIDE && counted ? words[stride + i] : 0u;
+        const float v = process<DT, WIDE, EACH>(El::to_f(x[i]), w, j, r, r_inv, fq, ps, bias);
+        const bool ok = !mask || ((mask[(lo + i) >> 5] >> ((lo + i) & 31)) & 1u);
+        y[i] = El::from_f(ok ? v : -INFINITY);
+    };
+    if (static_cast<const void*>(x) == static_cast<const void*>(y) && !mask) {
+        if (counted)
+            for (int i = threadIdx.x; i < n; i += kLogThreads)
+                if (words[i] || (WIDE && words[stride + i])) one(i);
+        return;
+    }
+    const int head = head_x == head_y ? (head_x < n ? head_x : n) : n;      // all singly when no boundary is shared
+    const int nv = (n - head) / E;
+    constexpr int U = 4;                                // vectors of a thread in flight
+    for (int i0 = threadIdx.x; i0 < nv; i0 += U * kLogThreads) {
+        uint4 q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * kLogThreads < nv) q[u] = __ldcs(reinterpret_cast<const uint4*>(x + head) + i0 + u * kLogThreads);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * kLogThreads, first = head + i * E;
+            if (i >= nv) break;
+            T xv[E];
+            *reinterpret_cast<uint4*>(xv) = q[u];
+            uint32_t w[E], any = 0u;
+            if (counted) {
+#pragma unroll
+                for (int e = 0; e < E; e += 4) {
+                    const uint4 c = *reinterpret_cast<const uint4*>(words + first + e);
+                    w[e] = c.x; w[e + 1] = c.y; w[e + 2] = c.z; w[e + 3] = c.w;
+                    any |= c.x | c.y | c.z | c.w;
+                    if (WIDE) {
+                        const uint4 d = *reinterpret_cast<const uint4*>(words + stride + first + e);
+                        any |= d.x | d.y | d.z | d.w;
+                    }
+                }
+            }
+            if (any) {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    xv[e] = El::from_f(process<DT, WIDE, EACH>(El::to_f(xv[e]), w[e], WIDE ? words[stride + first + e] : 0u,
+                                                               r, r_inv, fq, ps, bias));
+            }
+            if (mask) {
+                const int64_t at = lo + first;
+                uint32_t bits = mask[at >> 5];
+                const int sh = (int)(at & 31);
+                if (sh + E > 32) bits = __funnelshift_r(bits, mask[(at >> 5) + 1], sh);
+                else bits >>= sh;
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (!((bits >> e) & 1u)) xv[e] = El::from_f(-INFINITY);
+            }
+            __stcs(reinterpret_cast<uint4*>(y + head) + i, *reinterpret_cast<const uint4*>(xv));
+        }
+    }
+    for (int i = threadIdx.x; i < head; i += kLogThreads) one(i);
+    for (int i = head + nv * E + threadIdx.x; i < n; i += kLogThreads) one(i);
 }
 
 template <int DT, bool WIDE, bool EACH>
 int launch(LogArgs a, int64_t B, cudaStream_t stream) {
-    constexpr int kCluster = 8;
-    int64_t slice = ((a.V + kCluster - 1) / kCluster + 127) / 128 * 128;
-    slice = std::min<int64_t>(slice, 196608 / (4 * Count<WIDE>::kWords) / 128 * 128);
+    // Slices of 1024 to 8192 entries: four CTAs per SM if the rows allow it, and
+    // no more slices than that, since each reads the whole history of its row.
+    const int64_t want = std::max<int64_t>(1, 4 * 148 / B);
+    int64_t slice = std::min<int64_t>(8192, std::max<int64_t>(1024, (a.V + want - 1) / want));
+    slice = (slice + 127) / 128 * 128;
     a.slice = (int)slice;
-    const size_t smem = (size_t)slice * 4 * Count<WIDE>::kWords;
+    a.slices = (int)((a.V + slice - 1) / slice);
+    if (B * a.slices > INT32_MAX) return fail(NT_ERR_ARG, "nt_logits_process: too many rows");
+    const bool counted = (a.tokens && a.L > 0) || a.NB > 0;
+    const size_t smem = counted ? (size_t)(slice + 16 / (DT == NT_F32 ? 4 : 2)) * 4 * Count<WIDE>::kWords : 0;
     auto kern = logits_kernel<DT, WIDE, EACH>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 8200 * 4 * Count<WIDE>::kWords);
     if (e != cudaSuccess) return fail(NT_ERR_CUDA, "nt_logits_process: %s", cudaGetErrorString(e));
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(B * kCluster));
-    cfg.blockDim = dim3(kLogThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kCluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kern, a);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        return fail(NT_ERR_CUDA, "logits_kernel launch failed: %s", cudaGetErrorString(e));
-    }
+    kern<<<(unsigned)(B * a.slices), kLogThreads, smem, stream>>>(a);
     return check_launch("logits_kernel");
 }
 
