@@ -591,8 +591,10 @@ template <int DT, int D, int W>
 int launch_kv_attention(const KvAttnArgs& a, int64_t B, cudaStream_t stream) {
     const dim3 grid((unsigned)a.splits, (unsigned)(a.H * a.row_tiles), (unsigned)B);
     const size_t smem = std::max(kRingBytes<D, W>, sizeof(float) * W * kRows * (D + 2));
-    cudaError_t e = cudaFuncSetAttribute(kv_attention_kernel<DT, D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return fail(NT_ERR_CUDA, "nt_kv_attention: %s", cudaGetErrorString(e));
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kv_attention_kernel<DT, D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return fail(NT_ERR_CUDA, "nt_kv_attention: %s", cudaGetErrorString(e));
+    }
     kv_attention_kernel<DT, D, W><<<grid, W * 32, smem, stream>>>(a);
     const int rc = check_launch("kv_attention_kernel");
     if (rc != NT_OK || a.splits == 1) return rc;
@@ -605,7 +607,7 @@ int launch_kv_attention(const KvAttnArgs& a, int64_t B, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<DT, D>, a);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<DT, D>, a);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return fail(NT_ERR_CUDA, "kv_attention_join_kernel launch failed: %s", cudaGetErrorString(e));

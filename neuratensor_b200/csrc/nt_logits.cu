@@ -209,8 +209,10 @@ int launch(LogArgs a, int64_t B, cudaStream_t stream) {
     const bool counted = (a.tokens && a.L > 0) || a.NB > 0;
     const size_t smem = counted ? (size_t)(slice + 16 / (DT == NT_F32 ? 4 : 2)) * 4 * Count<WIDE>::kWords : 0;
     auto kern = logits_kernel<DT, WIDE, EACH>;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 8200 * 4 * Count<WIDE>::kWords);
-    if (e != cudaSuccess) return fail(NT_ERR_CUDA, "nt_logits_process: %s", cudaGetErrorString(e));
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return fail(NT_ERR_CUDA, "nt_logits_process: %s", cudaGetErrorString(e));
+    }
     kern<<<(unsigned)(B * a.slices), kLogThreads, smem, stream>>>(a);
     return check_launch("logits_kernel");
 }

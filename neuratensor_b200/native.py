@@ -7,8 +7,8 @@ missing or the tensors are not on an sm_100 GPU, the call raises.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 import math
 import os
 import threading
@@ -118,24 +118,24 @@ _checked_devices = set()
 
 
 def _require_cuda(*ts: Optional[Tensor]) -> torch.device:
-    dev = None
+    idx = first = None
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise RuntimeError("neuratensor_b200 runs its hot path on CUDA (sm_100 / B200) only; "
-                               f"got a tensor on {t.device}")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
-    if dev is None:
+        i = t.get_device()                        # -1 for a CPU tensor
+        if idx is None:
+            idx, first = i, t
+        if i != idx or not t.is_cuda:
+            if not t.is_cuda:
+                raise RuntimeError("neuratensor_b200 runs its hot path on CUDA (sm_100 / B200) only; "
+                                   f"got a tensor on {t.device}")
+            raise RuntimeError(f"tensors on different devices: {first.device} and {t.device}")
+    if first is None:
         raise RuntimeError("no CUDA tensor given")
-    idx = dev.index if dev.index is not None else torch.cuda.current_device()
     if idx not in _checked_devices:
         _check("nt_device_supported", load().nt_device_supported(idx))
         _checked_devices.add(idx)
-    return dev
+    return first.device
 
 
 def _dtype_code(t: Tensor) -> int:
@@ -460,16 +460,23 @@ def lm_head(x: Tensor, gamma: Tensor, W: Tensor, workspace: Optional[Tensor] = N
 #  cache, attention over it, penalties on logits                               #
 # --------------------------------------------------------------------------- #
 
-_NO_GUARD = contextlib.nullcontext()
+def _launch(dev: torch.device, name: str, *args) -> None:
+    """Calls a C entry point with `dev` current and its current stream as the last argument.
+
+    These calls are short (a step makes several per layer), so the stream is read as the
+    raw handle and the device switched only when it has to be."""
+    fn = getattr(_lib, name)
+    if dev.index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc != 0:
+        _check(name, rc)
 
 
-def _guard(dev: torch.device):
-    """Makes `dev` current for a launch when it is not."""
-    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-
-def _refuse_grad(fn: str, *ts: Optional[Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+def _refuse_grad(fn: str, t: Tensor, u: Optional[Tensor] = None) -> None:
+    if (t.requires_grad or (u is not None and u.requires_grad)) and torch.is_grad_enabled():
         raise RuntimeError(f"{fn} has no backward; detach the inputs or run under torch.no_grad()")
 
 
@@ -506,7 +513,7 @@ def rotary(x: Tensor, positions: Tensor, inv_freq: Tensor, layout: str = "half",
     by positions * inv_freq[i], taken in float64, and is multiplied by mscale; one
     rounding.  inverse turns backwards.  out may be x (in place).  Differentiable in x
     (not with out)."""
-    if torch.is_grad_enabled() and (x.requires_grad or inv_freq.requires_grad):
+    if (x.requires_grad or inv_freq.requires_grad) and torch.is_grad_enabled():
         if inv_freq.requires_grad:
             raise RuntimeError("rotary has no gradient for inv_freq; detach it")
         if out is not None:
@@ -528,30 +535,41 @@ def _rotary(x, positions, inv_freq, layout, mscale, inverse, out):
     R = 2 * inv_freq.numel()
     if not 2 <= R <= D:
         raise ValueError(f"{R} rotated dimensions do not fit a head of {D}")
-    positions = _ints(positions, torch.int64, "positions")
+    if positions.dtype != torch.int64:
+        positions = _ints(positions, torch.int64, "positions")
     if positions.shape != (B, T):
         if positions.dim() not in (1, 2) or positions.shape[-1] != T:
             raise ValueError(f"positions must be [T] or [B, T] = {(B, T)}, got {tuple(positions.shape)}")
         positions = positions.expand(B, T)
-    if T > 1 and positions.stride(1) != 1:
+    p_sb, p_st = positions.stride()
+    if p_st != 1 and T > 1:
         positions = positions.contiguous()
-    if x.stride(3) != 1 and D > 1:
+        p_sb = T
+    x_sb, x_st, x_sh, unit = x.stride()
+    if unit != 1 and D > 1:
         x = x.contiguous()
+        x_sb, x_st, x_sh, _ = x.stride()
     if out is None:
-        out = torch.empty((B, T, H, D), dtype=x.dtype, device=dev)
-    else:
-        if out.shape != x.shape or out.dtype != x.dtype or out.stride(3) != 1:
-            raise ValueError("out must have x's shape and dtype and unit stride in D")
-        if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
-            raise ValueError("out must not overlap itself")
-    inv_freq = inv_freq.contiguous()
-    with _guard(dev):
-        rc = load().nt_rotary(code, B, T, H, D, R, int(layout == "interleaved"), int(inverse), float(mscale),
-                              x.data_ptr(), x.stride(0), x.stride(1), x.stride(2), positions.data_ptr(),
-                              positions.stride(0), inv_freq.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
-                              out.stride(2), torch.cuda.current_stream(dev).cuda_stream)
-    _check("nt_rotary", rc)
+        out = x.new_empty((B, T, H, D))
+    elif out.shape != x.shape or out.dtype != x.dtype or out.stride(3) != 1:
+        raise ValueError("out must have x's shape and dtype and unit stride in D")
+    elif any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+        raise ValueError("out must not overlap itself")
+    y_sb, y_st, y_sh, _ = out.stride()
+    _launch(dev, "nt_rotary", code, B, T, H, D, R, layout == "interleaved", inverse, mscale, x.data_ptr(), x_sb, x_st, x_sh,
+            positions.data_ptr(), p_sb, inv_freq.contiguous().data_ptr(), out.data_ptr(), y_sb, y_st, y_sh)
     return out
+
+
+def _row_ints(fn: str, what: str, t: Optional[Tensor], B: int) -> Optional[Tensor]:
+    """An integer per row as contiguous int32 [B]."""
+    if t is None:
+        return None
+    if t.shape != (B,):
+        raise ValueError(f"{fn}: {what} must be [{B}], got {tuple(t.shape)}")
+    if t.dtype != torch.int32:
+        t = _ints(t, torch.int32, what)
+    return t.contiguous()
 
 
 def _cache_args(fn, B, D, k_codes, k_scale, v_codes, v_scale, table, lengths, counts):
@@ -566,17 +584,10 @@ def _cache_args(fn, B, D, k_codes, k_scale, v_codes, v_scale, table, lengths, co
     for t in (k_scale, v_scale):
         if t.dtype != torch.float32 or t.shape != (n, H) or not t.is_contiguous():
             raise ValueError(f"{fn}: scales must be contiguous float32 [pages, heads] = {(n, H)}")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != B or (table.shape[1] > 1 and
-                                                                               table.stride(1) != 1):
+    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != B or (table.stride(1) != 1 and
+                                                                               table.shape[1] > 1):
         raise ValueError(f"{fn}: table must be int32 [{B}, blocks] with unit stride")
-    lengths = _ints(lengths, torch.int32, "lengths").contiguous()
-    if lengths.shape != (B,):
-        raise ValueError(f"{fn}: lengths must be [{B}], got {tuple(lengths.shape)}")
-    if counts is not None:
-        counts = _ints(counts, torch.int32, "counts").contiguous()
-        if counts.shape != (B,):
-            raise ValueError(f"{fn}: counts must be [{B}], got {tuple(counts.shape)}")
-    return H, P, n, table.shape[1], lengths, counts
+    return H, P, n, table.shape[1], _row_ints(fn, "lengths", lengths, B), _row_ints(fn, "counts", counts, B)
 
 
 def kv_append(k: Tensor, v: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: Tensor, v_scale: Tensor, table: Tensor,
@@ -608,13 +619,16 @@ def kv_append(k: Tensor, v: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: T
         k = k.contiguous()
     if v.stride(3) != 1:
         v = v.contiguous()
-    with _guard(dev):
-        rc = load().nt_kv_append(code, B, T, H, D, P, n, blocks, k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-                                 v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), k_codes.data_ptr(),
-                                 k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
-                                 table.stride(0), lengths.data_ptr(), None if counts is None else counts.data_ptr(),
-                                 torch.cuda.current_stream(dev).cuda_stream)
-    _check("nt_kv_append", rc)
+    k_sb, k_st, k_sh, _ = k.stride()
+    v_sb, v_st, v_sh, _ = v.stride()
+    _launch(dev, "nt_kv_append", code, B, T, H, D, P, n, blocks, k.data_ptr(), k_sb, k_st, k_sh, v.data_ptr(), v_sb, v_st,
+            v_sh, k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
+            table.stride(0), lengths.data_ptr(), None if counts is None else counts.data_ptr())
+
+
+@functools.lru_cache(maxsize=256)
+def _kv_attention_bytes(*sizes: int) -> int:
+    return load().nt_kv_attention_workspace_bytes(*sizes)
 
 
 def kv_attention(q: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: Tensor, v_scale: Tensor, table: Tensor,
@@ -641,18 +655,14 @@ def kv_attention(q: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: Tensor, v
     win = -1 if window is None else int(window)
     if q.stride(3) != 1:
         q = q.contiguous()
-    out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=dev)
-    L = load()
-    nbytes = L.nt_kv_attention_workspace_bytes(B, T, Hq, H, D, P, blocks, win)
-    ws = _workspace(nbytes, dev) if nbytes else None
-    with _guard(dev):
-        rc = L.nt_kv_attention(code, B, T, Hq, H, D, P, n, blocks, win, 1.0 / math.sqrt(D) if scale is None else scale,
-                               q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), k_codes.data_ptr(),
-                               k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
-                               table.stride(0), lengths.data_ptr(), None if counts is None else counts.data_ptr(),
-                               out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
-                               torch.cuda.current_stream(dev).cuda_stream)
-    _check("nt_kv_attention", rc)
+    q_sb, q_st, q_sh, _ = q.stride()
+    out = q.new_empty((B, T, Hq, D))
+    nbytes = _kv_attention_bytes(B, T, Hq, H, D, P, blocks, win)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _launch(dev, "nt_kv_attention", code, B, T, Hq, H, D, P, n, blocks, win, 1.0 / math.sqrt(D) if scale is None else scale,
+            q.data_ptr(), q_sb, q_st, q_sh, k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(),
+            table.data_ptr(), table.stride(0), lengths.data_ptr(), None if counts is None else counts.data_ptr(),
+            out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     return out
 
 
@@ -703,14 +713,8 @@ def logits_process(logits: Tensor, tokens: Optional[Tensor] = None, lengths: Opt
         tok_ld = tokens.stride(0)
     elif lengths is not None or prompt_lengths is not None:
         raise ValueError("lengths of a history that is not given")
-    rows = []
-    for name, t in (("lengths", lengths), ("prompt_lengths", prompt_lengths)):
-        if t is not None:
-            t = _ints(t, torch.int32, name).contiguous()
-            if t.shape != (B,):
-                raise ValueError(f"{name} must be [{B}], got {tuple(t.shape)}")
-        rows.append(t)
-    lengths, prompt_lengths = rows
+    lengths = _row_ints("logits_process", "lengths", lengths, B)
+    prompt_lengths = _row_ints("logits_process", "prompt_lengths", prompt_lengths, B)
     if each and prompt_lengths is not None:
         raise ValueError("a repetition penalty per occurrence takes no prompt_lengths")
     rep, rep_all = _per_row("repetition", repetition, B, 1.0)
@@ -742,17 +746,16 @@ def logits_process(logits: Tensor, tokens: Optional[Tensor] = None, lengths: Opt
             allowed = allowed.contiguous()
         allowed_ld = allowed.stride(0) if allowed.shape[0] == B else 0
     if out is None:
-        out = torch.empty((B, V), dtype=logits.dtype, device=dev)
+        out = logits.new_empty((B, V))
     elif out.shape != logits.shape or out.dtype != logits.dtype or (V > 1 and out.stride(1) != 1) or \
             (B > 1 and out.stride(0) < V):
         raise ValueError("out must be [B, V] in the logits' dtype with unit column stride")
-    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    with _guard(dev):
-        rc = load().nt_logits_process(code, B, V, logits.data_ptr(), logits.stride(0), p(tokens), tok_ld, L, p(lengths),
-                                      p(prompt_lengths), int(each), p(rep), rep_all, p(fq), fq_all, p(ps), ps_all,
-                                      p(bias_ids), ids_ld, p(bias), bias_ld, NB, p(allowed), allowed_ld, out.data_ptr(),
-                                      out.stride(0), torch.cuda.current_stream(dev).cuda_stream)
-    _check("nt_logits_process", rc)
+    held = (tokens, lengths, prompt_lengths, rep, fq, ps, bias_ids, bias, allowed)      # until the launch
+    tokens, lengths, prompt_lengths, rep, fq, ps, bias_ids, bias, allowed = [
+        None if t is None else t.data_ptr() for t in held]
+    _launch(dev, "nt_logits_process", code, B, V, logits.data_ptr(), logits.stride(0), tokens, tok_ld, L, lengths,
+            prompt_lengths, each, rep, rep_all, fq, fq_all, ps, ps_all, bias_ids, ids_ld, bias, bias_ld, NB, allowed,
+            allowed_ld, out.data_ptr(), out.stride(0))
     return out
 
 
