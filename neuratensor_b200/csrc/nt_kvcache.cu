@@ -11,10 +11,12 @@
 // a block whose scale grows is exact down to e4m3's subnormals, so filling a
 // block token by token loses nothing against filling it at once.
 //
-// One block of threads per (sequence, touched page, head) and side (k or v):
-// the new values are read once into registers, their largest magnitude is
-// reduced, and the codes are written; 8 values per thread and step (16 bytes
-// of bf16 in, 8 bytes of codes out).  Bound by HBM for prompts, by launch
+// One CTA of 64 or 128 threads per (sequence, touched page, head) and side (k or
+// v): the new values are read once into registers, their largest magnitude is
+// reduced, and the codes are written; 8 values per thread and step (16 bytes of
+// bf16 in, 8 bytes of codes out).  Bound by HBM for prompts (8 of up to 8192
+// tokens, 16 heads of 128: 112 us with 128 threads that looked the page up before
+// they read, 84 us so; several units to a CTA of 256 threads 92 us), by launch
 // latency for single tokens.
 #include "nt_kernels.cuh"
 
@@ -23,7 +25,8 @@
 namespace nt {
 namespace {
 
-constexpr int kAppThreads = 128;
+// Threads of a block of P x D values, eight vectors of eight values each or fewer.
+template <int D, int P> constexpr int kAppThreadsOf = P * D / 64 > 64 ? P * D / 64 : 64;
 
 struct AppendArgs {
     int64_t T; int H; int64_t n_pages, n_blocks;
@@ -57,35 +60,56 @@ __device__ __forceinline__ int block_exponent(float amax) {
 }
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-template <int DT>
-__device__ __forceinline__ void load8(const typename Elem<DT>::T* p, bool vec, float (&v)[8]) {
-    if constexpr (DT == NT_BF16) {
-        if (vec) {
-            const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
-            return;
-        }
-    } else if (vec) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = Elem<DT>::load(p + i);
-}
-
-// NV: vectors of 8 values per thread, P * D / 8 / kAppThreads.
-template <int DT, int D, int P>
-__global__ void __launch_bounds__(kAppThreads) kv_append_kernel(AppendArgs a, int vec) {
+// Eight values as they are read.
+template <int DT> struct Raw {
     using T = typename Elem<DT>::T;
+    static constexpr int W = 8 * (int)sizeof(T) / 16;
+    uint4 w[W];
+    __device__ __forceinline__ void load(const T* p, bool vec) {
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(w)[i] = p[i];
+        }
+    }
+    __device__ __forceinline__ float at(int i) const {
+        const uint32_t u = reinterpret_cast<const uint32_t*>(w)[DT == NT_BF16 ? i / 2 : i];
+        return __uint_as_float(DT != NT_BF16 ? u : i & 1 ? u & 0xffff0000u : u << 16);
+    }
+    // Largest magnitude, NaN ignored; infinity where there is one.
+    __device__ __forceinline__ float amax() const {
+        float m = 0.f;
+        if constexpr (DT == NT_BF16) {
+            const uint32_t* u = reinterpret_cast<const uint32_t*>(w);
+            uint32_t p = u[0] & 0x7fff7fffu;
+#pragma unroll
+            for (int i = 1; i < 4; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(p) : "r"(u[i] & 0x7fff7fffu));
+            m = fmaxf(fmaxf(m, __uint_as_float(p << 16)), __uint_as_float(p & 0xffff0000u));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(at(i)));
+        }
+        return m;
+    }
+    __device__ __forceinline__ float amax_finite() const {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float v = fabsf(at(i));
+            if (v <= 3.402823466e38f) m = fmaxf(m, v);
+        }
+        return m;
+    }
+};
+
+template <int DT, int D, int P>
+__global__ void __launch_bounds__(kAppThreadsOf<D, P>) kv_append_kernel(const __grid_constant__ AppendArgs a, int vec) {
+    using T = typename Elem<DT>::T;
+    constexpr int kAppThreads = kAppThreadsOf<D, P>;
     constexpr int CH = D / 8;                           // vectors of a row
-    constexpr int NV = P * CH / kAppThreads;
+    constexpr int NV = P * CH / kAppThreads;            // vectors of a thread
     static_assert(NV >= 1 && NV * kAppThreads == P * CH, "a block's vectors divide among the threads");
     const int h = blockIdx.x % a.H, side = blockIdx.x / a.H;
     const int64_t b = blockIdx.z;
@@ -96,30 +120,32 @@ __global__ void __launch_bounds__(kAppThreads) kv_append_kernel(AppendArgs a, in
     }
     const int64_t blk = start / P + blockIdx.y, base = blk * P;
     if (cnt == 0 || base >= len) return;
+    const int lo = (int)(start > base ? start - base : 0);                // first new slot; older ones before it
+    const int hi = (int)(len - base < P ? len - base : P);
+    const T* x = static_cast<const T*>(a.x[side]) + b * a.sb[side] + (int64_t)h * a.sh[side];
+    // the values are on their way before the page is known
+    Raw<DT> raw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int idx = threadIdx.x + i * kAppThreads, slot = idx / CH, c = idx % CH;
+        if (slot >= lo && slot < hi) raw[i].load(x + (base + slot - start) * a.st[side] + c * 8, vec);
+    }
     const int64_t page = a.table[b * a.table_sb + blk];
     if (page < 0 || page >= a.n_pages) {
         if (threadIdx.x == 0) atomicOr(a.err, ERRF_BAD_ARG);
         return;
     }
-    const int lo = (int)(start > base ? start - base : 0);                // first new slot; older ones before it
-    const int hi = (int)(len - base < P ? len - base : P);
     uint8_t* codes = a.codes[side] + (page * a.H + h) * (int64_t)(P * D);
     float* sp = a.scale[side] + page * a.H + h;
-    const T* x = static_cast<const T*>(a.x[side]) + b * a.sb[side] + (int64_t)h * a.sh[side];
     const float s_old = lo > 0 ? *sp : 0.f;
 
-    float v[NV][8];
     float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int idx = threadIdx.x + i * kAppThreads, slot = idx / CH, c = idx % CH;
+        const int slot = (threadIdx.x + i * kAppThreads) / CH;
         if (slot >= lo && slot < hi) {
-            load8<DT>(x + (base + slot - start) * a.st[side] + c * 8, vec, v[i]);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float m = fabsf(v[i][k]);
-                if (m <= 3.402823466e38f) amax = fmaxf(amax, m);           // finite values only
-            }
+            const float m = raw[i].amax();
+            amax = fmaxf(amax, m <= 3.402823466e38f ? m : raw[i].amax_finite());
         }
     }
     __shared__ float red[kAppThreads / 32];
@@ -131,27 +157,34 @@ __global__ void __launch_bounds__(kAppThreads) kv_append_kernel(AppendArgs a, in
     for (int w = 0; w < kAppThreads / 32; ++w) amax = fmaxf(amax, red[w]);
     const float s_blk = exp2i(block_exponent(amax));
     const float s = fmaxf(s_blk, s_old);
-    // 1/s exactly: an exponent flip (a scale given by hand may be any value, so divide then)
-    const float inv = 1.f / s;
-    const float ratio = s_old * inv;
-    const bool grown = lo > 0 && s > s_old;
+    const float inv = 1.f / s;                          // exact: scales are powers of two
+    uint2* dst = reinterpret_cast<uint2*>(codes) + threadIdx.x;
+    auto encode = [&](int i) {
+        uint2 w;
+        w.x = e4m3x4(raw[i].at(0) * inv, raw[i].at(1) * inv, raw[i].at(2) * inv, raw[i].at(3) * inv);
+        w.y = e4m3x4(raw[i].at(4) * inv, raw[i].at(5) * inv, raw[i].at(6) * inv, raw[i].at(7) * inv);
+        dst[i * kAppThreads] = w;
+    };
+    if (lo == 0 && hi == P) {                           // all pages of a prompt but its first and last
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int idx = threadIdx.x + i * kAppThreads, slot = idx / CH;
-        uint2* dst = reinterpret_cast<uint2*>(codes) + idx;
-        if (slot >= lo && slot < hi) {
-            uint2 w;
-            w.x = e4m3x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-            w.y = e4m3x4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
-            *dst = w;
-        } else if (grown && slot < lo) {
-            uint2 w = *dst;
-            float f[4];
-            from_e4m3x4(w.x, f);
-            w.x = e4m3x4(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
-            from_e4m3x4(w.y, f);
-            w.y = e4m3x4(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
-            *dst = w;
+        for (int i = 0; i < NV; ++i) encode(i);
+    } else {
+        const float ratio = s_old * inv;
+        const bool grown = lo > 0 && s > s_old;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int slot = (threadIdx.x + i * kAppThreads) / CH;
+            if (slot >= lo && slot < hi) {
+                encode(i);
+            } else if (grown && slot < lo) {
+                uint2 w = dst[i * kAppThreads];
+                float f[4];
+                from_e4m3x4(w.x, f);
+                w.x = e4m3x4(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+                from_e4m3x4(w.y, f);
+                w.y = e4m3x4(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+                dst[i * kAppThreads] = w;
+            }
         }
     }
     if (threadIdx.x == 0) *sp = s;
@@ -162,7 +195,7 @@ int launch_append(const AppendArgs& a, int64_t B, int vec, cudaStream_t stream) 
     const int64_t blocks = (a.T + P - 2) / P + 1;      // pages that T tokens can touch
     if (blocks > 65535) return fail(NT_ERR_ARG, "nt_kv_append: %lld tokens in one call", (long long)a.T);
     const dim3 grid((unsigned)(2 * a.H), (unsigned)blocks, (unsigned)B);
-    kv_append_kernel<DT, D, P><<<grid, kAppThreads, 0, stream>>>(a, vec);
+    kv_append_kernel<DT, D, P><<<grid, kAppThreadsOf<D, P>, 0, stream>>>(a, vec);
     return check_launch("kv_append_kernel");
 }
 
