@@ -13,6 +13,8 @@ from .core.model import NeuraTensorModel, ModelConfig, SlidingWindowAttention, R
 from .core.snn import LIFLayer, AdaptiveLIFLayer
 from .core.ssm import SelectiveSSMLayer, SSMLayer
 from .core.fused import FusedSpikeBlock, FusedSNNSSMBlock, BlockState
+from .core.cache import AttentionCache
+from .core.rotary import rotary_frequencies
 from .config.presets import get_preset, list_presets, PRESETS
 from .inference.engine import InferenceEngine, InferenceResult
 from .backends.detect import detect_backend
@@ -21,5 +23,5 @@ NeuraTensor = NeuraTensorModel
 
 __all__ = ["NeuraTensor", "NeuraTensorModel", "ModelConfig", "LIFLayer", "AdaptiveLIFLayer", "SelectiveSSMLayer",
            "SSMLayer", "FusedSpikeBlock", "FusedSNNSSMBlock", "BlockState", "SlidingWindowAttention",
-           "RotaryEmbedding", "get_preset", "list_presets", "PRESETS", "InferenceEngine", "InferenceResult",
+           "RotaryEmbedding", "AttentionCache", "rotary_frequencies", "get_preset", "list_presets", "PRESETS", "InferenceEngine", "InferenceResult",
            "detect_backend", "__version__"]

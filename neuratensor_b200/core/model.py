@@ -13,17 +13,23 @@ The spike blocks, the embedding gather, the sliding-window attention layers
 tied lm_head (bf16 logits on the tcgen05 GEMM) run on the native kernels.
 The forward collects every block's spike count in one device buffer and
 reads it once, instead of the reference's three host syncs per block.
+
+Beyond the reference, the attention layers can keep an 8-bit cache between
+calls (``core/cache.py``; the reference's are stateless), and ``generate``
+takes frequency and presence penalties, biases and masks beside the
+repetition penalty, all on the device (``native.logits_process``).
 """
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Tuple
+from typing import Callable, Dict, List, Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
 
+from .cache import AttentionCache
 from .fused import BlockState, FusedSpikeBlock, rate_like_reference
 
 
@@ -137,6 +143,44 @@ class SlidingWindowAttention(nn.Module):
         return native.attention_forward(x, self.norm.weight, self.qkv.weight, self.o_proj.weight, self.n_heads,
                                         self.window, cos, sin, workspace=workspace)
 
+    def forward_cached(self, x: Tensor, cache: AttentionCache, layer: str) -> Tensor:
+        """The layer with a memory: x [B, T, d_model], the last T of cache.lengths tokens.
+
+        The first call of a sequence is the plain layer (its keys are all in x) and
+        leaves its window in the cache; later calls attend over the cache."""
+        from .. import native
+        B, T, dm = x.shape
+        H, hd = self.n_heads, self.head_dim
+        freq = getattr(self, "_rope_freq", None)
+        src = self.rope.inv_freq
+        if freq is None or freq[0] != (src.data_ptr(), src._version, x.device):
+            freq = self._rope_freq = ((src.data_ptr(), src._version, x.device), src.to(x.device, torch.float32))
+        freq = freq[1]
+        before = cache.filled - T                       # tokens of the sequences ahead of x
+
+        def heads(a: int, b: int) -> Tensor:            # q | k | v heads [B, b - a, 3H, hd] of tokens a..b-1 of x
+            qkv = native.lm_head(x[:, a:b], self.norm.weight, self.qkv.weight)      # RMSNorm and one projection
+            return qkv.view(B, b - a, 3 * H, hd)
+
+        if before == 0:
+            # the window of the tokens to come, from a page's first slot on
+            a = max(0, T - self.window) // cache.page * cache.page
+            qkv = heads(a, T)
+            k = native.rotary(qkv[:, :, H:2 * H], torch.arange(a, T, device=x.device), freq)
+            cache.append(layer, k, qkv[:, :, 2 * H:], cache.lengths)
+            return self.forward(x)
+        out = []
+        for a in range(0, T, cache.max_step):
+            b = min(T, a + cache.max_step)
+            qkv = heads(a, b)
+            lengths = cache.lengths - (T - b) if b < T else cache.lengths
+            pos = lengths[:, None] + torch.arange(a - b, 0, device=x.device)
+            native.rotary(qkv[:, :, :2 * H], pos, freq, out=qkv[:, :, :2 * H])
+            cache.append(layer, qkv[:, :, H:2 * H], qkv[:, :, 2 * H:], lengths)
+            out.append(cache.attend(layer, qkv[:, :, :H], lengths).view(B, b - a, dm))
+        o = out[0] if len(out) == 1 else torch.cat(out, dim=1)
+        return F.linear(o, self.o_proj.weight.to(x.dtype)) + x
+
     def forward_torch(self, x: Tensor) -> Tensor:
         """The reference's op sequence (fp32, CPU tensors, head dims other than 64 and 128)."""
         B, T, _ = x.shape
@@ -215,11 +259,13 @@ class NeuraTensorModel(nn.Module):
         return max(1, self.MAX_ACTIVATION_ELEMS // (max(seq, 1) * width))
 
     def forward_device(self, input_ids: Tensor, states: Optional[List[Optional[BlockState]]] = None,
-                       workspace: Optional[Tensor] = None, last_only: bool = False):
+                       workspace: Optional[Tensor] = None, last_only: bool = False,
+                       attn_cache: Optional[AttentionCache] = None):
         """Forward without any host sync: returns (logits, states, per-layer spike counts on device).
 
         ``last_only``: logits of the last position only ([B, 1, vocab]), as a
-        generation prefill needs them."""
+        generation prefill needs them.  ``attn_cache``: the attention layers see
+        the tokens of earlier calls with it, and it moves on by this call's."""
         if states is None:
             states = [None] * len(self.blocks)
         if input_ids.shape[1] > self.config.max_seq_len:
@@ -228,14 +274,19 @@ class NeuraTensorModel(nn.Module):
                           f"{self.config.max_seq_len}; truncating.", UserWarning, stacklevel=3)
             input_ids = input_ids[:, : self.config.max_seq_len]
         B, T = input_ids.shape
+        if attn_cache is not None:
+            if attn_cache.batch != B:
+                raise ValueError(f"the attention cache is for {attn_cache.batch} sequences, got {B}")
+            attn_cache.advance(T)
         g = self.group_size(T)
         if B <= g:
-            return self._forward_rows(input_ids, states, workspace, last_only)
+            return self._forward_rows(input_ids, states, workspace, last_only, attn_cache)
         parts = []
         for a in range(0, B, g):
             sub = [None if s is None else BlockState(membrane=s.membrane[a:a + g], ssm_state=s.ssm_state[a:a + g])
                    for s in states]
-            parts.append(self._forward_rows(input_ids[a:a + g], sub, workspace, last_only))
+            part = None if attn_cache is None else attn_cache.rows(a, min(a + g, B))
+            parts.append(self._forward_rows(input_ids[a:a + g], sub, workspace, last_only, part))
         logits = torch.cat([p[0] for p in parts])
         state_cls = self.blocks[0]._state_cls
         new_states = [state_cls(membrane=torch.cat([p[1][i].membrane for p in parts]),
@@ -245,7 +296,7 @@ class NeuraTensorModel(nn.Module):
         return logits, new_states, counts
 
     def _forward_rows(self, input_ids: Tensor, states: List[Optional[BlockState]], workspace: Optional[Tensor],
-                      last_only: bool):
+                      last_only: bool, attn_cache: Optional[AttentionCache] = None):
         from .. import native
         x = native.embedding(input_ids, self.embedding.weight)
         counts = torch.zeros(len(self.blocks), dtype=torch.int64, device=x.device)
@@ -257,7 +308,8 @@ class NeuraTensorModel(nn.Module):
                 new_states.append(ns)
                 key = str(i)
                 if key in self.attn_layers:
-                    x = self.attn_layers[key](x)
+                    attn = self.attn_layers[key]
+                    x = attn(x) if attn_cache is None else attn.forward_cached(x, attn_cache, key)
             if last_only:
                 x = x[:, -1:]
             # final RMSNorm + tied lm_head on the tcgen05 GEMM; the block
@@ -286,60 +338,98 @@ class NeuraTensorModel(nn.Module):
         return sum(p.numel() for p in self.parameters() if p.requires_grad)
 
     @torch.no_grad()
-    def step_graph(self, batch: int, seq: int, device, dtype):
-        """The captured forward for this (batch, length) (``inference/decode.py``).
+    def step_graph(self, batch: int, seq: int, device, dtype, cache_tokens: int = 0):
+        """The captured forward for this (batch, length) (``inference/decode.py``);
+        with ``cache_tokens`` the graph has an attention cache of its own for that many
+        tokens a sequence (``graph.attn_cache``).
         A graph holds raw addresses, so it is rebuilt when a parameter changes
         (version or storage) or an attention layer's RoPE tables were rebuilt;
         the four most recently used shapes are kept."""
         from ..inference.decode import StepGraph
         sig = (tuple((p.data_ptr(), p._version) for p in self.parameters()),
                tuple((a.rope.cos_cached.data_ptr(), a.rope.sin_cached.data_ptr()) for a in self.attn_layers.values()))
-        key = (batch, seq, str(device), dtype)
+        key = (batch, seq, str(device), dtype, cache_tokens)
         cache = self.__dict__.setdefault("_step_graphs", {})
         hit = cache.pop(key, None)
         if hit is None or hit[0] != sig:
             hit = None
             while len(cache) >= 4:
                 cache.pop(next(iter(cache)))
-            hit = (sig, StepGraph(self, batch, seq, torch.device(device), dtype))
+            hit = (sig, StepGraph(self, batch, seq, torch.device(device), dtype, cache_tokens))
         cache[key] = hit                          # most recently used last
         return hit[1]
 
-    def decode_graph(self, batch: int, device, dtype):
+    def decode_graph(self, batch: int, device, dtype, cache_tokens: int = 0):
         """The captured single-token step for this batch size."""
-        return self.step_graph(batch, 1, device, dtype)
+        return self.step_graph(batch, 1, device, dtype, cache_tokens)
 
     def generate(self, input_ids: Tensor, max_new_tokens: int = 50, temperature: float = 1.0, top_k: int = 50,
                  top_p: float = 1.0, repetition_penalty: float = 1.0, stop_tokens: Optional[List[int]] = None,
                  states: Optional[List[Optional[BlockState]]] = None,
-                 use_graph: bool = True) -> Tuple[Tensor, List[BlockState]]:
+                 use_graph: bool = True, attn_cache: Union[bool, AttentionCache] = False,
+                 frequency_penalty: float = 0.0, presence_penalty: float = 0.0,
+                 logit_bias: Optional[Dict[int, float]] = None,
+                 allowed: Union[None, Tensor, Callable[[Tensor], Optional[Tensor]]] = None
+                 ) -> Tuple[Tensor, List[BlockState]]:
         """Autoregressive sampling with carried block state (model.py:301-370).
 
         On CUDA the per-token steps replay one captured graph of the whole model
         (``inference/decode.py``); ``use_graph=False`` runs them one launch at a
-        time.  Both run the same kernels on the same inputs."""
+        time.  Both run the same kernels on the same inputs.
+
+        Beyond the reference: ``attn_cache`` lets the attention layers see their window
+        of earlier tokens instead of the new one alone (True: for this call; an
+        ``AttentionCache`` carries on and is left behind the last token that was run);
+        ``frequency_penalty`` and ``presence_penalty`` are taken off per occurrence of a
+        generated token and for any; ``logit_bias`` maps token ids to what is added;
+        ``allowed`` is a mask of the tokens that may come next, boolean [B or 1, vocab] or
+        the int32 words of ``native.pack_allowed``, or a function of the tokens so far
+        that returns one (or None)."""
+        from .. import native
         self.eval()
         out = input_ids
+        B, prompt = out.shape
         stop = set(stop_tokens or [])
-        logits, states, _ = self.forward_device(out, states, last_only=True)
+        want_graph = use_graph and out.is_cuda and max_new_tokens > 1
+        graph = cache = None
+        if isinstance(attn_cache, AttentionCache):
+            cache, want_graph = attn_cache, False       # a graph has its own
+        elif attn_cache:
+            tokens = min(prompt, self.config.max_seq_len) + max_new_tokens
+            if want_graph:
+                tokens = -(-tokens // 1024) * 1024      # so that calls of other lengths find the same graph
+                graph = self.decode_graph(B, out.device, self.lm_head.weight.dtype, tokens)
+                cache = graph.attn_cache
+                cache.reset()
+            else:
+                cache = AttentionCache(self.config, B, tokens, out.device)
+        logits, states, _ = self.forward_device(out, states, last_only=True, attn_cache=cache)
         nxt_logits = logits[:, -1, :]
-        graph = None
-        if use_graph and out.is_cuda and max_new_tokens > 1:
-            graph = self.decode_graph(out.shape[0], out.device, logits.dtype)
+        if want_graph:
+            graph = graph or self.decode_graph(B, out.device, logits.dtype)
             graph.load_states(states)
+        made = torch.full((B,), prompt, dtype=torch.int32, device=out.device) if frequency_penalty or presence_penalty else None
+        bias_ids = bias = None
+        if logit_bias:
+            bias_ids = torch.tensor([list(logit_bias)], dtype=torch.int64, device=out.device).expand(B, -1)
+            bias = torch.tensor([list(logit_bias.values())], dtype=torch.float32, device=out.device).expand(B, -1)
+        words = lambda m: native.pack_allowed(m) if m is not None and m.dtype == torch.bool else m  # noqa: E731
+        fixed = None if callable(allowed) else words(allowed)
         # top_k = 1 without nucleus filtering leaves the tied row maxima with
         # equal probability: one kernel picks among them with a uniform drawn
         # here for every step at once (the other filters run as written)
         greedy = out.is_cuda and top_k == 1 and top_p >= 1.0
         if greedy:
-            from .. import native
             u_all = torch.rand((max_new_tokens, out.shape[0]), device=out.device)
         for step in range(max_new_tokens):
             if repetition_penalty != 1.0:
-                for b in range(out.shape[0]):
-                    for tok in out[b].tolist():
-                        v = nxt_logits[b, tok]
-                        nxt_logits[b, tok] = v / repetition_penalty if v > 0 else v * repetition_penalty
+                # once per occurrence, as the reference's loop over out[b] does
+                native.logits_process(nxt_logits, tokens=out, repetition=repetition_penalty, each=True, out=nxt_logits)
+            mask = words(allowed(out)) if callable(allowed) else fixed
+            if made is not None or bias is not None or mask is not None:
+                native.logits_process(nxt_logits, tokens=out if made is not None else None, prompt_lengths=made,
+                                      frequency=frequency_penalty, presence=presence_penalty, bias_ids=bias_ids, bias=bias,
+                                      allowed=mask, out=nxt_logits)
             if temperature != 1.0:
                 nxt_logits = nxt_logits / temperature
             if greedy:
@@ -361,7 +451,7 @@ class NeuraTensorModel(nn.Module):
             if graph is not None:
                 nxt_logits = graph.step(tok).clone()
             else:
-                logits, states, _ = self.forward_device(tok, states)
+                logits, states, _ = self.forward_device(tok, states, attn_cache=cache)
                 nxt_logits = logits[:, -1, :]
         if graph is not None:
             states = graph.states()

@@ -11,7 +11,9 @@ a (batch, length) shape:
   buffers stand for "no state", which the kernels treat as zeros);
 * the captured region runs the forward on them and copies the new states back
   into the static state buffers, so replay k+1 continues from replay k;
-* static outputs: the logits [B, T, vocab] and the per-layer spike counts.
+* static outputs: the logits [B, T, vocab] and the per-layer spike counts;
+* with an attention cache (``cache_tokens``): the graph's own, whose lengths the
+  captured region moves on; ``generate`` fills it from the prompt.
 
 The graph holds raw device addresses: it owns its workspace, and the model
 rebuilds it when a parameter changes or a RoPE table is rebuilt
@@ -24,13 +26,15 @@ from typing import List, Optional
 import torch
 from torch import Tensor
 
+from ..core.cache import AttentionCache
 from ..core.fused import BlockState
 
 
 class StepGraph:
     """A captured forward for one (batch, length), device and dtype."""
 
-    def __init__(self, model, batch: int, seq: int, device: torch.device, dtype: torch.dtype) -> None:
+    def __init__(self, model, batch: int, seq: int, device: torch.device, dtype: torch.dtype,
+                 cache_tokens: int = 0) -> None:
         from .. import native
         cfg = model.config
         di = cfg.d_model * cfg.expand
@@ -47,6 +51,7 @@ class StepGraph:
         self.mem, self.st = self._split(self.flat)
         nbytes = native.block_workspace_bytes(dtype, batch, seq, cfg.d_model, di, cfg.d_state)
         self.ws = torch.empty(nbytes, dtype=torch.uint8, device=device)   # owned: the graph keeps its address
+        self.attn_cache = AttentionCache(cfg, batch, cache_tokens, device, max_step=max(seq, 1)) if cache_tokens else None
         self.logits: Optional[Tensor] = None
         self.counts: Optional[Tensor] = None
         self.graph = torch.cuda.CUDAGraph()
@@ -56,7 +61,8 @@ class StepGraph:
         return [BlockState(membrane=m, ssm_state=s) for m, s in zip(self.mem, self.st)]
 
     def _forward(self):
-        logits, new_states, counts = self.model.forward_device(self.tok, self._states(), workspace=self.ws)
+        logits, new_states, counts = self.model.forward_device(self.tok, self._states(), workspace=self.ws,
+                                                               attn_cache=self.attn_cache)
         for i, ns in enumerate(new_states):
             self.mem[i].copy_(ns.membrane)
             self.st[i].copy_(ns.ssm_state)
@@ -64,6 +70,10 @@ class StepGraph:
 
     def _capture(self) -> None:
         dev = self.tok.device
+        seq = self.tok.shape[1]
+        if self.attn_cache is not None:
+            # a step: tokens are ahead of it (zeros here, which reset() forgets)
+            self.attn_cache.advance(seq)
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(side), torch.no_grad():
@@ -74,6 +84,8 @@ class StepGraph:
         torch.cuda.current_stream(dev).wait_stream(side)
         with torch.no_grad(), torch.cuda.graph(self.graph):
             self.logits, self.counts = self._forward()
+        if self.attn_cache is not None:
+            self.attn_cache.reset()
 
     def load_states(self, states: Optional[List[Optional[BlockState]]]) -> None:
         """Start the next replay from `states` (None, or None entries: zero state)."""
@@ -91,6 +103,8 @@ class StepGraph:
 
     def replay(self, tok: Tensor) -> Tensor:
         """Run the captured forward on token ids `tok` [B, T]; returns the static logits."""
+        if self.attn_cache is not None:
+            self.attn_cache.move(self.tok.shape[1])
         self.tok.copy_(tok, non_blocking=True)
         self.graph.replay()
         return self.logits

@@ -148,15 +148,18 @@ class InferenceEngine:
     @torch.no_grad()
     def generate(self, input_ids: Tensor, max_new_tokens: int = 64, temperature: float = 1.0, top_k: int = 50,
                  top_p: float = 1.0, repetition_penalty: float = 1.0, stop_tokens: Optional[List[int]] = None,
-                 reset_state: bool = True) -> Tensor:
-        """Returns [B, T + generated] token ids (engine.py:180-208)."""
+                 reset_state: bool = True, **more) -> Tensor:
+        """Returns [B, T + generated] token ids (engine.py:180-208).
+
+        ``more``: the model's own arguments beyond the reference (``attn_cache``,
+        ``frequency_penalty``, ``presence_penalty``, ``logit_bias``, ``allowed``)."""
         if reset_state:
             self.reset_state()
         ids = input_ids.to(self.device)
         with torch.autocast(device_type="cuda", dtype=self.dtype, enabled=self.dtype != torch.float32):
             out, states = self.model.generate(ids, max_new_tokens=max_new_tokens, temperature=temperature,
                                               top_k=top_k, top_p=top_p, repetition_penalty=repetition_penalty,
-                                              stop_tokens=stop_tokens, states=self._states)
+                                              stop_tokens=stop_tokens, states=self._states, **more)
         self._states = states
         return out
 
