@@ -72,7 +72,7 @@ __device__ __forceinline__ float process(float x, uint32_t w, uint32_t j, float 
 }
 
 template <int DT, bool WIDE, bool EACH>
-__global__ void __launch_bounds__(kLogThreads) logits_kernel(const __grid_constant__ LogArgs a) {
+__global__ void __launch_bounds__(kLogThreads, 6) logits_kernel(const __grid_constant__ LogArgs a) {
     using El = Elem<DT>;
     using T = typename El::T;
     using K = Count<WIDE>;
@@ -98,6 +98,28 @@ __global__ void __launch_bounds__(kLogThreads) logits_kernel(const __grid_consta
     len = len < 0 ? 0 : (len > a.L ? a.L : len);
     const bool counted = len > 0 || a.NB > 0;
 
+    const bool touched_only = static_cast<const void*>(x) == static_cast<const void*>(y) && !mask;
+    const int head = head_x == head_y ? (head_x < n ? head_x : n) : n;      // all singly when no boundary is shared
+    const int nv = touched_only ? 0 : (n - head) / E;
+    // vectors of a thread in flight, with their mask bits (loading the first ones before
+    // the history is counted cost registers, and so CTAs per SM: 84 us against 70)
+    constexpr int U = 4;
+    uint4 q[U];
+    uint32_t bits[U];
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * kLogThreads;
+            bits[u] = ~0u;
+            if (i >= nv) continue;
+            q[u] = __ldcs(reinterpret_cast<const uint4*>(x + head) + i);
+            if (mask) {
+                const uint32_t at = (uint32_t)lo + head + i * E, sh = at & 31;
+                bits[u] = __ldg(mask + (at >> 5)) >> sh;
+                if (sh + E > 32) bits[u] |= __ldg(mask + (at >> 5) + 1) << (32 - sh);
+            }
+        }
+    };
     if (counted) {
         for (int i = threadIdx.x; i < stride * K::kWords / 4; i += kLogThreads)
             reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
@@ -140,20 +162,14 @@ __global__ void __launch_bounds__(kLogThreads) logits_kernel(const __grid_consta
         const bool ok = !mask || ((mask[(lo + i) >> 5] >> ((lo + i) & 31)) & 1u);
         y[i] = El::from_f(ok ? v : -INFINITY);
     };
-    if (static_cast<const void*>(x) == static_cast<const void*>(y) && !mask) {
+    if (touched_only) {
         if (counted)
             for (int i = threadIdx.x; i < n; i += kLogThreads)
                 if (words[i] || (WIDE && words[stride + i])) one(i);
         return;
     }
-    const int head = head_x == head_y ? (head_x < n ? head_x : n) : n;      // all singly when no boundary is shared
-    const int nv = (n - head) / E;
-    constexpr int U = 4;                                // vectors of a thread in flight
     for (int i0 = threadIdx.x; i0 < nv; i0 += U * kLogThreads) {
-        uint4 q[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i0 + u * kLogThreads < nv) q[u] = __ldcs(reinterpret_cast<const uint4*>(x + head) + i0 + u * kLogThreads);
+        load(i0);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * kLogThreads, first = head + i * E;
@@ -179,16 +195,9 @@ __global__ void __launch_bounds__(kLogThreads) logits_kernel(const __grid_consta
                     xv[e] = El::from_f(process<DT, WIDE, EACH>(El::to_f(xv[e]), w[e], WIDE ? words[stride + first + e] : 0u,
                                                                r, r_inv, fq, ps, bias));
             }
-            if (mask) {
-                const int64_t at = lo + first;
-                uint32_t bits = mask[at >> 5];
-                const int sh = (int)(at & 31);
-                if (sh + E > 32) bits = __funnelshift_r(bits, mask[(at >> 5) + 1], sh);
-                else bits >>= sh;
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (!((bits >> e) & 1u)) xv[e] = El::from_f(-INFINITY);
-            }
+            for (int e = 0; e < E; ++e)
+                if (!((bits[u] >> e) & 1u)) xv[e] = El::from_f(-INFINITY);
             __stcs(reinterpret_cast<uint4*>(y + head) + i, *reinterpret_cast<const uint4*>(xv));
         }
     }
