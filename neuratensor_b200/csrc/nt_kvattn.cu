@@ -23,8 +23,7 @@
 //
 // Softmax is online, in float32, base 2: a warp keeps its rows' running
 // maximum, sum and output over its tiles; the warps of a CTA join in shared
-// memory, and the CTAs of a long sequence (`chunk` tiles each) in a second
-// kernel, in a fixed order.  Probabilities are held as 2^14 p in f16 (11 bits;
+// memory, and the CTAs that share a head in a second kernel, in a fixed order.  Probabilities are held as 2^14 p in f16 (11 bits;
 // small ones reach down to 2^-38 of the largest) for bf16 outputs, whose own
 // rounding is 2^-9, and as an f16 pair for float32.
 #include "nt_kernels.cuh"
@@ -53,7 +52,7 @@ struct KvAttnArgs {
     const int32_t* table; int64_t table_sb;
     const int32_t* lengths; const int32_t* counts;
     void* out;
-    float* part;                       // [B, H * row_tiles, splits] x ([kRows][D] sums, [kRows] maxima, [kRows] totals)
+    float* part;                       // partial rows: [kRows][D] sums, [kRows] maxima, [kRows] totals
     unsigned* err;
 };
 
@@ -127,22 +126,18 @@ template <int D> __device__ __forceinline__ int v_swz(int row) { return D == 128
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-// W warps per CTA, 16 to an SM (128 registers a thread).
+// Tiles [first, last) of one row tile of head h, sequence b, by the W warps of a
+// CTA: the rows themselves when these are all of its tiles, else unnormalised sums
+// with their maxima and totals in `part`.
 template <int DT, int D, int W>
-__global__ void __launch_bounds__(W * 32, 16 / W) kv_attention_kernel(const __grid_constant__ KvAttnArgs a) {
+__device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, int row_tile, const Span& s, int first,
+                                       int last, float* part, unsigned char* smem) {
     using El = Elem<DT>;
     using T = typename El::T;
     constexpr int KS = D / 16;                 // k-steps of the first product
     constexpr int MT = D / 16;                 // 16-dimension tiles of the second
     constexpr bool kPair = DT == NT_F32;       // a second product with what f16 leaves of q and of the weights
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int split = blockIdx.x, h = blockIdx.y / a.row_tiles, row_tile = blockIdx.y % a.row_tiles;
-    const int64_t b = blockIdx.z;
-    const Span s = span_of(a, b, row_tile);
-    if (s.bad && split == 0 && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(a.err, ERRF_BAD_ARG);
-    const int first = split * a.chunk, last = min(first + a.chunk, s.tiles);
-    if (split > 0 && first >= s.tiles) return;
-
     const int row = row_tile * kRows + g, t = row / a.G;
     const bool live = t < s.cnt;
     // in the products a lane holds rows 2c and 2c + 1: their positions
@@ -221,7 +216,6 @@ __global__ void __launch_bounds__(W * 32, 16 / W) kv_attention_kernel(const __gr
     int f_page = -1, c_page = -1;
     float f_ks = 0.f, f_vs = 0.f, c_ks = 0.f, c_vs = 0.f;
     bool bad_page = false;
-    extern __shared__ __align__(128) unsigned char smem[];
     unsigned char* ring = smem + warp * (kStages * 2 * kTileBytes<D>);
     const uint32_t ring_u32 = smem_u32(ring);
     auto fetch = [&](int i) {
@@ -448,7 +442,6 @@ __global__ void __launch_bounds__(W * 32, 16 / W) kv_attention_kernel(const __gr
         l1 += __shfl_xor_sync(0xffffffffu, l1, k);
     }
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // join the warps
     __syncthreads();                                    // all rings are read: their memory takes the sums
     float (*so)[kRows][D] = reinterpret_cast<float (*)[kRows][D]>(smem);
@@ -468,8 +461,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) kv_attention_kernel(const __gr
     }
     __syncthreads();
     const int rows = min(kRows, a.T * a.G - row_tile * kRows);
-    const int64_t part_at = (b * gridDim.y + blockIdx.y) * a.splits + split;
-    const bool alone = s.tiles <= a.chunk;              // this CTA has seen all keys
+    const bool alone = last - first == s.tiles;         // this CTA has seen all keys
     for (int i = threadIdx.x; i < rows * D; i += (W * 32)) {
         const int r = i / D, d = i % D;
         float mm = -INFINITY;
@@ -489,7 +481,6 @@ __global__ void __launch_bounds__(W * 32, 16 / W) kv_attention_kernel(const __gr
             T* out = static_cast<T*>(a.out) + ((b * a.T + tt) * (int64_t)(a.H * a.G) + h * a.G + rr % a.G) * D + d;
             *out = El::from_f(tt < s.cnt && tot != 0.f ? sum / tot : 0.f);
         } else {
-            float* part = a.part + part_at * (kRows * (D + 2));
             part[i] = sum;
             if (d == 0) {
                 part[kRows * D + r] = mm;
@@ -499,12 +490,86 @@ __global__ void __launch_bounds__(W * 32, 16 / W) kv_attention_kernel(const __gr
     }
 }
 
-// Joins the chunks of one query row: warp w takes chunks w, w + 4, ..., a lane D/32
+// W warps per CTA, 16 to an SM (128 registers a thread).  A CTA takes `chunk`
+// tiles of one row tile.
+template <int DT, int D, int W>
+__global__ void __launch_bounds__(W * 32, 16 / W) kv_attention_kernel(const __grid_constant__ KvAttnArgs a) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int split = blockIdx.x, h = blockIdx.y / a.row_tiles, row_tile = blockIdx.y % a.row_tiles;
+    const int64_t b = blockIdx.z;
+    const Span s = span_of(a, b, row_tile);
+    if (s.bad && split == 0 && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(a.err, ERRF_BAD_ARG);
+    const int first = split * a.chunk, last = min(first + a.chunk, s.tiles);
+    if (split > 0 && first >= s.tiles) return;
+    float* part = a.part + ((b * gridDim.y + blockIdx.y) * a.splits + split) * (kRows * (D + 2));
+    attend<DT, D, W>(a, b, h, row_tile, s, first, last, part, smem);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Ragged sequences, in even shares: all tiles of all heads and sequences in a row
+// (sequence by sequence, head by head) are cut into gridDim.x shares of `share`
+// tiles, so every CTA works equally long whatever the lengths.  A CTA leaves at
+// most two partial rows: of the head its share begins in (slot 0) and of the one it
+// ends in (slot 1).  One row tile per head; up to kEvenBatch sequences.
+constexpr int kEvenBatch = 512;
+constexpr int kEvenLeast = 8;          // tiles of a share at least
+
+// before[i] = tiles per head of the sequences before i, for i <= B; all threads of the CTA take part.
+__device__ __forceinline__ void tiles_before(const KvAttnArgs& a, int B, int* before, bool flag) {
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x < 32) {
+        int sum = 0;
+        for (int i0 = 0; i0 < B; i0 += 32) {
+            int n = 0;
+            if (i0 + lane < B) {
+                const Span s = span_of(a, i0 + lane, 0);
+                n = s.tiles;
+                if (s.bad && flag) atomicOr(a.err, ERRF_BAD_ARG);
+            }
+#pragma unroll
+            for (int k = 1; k < 32; k *= 2) {
+                const int up = __shfl_up_sync(0xffffffffu, n, k);
+                if (lane >= k) n += up;
+            }
+            if (i0 + lane < B) before[i0 + lane + 1] = sum + n;
+            sum += __shfl_sync(0xffffffffu, n, 31);
+        }
+        if (lane == 0) before[0] = 0;
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ int64_t share_of(int64_t total, int ctas) {
+    const int64_t n = (total + ctas - 1) / ctas;
+    return n > kEvenLeast ? n : kEvenLeast;
+}
+
+template <int DT, int D, int W>
+__global__ void __launch_bounds__(W * 32, 16 / W) kv_attention_even_kernel(const __grid_constant__ KvAttnArgs a, int B) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int before[kEvenBatch + 1];
+    tiles_before(a, B, before, blockIdx.x == 0);
+    const int64_t total = (int64_t)before[B] * a.H, share = share_of(total, gridDim.x);
+    const int64_t begin = blockIdx.x * share, end = begin + share < total ? begin + share : total;
+    int b = 0;
+    for (int64_t at = begin; at < end;) {
+        while ((int64_t)before[b + 1] * a.H <= at) ++b;
+        const Span s = span_of(a, b, 0);
+        const int64_t rel = at - (int64_t)before[b] * a.H;
+        const int h = (int)(rel / s.tiles), first = (int)(rel - (int64_t)h * s.tiles);
+        const int last = (int)(end - at < s.tiles - first ? first + (end - at) : s.tiles);
+        attend<DT, D, W>(a, b, h, 0, s, first, last, a.part + (2 * (int64_t)blockIdx.x + (at != begin)) * (kRows * (D + 2)), smem);
+        at += last - first;
+        __syncthreads();                                // the sums are read before the next ring is filled
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Joins the chunks of one query row: warp w takes chunks w, w + 8, ..., a lane D/32
 // dimensions, so the order of the sums is fixed.  Launched as a programmatic
 // dependent of the main kernel: its own launch is over when the last chunk is written.
-constexpr int kJoinWarps = 4;
-template <int DT, int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) kv_attention_join_kernel(const __grid_constant__ KvAttnArgs a) {
+constexpr int kJoinWarps = 8;
+template <int DT, int D, bool EVEN>
+__global__ void __launch_bounds__(kJoinWarps * 32) kv_attention_join_kernel(const __grid_constant__ KvAttnArgs a, int B, int ctas) {
     using El = Elem<DT>;
     using T = typename El::T;
     constexpr int E = D / 32;
@@ -512,26 +577,49 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv_attention_join_kernel(cons
     const int64_t b = blockIdx.z;
     const int row = t * a.G + hq % a.G, row_tile = row / kRows, r = row % kRows, y = h * a.row_tiles + row_tile;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Span s = span_of(a, b, row_tile);
-    const int n = (s.tiles + a.chunk - 1) / a.chunk;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (n <= 1) return;                                 // its CTA wrote the row
     constexpr int kPart = kRows * (D + 2);
-    const float* part = a.part + (b * (int64_t)(a.H * a.row_tiles) + y) * a.splits * kPart;
-    const float* ms = part + kRows * D + r;             // chunk maxima, kPart apart; the totals kRows behind them
+    const Span s = span_of(a, b, row_tile);
+    int n;                                              // partial rows, kPart apart
+    const float* part;
+    if constexpr (EVEN) {
+        __shared__ int before[kEvenBatch + 1];
+        tiles_before(a, B, before, false);
+        const int64_t share = share_of((int64_t)before[B] * a.H, ctas);
+        const int64_t g0 = (int64_t)before[b] * a.H + (int64_t)h * s.tiles, c0 = g0 / share;
+        n = s.tiles ? (int)((g0 + s.tiles - 1) / share - c0 + 1) : 0;
+        // the head begins in CTA c0, in its slot 1 unless the share begins with it, and goes on in slots 0
+        part = a.part + 2 * c0 * kPart;
+        if (g0 != c0 * share) part += kPart;
+    } else {
+        n = (s.tiles + a.chunk - 1) / a.chunk;
+        part = a.part + (b * (int64_t)(a.H * a.row_tiles) + y) * a.splits * kPart;
+    }
+    // where partial row i is: two slots a CTA when EVEN, the first possibly the second slot
+    const int64_t step = EVEN ? 2 * kPart : kPart;
+    const int64_t back = EVEN && n > 1 && ((part - a.part) / kPart & 1) ? kPart : 0;
+    auto at = [&](int i) { return part + i * step - (i ? back : 0); };
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (n == 1) return;                                 // its CTA wrote the row
+    if (n == 0) {                                       // a CTA wrote it, or in even shares none
+        if (EVEN)
+            for (int d = threadIdx.x; d < D; d += kJoinWarps * 32)
+                static_cast<T*>(a.out)[((b * a.T + t) * (int64_t)heads + hq) * D + d] = El::from_f(0.f);
+        return;
+    }
+    const int mr = kRows * D + r;                       // a partial row's maximum; its total kRows behind
     float m = -INFINITY;
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, ms[(int64_t)i * kPart]);
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, at(i)[mr]);
 #pragma unroll
     for (int k = 16; k; k /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
     const float base = m == -INFINITY ? 0.f : m;
     float sum[E], tot = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = warp; i < n; i += kJoinWarps) {
-        const float* pi = part + (int64_t)i * kPart;
-        const float f = ex2(pi[kRows * D + r] - base);
-        tot = fmaf(f, pi[kRows * D + kRows + r], tot);
+        const float* pi = at(i);
+        const float f = ex2(pi[mr] - base);
+        tot = fmaf(f, pi[mr + kRows], tot);
         float v[E];
         if constexpr (E == 4) {
             const float4 q = *reinterpret_cast<const float4*>(pi + r * D + lane * E);
@@ -560,9 +648,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv_attention_join_kernel(cons
 }
 
 // Warps per CTA, tiles per CTA and CTAs per row tile, from sizes the host knows (not the lengths).
-struct Plan { int row_tiles, warps, chunk, splits; int64_t part_bytes; };
+struct Plan { int row_tiles, warps, chunk, splits, even; int64_t part_bytes; };
 Plan plan_of(int64_t B, int64_t T, int64_t G, int64_t H, int64_t D, int64_t page, int64_t n_blocks, int64_t window) {
-    Plan pl;
+    Plan pl{};
     pl.row_tiles = (int)((T * G + kRows - 1) / kRows);
     int64_t span = n_blocks * page;
     if (window >= 0) span = std::min(span, window + std::min<int64_t>(T, kRows) + kTile);
@@ -573,11 +661,19 @@ Plan plan_of(int64_t B, int64_t T, int64_t G, int64_t H, int64_t D, int64_t page
         pl.warps = 8;
         pl.chunk = (int)tiles;
         pl.splits = 1;
+    } else if (window < 0 && pl.row_tiles == 1 && B <= kEvenBatch && base <= 8 * 148) {
+        // lengths that the host does not know: even shares for one wave of eight CTAs per SM, unless
+        // there are more heads than that (us, even shares against chunks or whole heads: 8 ragged
+        // caches of up to 65536 tokens x 8 heads 100 : 105, one of 131072 x 8 63 : 81, 64 of up to
+        // 8192 x 16 214 : 235; but 200 of up to 2000 x 8 124 : 98)
+        pl.warps = 2;
+        pl.even = (int)std::min<int64_t>(8 * 148, (base * tiles + kEvenLeast - 1) / kEvenLeast);
+        pl.part_bytes = 2 * (int64_t)pl.even * kRows * (D + 2) * (int64_t)sizeof(float);
+        return pl;
     } else {
-        // CTAs of two warps: one wave of eight per SM where a window makes the sequences alike;
-        // half as many again, for a table's capacity, where they are ragged
-        // (8 caches of up to 65536 tokens: 8 per SM 130 us, 12 111 us, 24 114 us;
-        // 24 drafts, window 1001: 8 14.5 us, 12 17.4 us)
+        // CTAs of two warps: one wave of eight per SM where a window makes the sequences
+        // alike, half as many again, for a table's capacity, where they are ragged
+        // (24 drafts, window 1001: 8 14.5 us, 12 17.4 us)
         pl.warps = 2;
         const int64_t want = std::max<int64_t>(1, (window >= 0 ? 8 : 12) * 148 / std::max<int64_t>(1, base));
         pl.chunk = (int)std::max<int64_t>(2 * pl.warps, (tiles + want - 1) / want);
@@ -587,17 +683,8 @@ Plan plan_of(int64_t B, int64_t T, int64_t G, int64_t H, int64_t D, int64_t page
     return pl;
 }
 
-template <int DT, int D, int W>
-int launch_kv_attention(const KvAttnArgs& a, int64_t B, cudaStream_t stream) {
-    const dim3 grid((unsigned)a.splits, (unsigned)(a.H * a.row_tiles), (unsigned)B);
-    const size_t smem = std::max(kRingBytes<D, W>, sizeof(float) * W * kRows * (D + 2));
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kv_attention_kernel<DT, D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return fail(NT_ERR_CUDA, "nt_kv_attention: %s", cudaGetErrorString(e));
-    }
-    kv_attention_kernel<DT, D, W><<<grid, W * 32, smem, stream>>>(a);
-    const int rc = check_launch("kv_attention_kernel");
-    if (rc != NT_OK || a.splits == 1) return rc;
+template <int DT, int D, bool EVEN>
+int launch_join(const KvAttnArgs& a, int64_t B, int ctas, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(a.T * a.H * a.G), 1, (unsigned)B);
     cfg.blockDim = dim3(kJoinWarps * 32);
@@ -607,7 +694,7 @@ int launch_kv_attention(const KvAttnArgs& a, int64_t B, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<DT, D>, a);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<DT, D, EVEN>, a, (int)B, ctas);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return fail(NT_ERR_CUDA, "kv_attention_join_kernel launch failed: %s", cudaGetErrorString(e));
@@ -615,9 +702,29 @@ int launch_kv_attention(const KvAttnArgs& a, int64_t B, cudaStream_t stream) {
     return check_launch("kv_attention_join_kernel");
 }
 
+template <int DT, int D, int W>
+int launch_kv_attention(const KvAttnArgs& a, int64_t B, int even, cudaStream_t stream) {
+    const size_t smem = std::max(kRingBytes<D, W>, sizeof(float) * W * kRows * (D + 2));
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kv_attention_kernel<DT, D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return fail(NT_ERR_CUDA, "nt_kv_attention: %s", cudaGetErrorString(e));
+    }
+    if constexpr (W == 2) {
+        if (even) {
+            kv_attention_even_kernel<DT, D, W><<<even, W * 32, smem, stream>>>(a, (int)B);
+            const int rc = check_launch("kv_attention_even_kernel");
+            return rc != NT_OK ? rc : launch_join<DT, D, true>(a, B, even, stream);
+        }
+    }
+    const dim3 grid((unsigned)a.splits, (unsigned)(a.H * a.row_tiles), (unsigned)B);
+    kv_attention_kernel<DT, D, W><<<grid, W * 32, smem, stream>>>(a);
+    const int rc = check_launch("kv_attention_kernel");
+    return rc != NT_OK || a.splits == 1 ? rc : launch_join<DT, D, false>(a, B, 0, stream);
+}
+
 template <int DT, int D>
-int launch_warps(const KvAttnArgs& a, int64_t B, int warps, cudaStream_t stream) {
-    return warps == 8 ? launch_kv_attention<DT, D, 8>(a, B, stream) : launch_kv_attention<DT, D, 2>(a, B, stream);
+int launch_planned(const KvAttnArgs& a, int64_t B, const Plan& pl, cudaStream_t stream) {
+    return pl.warps == 8 ? launch_kv_attention<DT, D, 8>(a, B, 0, stream) : launch_kv_attention<DT, D, 2>(a, B, pl.even, stream);
 }
 
 }  // namespace
@@ -675,8 +782,8 @@ int nt_kv_attention(int dtype, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, in
     a.err = device_error_word(dev);
     if (!a.err) return fail(NT_ERR_CUDA, "nt_kv_attention: error word unavailable");
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (dtype == NT_F32) return D == 64 ? launch_warps<NT_F32, 64>(a, B, pl.warps, st) : launch_warps<NT_F32, 128>(a, B, pl.warps, st);
-    return D == 64 ? launch_warps<NT_BF16, 64>(a, B, pl.warps, st) : launch_warps<NT_BF16, 128>(a, B, pl.warps, st);
+    if (dtype == NT_F32) return D == 64 ? launch_planned<NT_F32, 64>(a, B, pl, st) : launch_planned<NT_F32, 128>(a, B, pl, st);
+    return D == 64 ? launch_planned<NT_BF16, 64>(a, B, pl, st) : launch_planned<NT_BF16, 128>(a, B, pl, st);
 }
 
 }  // extern "C"

@@ -422,6 +422,35 @@ def test_kv_attention_against_definition(nat, dtype, P, D, T, H, G, lengths, cou
         assert (o[b, c:] == 0).all()
 
 
+@pytest.mark.parametrize("B,H,G,longest,window", [(70, 2, 1, 900, None), (520, 1, 2, 200, None), (300, 4, 1, 60, None), (9, 1, 8, 1300, None),
+                                                  (150, 2, 1, 700, 33), (2, 1, 1, 1536, None)])
+def test_kv_attention_many_ragged_sequences(nat, B, H, G, longest, window):
+    """Shares of the work that begin and end inside sequences, sequences without keys between them, batches
+    of every size that the plan tells apart; twice the same bits, and bad sequences flagged and zero."""
+    P, D = 16, 64
+    g = torch.Generator().manual_seed(B)
+    lengths = torch.randint(0, longest + 1, (B,), generator=g).tolist()
+    lengths[-1] = longest
+    counts = [min(1, n) for n in lengths]
+    counts[B // 2] = 0
+    cache, table = make_cache(B, 96, H, P, D, 40)
+    fill(cache, table, lengths, H, P, D, 41)
+    q = torch.randn(B, 1, H * G, D, device=DEV, generator=gen(42)).to(BF16)
+    n = torch.tensor(lengths, device=DEV, dtype=torch.int32)
+    c = torch.tensor(counts, device=DEV, dtype=torch.int32)
+    o = nat.kv_attention(q, *cache, table, n, counts=c, window=window)
+    want, tol = attention64(q, cache, table, lengths, counts, window, P)
+    close(o, want, half(BF16), tol)
+    assert torch.equal(o, nat.kv_attention(q, *cache, table, n, counts=c, window=window))
+    assert nat.device_error_flags(0) == 0
+    n[0], c[0] = 97 * P, 1                                   # past the table
+    n[1], c[1] = 3, 2                                        # more than T
+    o2 = nat.kv_attention(q, *cache, table, n, counts=c, window=window)
+    assert nat.device_error_flags(0) == 8
+    assert (o2[:2] == 0).all()
+    close(o2[2:], want[2:], half(BF16), tol[2:])
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_kv_attention_extreme_scales_and_scores(nat, dtype):
     """Pages whose scales are 2^60 apart, sharp and flat rows, tiny and large queries, a scale of its own."""
