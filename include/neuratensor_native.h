@@ -269,7 +269,8 @@ NT_API int nt_window_attention(int dtype, int64_t B, int64_t T, int64_t n_heads,
  * at position p turns by the angle p * inv_freq[i], taken in float64:
  *   y1 = m (x1 cos - x2 sin),  y2 = m (x2 cos + x1 sin),  m = mscale,
  * in float32 with one rounding to `dtype`.  inverse != 0 turns backwards (the
- * gradient of the forward call with the same arguments).  positions: int64,
+ * gradient of the forward call with the same arguments).  y is x or does not
+ * overlap it; D <= 2048.  positions: int64,
  * row b starts at positions + b*p_sb (p_sb = 0: shared by the batch);
  * inv_freq: [R/2] float32. */
 NT_API int nt_rotary(int dtype, int64_t B, int64_t T, int64_t H, int64_t D, int64_t R, int interleaved,
@@ -293,7 +294,8 @@ NT_API int nt_rotary(int dtype, int64_t B, int64_t T, int64_t H, int64_t D, int6
  * block's scale when the block holds older tokens; older codes are re-encoded
  * when it grows.  Codes: x / s rounded to nearest even, saturating; NaN stays
  * NaN.  Slots behind the new tokens are left as they are.  A page that is
- * written must belong to one sequence.  A sequence with counts outside [0, T],
+ * written must belong to one sequence and stand once among its blocks; calls that
+ * write the same pages must not overlap.  A sequence with counts outside [0, T],
  * lengths < counts or lengths past the table, and a page outside
  * [0, n_pages), is skipped and sets the bad-argument bit of the device error
  * word. */

@@ -411,6 +411,8 @@ class NeuraTensorModel(nn.Module):
         made = torch.full((B,), prompt, dtype=torch.int32, device=out.device) if frequency_penalty or presence_penalty else None
         bias_ids = bias = None
         if logit_bias:
+            if not all(0 <= i < self.config.vocab_size for i in logit_bias):
+                raise ValueError(f"logit_bias names tokens outside the vocabulary of {self.config.vocab_size}")
             bias_ids = torch.tensor([list(logit_bias)], dtype=torch.int64, device=out.device).expand(B, -1)
             bias = torch.tensor([list(logit_bias.values())], dtype=torch.float32, device=out.device).expand(B, -1)
         words = lambda m: native.pack_allowed(m) if m is not None and m.dtype == torch.bool else m  # noqa: E731

@@ -146,6 +146,53 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
     // every row of the CTA sees all of a tile when it lies in [all_lo, all_hi)
     const int all_hi = s.start + row_tile * kRows / a.G + 1, all_lo = a.window >= 0 ? s.hi - 1 - a.window : 0;
 
+    // o[j]: dimensions g*D/8 + 2j (rows 2c, 2c+1) and g*D/8 + 2j + 1 (the same rows), in units of v_unit
+    float o[MT][4];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, v_unit = 0.f, inv_unit = 0.f;
+
+    // This warp's tiles are first + warp + W * i, i < mine.  Lane j holds the
+    // page and the scales of the j-th of 32 tiles: f_* for the tiles being
+    // fetched, c_* for those being computed, at most two behind.
+    const int mine = last - first > warp ? (last - first - warp + W - 1) / W : 0;
+    const int32_t* table = a.table + b * a.table_sb;
+    int f_page = -1, c_page = -1;
+    float f_ks = 0.f, f_vs = 0.f, c_ks = 0.f, c_vs = 0.f;
+    bool bad_page = false;
+    unsigned char* ring = smem + warp * (kStages * 2 * kTileBytes<D>);
+    const uint32_t ring_u32 = smem_u32(ring);
+    auto fetch = [&](int i) {
+        if ((i & 31) == 0) {
+            f_page = -1;
+            if (i + lane < mine) {
+                const int pg = table[(s.lo16 + (first + warp + W * (i + lane)) * kTile) >> a.page_shift];
+                if (pg < 0 || pg >= a.n_pages) {
+                    bad_page = true;
+                } else {
+                    f_page = pg;
+                    f_ks = __ldg(a.ks + (int64_t)pg * a.H + h);
+                    f_vs = __ldg(a.vs + (int64_t)pg * a.H + h);
+                }
+            }
+        }
+        const int pg = __shfl_sync(0xffffffffu, f_page, i & 31);
+        if (pg >= 0 && i < mine) {
+            const int slot = ((first + warp + W * i) * kTile + s.lo16) & ((1 << a.page_shift) - 1);
+            const int64_t off = ((((int64_t)pg * a.H + h) << a.page_shift) + slot) * D + lane * 16;
+            const uint32_t dst = ring_u32 + (i % kStages) * (2 * kTileBytes<D>);
+            constexpr int CH = D / 16;                  // chunks of a row
+#pragma unroll
+            for (int j = 0; j < kTileBytes<D> / 512; ++j) {
+                const int row = j * (32 / CH) + lane / CH, ch = lane % CH;
+                cp16(dst + row * D + ((ch ^ k_swz<D>(row)) << 4), a.kc + off + j * 512);
+                cp16(dst + kTileBytes<D> + row * D + ((ch ^ v_swz<D>(row)) << 4), a.vc + off + j * 512);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    fetch(0);                                           // on its way while q is read
+
     // q rows in f16, scaled by a power of two so that the largest value is in [2^13, 2^14)
     uint32_t qh[KS][2], ql[KS][2];
     float q_inv = 1.f;
@@ -202,52 +249,6 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
 
     const float qi0 = __shfl_sync(0xffffffffu, q_inv, 8 * c), qi1 = __shfl_sync(0xffffffffu, q_inv, 8 * c + 4);
 
-    // o[j]: dimensions g*D/8 + 2j (rows 2c, 2c+1) and g*D/8 + 2j + 1 (the same rows), in units of v_unit
-    float o[MT][4];
-#pragma unroll
-    for (int j = 0; j < MT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, v_unit = 0.f, inv_unit = 0.f;
-
-    // This warp's tiles are first + warp + W * i, i < mine.  Lane j holds the
-    // page and the scales of the j-th of 32 tiles: f_* for the tiles being
-    // fetched, c_* for those being computed, at most two behind.
-    const int mine = last - first > warp ? (last - first - warp + W - 1) / W : 0;
-    const int32_t* table = a.table + b * a.table_sb;
-    int f_page = -1, c_page = -1;
-    float f_ks = 0.f, f_vs = 0.f, c_ks = 0.f, c_vs = 0.f;
-    bool bad_page = false;
-    unsigned char* ring = smem + warp * (kStages * 2 * kTileBytes<D>);
-    const uint32_t ring_u32 = smem_u32(ring);
-    auto fetch = [&](int i) {
-        if ((i & 31) == 0) {
-            f_page = -1;
-            if (i + lane < mine) {
-                const int pg = table[(s.lo16 + (first + warp + W * (i + lane)) * kTile) >> a.page_shift];
-                if (pg < 0 || pg >= a.n_pages) {
-                    bad_page = true;
-                } else {
-                    f_page = pg;
-                    f_ks = __ldg(a.ks + (int64_t)pg * a.H + h);
-                    f_vs = __ldg(a.vs + (int64_t)pg * a.H + h);
-                }
-            }
-        }
-        const int pg = __shfl_sync(0xffffffffu, f_page, i & 31);
-        if (pg >= 0 && i < mine) {
-            const int slot = ((first + warp + W * i) * kTile + s.lo16) & ((1 << a.page_shift) - 1);
-            const int64_t off = ((((int64_t)pg * a.H + h) << a.page_shift) + slot) * D + lane * 16;
-            const uint32_t dst = ring_u32 + (i % kStages) * (2 * kTileBytes<D>);
-            constexpr int CH = D / 16;                  // chunks of a row
-#pragma unroll
-            for (int j = 0; j < kTileBytes<D> / 512; ++j) {
-                const int row = j * (32 / CH) + lane / CH, ch = lane % CH;
-                cp16(dst + row * D + ((ch ^ k_swz<D>(row)) << 4), a.kc + off + j * 512);
-                cp16(dst + kTileBytes<D> + row * D + ((ch ^ v_swz<D>(row)) << 4), a.vc + off + j * 512);
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    fetch(0);
     for (int i = 0; i < mine; ++i) {
         if ((i & 31) == 0) {
             c_page = f_page;
@@ -651,6 +652,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv_attention_join_kernel(cons
 struct Plan { int row_tiles, warps, chunk, splits, even; int64_t part_bytes; };
 Plan plan_of(int64_t B, int64_t T, int64_t G, int64_t H, int64_t D, int64_t page, int64_t n_blocks, int64_t window) {
     Plan pl{};
+    window = std::min<int64_t>(window, INT32_MAX / 2);
     pl.row_tiles = (int)((T * G + kRows - 1) / kRows);
     int64_t span = n_blocks * page;
     if (window >= 0) span = std::min(span, window + std::min<int64_t>(T, kRows) + kTile);
@@ -661,7 +663,8 @@ Plan plan_of(int64_t B, int64_t T, int64_t G, int64_t H, int64_t D, int64_t page
         pl.warps = 8;
         pl.chunk = (int)tiles;
         pl.splits = 1;
-    } else if (window < 0 && pl.row_tiles == 1 && B <= kEvenBatch && base <= 8 * 148) {
+    } else if (window < 0 && pl.row_tiles == 1 && B <= kEvenBatch && base <= 8 * 148 &&
+               B * tiles < INT32_MAX) {
         // lengths that the host does not know: even shares for one wave of eight CTAs per SM, unless
         // there are more heads than that (us, even shares against chunks or whole heads: 8 ragged
         // caches of up to 65536 tokens x 8 heads 100 : 105, one of 131072 x 8 63 : 81, 64 of up to

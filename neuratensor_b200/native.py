@@ -511,8 +511,8 @@ def rotary(x: Tensor, positions: Tensor, inv_freq: Tensor, layout: str = "half",
     rows; inv_freq: [R/2] float32, the first R <= D dimensions turn and the rest are
     copied.  layout "half" pairs (i, i + R/2), "interleaved" (2i, 2i + 1).  Pair i turns
     by positions * inv_freq[i], taken in float64, and is multiplied by mscale; one
-    rounding.  inverse turns backwards.  out may be x (in place).  Differentiable in x
-    (not with out)."""
+    rounding.  inverse turns backwards.  out may be x (in place), or must not overlap it.
+    Differentiable in x (not with out).  Heads of at most 2048 dimensions."""
     if (x.requires_grad or inv_freq.requires_grad) and torch.is_grad_enabled():
         if inv_freq.requires_grad:
             raise RuntimeError("rotary has no gradient for inv_freq; detach it")
@@ -601,7 +601,8 @@ def kv_append(k: Tensor, v: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: T
     ones; counts [B] (None: T): how many of the T rows are new, rows 0..counts-1, which
     become the last counts positions.  A page's scale grows with its largest value, and
     its older codes are re-encoded then.  A page that is written must belong to one
-    sequence; a bad length, count or page is skipped and flagged (device_error_flags)."""
+    sequence and stand once among its blocks; a bad length, count or page is skipped and
+    flagged (device_error_flags)."""
     _refuse_grad("kv_append", k, v)
     dev = _require_cuda(k, v, k_codes, k_scale, v_codes, v_scale, table, lengths, counts)
     code = _dtype_code(k)

@@ -197,6 +197,8 @@ def test_generate_penalties_biases_and_masks():
 
     out = eng.generate(ids, max_new_tokens=9, top_k=50, allowed=even_then_odd, attn_cache=True)
     assert torch.equal(out[:, 10:] % 2, (torch.arange(10, 19, device=DEV) % 2).expand(2, -1))
+    with pytest.raises(ValueError, match="outside the vocabulary"):
+        eng.generate(ids, max_new_tokens=2, logit_bias={1000: 1.0})
     from neuratensor_b200 import native
     assert native.device_error_flags(0) == 0
 

@@ -530,6 +530,17 @@ def test_kv_attention_strided_q_other_stream_and_graph(nat):
     for g in graphs:
         g.replay()
     assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+    # a table wide enough that the work is shared between CTAs and joined by a second kernel
+    wide = torch.cat([table, table.flip(1), table, table.flip(1), table], 1)
+    first = nat.kv_attention(q, *cache, wide, n)
+    close(first, *(lambda w, t: (w, half(BF16), t))(*attention64(q, cache, table, lengths, [1] * B, None, P)))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        joined = nat.kv_attention(q, *cache, wide, n)
+    for _ in range(3):
+        joined.zero_()
+        g.replay()
+        assert torch.equal(joined, first)
     n -= torch.tensor([1, 0, 37, 60], device=DEV, dtype=torch.int32)
     want = nat.kv_attention(q, *cache, table, n)
     graphs[0].replay()
@@ -590,6 +601,7 @@ def test_kv_refusals(nat):
         nat.kv_attention(x.clone().requires_grad_(), *cache, table, n)
     with pytest.raises(RuntimeError, match="CUDA"):
         nat.kv_attention(x, *cache, table, n.cpu())
+    assert nat.kv_attention(x, *cache, table, n, window=2 ** 63 - 1).shape == (B, T, H, D)     # as good as none
     assert nat.kv_attention(x[:, :0], *cache, table, n).shape == (B, 0, H, D)
     assert nat.kv_attention(x[:0], *cache, table[:0], n[:0]).shape == (0, T, H, D)
 

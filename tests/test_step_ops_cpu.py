@@ -21,7 +21,7 @@ def rotary(L, dtype=0, B=1, T=2, H=3, D=64, R=64, x=FAKE, y=FAKE, pos=FAKE, freq
 
 @pytest.mark.parametrize("bad,status,text", [
     (dict(dtype=2), 2, "dtype"), (dict(R=63), 1, "even"), (dict(R=66), 1, "even"), (dict(R=0), 1, "even"), (dict(B=-1), 1, "sizes"),
-    (dict(D=0), 1, "sizes"), (dict(x=None), 1, "null"), (dict(pos=None), 1, "null"), (dict(freq=None), 1, "null"),
+    (dict(D=0), 1, "sizes"), (dict(D=2050, R=64), 1, "sizes"), (dict(x=None), 1, "null"), (dict(pos=None), 1, "null"), (dict(freq=None), 1, "null"),
     (dict(y=None), 1, "null"), (dict(ys=(1, 2, 3)), 1, "in place")])
 def test_rotary_status(nat, bad, status, text):
     L = nat.load()
@@ -74,6 +74,7 @@ def test_attention_workspace_covers_long_caches(nat):
     assert attention(L, Hq=32, H=8, D=128, page=64, blocks=2048, ws=FAKE, nbytes=need - 1) == 6
     assert L.nt_kv_attention_workspace_bytes(1, 1, 10, 10, 64, 16, 4, -1) == 0        # one CTA per head sees all of it
     assert L.nt_kv_attention_workspace_bytes(0, 1, 1, 1, 64, 16, 4, -1) == 0
+    assert L.nt_kv_attention_workspace_bytes(1, 1, 10, 10, 64, 16, 4, 2 ** 63 - 1) == 0
 
 
 def logits(L, dtype=0, B=1, V=100, x=FAKE, tokens=FAKE, n=5, prompts=None, each=0, rep=1.0, ids=None, nb=0, out=FAKE, ldo=100):
