@@ -265,7 +265,7 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
             const unsigned char* vt = kt + kTileBytes<D>;
             const float ks = __shfl_sync(0xffffffffu, c_ks, i & 31), vs = __shfl_sync(0xffffffffu, c_vs, i & 31);
             // scores: d[0], d[1] key g of the tile, d[2], d[3] key g + 8, for rows 2c and 2c + 1
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            float d[4] = {0.f, 0.f, 0.f, 0.f}, d2[4] = {0.f, 0.f, 0.f, 0.f};     // two chains of products
 #pragma unroll
             for (int j = 0; j < D / 64; ++j) {
                 const int at = g * D + (((4 * j + c) ^ k_swz<D>(g)) << 4);
@@ -274,10 +274,13 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const uint32_t a0 = cvt_lo(ku[k]), a1 = cvt_lo(kw[k]), a2 = cvt_hi(ku[k]), a3 = cvt_hi(kw[k]);
-                    mma_f16(d, a0, a1, a2, a3, qh[4 * j + k][0], qh[4 * j + k][1], d[0], d[1], d[2], d[3]);
-                    if constexpr (kPair) mma_f16(d, a0, a1, a2, a3, ql[4 * j + k][0], ql[4 * j + k][1], d[0], d[1], d[2], d[3]);
+                    float (&e)[4] = k & 1 ? d2 : d;
+                    mma_f16(e, a0, a1, a2, a3, qh[4 * j + k][0], qh[4 * j + k][1], e[0], e[1], e[2], e[3]);
+                    if constexpr (kPair) mma_f16(e, a0, a1, a2, a3, ql[4 * j + k][0], ql[4 * j + k][1], e[0], e[1], e[2], e[3]);
                 }
             }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) d[k] += d2[k];
             float sc[2][2] = {{d[0] * (qi0 * ks), d[1] * (qi1 * ks)}, {d[2] * (qi0 * ks), d[3] * (qi1 * ks)}};
             const bool whole = key0 >= all_lo && key0 >= s.lo && key0 + kTile <= all_hi;
             if (!whole) {
