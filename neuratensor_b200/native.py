@@ -475,6 +475,11 @@ def _launch(dev: torch.device, name: str, *args) -> None:
         _check(name, rc)
 
 
+def _like(t: Tensor) -> Tensor:
+    """An uninitialised contiguous tensor of t's shape, dtype and device."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _refuse_grad(fn: str, t: Tensor, u: Optional[Tensor] = None) -> None:
     if (t.requires_grad or (u is not None and u.requires_grad)) and torch.is_grad_enabled():
         raise RuntimeError(f"{fn} has no backward; detach the inputs or run under torch.no_grad()")
@@ -550,7 +555,7 @@ def _rotary(x, positions, inv_freq, layout, mscale, inverse, out):
         x = x.contiguous()
         x_sb, x_st, x_sh, _ = x.stride()
     if out is None:
-        out = x.new_empty((B, T, H, D))
+        out = _like(x)
     elif out.shape != x.shape or out.dtype != x.dtype or out.stride(3) != 1:
         raise ValueError("out must have x's shape and dtype and unit stride in D")
     elif any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
@@ -657,7 +662,7 @@ def kv_attention(q: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: Tensor, v
     if q.stride(3) != 1:
         q = q.contiguous()
     q_sb, q_st, q_sh, _ = q.stride()
-    out = q.new_empty((B, T, Hq, D))
+    out = _like(q)
     nbytes = _kv_attention_bytes(B, T, Hq, H, D, P, blocks, win)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _launch(dev, "nt_kv_attention", code, B, T, Hq, H, D, P, n, blocks, win, 1.0 / math.sqrt(D) if scale is None else scale,
@@ -747,7 +752,7 @@ def logits_process(logits: Tensor, tokens: Optional[Tensor] = None, lengths: Opt
             allowed = allowed.contiguous()
         allowed_ld = allowed.stride(0) if allowed.shape[0] == B else 0
     if out is None:
-        out = logits.new_empty((B, V))
+        out = _like(logits)
     elif out.shape != logits.shape or out.dtype != logits.dtype or (V > 1 and out.stride(1) != 1) or \
             (B > 1 and out.stride(0) < V):
         raise ValueError("out must be [B, V] in the logits' dtype with unit column stride")
