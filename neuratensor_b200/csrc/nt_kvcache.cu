@@ -16,7 +16,7 @@
 // reduced, and the codes are written; 8 values per thread and step (16 bytes of
 // bf16 in, 8 bytes of codes out).  Bound by HBM for prompts (8 of up to 8192
 // tokens, 16 heads of 128: 112 us with 128 threads that looked the page up before
-// they read, 84 us so; several units to a CTA of 256 threads 92 us), by launch
+// they read, 72 us so; several units to a CTA of 256 threads 92 us), by launch
 // latency for single tokens.
 #include "nt_kernels.cuh"
 
@@ -65,8 +65,8 @@ template <int DT> struct Raw {
     using T = typename Elem<DT>::T;
     static constexpr int W = 8 * (int)sizeof(T) / 16;
     uint4 w[W];
-    __device__ __forceinline__ void load(const T* p, bool vec) {
-        if (vec) {
+    template <bool VEC> __device__ __forceinline__ void load(const T* p) {
+        if constexpr (VEC) {
 #pragma unroll
             for (int i = 0; i < W; ++i) w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
         } else {
@@ -104,8 +104,9 @@ template <int DT> struct Raw {
     }
 };
 
-template <int DT, int D, int P>
-__global__ void __launch_bounds__(kAppThreadsOf<D, P>) kv_append_kernel(const __grid_constant__ AppendArgs a, int vec) {
+// VEC: rows allow 16-byte loads.
+template <int DT, int D, int P, bool VEC>
+__global__ void __launch_bounds__(kAppThreadsOf<D, P>) kv_append_kernel(const __grid_constant__ AppendArgs a) {
     using T = typename Elem<DT>::T;
     constexpr int kAppThreads = kAppThreadsOf<D, P>;
     constexpr int CH = D / 8;                           // vectors of a row
@@ -122,30 +123,49 @@ __global__ void __launch_bounds__(kAppThreadsOf<D, P>) kv_append_kernel(const __
     if (cnt == 0 || base >= len) return;
     const int lo = (int)(start > base ? start - base : 0);                // first new slot; older ones before it
     const int hi = (int)(len - base < P ? len - base : P);
-    const T* x = static_cast<const T*>(a.x[side]) + b * a.sb[side] + (int64_t)h * a.sh[side];
+    const bool full = lo == 0 && hi == P;               // all pages of a prompt but its first and last
+    const int64_t st = side ? a.st[1] : a.st[0];
+    const T* x = static_cast<const T*>(side ? a.x[1] : a.x[0]) + b * (side ? a.sb[1] : a.sb[0]) +
+                 (int64_t)h * (side ? a.sh[1] : a.sh[0]) + (base - start + threadIdx.x / CH) * st + threadIdx.x % CH * 8;
+    const int64_t step = kAppThreads / CH * st;
     // the values are on their way before the page is known
     Raw<DT> raw[NV];
+    if (full) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int idx = threadIdx.x + i * kAppThreads, slot = idx / CH, c = idx % CH;
-        if (slot >= lo && slot < hi) raw[i].load(x + (base + slot - start) * a.st[side] + c * 8, vec);
+        for (int i = 0; i < NV; ++i) raw[i].template load<VEC>(x + i * step);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int slot = (threadIdx.x + i * kAppThreads) / CH;
+            if (slot >= lo && slot < hi) raw[i].template load<VEC>(x + i * step);
+        }
     }
     const int64_t page = a.table[b * a.table_sb + blk];
     if (page < 0 || page >= a.n_pages) {
         if (threadIdx.x == 0) atomicOr(a.err, ERRF_BAD_ARG);
         return;
     }
-    uint8_t* codes = a.codes[side] + (page * a.H + h) * (int64_t)(P * D);
-    float* sp = a.scale[side] + page * a.H + h;
+    uint8_t* codes = (side ? a.codes[1] : a.codes[0]) + (page * a.H + h) * (int64_t)(P * D);
+    float* sp = (side ? a.scale[1] : a.scale[0]) + page * a.H + h;
     const float s_old = lo > 0 ? *sp : 0.f;
 
     float amax = 0.f;
+    if (full) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int slot = (threadIdx.x + i * kAppThreads) / CH;
-        if (slot >= lo && slot < hi) {
-            const float m = raw[i].amax();
-            amax = fmaxf(amax, m <= 3.402823466e38f ? m : raw[i].amax_finite());
+        for (int i = 0; i < NV; ++i) amax = fmaxf(amax, raw[i].amax());
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int slot = (threadIdx.x + i * kAppThreads) / CH;
+            if (slot >= lo && slot < hi) amax = fmaxf(amax, raw[i].amax());
+        }
+    }
+    if (amax > 3.402823466e38f) {                       // an infinity: the finite values' maximum is wanted
+        amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int slot = (threadIdx.x + i * kAppThreads) / CH;
+            if (slot >= lo && slot < hi) amax = fmaxf(amax, raw[i].amax_finite());
         }
     }
     __shared__ float red[kAppThreads / 32];
@@ -165,7 +185,7 @@ __global__ void __launch_bounds__(kAppThreadsOf<D, P>) kv_append_kernel(const __
         w.y = e4m3x4(raw[i].at(4) * inv, raw[i].at(5) * inv, raw[i].at(6) * inv, raw[i].at(7) * inv);
         dst[i * kAppThreads] = w;
     };
-    if (lo == 0 && hi == P) {                           // all pages of a prompt but its first and last
+    if (full) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) encode(i);
     } else {
@@ -195,7 +215,8 @@ int launch_append(const AppendArgs& a, int64_t B, int vec, cudaStream_t stream) 
     const int64_t blocks = (a.T + P - 2) / P + 1;      // pages that T tokens can touch
     if (blocks > 65535) return fail(NT_ERR_ARG, "nt_kv_append: %lld tokens in one call", (long long)a.T);
     const dim3 grid((unsigned)(2 * a.H), (unsigned)blocks, (unsigned)B);
-    kv_append_kernel<DT, D, P><<<grid, kAppThreadsOf<D, P>, 0, stream>>>(a, vec);
+    if (vec) kv_append_kernel<DT, D, P, true><<<grid, kAppThreadsOf<D, P>, 0, stream>>>(a);
+    else kv_append_kernel<DT, D, P, false><<<grid, kAppThreadsOf<D, P>, 0, stream>>>(a);
     return check_launch("kv_append_kernel");
 }
 
