@@ -9,11 +9,17 @@
 // final, so a CTA owns a slice of one row's vocabulary, with a counter per entry
 // in shared memory: it reads the row's whole history (from L2 for all slices
 // but the first), counts what falls into its slice, and then streams the slice.
-// Several CTAs share an SM, so one streams while another counts.  (A cluster of
-// CTAs per row that read the history once and counted into each other's shared
-// memory was slower: 131 us against 70 us for 250 x 131072 float32 with 4000 tokens of
-// history, 21.5 against 13.3 us for 64 x 32000 bf16 with 8704.)  Integer counters: the
-// order of arrival changes nothing.
+// Five CTAs share an SM, so some stream while others count.  Integer counters:
+// the order of arrival changes nothing.
+//
+// 250 x 131072 float32 with 4000 tokens of history, 300 biases and a mask: 67 us,
+// where the stream alone takes 44, the history 13, lookups at its touched entries,
+// biases and mask the rest; 64 x 32000 bf16 with 8704 tokens 14 us.  Measured
+// against this at the first size: the history counted once per cluster into
+// distributed shared memory 96 to 131 us; a list of touched entries put right
+// after an unchanged stream 89; a second kernel with a hash table per row 86.
+// The registers of a CTA decide: four vectors and eight tokens of a thread in
+// flight cost a CTA per SM or spills (69 to 78 us).
 //
 // A counter holds the index (plus one) of the last bias entry of the token, the
 // number of occurrences after the prompt, and one bit for an occurrence at all:
@@ -25,6 +31,7 @@
 #include "nt_kernels.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace nt {
 namespace {
@@ -53,33 +60,35 @@ template <bool WIDE> struct Count {
     static constexpr int kWords = WIDE ? 2 : 1;
 };
 
-// One logit: the penalties of its counter w, bias entry j - 1 (0: none).
+// One logit: the penalties of its counter w, bias entry j - 1 (0: none).  Without
+// branches for the penalties: an entry that was not met is multiplied by one and
+// loses zero, which leaves it as it is, and the lanes of a warp stay together.
 template <int DT, bool WIDE, bool EACH>
 __device__ __forceinline__ float process(float x, uint32_t w, uint32_t j, float r, float r_inv, float fq, float ps,
                                          const float* bias) {
-    if ((w | j) != 0) {
-        const uint32_t made = WIDE ? w & 0x7fffffffu : (w >> 16) & 0x7fffu;
-        if constexpr (EACH) {
-            for (uint32_t i = 0; i < made; ++i) x = Elem<DT>::rnd(x > 0.f ? x * r_inv : x * r);
-        } else {
-            if (made || (w >> 31)) x = x > 0.f ? x * r_inv : x * r;
-        }
-        if (made) x -= fmaf(fq, (float)made, ps);
-        if (!WIDE) j = w & 0xffffu;
-        if (j) x += __ldg(bias + (j - 1));
+    const uint32_t made = WIDE ? w & 0x7fffffffu : (w >> 16) & 0x7fffu;
+    if (!WIDE) j = w & 0xffffu;
+    if constexpr (EACH) {
+        for (uint32_t i = 0; i < made; ++i) x = Elem<DT>::rnd(x > 0.f ? x * r_inv : x * r);
+    } else {
+        const float f = x > 0.f ? r_inv : r;
+        x *= (WIDE ? w : w >> 16) ? f : 1.f;
     }
+    x -= made ? fmaf(fq, (float)made, ps) : 0.f;
+    if (j) x += __ldg(bias + (j - 1));
     return x;
 }
 
-template <int DT, bool WIDE, bool EACH>
-__global__ void __launch_bounds__(kLogThreads, 6) logits_kernel(const __grid_constant__ LogArgs a) {
+// COUNTED: there is a history or there are biases.  MASK: there is a mask.
+template <int DT, bool COUNTED, bool MASK, bool WIDE, bool EACH>
+__global__ void __launch_bounds__(kLogThreads, 5) logits_kernel(const __grid_constant__ LogArgs a) {
     using El = Elem<DT>;
     using T = typename El::T;
     using K = Count<WIDE>;
     constexpr int E = 16 / (int)sizeof(T);
     extern __shared__ __align__(16) uint32_t smem[];
     const int64_t b = blockIdx.x / a.slices;
-    const int64_t lo = (int64_t)(blockIdx.x % a.slices) * a.slice;
+    const int lo = (int)(blockIdx.x % a.slices) * a.slice;
     const int n = (int)(a.V - lo < a.slice ? a.V - lo : a.slice);
     const T* x = static_cast<const T*>(a.x) + b * a.ld + lo;
     T* y = static_cast<T*>(a.out) + b * a.ldo + lo;
@@ -87,53 +96,36 @@ __global__ void __launch_bounds__(kLogThreads, 6) logits_kernel(const __grid_con
     // words[i], shifted so that those of a vector are 16-byte aligned too.
     const int head_x = (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T);
     const int head_y = (int)((16 - (reinterpret_cast<uintptr_t>(y) & 15)) & 15) / (int)sizeof(T);
-    const int pad = (E - head_x) & (E - 1);
-    uint32_t* words = smem + pad;
+    uint32_t* words = smem + ((E - head_x) & (E - 1));
     const int stride = a.slice + E;                     // from the counters to the bias indices when wide
-    const float r = a.rep ? a.rep[b] : a.rep_all, fq = a.freq ? a.freq[b] : a.freq_all, ps = a.pres ? a.pres[b] : a.pres_all;
-    const float r_inv = 1.f / r;
-    const uint32_t* mask = a.allowed ? a.allowed + b * a.allowed_ld : nullptr;
-    const float* bias = a.NB ? a.bias + b * a.bias_ld : nullptr;
-    int len = a.tokens ? (a.lengths ? a.lengths[b] : a.L) : 0;
-    len = len < 0 ? 0 : (len > a.L ? a.L : len);
-    const bool counted = len > 0 || a.NB > 0;
-
-    const bool touched_only = static_cast<const void*>(x) == static_cast<const void*>(y) && !mask;
-    const int head = head_x == head_y ? (head_x < n ? head_x : n) : n;      // all singly when no boundary is shared
-    const int nv = touched_only ? 0 : (n - head) / E;
-    // vectors of a thread in flight, with their mask bits (loading the first ones before
-    // the history is counted cost registers, and so CTAs per SM: 84 us against 70)
-    constexpr int U = 4;
-    uint4 q[U];
-    uint32_t bits[U];
-    auto load = [&](int i0) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * kLogThreads;
-            bits[u] = ~0u;
-            if (i >= nv) continue;
-            q[u] = __ldcs(reinterpret_cast<const uint4*>(x + head) + i);
-            if (mask) {
-                const uint32_t at = (uint32_t)lo + head + i * E, sh = at & 31;
-                bits[u] = __ldg(mask + (at >> 5)) >> sh;
-                if (sh + E > 32) bits[u] |= __ldg(mask + (at >> 5) + 1) << (32 - sh);
-            }
-        }
-    };
-    if (counted) {
+    const uint32_t* mask = MASK ? a.allowed + b * a.allowed_ld : nullptr;
+    float r = 1.f, r_inv = 1.f, fq = 0.f, ps = 0.f;
+    const float* bias = nullptr;
+    if constexpr (COUNTED) {
+        r = a.rep ? a.rep[b] : a.rep_all;
+        r_inv = 1.f / r;
+        fq = a.freq ? a.freq[b] : a.freq_all;
+        ps = a.pres ? a.pres[b] : a.pres_all;
+        if (a.NB) bias = a.bias + b * a.bias_ld;
+        int len = a.L > 0 ? (a.lengths ? a.lengths[b] : a.L) : 0;
+        len = len < 0 ? 0 : (len > a.L ? a.L : len);
         for (int i = threadIdx.x; i < stride * K::kWords / 4; i += kLogThreads)
             reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
         const int prompt = a.prompts ? a.prompts[b] : 0;
         const int64_t* tok = a.tokens + b * a.tok_ld;
-        constexpr int R = 8;                            // tokens of a thread in flight
-        for (int i0 = threadIdx.x; i0 < len; i0 += R * kLogThreads) {
+        constexpr int R = 4;                            // tokens of a thread in flight
+        auto count = [&](int i0, auto all) {
+            constexpr bool whole = decltype(all)::value;
             uint32_t v[R];
 #pragma unroll
             for (int k = 0; k < R; ++k) {
                 const int i = i0 + k * kLogThreads;
-                const int64_t t = i < len ? __ldg(tok + i) : -1;
-                v[k] = (uint64_t)t >> 32 ? ~0u : (uint32_t)t - (uint32_t)lo;
+                v[k] = ~0u;
+                if (whole || i < len) {
+                    const int2 t = __ldg(reinterpret_cast<const int2*>(tok) + i);
+                    if (t.y == 0) v[k] = (uint32_t)t.x - (uint32_t)lo;
+                }
             }
 #pragma unroll
             for (int k = 0; k < R; ++k)
@@ -141,7 +133,10 @@ __global__ void __launch_bounds__(kLogThreads, 6) logits_kernel(const __grid_con
                     if (i0 + k * kLogThreads >= prompt) atomicAdd(words + v[k], K::kOne);
                     else atomicOr(words + v[k], K::kSeen);
                 }
-        }
+        };
+        int i0 = threadIdx.x;
+        for (; i0 + (R - 1) * kLogThreads < len; i0 += R * kLogThreads) count(i0, std::true_type{});
+        if (i0 < len) count(i0, std::false_type{});
         __syncthreads();
         if (a.NB) {
             const int64_t* ids = a.ids + b * a.ids_ld;
@@ -157,55 +152,83 @@ __global__ void __launch_bounds__(kLogThreads, 6) logits_kernel(const __grid_con
         }
     }
     auto one = [&](int i) {                             // a single entry
-        const uint32_t w = counted ? words[i] : 0u, j = WIDE && counted ? words[stride + i] : 0u;
-        const float v = process<DT, WIDE, EACH>(El::to_f(x[i]), w, j, r, r_inv, fq, ps, bias);
-        const bool ok = !mask || ((mask[(lo + i) >> 5] >> ((lo + i) & 31)) & 1u);
-        y[i] = El::from_f(ok ? v : -INFINITY);
+        float v = El::to_f(x[i]);
+        if (COUNTED) v = process<DT, WIDE, EACH>(v, words[i], WIDE ? words[stride + i] : 0u, r, r_inv, fq, ps, bias);
+        if (MASK && !((mask[(lo + i) >> 5] >> ((lo + i) & 31)) & 1u)) v = -INFINITY;
+        y[i] = El::from_f(v);
     };
-    if (touched_only) {
-        if (counted)
+    if (!MASK && static_cast<const void*>(x) == static_cast<const void*>(y)) {
+        if (COUNTED)
             for (int i = threadIdx.x; i < n; i += kLogThreads)
                 if (words[i] || (WIDE && words[stride + i])) one(i);
         return;
     }
-    for (int i0 = threadIdx.x; i0 < nv; i0 += U * kLogThreads) {
-        load(i0);
+    const int head = head_x == head_y ? (head_x < n ? head_x : n) : n;      // all singly when no boundary is shared
+    const int nv = (n - head) / E;
+    constexpr int U = 3;                                // vectors of a thread in flight, with their mask bits
+    auto vectors = [&](int i0, auto all) {
+        constexpr bool whole = decltype(all)::value;
+        const uint4* src = reinterpret_cast<const uint4*>(x + head) + i0;
+        uint4* dst = reinterpret_cast<uint4*>(y + head) + i0;
+        uint4 q[U];
+        uint32_t off[U];                                // which entries the mask takes out
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * kLogThreads, first = head + i * E;
-            if (i >= nv) break;
-            T xv[E];
-            *reinterpret_cast<uint4*>(xv) = q[u];
-            uint32_t w[E], any = 0u;
-            if (counted) {
+            off[u] = 0u;
+            if (whole || i0 + u * kLogThreads < nv) {
+                q[u] = __ldcs(src + u * kLogThreads);
+                if constexpr (MASK) {
+                    const uint32_t at = (uint32_t)(lo + head + (i0 + u * kLogThreads) * E), sh = at & 31;
+                    uint32_t bits = __ldg(mask + (at >> 5)) >> sh;
+                    if (head && sh + E > 32) bits |= __ldg(mask + (at >> 5) + 1) << (32 - sh);
+                    off[u] = ~bits & ((1u << E) - 1u);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (!(whole || i0 + u * kLogThreads < nv)) continue;
+            T v[E];
+            if constexpr (COUNTED) {
+                const uint32_t* c = words + head + (i0 + u * kLogThreads) * E;
+                uint32_t w[E], any = 0u;
 #pragma unroll
                 for (int e = 0; e < E; e += 4) {
-                    const uint4 c = *reinterpret_cast<const uint4*>(words + first + e);
-                    w[e] = c.x; w[e + 1] = c.y; w[e + 2] = c.z; w[e + 3] = c.w;
-                    any |= c.x | c.y | c.z | c.w;
+                    const uint4 t = *reinterpret_cast<const uint4*>(c + e);
+                    w[e] = t.x; w[e + 1] = t.y; w[e + 2] = t.z; w[e + 3] = t.w;
+                    any |= t.x | t.y | t.z | t.w;
                     if (WIDE) {
-                        const uint4 d = *reinterpret_cast<const uint4*>(words + stride + first + e);
+                        const uint4 d = *reinterpret_cast<const uint4*>(c + stride + e);
                         any |= d.x | d.y | d.z | d.w;
                     }
                 }
+                if (any) {
+                    *reinterpret_cast<uint4*>(v) = q[u];
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        v[e] = El::from_f(process<DT, WIDE, EACH>(El::to_f(v[e]), w[e], WIDE ? c[stride + e] : 0u, r, r_inv,
+                                                                  fq, ps, bias));
+                    q[u] = *reinterpret_cast<const uint4*>(v);
+                }
             }
-            if (any) {
+            if (MASK && off[u]) {
+                *reinterpret_cast<uint4*>(v) = q[u];
 #pragma unroll
                 for (int e = 0; e < E; ++e)
-                    xv[e] = El::from_f(process<DT, WIDE, EACH>(El::to_f(xv[e]), w[e], WIDE ? words[stride + first + e] : 0u,
-                                                               r, r_inv, fq, ps, bias));
+                    if ((off[u] >> e) & 1u) v[e] = El::from_f(-INFINITY);
+                q[u] = *reinterpret_cast<const uint4*>(v);
             }
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (!((bits[u] >> e) & 1u)) xv[e] = El::from_f(-INFINITY);
-            __stcs(reinterpret_cast<uint4*>(y + head) + i, *reinterpret_cast<const uint4*>(xv));
+            __stcs(dst + u * kLogThreads, q[u]);
         }
-    }
+    };
+    int i0 = threadIdx.x;
+    for (; i0 + (U - 1) * kLogThreads < nv; i0 += U * kLogThreads) vectors(i0, std::true_type{});
+    if (i0 < nv) vectors(i0, std::false_type{});
     for (int i = threadIdx.x; i < head; i += kLogThreads) one(i);
     for (int i = head + nv * E + threadIdx.x; i < n; i += kLogThreads) one(i);
 }
 
-template <int DT, bool WIDE, bool EACH>
+template <int DT, bool COUNTED, bool WIDE, bool EACH>
 int launch(LogArgs a, int64_t B, cudaStream_t stream) {
     // Slices of 1024 to 8192 entries: four CTAs per SM if the rows allow it, and
     // no more slices than that, since each reads the whole history of its row.
@@ -215,9 +238,8 @@ int launch(LogArgs a, int64_t B, cudaStream_t stream) {
     a.slice = (int)slice;
     a.slices = (int)((a.V + slice - 1) / slice);
     if (B * a.slices > INT32_MAX) return fail(NT_ERR_ARG, "nt_logits_process: too many rows");
-    const bool counted = (a.tokens && a.L > 0) || a.NB > 0;
-    const size_t smem = counted ? (size_t)(slice + 16 / (DT == NT_F32 ? 4 : 2)) * 4 * Count<WIDE>::kWords : 0;
-    auto kern = logits_kernel<DT, WIDE, EACH>;
+    const size_t smem = COUNTED ? (size_t)(slice + 16 / (DT == NT_F32 ? 4 : 2)) * 4 * Count<WIDE>::kWords : 0;
+    auto kern = a.allowed ? logits_kernel<DT, COUNTED, true, WIDE, EACH> : logits_kernel<DT, COUNTED, false, WIDE, EACH>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return fail(NT_ERR_CUDA, "nt_logits_process: %s", cudaGetErrorString(e));
@@ -228,9 +250,10 @@ int launch(LogArgs a, int64_t B, cudaStream_t stream) {
 
 template <int DT>
 int launch_dt(const LogArgs& a, int64_t B, bool each, cudaStream_t stream) {
-    const bool small = a.L < (1 << 15) && a.NB < (1 << 16) - 1;
-    if (small) return each ? launch<DT, false, true>(a, B, stream) : launch<DT, false, false>(a, B, stream);
-    return each ? launch<DT, true, true>(a, B, stream) : launch<DT, true, false>(a, B, stream);
+    if (a.L == 0 && a.NB == 0) return launch<DT, false, false, false>(a, B, stream);
+    const bool wide = a.L >= (1 << 15) || a.NB >= (1 << 16) - 1;
+    if (wide) return each ? launch<DT, true, true, true>(a, B, stream) : launch<DT, true, true, false>(a, B, stream);
+    return each ? launch<DT, true, false, true>(a, B, stream) : launch<DT, true, false, false>(a, B, stream);
 }
 
 }  // namespace
