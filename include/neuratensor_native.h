@@ -349,6 +349,14 @@ NT_API int nt_logits_process(int dtype, int64_t B, int64_t V, const void* logits
                              const int64_t* bias_ids, int64_t ids_ld, const float* bias, int64_t bias_ld, int64_t NB,
                              const uint32_t* allowed, int64_t allowed_ld, void* out, int64_t ldo, void* stream);
 
+/* The four entry points above with their arguments in one array, for bindings
+ * that pay for every argument they convert (a step makes several short calls
+ * per layer): `words` holds the arguments in order, 8 bytes each, integers as
+ * int64, pointers as their address, floats as double; n_words must be the entry
+ * point's number of arguments. */
+enum { NT_ENTRY_ROTARY = 0, NT_ENTRY_KV_APPEND = 1, NT_ENTRY_KV_ATTENTION = 2, NT_ENTRY_LOGITS_PROCESS = 3 };
+NT_API int nt_call_packed(int entry, const void* words, int64_t n_words);
+
 #ifdef __cplusplus
 }
 #endif

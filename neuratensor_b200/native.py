@@ -11,6 +11,7 @@ import ctypes
 import functools
 import math
 import os
+import struct
 import threading
 from typing import Optional, Tuple, Union
 
@@ -72,6 +73,7 @@ _SIGS = {
                         _I32),
     "nt_logits_process": ([_I32, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P, _I32] + [_P, _F32] * 3 +
                           [_P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P], _I32),
+    "nt_call_packed": ([_I32, ctypes.c_char_p, _I64], _I32),
 }
 
 EXPORTED = tuple(_SIGS)
@@ -117,25 +119,29 @@ def _stream(dev: torch.device) -> ctypes.c_void_p:
 _checked_devices = set()
 
 
-def _require_cuda(*ts: Optional[Tensor]) -> torch.device:
-    idx = first = None
+def _device_index(*ts: Optional[Tensor]) -> int:
+    """The CUDA device that all of `ts` are on."""
+    idx = None
     for t in ts:
-        if t is None:
-            continue
-        i = t.get_device()                        # -1 for a CPU tensor
-        if idx is None:
-            idx, first = i, t
-        if i != idx or not t.is_cuda:
-            if not t.is_cuda:
-                raise RuntimeError("neuratensor_b200 runs its hot path on CUDA (sm_100 / B200) only; "
-                                   f"got a tensor on {t.device}")
-            raise RuntimeError(f"tensors on different devices: {first.device} and {t.device}")
-    if first is None:
+        if t is not None:
+            i = t.get_device()                    # -1 for a CPU tensor
+            if i != idx:
+                if i < 0 or not t.is_cuda:
+                    raise RuntimeError("neuratensor_b200 runs its hot path on CUDA (sm_100 / B200) only; "
+                                       f"got a tensor on {t.device}")
+                if idx is not None:
+                    raise RuntimeError(f"tensors on different devices: cuda:{idx} and {t.device}")
+                idx = i
+    if idx is None:
         raise RuntimeError("no CUDA tensor given")
     if idx not in _checked_devices:
         _check("nt_device_supported", load().nt_device_supported(idx))
         _checked_devices.add(idx)
-    return first.device
+    return idx
+
+
+def _require_cuda(*ts: Optional[Tensor]) -> torch.device:
+    return torch.device("cuda", _device_index(*ts))
 
 
 def _dtype_code(t: Tensor) -> int:
@@ -460,19 +466,30 @@ def lm_head(x: Tensor, gamma: Tensor, W: Tensor, workspace: Optional[Tensor] = N
 #  cache, attention over it, penalties on logits                               #
 # --------------------------------------------------------------------------- #
 
-def _launch(dev: torch.device, name: str, *args) -> None:
-    """Calls a C entry point with `dev` current and its current stream as the last argument.
+# entry point -> (its number, number of arguments, packer) for nt_call_packed
+_PACKED = {"nt_rotary": (0, 21, struct.Struct("=8qd12q").pack), "nt_kv_append": (1, 25, struct.Struct("=25q").pack),
+           "nt_kv_attention": (2, 27, struct.Struct("=10qd16q").pack),
+           "nt_logits_process": (3, 27, struct.Struct("=11qqdqdqd10q").pack)}
 
-    These calls are short (a step makes several per layer), so the stream is read as the
-    raw handle and the device switched only when it has to be."""
-    fn = getattr(_lib, name)
-    if dev.index == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+
+def _launch(index: int, name: str, *args) -> None:
+    """Calls an entry point with device `index` current and its current stream as the last argument.
+
+    These calls are short (a step makes several per layer), so their arguments go over in
+    one piece, the stream is read as the raw handle and the device switched only when it has to be."""
+    entry, n, pack = _PACKED[name]
+    words = pack(*args, torch._C._cuda_getCurrentRawStream(index))
+    if index == torch._C._cuda_getDevice():
+        rc = _lib.nt_call_packed(entry, words, n)
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+        with torch.cuda.device(index):
+            rc = _lib.nt_call_packed(entry, words, n)
     if rc != 0:
         _check(name, rc)
+
+
+def _ptr(t: Optional[Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _like(t: Tensor) -> Tensor:
@@ -528,7 +545,7 @@ def rotary(x: Tensor, positions: Tensor, inv_freq: Tensor, layout: str = "half",
 
 
 def _rotary(x, positions, inv_freq, layout, mscale, inverse, out):
-    dev = _require_cuda(x, positions, inv_freq, out)
+    index = _device_index(x, positions, inv_freq, out)
     code = _dtype_code(x)
     if x.dim() != 4:
         raise ValueError(f"x must be [B, T, H, D], got {tuple(x.shape)}")
@@ -561,8 +578,9 @@ def _rotary(x, positions, inv_freq, layout, mscale, inverse, out):
     elif any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
         raise ValueError("out must not overlap itself")
     y_sb, y_st, y_sh, _ = out.stride()
-    _launch(dev, "nt_rotary", code, B, T, H, D, R, layout == "interleaved", inverse, mscale, x.data_ptr(), x_sb, x_st, x_sh,
-            positions.data_ptr(), p_sb, inv_freq.contiguous().data_ptr(), out.data_ptr(), y_sb, y_st, y_sh)
+    inv_freq = inv_freq.contiguous()
+    _launch(index, "nt_rotary", code, B, T, H, D, R, layout == "interleaved", inverse, mscale, x.data_ptr(), x_sb, x_st, x_sh,
+            positions.data_ptr(), p_sb, inv_freq.data_ptr(), out.data_ptr(), y_sb, y_st, y_sh)
     return out
 
 
@@ -609,7 +627,7 @@ def kv_append(k: Tensor, v: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: T
     sequence and stand once among its blocks; a bad length, count or page is skipped and
     flagged (device_error_flags)."""
     _refuse_grad("kv_append", k, v)
-    dev = _require_cuda(k, v, k_codes, k_scale, v_codes, v_scale, table, lengths, counts)
+    index = _device_index(k, v, k_codes, k_scale, v_codes, v_scale, table, lengths, counts)
     code = _dtype_code(k)
     if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError(f"k and v must be [B, T, H, D] of one dtype, got {tuple(k.shape)} {k.dtype} and "
@@ -627,9 +645,9 @@ def kv_append(k: Tensor, v: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: T
         v = v.contiguous()
     k_sb, k_st, k_sh, _ = k.stride()
     v_sb, v_st, v_sh, _ = v.stride()
-    _launch(dev, "nt_kv_append", code, B, T, H, D, P, n, blocks, k.data_ptr(), k_sb, k_st, k_sh, v.data_ptr(), v_sb, v_st,
+    _launch(index, "nt_kv_append", code, B, T, H, D, P, n, blocks, k.data_ptr(), k_sb, k_st, k_sh, v.data_ptr(), v_sb, v_st,
             v_sh, k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
-            table.stride(0), lengths.data_ptr(), None if counts is None else counts.data_ptr())
+            table.stride(0), lengths.data_ptr(), _ptr(counts))
 
 
 @functools.lru_cache(maxsize=256)
@@ -647,7 +665,7 @@ def kv_attention(q: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: Tensor, v
     window only those from position - window on.  Other rows are zero.  scale: of the
     scores, 1/sqrt(D) by default."""
     _refuse_grad("kv_attention", q)
-    dev = _require_cuda(q, k_codes, k_scale, v_codes, v_scale, table, lengths, counts)
+    index = _device_index(q, k_codes, k_scale, v_codes, v_scale, table, lengths, counts)
     code = _dtype_code(q)
     if q.dim() != 4:
         raise ValueError(f"q must be [B, T, H, D], got {tuple(q.shape)}")
@@ -665,20 +683,21 @@ def kv_attention(q: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: Tensor, v
     out = _like(q)
     nbytes = _kv_attention_bytes(B, T, Hq, H, D, P, blocks, win)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _launch(dev, "nt_kv_attention", code, B, T, Hq, H, D, P, n, blocks, win, 1.0 / math.sqrt(D) if scale is None else scale,
+    _launch(index, "nt_kv_attention", code, B, T, Hq, H, D, P, n, blocks, win, D ** -0.5 if scale is None else scale,
             q.data_ptr(), q_sb, q_st, q_sh, k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(),
-            table.data_ptr(), table.stride(0), lengths.data_ptr(), None if counts is None else counts.data_ptr(),
-            out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
+            table.data_ptr(), table.stride(0), lengths.data_ptr(), _ptr(counts), out.data_ptr(), _ptr(ws), nbytes)
     return out
 
 
-def _per_row(name: str, v, B: int, none: float) -> Tuple[Optional[Tensor], float]:
+def _per_row(name: str, v, B: int, none: float, index: int) -> Tuple[Optional[Tensor], float]:
     """A penalty as ([B] float32, unused) or (None, scalar)."""
     if v is None:
         return None, none
     if isinstance(v, Tensor):
         if v.shape != (B,):
             raise ValueError(f"{name} must be a number or [{B}], got {tuple(v.shape)}")
+        if v.get_device() != index:
+            raise RuntimeError(f"{name} must be on CUDA device {index}, got {v.device}")
         return _c(v, torch.float32), none
     return None, float(v)
 
@@ -700,8 +719,7 @@ def logits_process(logits: Tensor, tokens: Optional[Tensor] = None, lengths: Opt
     word v // 32 makes the logit -inf (pack_allowed).  float32 arithmetic, one rounding;
     out may be logits."""
     _refuse_grad("logits_process", logits, bias)
-    dev = _require_cuda(logits, tokens, lengths, prompt_lengths, bias_ids, bias, allowed, out,
-                        *(t for t in (repetition, frequency, presence) if isinstance(t, Tensor)))
+    index = _device_index(logits, tokens, lengths, prompt_lengths, bias_ids, bias, allowed, out)
     code = _dtype_code(logits)
     if logits.dim() != 2:
         raise ValueError(f"logits must be [B, V], got {tuple(logits.shape)}")
@@ -723,9 +741,9 @@ def logits_process(logits: Tensor, tokens: Optional[Tensor] = None, lengths: Opt
     prompt_lengths = _row_ints("logits_process", "prompt_lengths", prompt_lengths, B)
     if each and prompt_lengths is not None:
         raise ValueError("a repetition penalty per occurrence takes no prompt_lengths")
-    rep, rep_all = _per_row("repetition", repetition, B, 1.0)
-    fq, fq_all = _per_row("frequency", frequency, B, 0.0)
-    ps, ps_all = _per_row("presence", presence, B, 0.0)
+    rep, rep_all = _per_row("repetition", repetition, B, 1.0, index)
+    fq, fq_all = _per_row("frequency", frequency, B, 0.0, index)
+    ps, ps_all = _per_row("presence", presence, B, 0.0, index)
     if rep is None and not (rep_all > 0.0 and math.isfinite(rep_all)):
         raise ValueError(f"repetition must be above 0, got {rep_all}")
     NB = ids_ld = bias_ld = 0
@@ -756,12 +774,9 @@ def logits_process(logits: Tensor, tokens: Optional[Tensor] = None, lengths: Opt
     elif out.shape != logits.shape or out.dtype != logits.dtype or (V > 1 and out.stride(1) != 1) or \
             (B > 1 and out.stride(0) < V):
         raise ValueError("out must be [B, V] in the logits' dtype with unit column stride")
-    held = (tokens, lengths, prompt_lengths, rep, fq, ps, bias_ids, bias, allowed)      # until the launch
-    tokens, lengths, prompt_lengths, rep, fq, ps, bias_ids, bias, allowed = [
-        None if t is None else t.data_ptr() for t in held]
-    _launch(dev, "nt_logits_process", code, B, V, logits.data_ptr(), logits.stride(0), tokens, tok_ld, L, lengths,
-            prompt_lengths, each, rep, rep_all, fq, fq_all, ps, ps_all, bias_ids, ids_ld, bias, bias_ld, NB, allowed,
-            allowed_ld, out.data_ptr(), out.stride(0))
+    _launch(index, "nt_logits_process", code, B, V, logits.data_ptr(), logits.stride(0), _ptr(tokens), tok_ld, L,
+            _ptr(lengths), _ptr(prompt_lengths), each, _ptr(rep), rep_all, _ptr(fq), fq_all, _ptr(ps), ps_all,
+            _ptr(bias_ids), ids_ld, _ptr(bias), bias_ld, NB, _ptr(allowed), allowed_ld, out.data_ptr(), out.stride(0))
     return out
 
 

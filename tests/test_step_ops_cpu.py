@@ -115,3 +115,32 @@ def test_pack_allowed_words():
     assert words.dtype == torch.int32 and words.tolist() == [[-2 ** 31 + 1, 1, 32], [-1, -1, 63]]
     with pytest.raises(ValueError):
         native.pack_allowed(mask.int())
+
+
+def test_packed_calls_are_the_calls(nat):
+    """nt_call_packed reads the arguments in their order: the same refusals, by the argument that is wrong."""
+    L = nat.load()
+
+    def call(name, *args):
+        entry, n, pack = nat._PACKED[name]
+        words = pack(*args)
+        assert len(words) == 8 * n
+        return L.nt_call_packed(entry, words, n), L.nt_last_error().decode()
+
+    X = 4096
+    assert call("nt_rotary", 0, 1, 2, 3, 64, 63, 0, 0, 1.0, X, 1, 2, 3, X, 2, X, X, 1, 2, 3, 0) == (
+        1, "nt_rotary: rotated part 63 of 64 must be even, 2..D")
+    assert call("nt_rotary", 0, 1, 2, 3, 64, 64, 0, 0, 1.0, X, 1, 2, 3, X, 2, X, X, 1, 2, 4, 0)[1].endswith("equal strides")
+    assert call("nt_rotary", 0, 0, 2, 3, 64, 64, 0, 0, 1.0, *[0] * 12)[0] == 0
+    assert call("nt_kv_append", 1, 1, 1, 2, 64, 48, 4, 2, *[X] * 17)[1].startswith("nt_kv_append: page of 48 tokens")
+    assert call("nt_kv_append", 1, 1, 1, 2, 64, 16, 4, 2, X, 0, 0, 0, X, 0, 0, 0, X, X, X, 0, X, 2, X, 0, 0)[1].endswith("null pointer")
+    assert call("nt_kv_append", 1, 1, 0, 2, 64, 16, 4, 2, *[0] * 17)[0] == 0
+    args = (1, 1, 1, 32, 8, 128, 64, 4, 2048, -1, 1.0, X, 0, 0, 0, X, X, X, X, X, 2, X, 0, X)
+    need = L.nt_kv_attention_workspace_bytes(1, 1, 32, 8, 128, 64, 2048, -1)
+    assert call("nt_kv_attention", *args, X, need - 1, 0) == (6, f"nt_kv_attention: workspace {need - 1} < {need} bytes")
+    args = (0, 1, 100, X, 100, X, 5, 5, 0, 0, 0, 0, -0.5, 0, 0.0, 0, 0.0, 0, 0, 0, 0, 0, 0, 0, X, 101, 0)
+    assert call("nt_logits_process", *args)[1].endswith("in place needs equal row strides")
+    args = args[:-2] + (100, 0)
+    assert call("nt_logits_process", *args)[1].endswith("must be above 0")
+    for entry, words, n, text in ((4, b"", 0, "entry 4"), (-1, b"", 0, "entry -1"), (0, None, 21, "null"), (0, bytes(8), 1, "takes 21")):
+        assert L.nt_call_packed(entry, words, n) == 1 and text in L.nt_last_error().decode()
