@@ -676,7 +676,7 @@ def kv_attention(q: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: Tensor, v
         raise ValueError(f"kv_attention: {Hq} query heads over {H} cached heads")
     if window is not None and window < 0:
         raise ValueError(f"kv_attention: window must be None or >= 0, got {window}")
-    win = -1 if window is None else int(window)
+    win = -1 if window is None else min(int(window), 2 ** 31)      # as good as none from there on
     if q.stride(3) != 1:
         q = q.contiguous()
     q_sb, q_st, q_sh, _ = q.stride()
