@@ -6,14 +6,15 @@
 //
 // Bound by HBM: a step reads every visible code once (one byte per element)
 // and does two flops per query row with it.  Each warp streams its own tiles of
-// 16 keys through a ring in shared memory (16-byte cp.async, two tiles ahead of
-// the arithmetic, no barrier between warps), and the tensor cores (mma m16n8k16,
-// f16 in, float32 sums) do the products that would cost the CUDA cores a
-// conversion and an FMA per element.  The cached operand is the 16-row one of
+// 16 keys through a ring in shared memory (16-byte cp.async, one tile ahead of
+// the arithmetic, no barrier between warps; three stages take no less time, four
+// cost CTAs), and the tensor cores (mma m16n8k16, f16 in, float32 sums) do the
+// products that would cost the CUDA cores a conversion and an FMA per element.  The cached operand is the 16-row one of
 // each product (keys of K, then dimensions of V^T), the query rows of one cached
 // head the 8 columns: up to eight shared heads of a step, or a draft of a few
-// tokens.  e4m3 codes and bf16 queries are exact in f16; float32 queries and
-// weights are split into two f16 and take each product twice.
+// tokens.  e4m3 codes are exact in f16, and so is a bf16 query down to 2^-27 of its
+// largest value; float32 queries and weights are split into two f16 and take each
+// product twice.
 //
 // The k order of a product is free, so a lane takes 16 consecutive dimensions
 // of a key (one 16-byte read) as its part of four k-steps, with q in the same
@@ -23,9 +24,14 @@
 //
 // Softmax is online, in float32, base 2: a warp keeps its rows' running
 // maximum, sum and output over its tiles; the warps of a CTA join in shared
-// memory, and the CTAs that share a head in a second kernel, in a fixed order.  Probabilities are held as 2^14 p in f16 (11 bits;
-// small ones reach down to 2^-38 of the largest) for bf16 outputs, whose own
-// rounding is 2^-9, and as an f16 pair for float32.
+// memory, and the CTAs that share a head in a second kernel, in a fixed order.
+// Probabilities are held as 2^14 p in f16 (11 bits; small ones reach down to 2^-38
+// of the largest) for bf16 outputs, whose own rounding is 2^-8, and as an f16 pair
+// for float32.
+//
+// 64 streams, 16 bf16 heads of 128, window 512 (134 MB of codes): 30.7 us a call,
+// 20.6 at the measured copy rate and ~8 of launch, look-ups and joining; 8 ragged
+// caches of up to 65536 tokens, 32 over 8 heads: 5.8 TB/s.
 #include "nt_kernels.cuh"
 
 #include <cuda_fp16.h>
@@ -154,7 +160,7 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
 
     // This warp's tiles are first + warp + W * i, i < mine.  Lane j holds the
     // page and the scales of the j-th of 32 tiles: f_* for the tiles being
-    // fetched, c_* for those being computed, at most two behind.
+    // fetched, c_* for those being computed, one behind.
     const int mine = last - first > warp ? (last - first - warp + W - 1) / W : 0;
     const int32_t* table = a.table + b * a.table_sb;
     int f_page = -1, c_page = -1;
