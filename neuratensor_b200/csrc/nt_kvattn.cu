@@ -7,14 +7,14 @@
 // Bound by HBM: a step reads every visible code once (one byte per element)
 // and does two flops per query row with it.  Each warp streams its own tiles of
 // 16 keys through a ring in shared memory (16-byte cp.async, one tile ahead of
-// the arithmetic, no barrier between warps; three stages take no less time, four
-// cost CTAs), and the tensor cores (mma m16n8k16, f16 in, float32 sums) do the
-// products that would cost the CUDA cores a conversion and an FMA per element.  The cached operand is the 16-row one of
+// the arithmetic, no barrier between warps), and the tensor cores (mma m16n8k16,
+// f16 in, float32 sums) do the products that would cost the CUDA cores a
+// conversion and an FMA per element.  The cached operand is the 16-row one of
 // each product (keys of K, then dimensions of V^T), the query rows of one cached
 // head the 8 columns: up to eight shared heads of a step, or a draft of a few
-// tokens.  e4m3 codes are exact in f16, and so is a bf16 query down to 2^-27 of its
-// largest value; float32 queries and weights are split into two f16 and take each
-// product twice.
+// tokens.  e4m3 codes are exact in f16, and so is a bf16 query of at least 2^-30
+// of its row's largest (scaled to [2^13, 2^14), where f16 ends at 2^-24); float32
+// queries and weights are split into two f16 and take each product twice.
 //
 // The k order of a product is free, so a lane takes 16 consecutive dimensions
 // of a key (one 16-byte read) as its part of four k-steps, with q in the same
@@ -29,9 +29,10 @@
 // of the largest) for bf16 outputs, whose own rounding is 2^-8, and as an f16 pair
 // for float32.
 //
-// 64 streams, 16 bf16 heads of 128, window 512 (134 MB of codes): 30.7 us a call,
-// 20.6 at the measured copy rate and ~8 of launch, look-ups and joining; 8 ragged
-// caches of up to 65536 tokens, 32 over 8 heads: 5.8 TB/s.
+// The kernel alone, caches flushed, for 64 streams of 16 bf16 heads of 128 with
+// window 512 (134 MB of codes) / 8 ragged caches of up to 65536 tokens, 32 heads
+// over 8: 34.9 / 101.7 us with a ring of two tiles, 36.0 / 104.7 with three,
+// 43.5 / 125.5 with four (two ahead; 32 KB a CTA).
 #include "nt_kernels.cuh"
 
 #include <cuda_fp16.h>
