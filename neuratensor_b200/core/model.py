@@ -21,6 +21,7 @@ repetition penalty, all on the device (``native.logits_process``).
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Callable, Dict, List, Optional, Tuple, Union
 
@@ -194,6 +195,31 @@ class SlidingWindowAttention(nn.Module):
         else:
             o = F.scaled_dot_product_attention(q, k, v, attn_mask=self._window_mask(T, x.device))
         return self.o_proj(o.transpose(1, 2).reshape(B, T, self.d_model)) + x
+
+
+# the largest penalty or bias of `generate`: its sum over a history stays finite in bf16 too
+MAX_BIAS = 1e20
+
+
+def allowed_words(mask: Optional[Tensor], batch: int, vocab: int) -> Optional[Tensor]:
+    """A mask of the tokens that may come next as the words of ``native.pack_allowed``,
+    checked for a token in every row (one read of the device)."""
+    if mask is None:
+        return None
+    from .. import native
+    n = vocab if mask.dtype == torch.bool else (vocab + 31) // 32
+    if mask.dtype not in (torch.bool, torch.int32, torch.uint32) or mask.dim() != 2 or mask.shape[0] not in (1, batch) \
+            or mask.shape[1] < n:
+        raise ValueError(f"allowed must be boolean [{batch} or 1, {vocab}] or int32 words [{batch} or 1, {(vocab + 31) // 32}], "
+                         f"got {mask.dtype} {tuple(mask.shape)}")
+    words = native.pack_allowed(mask) if mask.dtype == torch.bool else mask
+    bits = words.view(torch.int32)
+    some = (bits[:, :vocab // 32] != 0).any(1)
+    if vocab % 32:
+        some = some | ((bits[:, vocab // 32] & ((1 << vocab % 32) - 1)) != 0)
+    if not bool(some.all()):
+        raise ValueError("allowed leaves no token for a sequence")
+    return words
 
 
 class NeuraTensorModel(nn.Module):
@@ -384,11 +410,26 @@ class NeuraTensorModel(nn.Module):
         generated token and for any; ``logit_bias`` maps token ids to what is added;
         ``allowed`` is a mask of the tokens that may come next, boolean [B or 1, vocab] or
         the int32 words of ``native.pack_allowed``, or a function of the tokens so far
-        that returns one (or None)."""
+        that returns one (or None).  Penalties and biases are finite (at most 1e20), and a
+        mask that leaves a sequence no token is refused; a function's is read for that at
+        every step."""
         from .. import native
         self.eval()
         out = input_ids
         B, prompt = out.shape
+        # what would leave a row without a finite largest logit is refused before anything runs:
+        # sampling from its probabilities, all NaN, fails on the device
+        for name, v in (("frequency_penalty", frequency_penalty), ("presence_penalty", presence_penalty)):
+            if not abs(v) <= MAX_BIAS:
+                raise ValueError(f"{name} must be at most {MAX_BIAS:g} in size, got {v}")
+        if not math.isfinite(repetition_penalty) or repetition_penalty == 0:
+            raise ValueError(f"repetition_penalty must be finite and not 0, got {repetition_penalty}")
+        for i, v in (logit_bias or {}).items():
+            if not 0 <= i < self.config.vocab_size:
+                raise ValueError(f"logit_bias names token {i} outside the vocabulary of {self.config.vocab_size}")
+            if not abs(v) <= MAX_BIAS:
+                raise ValueError(f"logit_bias must be at most {MAX_BIAS:g} in size, got {v} for token {i}")
+        fixed = None if callable(allowed) else allowed_words(allowed, B, self.config.vocab_size)
         stop = set(stop_tokens or [])
         want_graph = use_graph and out.is_cuda and max_new_tokens > 1
         graph = cache = None
@@ -411,12 +452,8 @@ class NeuraTensorModel(nn.Module):
         made = torch.full((B,), prompt, dtype=torch.int32, device=out.device) if frequency_penalty or presence_penalty else None
         bias_ids = bias = None
         if logit_bias:
-            if not all(0 <= i < self.config.vocab_size for i in logit_bias):
-                raise ValueError(f"logit_bias names tokens outside the vocabulary of {self.config.vocab_size}")
             bias_ids = torch.tensor([list(logit_bias)], dtype=torch.int64, device=out.device).expand(B, -1)
             bias = torch.tensor([list(logit_bias.values())], dtype=torch.float32, device=out.device).expand(B, -1)
-        words = lambda m: native.pack_allowed(m) if m is not None and m.dtype == torch.bool else m  # noqa: E731
-        fixed = None if callable(allowed) else words(allowed)
         # top_k = 1 without nucleus filtering leaves the tied row maxima with
         # equal probability: one kernel picks among them with a uniform drawn
         # here for every step at once (the other filters run as written)
@@ -427,7 +464,7 @@ class NeuraTensorModel(nn.Module):
             if repetition_penalty != 1.0:
                 # once per occurrence, as the reference's loop over out[b] does
                 native.logits_process(nxt_logits, tokens=out, repetition=repetition_penalty, each=True, out=nxt_logits)
-            mask = words(allowed(out)) if callable(allowed) else fixed
+            mask = allowed_words(allowed(out), B, self.config.vocab_size) if callable(allowed) else fixed
             if made is not None or bias is not None or mask is not None:
                 native.logits_process(nxt_logits, tokens=out if made is not None else None, prompt_lengths=made,
                                       frequency=frequency_penalty, presence=presence_penalty, bias_ids=bias_ids, bias=bias,
@@ -446,6 +483,9 @@ class NeuraTensorModel(nn.Module):
                 srt = srt.masked_fill(drop, float("-inf"))
                 nxt_logits = torch.zeros_like(nxt_logits).scatter_(-1, idx, srt)
             if not greedy:
+                # a penalty per occurrence can carry logits past the largest number
+                if repetition_penalty != 1.0 and not bool(nxt_logits.amax(-1).isfinite().all()):
+                    raise ValueError(f"repetition_penalty {repetition_penalty} leaves no finite logits to sample from")
                 tok = torch.multinomial(torch.softmax(nxt_logits, dim=-1), num_samples=1)
             out = torch.cat([out, tok], dim=1)
             if stop and tok.item() in stop:

@@ -31,6 +31,7 @@
 #include "nt_kernels.cuh"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace nt {
@@ -274,8 +275,11 @@ extern "C" int nt_logits_process(int dtype, int64_t B, int64_t V, const void* lo
     if (!logits || !out || (L > 0 && !tokens) || (NB > 0 && (!bias_ids || !bias)))
         return fail(NT_ERR_ARG, "nt_logits_process: null pointer");
     if (out == logits && ld != ldo) return fail(NT_ERR_ARG, "nt_logits_process: in place needs equal row strides");
+    if (!repetition && !each && !(repetition_all > 0.f))
+        return fail(NT_ERR_ARG, "nt_logits_process: repetition penalty must be above 0");
+    if (!repetition && each && (!std::isfinite(repetition_all) || repetition_all == 0.f))
+        return fail(NT_ERR_ARG, "nt_logits_process: a repetition penalty per occurrence must be finite and not 0");
     if (each && prompt_lengths) return fail(NT_ERR_ARG, "nt_logits_process: a penalty per occurrence takes no prompt lengths");
-    if (!repetition && !(repetition_all > 0.f)) return fail(NT_ERR_ARG, "nt_logits_process: repetition penalty must be above 0");
     LogArgs a{};
     a.V = V; a.x = logits; a.ld = ld;
     a.tokens = L > 0 ? tokens : nullptr; a.tok_ld = tok_ld; a.L = (int)L; a.lengths = lengths; a.prompts = prompt_lengths;

@@ -716,8 +716,9 @@ def logits_process(logits: Tensor, tokens: Optional[Tensor] = None, lengths: Opt
     taken off per occurrence and for any, counted from prompt_lengths[b] (None: 0) on.
     bias_ids [B, N] int64 and bias [B, N]: added to the logits of the ids (-1: none; of
     equal ids the last holds).  allowed: int32 words [B or 1, ceil(V / 32)]; a zero bit v % 32 of
-    word v // 32 makes the logit -inf (pack_allowed).  float32 arithmetic, one rounding;
-    out may be logits."""
+    word v // 32 makes the logit -inf (pack_allowed), all of a row without a bit: it has no
+    probabilities, so ask for them only where a token is left.  float32 arithmetic, one
+    rounding; out may be logits."""
     _refuse_grad("logits_process", logits, bias)
     index = _device_index(logits, tokens, lengths, prompt_lengths, bias_ids, bias, allowed, out)
     code = _dtype_code(logits)
@@ -744,8 +745,8 @@ def logits_process(logits: Tensor, tokens: Optional[Tensor] = None, lengths: Opt
     rep, rep_all = _per_row("repetition", repetition, B, 1.0, index)
     fq, fq_all = _per_row("frequency", frequency, B, 0.0, index)
     ps, ps_all = _per_row("presence", presence, B, 0.0, index)
-    if rep is None and not (rep_all > 0.0 and math.isfinite(rep_all)):
-        raise ValueError(f"repetition must be above 0, got {rep_all}")
+    if rep is None and not (math.isfinite(rep_all) and (rep_all > 0.0 or each and rep_all != 0.0)):
+        raise ValueError(f"repetition must be {'finite and not' if each else 'above'} 0, got {rep_all}")
     NB = ids_ld = bias_ld = 0
     if (bias_ids is None) != (bias is None):
         raise ValueError("bias_ids and bias go together")

@@ -226,3 +226,22 @@ def test_long_contexts_with_scaled_frequencies():
     want = m * rotate64(x, pos[None], parts.to(DEV))
     mag = m * (x.abs() + torch.cat([x[..., D // 2:], x[..., :D // 2]], -1).abs()).double()
     close(y, want, U32, 8 * U32 * mag)
+
+
+@pytest.mark.parametrize("top_k", [1, 50])
+def test_generate_refuses_a_step_without_tokens(top_k):
+    """A function whose mask runs empty at the third token: refused on the host, and the device goes on."""
+    from neuratensor_b200 import InferenceEngine, NeuraTensorModel, native
+    torch.manual_seed(12)
+    eng = InferenceEngine(NeuraTensorModel(config()), device=DEV, dtype=BF16)
+    ids = torch.randint(0, 1000, (2, 10))
+
+    def closing(tokens):
+        m = torch.ones(2, 1000, dtype=torch.bool, device=DEV)
+        m[1] = tokens.shape[1] < 12
+        return m
+
+    with pytest.raises(ValueError, match="leaves no token"):
+        eng.generate(ids, max_new_tokens=5, top_k=top_k, allowed=closing)
+    assert eng.generate(ids, max_new_tokens=2, top_k=top_k, allowed=closing).shape == (2, 12)
+    assert native.device_error_flags(0) == 0

@@ -1,5 +1,6 @@
 """Refusals of the generation-step entry points that need no GPU: a status and a message, never an abort."""
 import ctypes
+import math
 
 import pytest
 import torch
@@ -144,3 +145,57 @@ def test_packed_calls_are_the_calls(nat):
     assert call("nt_logits_process", *args)[1].endswith("must be above 0")
     for entry, words, n, text in ((4, b"", 0, "entry 4"), (-1, b"", 0, "entry -1"), (0, None, 21, "null"), (0, bytes(8), 1, "takes 21")):
         assert L.nt_call_packed(entry, words, n) == 1 and text in L.nt_last_error().decode()
+
+
+@pytest.mark.parametrize("more,text", [
+    (dict(allowed=torch.zeros(1, 70, dtype=torch.bool)), "leaves no token"),
+    (dict(allowed=torch.tensor([[True] * 70, [False] * 70])), "leaves no token"),            # of one sequence
+    (dict(allowed=torch.tensor([[0, 0, 1 << 6]], dtype=torch.int32)), "leaves no token"),    # a bit behind the vocabulary
+    (dict(allowed=torch.cat([torch.zeros(1, 70), torch.ones(1, 26)], 1).bool()), "leaves no token"),
+    (dict(allowed=torch.ones(1, 64, dtype=torch.bool)), "allowed must be"),
+    (dict(allowed=torch.ones(3, 70, dtype=torch.bool)), "allowed must be"),
+    (dict(allowed=torch.ones(1, 70)), "allowed must be"),
+    (dict(logit_bias={3: math.inf}), "logit_bias"),
+    (dict(logit_bias={3: -math.inf}), "logit_bias"),
+    (dict(logit_bias={3: math.nan}), "logit_bias"),
+    (dict(logit_bias={70: 1.0}), "logit_bias"),
+    (dict(logit_bias={-1: 1.0}), "logit_bias"),
+    (dict(frequency_penalty=math.nan), "frequency_penalty"),
+    (dict(frequency_penalty=-math.inf), "frequency_penalty"),
+    (dict(presence_penalty=math.inf), "presence_penalty"),
+    (dict(presence_penalty=1e21), "presence_penalty"),
+    (dict(repetition_penalty=0.0), "repetition_penalty"),
+    (dict(repetition_penalty=math.nan), "repetition_penalty"),
+])
+@pytest.mark.parametrize("top_k", [1, 50])
+def test_generate_refuses_what_cannot_be_sampled(more, text, top_k):
+    """Before anything runs: rows of logits without a finite largest value have no probabilities."""
+    from neuratensor_b200 import ModelConfig, NeuraTensorModel
+    model = NeuraTensorModel(ModelConfig(vocab_size=70, d_model=128, n_layers=2, d_state=16, max_seq_len=64, attn_every=2,
+                                         attn_heads=2, attn_window=8))
+    with pytest.raises(ValueError, match=text):
+        model.generate(torch.zeros(2, 3, dtype=torch.int64), max_new_tokens=2, top_k=top_k, **more)
+
+
+def test_allowed_words_of_a_step():
+    from neuratensor_b200.core.model import allowed_words
+    assert allowed_words(None, 2, 70) is None
+    last = torch.zeros(2, 70, dtype=torch.bool)
+    last[:, 69] = True
+    words = allowed_words(last, 2, 70)
+    assert words.tolist() == [[0, 0, 1 << 5]] * 2 and allowed_words(words, 2, 70) is words
+    top = torch.zeros(1, 64, dtype=torch.bool)
+    top[0, 63] = True                                        # the sign bit of a word
+    assert allowed_words(top, 2, 64).tolist() == [[0, -2 ** 31]]
+    with pytest.raises(ValueError, match="leaves no token"):
+        allowed_words(torch.zeros(2, 3, dtype=torch.int32), 2, 70)
+
+
+def test_repetition_per_occurrence_takes_what_the_loop_took(nat):
+    """v / r and v * r are defined for a negative r.  Every call has prompt lengths, which a penalty per
+    occurrence is refused for behind the check of r, so that none launches."""
+    L = nat.load()
+    for each, r, text in ((0, -1.5, "above 0"), (1, 0.0, "not 0"), (1, math.nan, "not 0"), (1, math.inf, "not 0"),
+                          (1, -1.5, "prompt lengths")):
+        assert logits(L, each=each, rep=r, prompts=FAKE) == 1
+        assert text in L.nt_last_error().decode()
