@@ -336,7 +336,8 @@ NT_API int nt_kv_attention(int dtype, int64_t B, int64_t T, int64_t Hq, int64_t 
  *   x = x + bias[b, j] for the last j with bias_ids[b, j] == v (int64, ids
  *       outside [0, V) are skipped)
  *   x = -inf where bit v % 32 of allowed[b, v / 32] is 0
- * in float32, one rounding to `dtype`; x/r is the product with float32 1/r.
+ * in float32, one rounding to `dtype`; x/r is the product with 1/r rounded to
+ * float32 (from the double when r is the scalar, as torch divides by a number).
  * Tokens outside [0, V) are skipped.  A penalty is a [B] float32 array, or the
  * scalar beside it when the pointer is NULL (1, 0, 0: none).  tokens, bias and
  * allowed may be NULL (L, NB 0).  allowed: uint32 words, row stride
@@ -344,7 +345,7 @@ NT_API int nt_kv_attention(int dtype, int64_t B, int64_t T, int64_t Hq, int64_t 
 NT_API int nt_logits_process(int dtype, int64_t B, int64_t V, const void* logits, int64_t ld,
                              const int64_t* tokens, int64_t tok_ld, int64_t L, const int32_t* lengths,
                              const int32_t* prompt_lengths, int each,
-                             const float* repetition, float repetition_all, const float* frequency,
+                             const float* repetition, double repetition_all, const float* frequency,
                              float frequency_all, const float* presence, float presence_all,
                              const int64_t* bias_ids, int64_t ids_ld, const float* bias, int64_t bias_ld, int64_t NB,
                              const uint32_t* allowed, int64_t allowed_ld, void* out, int64_t ldo, void* stream);

@@ -45,7 +45,7 @@ struct LogArgs {
     const int64_t* tokens; int64_t tok_ld; int L;
     const int32_t* lengths; const int32_t* prompts;
     const float* rep; const float* freq; const float* pres;
-    float rep_all, freq_all, pres_all;
+    float rep_all, rep_inv, freq_all, pres_all;   // rep_inv: 1 / rep_all, rounded from float64 as generate's loop has it
     const int64_t* ids; int64_t ids_ld; const float* bias; int64_t bias_ld; int NB;
     const uint32_t* allowed; int64_t allowed_ld;
     void* out; int64_t ldo;
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(kLogThreads, 5) logits_kernel(const __grid_con
     const float* bias = nullptr;
     if constexpr (COUNTED) {
         r = a.rep ? a.rep[b] : a.rep_all;
-        r_inv = 1.f / r;
+        r_inv = a.rep ? 1.f / r : a.rep_inv;
         fq = a.freq ? a.freq[b] : a.freq_all;
         ps = a.pres ? a.pres[b] : a.pres_all;
         if (a.NB) bias = a.bias + b * a.bias_ld;
@@ -264,7 +264,7 @@ using namespace nt;
 
 extern "C" int nt_logits_process(int dtype, int64_t B, int64_t V, const void* logits, int64_t ld, const int64_t* tokens,
                                  int64_t tok_ld, int64_t L, const int32_t* lengths, const int32_t* prompt_lengths, int each,
-                                 const float* repetition, float repetition_all, const float* frequency, float frequency_all,
+                                 const float* repetition, double repetition_all, const float* frequency, float frequency_all,
                                  const float* presence, float presence_all, const int64_t* bias_ids, int64_t ids_ld,
                                  const float* bias, int64_t bias_ld, int64_t NB, const uint32_t* allowed, int64_t allowed_ld,
                                  void* out, int64_t ldo, void* stream) {
@@ -275,16 +275,16 @@ extern "C" int nt_logits_process(int dtype, int64_t B, int64_t V, const void* lo
     if (!logits || !out || (L > 0 && !tokens) || (NB > 0 && (!bias_ids || !bias)))
         return fail(NT_ERR_ARG, "nt_logits_process: null pointer");
     if (out == logits && ld != ldo) return fail(NT_ERR_ARG, "nt_logits_process: in place needs equal row strides");
-    if (!repetition && !each && !(repetition_all > 0.f))
+    if (!repetition && !each && !(repetition_all > 0.0))
         return fail(NT_ERR_ARG, "nt_logits_process: repetition penalty must be above 0");
-    if (!repetition && each && (!std::isfinite(repetition_all) || repetition_all == 0.f))
+    if (!repetition && each && (!std::isfinite(repetition_all) || repetition_all == 0.0))
         return fail(NT_ERR_ARG, "nt_logits_process: a repetition penalty per occurrence must be finite and not 0");
     if (each && prompt_lengths) return fail(NT_ERR_ARG, "nt_logits_process: a penalty per occurrence takes no prompt lengths");
     LogArgs a{};
     a.V = V; a.x = logits; a.ld = ld;
     a.tokens = L > 0 ? tokens : nullptr; a.tok_ld = tok_ld; a.L = (int)L; a.lengths = lengths; a.prompts = prompt_lengths;
     a.rep = repetition; a.freq = frequency; a.pres = presence;
-    a.rep_all = repetition_all; a.freq_all = frequency_all; a.pres_all = presence_all;
+    a.rep_all = (float)repetition_all; a.rep_inv = (float)(1.0 / repetition_all); a.freq_all = frequency_all; a.pres_all = presence_all;
     a.ids = bias_ids; a.ids_ld = ids_ld; a.bias = bias; a.bias_ld = bias_ld; a.NB = (int)NB;
     a.allowed = allowed; a.allowed_ld = allowed_ld;
     a.out = out; a.ldo = ldo;

@@ -18,12 +18,13 @@ struct Words {
         p += 8;
         return v;
     }
-    float f() {
+    double d() {
         double v;
         memcpy(&v, p, 8);
         p += 8;
-        return (float)v;
+        return v;
     }
+    float f() { return (float)d(); }
     template <typename T> T* ptr() { return reinterpret_cast<T*>(static_cast<uintptr_t>(i())); }
 };
 
@@ -98,7 +99,7 @@ extern "C" int nt_call_packed(int entry, const void* words, int64_t n_words) {
     const int32_t* prompts = w.ptr<int32_t>();
     const int64_t each = w.i();
     const float* rep = w.ptr<float>();
-    const float rep_all = w.f();
+    const double rep_all = w.d();
     const float* freq = w.ptr<float>();
     const float freq_all = w.f();
     const float* pres = w.ptr<float>();

@@ -71,7 +71,7 @@ _SIGS = {
     "nt_kv_attention_workspace_bytes": ([_I64] * 8, _I64),
     "nt_kv_attention": ([_I32] + [_I64] * 9 + [_F32, _P, _I64, _I64, _I64] + [_P] * 5 + [_I64, _P, _P, _P, _P, _I64, _P],
                         _I32),
-    "nt_logits_process": ([_I32, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P, _I32] + [_P, _F32] * 3 +
+    "nt_logits_process": ([_I32, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P, _I32, _P, ctypes.c_double] + [_P, _F32] * 2 +
                           [_P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P], _I32),
     "nt_call_packed": ([_I32, ctypes.c_char_p, _I64], _I32),
 }

@@ -245,3 +245,32 @@ def test_generate_refuses_a_step_without_tokens(top_k):
         eng.generate(ids, max_new_tokens=5, top_k=top_k, allowed=closing)
     assert eng.generate(ids, max_new_tokens=2, top_k=top_k, allowed=closing).shape == (2, 12)
     assert native.device_error_flags(0) == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_negative_repetition_per_occurrence_is_the_loop(dtype):
+    from neuratensor_b200 import native
+    torch.manual_seed(13)
+    x = torch.randn(2, 50, device=DEV).to(dtype)
+    tokens = torch.randint(0, 50, (2, 120), device=DEV)
+    want, r = x.clone(), -1.07
+    for b in range(2):
+        for tok in tokens[b].tolist():
+            v = want[b, tok]
+            want[b, tok] = v / r if v > 0 else v * r
+    assert torch.equal(native.logits_process(x, tokens=tokens, repetition=r, each=True), want)
+
+
+@pytest.mark.parametrize("r", [1.05, 1.07, 1.1, 1.15, 1.3, 0.9])
+def test_repetition_per_occurrence_for_usual_penalties(r):
+    """Bit for bit the loop in float32, where 1 / r rounded from float64 is not 1 / float32(r) (not for the last two)."""
+    from neuratensor_b200 import native
+    torch.manual_seed(14)
+    x = torch.randn(2, 50, device=DEV)
+    tokens = torch.randint(0, 50, (2, 120), device=DEV)
+    want = x.clone()
+    for b in range(2):
+        for tok in tokens[b].tolist():
+            v = want[b, tok]
+            want[b, tok] = v / r if v > 0 else v * r
+    assert torch.equal(native.logits_process(x, tokens=tokens, repetition=r, each=True), want)
