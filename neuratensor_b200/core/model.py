@@ -418,7 +418,7 @@ class NeuraTensorModel(nn.Module):
         out = input_ids
         B, prompt = out.shape
         # what would leave a row without a finite largest logit is refused before anything runs:
-        # sampling from its probabilities, all NaN, fails on the device
+        # its probabilities are NaN, and there is nothing to sample
         for name, v in (("frequency_penalty", frequency_penalty), ("presence_penalty", presence_penalty)):
             if not abs(v) <= MAX_BIAS:
                 raise ValueError(f"{name} must be at most {MAX_BIAS:g} in size, got {v}")
