@@ -13,8 +13,9 @@
 // each product (keys of K, then dimensions of V^T), the query rows of one cached
 // head the 8 columns: up to eight shared heads of a step, or a draft of a few
 // tokens.  e4m3 codes are exact in f16, and so is a bf16 query of at least 2^-30
-// of its row's largest (scaled to [2^13, 2^14), where f16 ends at 2^-24); float32
-// queries and weights are split into two f16 and take each product twice.
+// of its row's largest (scaled to [2^13, 2^14), where f16 ends at 2^-24).  float32
+// queries, and the weights always, are split into two f16 (22 bits) and take
+// their product twice.
 //
 // The k order of a product is free, so a lane takes 16 consecutive dimensions
 // of a key (one 16-byte read) as its part of four k-steps, with q in the same
@@ -25,9 +26,13 @@
 // Softmax is online, in float32, base 2: a warp keeps its rows' running
 // maximum, sum and output over its tiles; the warps of a CTA join in shared
 // memory, and the CTAs that share a head in a second kernel, in a fixed order.
-// Probabilities are held as 2^14 p in f16 (11 bits; small ones reach down to 2^-38
-// of the largest) for bf16 outputs, whose own rounding is 2^-8, and as an f16 pair
-// for float32.
+// Probabilities are 2^14 p as a pair of f16, the second what the first leaves, for
+// bf16 outputs too, so that these are a float32 result rounded once (one f16, off
+// by 2^-12, changes one bf16 output in ten).  The second product hides behind the
+// codes' loads while a cached head has few query rows: between events, 39.0 us with
+// one f16 and with two for the 64 streams below, 138 and 140 for the ragged caches;
+// 8 tokens of 4 heads on each of 8 x 8 cached heads over up to 16384 keys: 107 to
+// 116 and 124.
 //
 // The kernel alone, caches flushed, for 64 streams of 16 bf16 heads of 128 with
 // window 512 (134 MB of codes) / 8 ragged caches of up to 65536 tokens, 32 heads
@@ -143,7 +148,7 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
     using T = typename El::T;
     constexpr int KS = D / 16;                 // k-steps of the first product
     constexpr int MT = D / 16;                 // 16-dimension tiles of the second
-    constexpr bool kPair = DT == NT_F32;       // a second product with what f16 leaves of q and of the weights
+    constexpr bool kPair = DT == NT_F32;       // a second product with what f16 leaves of q
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int row = row_tile * kRows + g, t = row / a.G;
     const bool live = t < s.cnt;
@@ -334,19 +339,11 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
             const float w00 = ex2(sc[0][0] - b0f) * fold, w01 = ex2(sc[0][1] - b1f) * fold;
             const float w10 = ex2(sc[1][0] - b0f) * fold, w11 = ex2(sc[1][1] - b1f) * fold;
             uint32_t pk0 = pack_h2(w00, w01), pk1 = pack_h2(w10, w11);
-            uint32_t bl0 = 0u, bl1 = 0u;
-            {
-                const float2 r0 = unpack_h2(pk0), r1 = unpack_h2(pk1);
-                if constexpr (kPair) {
-                    bl0 = transpose(pack_h2(w00 - r0.x, w01 - r0.y));
-                    bl1 = transpose(pack_h2(w10 - r1.x, w11 - r1.y));
-                    l0 = fmaf(w00 + w10, unfold, l0);
-                    l1 = fmaf(w01 + w11, unfold, l1);
-                } else {                                           // the weights that are used sum to one
-                    l0 = fmaf(r0.x + r1.x, unfold, l0);
-                    l1 = fmaf(r0.y + r1.y, unfold, l1);
-                }
-            }
+            const float2 rest0 = unpack_h2(pk0), rest1 = unpack_h2(pk1);
+            uint32_t bl0 = transpose(pack_h2(w00 - rest0.x, w01 - rest0.y));
+            uint32_t bl1 = transpose(pack_h2(w10 - rest1.x, w11 - rest1.y));
+            l0 = fmaf(w00 + w10, unfold, l0);
+            l1 = fmaf(w01 + w11, unfold, l1);
             uint32_t bh0 = transpose(pk0), bh1 = transpose(pk1);  // row g, keys 2c, 2c+1 and 2c+8, 2c+9
             uint32_t vw[4][D / 32];
             auto load_v = [&]() {
@@ -401,7 +398,7 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
                     uint32_t f[4];
                     v_tile(j, f);
                     mma_f16(o[j], f[0], f[1], f[2], f[3], bh0, bh1, o[j][0], o[j][1], o[j][2], o[j][3]);
-                    if constexpr (kPair) mma_f16(o[j], f[0], f[1], f[2], f[3], bl0, bl1, o[j][0], o[j][1], o[j][2], o[j][3]);
+                    mma_f16(o[j], f[0], f[1], f[2], f[3], bl0, bl1, o[j][0], o[j][1], o[j][2], o[j][3]);
                 }
             } else {
                 float f_out = plain ? 1.f : rel;
@@ -418,7 +415,7 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
                         float e[4];
                         v_tile(j, f);
                         mma_f16(e, f[0], f[1], f[2], f[3], bh0, bh1, 0.f, 0.f, 0.f, 0.f);
-                        if constexpr (kPair) mma_f16(e, f[0], f[1], f[2], f[3], bl0, bl1, e[0], e[1], e[2], e[3]);
+                        mma_f16(e, f[0], f[1], f[2], f[3], bl0, bl1, e[0], e[1], e[2], e[3]);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             o[j][k] = fmaf(f_out, e[k], o[j][k]);
