@@ -64,7 +64,7 @@ struct KvAttnArgs {
     const int32_t* table; int64_t table_sb;
     const int32_t* lengths; const int32_t* counts;
     void* out;
-    float* part;                       // partial rows: [kRows][D] sums, [kRows] maxima, [kRows] totals
+    float* part;                       // partial rows: [kRows][D] means, [kRows] maxima, [kRows] totals
     unsigned* err;
 };
 
@@ -139,8 +139,8 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 // Tiles [first, last) of one row tile of head h, sequence b, by the W warps of a
-// CTA: the rows themselves when these are all of its tiles, else unnormalised sums
-// with their maxima and totals in `part`.
+// CTA: the rows themselves when these are all of its tiles, else their means over
+// the tiles with their maxima and totals in `part`.
 template <int DT, int D, int W>
 __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, int row_tile, const Span& s, int first,
                                        int last, float* part, unsigned char* smem) {
@@ -450,16 +450,19 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
         l1 += __shfl_xor_sync(0xffffffffu, l1, k);
     }
 
-    // join the warps
-    __syncthreads();                                    // all rings are read: their memory takes the sums
+    // Join the warps.  A warp leaves the mean of the values that it saw, beside its
+    // maximum and total: a mean is no larger than the largest value, where a sum of
+    // cached values of 1e36 and more would pass float32's range.
+    const float r0 = l0 != 0.f ? 1.f / l0 : 0.f, r1 = l1 != 0.f ? 1.f / l1 : 0.f;
+    __syncthreads();                                    // all rings are read: their memory takes the means
     float (*so)[kRows][D] = reinterpret_cast<float (*)[kRows][D]>(smem);
     float (*sm)[kRows] = reinterpret_cast<float (*)[kRows]>(smem + sizeof(float) * W * kRows * D);
     float (*sl)[kRows] = sm + W;
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
         const int d = g * (D / 8) + 2 * j;
-        *reinterpret_cast<float2*>(&so[warp][2 * c][d]) = make_float2(o[j][0] * v_unit, o[j][2] * v_unit);
-        *reinterpret_cast<float2*>(&so[warp][2 * c + 1][d]) = make_float2(o[j][1] * v_unit, o[j][3] * v_unit);
+        *reinterpret_cast<float2*>(&so[warp][2 * c][d]) = make_float2(o[j][0] * r0 * v_unit, o[j][2] * r0 * v_unit);
+        *reinterpret_cast<float2*>(&so[warp][2 * c + 1][d]) = make_float2(o[j][1] * r1 * v_unit, o[j][3] * r1 * v_unit);
     }
     if (g == 0) {
         sm[warp][2 * c] = m0;
@@ -476,18 +479,19 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
 #pragma unroll
         for (int w = 0; w < W; ++w) mm = fmaxf(mm, sm[w][r]);
         const float base = mm == -INFINITY ? 0.f : mm;
-        float sum = 0.f, tot = 0.f;
+        float f[W], sum = 0.f, tot = 0.f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float f = ex2(sm[w][r] - base);
-            // a warp without keys holds zeros; a NaN row keeps its NaN
-            sum = fmaf(f, so[w][r][d], sum);
-            tot = fmaf(f, sl[w][r], tot);
+        for (int w = 0; w < W; ++w) {                   // a warp without keys holds zeros; a NaN row keeps its NaN
+            f[w] = ex2(sm[w][r] - base) * sl[w][r];
+            tot += f[w];
         }
+        const float inv = tot != 0.f ? 1.f / tot : 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) sum = fmaf(f[w] * inv, so[w][r][d], sum);
         if (alone) {
             const int rr = row_tile * kRows + r, tt = rr / a.G;
             T* out = static_cast<T*>(a.out) + ((b * a.T + tt) * (int64_t)(a.H * a.G) + h * a.G + rr % a.G) * D + d;
-            *out = El::from_f(tt < s.cnt && tot != 0.f ? sum / tot : 0.f);
+            *out = El::from_f(tt < s.cnt && tot != 0.f ? sum : 0.f);
         } else {
             part[i] = sum;
             if (d == 0) {
@@ -615,19 +619,29 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv_attention_join_kernel(cons
         return;
     }
     const int mr = kRows * D + r;                       // a partial row's maximum; its total kRows behind
-    float m = -INFINITY;
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, at(i)[mr]);
+    // the row's maximum and total: every warp takes them from all partial rows
+    float m = -INFINITY, tot = 0.f;
+    for (int i = lane; i < n; i += 32) {
+        const float mi = at(i)[mr], li = at(i)[mr + kRows], up = fmaxf(m, mi), base = up == -INFINITY ? 0.f : up;
+        tot = fmaf(ex2(mi - base), li, tot * ex2(m - base));
+        m = up;
+    }
 #pragma unroll
-    for (int k = 16; k; k /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+    for (int k = 16; k; k /= 2) {
+        const float mi = __shfl_xor_sync(0xffffffffu, m, k), li = __shfl_xor_sync(0xffffffffu, tot, k);
+        const float up = fmaxf(m, mi), base = up == -INFINITY ? 0.f : up;
+        tot = __fadd_rn(__fmul_rn(ex2(m - base), tot), __fmul_rn(ex2(mi - base), li));     // alike in every lane
+        m = up;
+    }
     const float base = m == -INFINITY ? 0.f : m;
-    float sum[E], tot = 0.f;
+    const float inv = tot != 0.f ? 1.f / tot : 0.f;
+    float sum[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = 0.f;
 #pragma unroll 8
     for (int i = warp; i < n; i += kJoinWarps) {
         const float* pi = at(i);
-        const float f = ex2(pi[mr] - base);
-        tot = fmaf(f, pi[mr + kRows], tot);
+        const float f = ex2(pi[mr] - base) * pi[mr + kRows] * inv;
         float v[E];
         if constexpr (E == 4) {
             const float4 q = *reinterpret_cast<const float4*>(pi + r * D + lane * E);
@@ -639,19 +653,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv_attention_join_kernel(cons
 #pragma unroll
         for (int e = 0; e < E; ++e) sum[e] = fmaf(f, v[e], sum[e]);
     }
-    __shared__ float ws[kJoinWarps][D], wt[kJoinWarps];
+    __shared__ float ws[kJoinWarps][D];
 #pragma unroll
     for (int e = 0; e < E; ++e) ws[warp][lane * E + e] = sum[e];
-    if (lane == 0) wt[warp] = tot;
     __syncthreads();
     for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) {
-        float x = 0.f, l = 0.f;
+        float x = 0.f;
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) {
-            x += ws[w][d];
-            l += wt[w];
-        }
-        static_cast<T*>(a.out)[((b * a.T + t) * (int64_t)heads + hq) * D + d] = El::from_f(t < s.cnt && l != 0.f ? x / l : 0.f);
+        for (int w = 0; w < kJoinWarps; ++w) x += ws[w][d];
+        static_cast<T*>(a.out)[((b * a.T + t) * (int64_t)heads + hq) * D + d] = El::from_f(t < s.cnt && tot != 0.f ? x : 0.f);
     }
 }
 

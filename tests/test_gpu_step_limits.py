@@ -29,3 +29,34 @@ def test_bf16_attention_is_float32_rounded_once(nat, T, G, D, P, lengths, window
     want, tol = attention64(q.float(), cache, table, lengths, [T] * B, window, P, scale=0.5)     # the bound of float32
     low, high = (want - tol).to(BF16).double(), (want + tol).to(BF16).double()
     assert ((o >= low) & (o <= high)).all(), f"{((o < low) | (o > high)).double().mean().item():.2g} of the outputs are outside"
+
+
+def large_cache(B, blocks, H, P, D, seed, code):
+    """Random finite codes, keys of about one, values of up to `code` times the pages' scales of 1."""
+    cache, table = make_cache(B, blocks, H, P, D, seed)
+    g = gen(seed + 1)
+    cache[0].copy_(torch.randn(cache[0].shape, device=DEV, generator=g).to(E4M3))
+    cache[2].copy_((code * (2 * torch.rand(cache[2].shape, device=DEV, generator=g) - 1)).to(E4M3))
+    cache[1].fill_(1.0)
+    cache[3].fill_(1.0)
+    return cache, table
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,T,H,G,D,P,lengths,window", [
+    (1, 1, 10, 1, 64, 16, [257], 256),                    # one CTA a head
+    (2, 1, 8, 4, 128, 64, [5000, 300], None),             # even shares
+    (2, 2, 3, 8, 64, 32, [2900, 1500], None)])            # chunks of row tiles
+def test_attention_over_the_largest_values(nat, dtype, B, T, H, G, D, P, lengths, window):  # noqa: F811
+    """The mean of values of up to 448 * 2^119, the last scale whose codes are all finite, is finite: every sum of
+    them on the way must be, too."""
+    cache, table = large_cache(B, -(-max(lengths) // P), H, P, D, 80, 448)
+    q = torch.randn(B, T, H * G, D, device=DEV, generator=gen(82)).to(dtype)
+    n = torch.tensor(lengths, device=DEV, dtype=torch.int32)
+    plain = nat.kv_attention(q, *cache, table, n, window=window)
+    want, tol = attention64(q, cache, table, lengths, [T] * B, window, P)
+    close(plain, want, half(dtype), tol)
+    for e in (100, 119):
+        cache[3].fill_(2.0 ** e)
+        o = nat.kv_attention(q, *cache, table, n, window=window)
+        assert torch.equal(o.double(), plain.double() * 2.0 ** e)      # a power of two on every value is one on the result
