@@ -13,7 +13,9 @@
 // each product (keys of K, then dimensions of V^T), the query rows of one cached
 // head the 8 columns: up to eight shared heads of a step, or a draft of a few
 // tokens.  e4m3 codes are exact in f16, and so is a bf16 query of at least 2^-30
-// of its row's largest (scaled to [2^13, 2^14), where f16 ends at 2^-24).  float32
+// of its row's largest (scaled to [2^13, 2^14), where f16 ends at 2^-24; rows whose
+// largest is below 2^-113 are scaled by 2^126, which brings every bf16 number into
+// f16).  float32
 // queries, and the weights always, are split into two f16 (22 bits) and take
 // their product twice.
 //
@@ -241,7 +243,7 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         int e = 127 + 13 - (int)(__float_as_uint(amax) >> 23);
-        e = amax > 0.f ? (e > 100 ? 100 : e) : 0;                       // >= -114
+        e = amax > 0.f ? (e > 126 ? 126 : e) : 0;                       // >= -114; 2^e and 2^-e are normal
         const float up = __uint_as_float((uint32_t)(127 + e) << 23);
         q_inv = __uint_as_float((uint32_t)(127 - e) << 23) * a.scale_log2;
 #pragma unroll

@@ -60,3 +60,32 @@ def test_attention_over_the_largest_values(nat, dtype, B, T, H, G, D, P, lengths
         cache[3].fill_(2.0 ** e)
         o = nat.kv_attention(q, *cache, table, n, window=window)
         assert torch.equal(o.double(), plain.double() * 2.0 ** e)      # a power of two on every value is one on the result
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("e", [-80, -100, -112, -120])
+def test_attention_of_the_smallest_queries(nat, dtype, e):  # noqa: F811
+    """Queries of 2^e with a scale of 2^-e have the scores of ordinary ones: a power of two on the query and its
+    inverse on the scale change no rounding while every number is normal."""
+    B, T, H, G, D, P, lengths = 2, 2, 2, 2, 64, 16, [100, 33]
+    cache, table = large_cache(B, 7, H, P, D, 85, 1)
+    q = torch.randn(B, T, H * G, D, device=DEV, generator=gen(86))
+    q = (torch.where(q.abs() < 2.0 ** -5, torch.zeros_like(q), q)).to(dtype)          # 2^-125 and above, or zero
+    n = torch.tensor(lengths, device=DEV, dtype=torch.int32)
+    want, tol = attention64(q, cache, table, lengths, [T] * B, None, P, scale=0.25)
+    plain = nat.kv_attention(q, *cache, table, n, scale=0.25)
+    close(plain, want, half(dtype), tol)
+    o = nat.kv_attention((q.double() * 2.0 ** e).to(dtype), *cache, table, n, scale=0.25 * 2.0 ** -e)
+    # q is split into f16 as before or, below 2^-113, from 2^7 on instead of 2^13: f16 still ends at 2^-31 of its largest
+    close(o, want, half(dtype), tol)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_of_subnormal_queries(nat, dtype):  # noqa: F811
+    B, T, H, G, D, P, lengths = 1, 1, 4, 1, 64, 16, [50]
+    cache, table = large_cache(B, 4, H, P, D, 87, 1)
+    q = (torch.randint(-100, 100, (B, T, H, D), device=DEV, generator=gen(88)).double() * 2.0 ** -133).to(dtype)
+    assert q.abs().max() > 0
+    n = torch.tensor(lengths, device=DEV, dtype=torch.int32)
+    want, tol = attention64(q, cache, table, lengths, [T], None, P, scale=2.0 ** 124)
+    close(nat.kv_attention(q, *cache, table, n, scale=2.0 ** 124), want, half(dtype), tol)
