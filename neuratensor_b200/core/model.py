@@ -65,8 +65,13 @@ class ModelConfig:
         return self.vocab_size * self.d_model + self.n_layers * block + self.n_attn_layers * attn + head
 
 
+def _stamp(t: Tensor) -> Tuple[int, int]:
+    """Tells a buffer's contents from later ones, for whoever holds the tensor as well (so that its id stays its own)."""
+    return id(t), 0 if t.is_inference() else t._version
+
+
 class RotaryEmbedding(nn.Module):
-    """Rotary position embedding tables (model.py:88-116)."""
+    """Rotary position embedding tables (model.py:88-116), rebuilt when ``inv_freq`` is replaced or written."""
 
     def __init__(self, dim: int, max_seq_len: int = 8192, base: float = 10000.0) -> None:
         super().__init__()
@@ -75,11 +80,21 @@ class RotaryEmbedding(nn.Module):
         self._max_cached = 0
         self.register_buffer("cos_cached", torch.empty(0), persistent=False)
         self.register_buffer("sin_cached", torch.empty(0), persistent=False)
+        self._made_from = (inv_freq, _stamp(inv_freq))      # what the tables hold the angles of
+
+    def _apply(self, fn, *args, **kw):
+        current = self._made_from[1] == _stamp(self.inv_freq)
+        super()._apply(fn, *args, **kw)
+        if current:                                         # moved or cast, the tables with it
+            self._made_from = (self.inv_freq, _stamp(self.inv_freq))
+        return self
 
     def _build_cache(self, seq_len: int, device, dtype) -> None:
-        if seq_len <= self._max_cached and self.cos_cached.dtype == dtype and self.cos_cached.device == device:
+        if seq_len <= self._max_cached and self.cos_cached.dtype == dtype and self.cos_cached.device == device \
+                and self._made_from[1] == _stamp(self.inv_freq):
             return
         self._max_cached = seq_len
+        self._made_from = (self.inv_freq, _stamp(self.inv_freq))
         pos = torch.arange(seq_len, device=device, dtype=torch.float32)
         ang = torch.outer(pos, self.inv_freq.to(device))
         ang = torch.cat([ang, ang], dim=-1)
@@ -152,11 +167,11 @@ class SlidingWindowAttention(nn.Module):
         from .. import native
         B, T, dm = x.shape
         H, hd = self.n_heads, self.head_dim
-        freq = getattr(self, "_rope_freq", None)
+        held = getattr(self, "_rope_freq", None)
         src = self.rope.inv_freq
-        if freq is None or freq[0] != (src.data_ptr(), src._version, x.device):
-            freq = self._rope_freq = ((src.data_ptr(), src._version, x.device), src.to(x.device, torch.float32))
-        freq = freq[1]
+        if held is None or held[0] != (_stamp(src), x.device):
+            held = self._rope_freq = ((_stamp(src), x.device), src, src.to(x.device, torch.float32))
+        freq = held[2]
         before = cache.filled - T                       # tokens of the sequences ahead of x
 
         def heads(a: int, b: int) -> Tensor:            # q | k | v heads [B, b - a, 3H, hd] of tokens a..b-1 of x
@@ -363,17 +378,24 @@ class NeuraTensorModel(nn.Module):
     def count_trainable_parameters(self) -> int:
         return sum(p.numel() for p in self.parameters() if p.requires_grad)
 
+    def _graph_signature(self, cache_tokens: int):
+        """What a captured forward reads besides its own buffers.  With an attention cache the layers rotate
+        by their frequencies (``forward_cached``), without one by their tables of them."""
+        layers = self.attn_layers.values()
+        return (tuple((p.data_ptr(), p._version) for p in self.parameters()),
+                tuple(_stamp(a.rope.inv_freq) for a in layers),
+                () if cache_tokens else tuple((a.rope.cos_cached.data_ptr(), a.rope.sin_cached.data_ptr()) for a in layers))
+
     @torch.no_grad()
     def step_graph(self, batch: int, seq: int, device, dtype, cache_tokens: int = 0):
         """The captured forward for this (batch, length) (``inference/decode.py``);
         with ``cache_tokens`` the graph has an attention cache of its own for that many
         tokens a sequence (``graph.attn_cache``).
         A graph holds raw addresses, so it is rebuilt when a parameter changes
-        (version or storage) or an attention layer's RoPE tables were rebuilt;
-        the four most recently used shapes are kept."""
+        (version or storage), an attention layer's frequencies do, or, where it reads
+        them, its RoPE tables were rebuilt; the four most recently used shapes are kept."""
         from ..inference.decode import StepGraph
-        sig = (tuple((p.data_ptr(), p._version) for p in self.parameters()),
-               tuple((a.rope.cos_cached.data_ptr(), a.rope.sin_cached.data_ptr()) for a in self.attn_layers.values()))
+        sig = self._graph_signature(cache_tokens)
         key = (batch, seq, str(device), dtype, cache_tokens)
         cache = self.__dict__.setdefault("_step_graphs", {})
         hit = cache.pop(key, None)
@@ -381,7 +403,8 @@ class NeuraTensorModel(nn.Module):
             hit = None
             while len(cache) >= 4:
                 cache.pop(next(iter(cache)))
-            hit = (sig, StepGraph(self, batch, seq, torch.device(device), dtype, cache_tokens))
+            graph = StepGraph(self, batch, seq, torch.device(device), dtype, cache_tokens)
+            hit = (self._graph_signature(cache_tokens), graph)      # its warm-up may have built the tables
         cache[key] = hit                          # most recently used last
         return hit[1]
 

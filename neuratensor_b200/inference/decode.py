@@ -16,8 +16,8 @@ a (batch, length) shape:
   captured region moves on; ``generate`` fills it from the prompt.
 
 The graph holds raw device addresses: it owns its workspace, and the model
-rebuilds it when a parameter changes or a RoPE table is rebuilt
-(``NeuraTensorModel.step_graph``).  Sampling stays eager on the logits.
+rebuilds it when a parameter or an attention layer's frequencies change or a RoPE
+table that it reads is rebuilt (``NeuraTensorModel.step_graph``).  Sampling stays eager on the logits.
 """
 from __future__ import annotations
 
@@ -56,6 +56,9 @@ class StepGraph:
         self.counts: Optional[Tensor] = None
         self.graph = torch.cuda.CUDAGraph()
         self._capture()
+        # the captured addresses outlive a rebuild of what they belong to
+        self.rotations = [(a.rope.inv_freq, a.rope.cos_cached, a.rope.sin_cached, getattr(a, "_rope_freq", None))
+                          for a in model.attn_layers.values()]
 
     def _states(self) -> List[BlockState]:
         return [BlockState(membrane=m, ssm_state=s) for m, s in zip(self.mem, self.st)]

@@ -1,0 +1,62 @@
+"""What the model keeps between calls of generate, without a GPU."""
+import copy
+
+import pytest
+import torch
+
+
+def config(**kw):
+    from neuratensor_b200 import ModelConfig
+    return ModelConfig(**{**dict(vocab_size=70, d_model=128, n_layers=4, d_state=16, max_seq_len=64, attn_every=2,
+                                 attn_heads=2, attn_window=8), **kw})
+
+
+@pytest.mark.parametrize("how", ["replaced", "written"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tables_follow_the_frequencies(how, dtype):
+    from neuratensor_b200 import RotaryEmbedding
+    rope, x = RotaryEmbedding(64), torch.zeros(1, 9, 64, dtype=dtype)
+    before = rope(x)[0]
+    assert rope(x)[0].data_ptr() == before.data_ptr()               # kept as long as nothing changes
+    f = rope.inv_freq / 8
+    if how == "replaced":
+        rope.inv_freq = f
+    else:
+        rope.inv_freq.copy_(f)
+    cos, sin = rope(x)
+    ang = torch.outer(torch.arange(9.0), f).repeat(1, 2)
+    assert torch.equal(cos, ang.cos().to(dtype)) and torch.equal(sin, ang.sin().to(dtype))
+    assert rope(x)[0].data_ptr() == cos.data_ptr()
+
+
+def test_moved_and_copied_tables_stay():
+    """A cast or a copy of the module takes its tables along, as it does for the reference's."""
+    from neuratensor_b200 import RotaryEmbedding
+    rope, x = RotaryEmbedding(64), torch.zeros(1, 9, 64, dtype=torch.bfloat16)
+    table = rope(x.float())[0]
+    other = copy.deepcopy(rope)
+    assert torch.equal(other(x.float())[0], table) and other._made_from[0] is other.inv_freq
+    rope = rope.to(torch.bfloat16)
+    assert torch.equal(rope(x)[0], table.to(torch.bfloat16))
+    rope.inv_freq.mul_(0.5)
+    assert not torch.equal(rope(x)[0], table.to(torch.bfloat16))
+
+
+def test_a_captured_step_is_told_of_new_frequencies():
+    """A captured step with an attention cache reads the frequencies, one without reads the tables."""
+    from neuratensor_b200 import NeuraTensorModel
+    model = NeuraTensorModel(config()).to(torch.bfloat16)
+    rope = next(iter(model.attn_layers.values())).rope
+    sig = model._graph_signature
+    x = torch.zeros(1, 9, 64, dtype=torch.bfloat16)
+    with_cache, without = sig(1024), sig(0)
+    rope(x)                                                         # tables, and longer ones
+    assert sig(1024) == with_cache and sig(0) != without
+    with_cache, without = sig(1024), sig(0)
+    rope(torch.zeros(1, 20, 64, dtype=torch.bfloat16))
+    assert sig(1024) == with_cache and sig(0) != without
+    for change in (lambda: rope.inv_freq.mul_(0.5), lambda: setattr(rope, "inv_freq", rope.inv_freq.clone())):
+        with_cache, without, kept = sig(1024), sig(0), rope.inv_freq
+        change()
+        assert sig(1024) != with_cache and sig(0) != without
+        del kept

@@ -1,0 +1,74 @@
+"""Generation with an attention memory, from call to call (B200)."""
+import pytest
+import torch
+
+from test_gpu_generate_memory import config
+from test_gpu_step_ops import BF16, DEV, E4M3, F32
+
+pytestmark = pytest.mark.gpu
+
+
+def steps(model, ids, tokens, graph):
+    """Logits of the prompt's last position and of each of `tokens` [n, B], with a memory, captured or not."""
+    from neuratensor_b200 import AttentionCache
+    dtype = model.lm_head.weight.dtype
+    with torch.no_grad():
+        if graph:
+            g = model.decode_graph(ids.shape[0], ids.device, dtype, 1024)
+            cache = g.attn_cache
+            cache.reset()
+        else:
+            cache = AttentionCache(model.config, ids.shape[0], 1024, DEV)
+        logits, states, _ = model.forward_device(ids, last_only=True, attn_cache=cache)
+        out = [logits[:, -1].clone()]
+        if graph:
+            g.load_states(states)
+        for tok in tokens:
+            if graph:
+                out.append(g.step(tok[:, None]).clone())
+            else:
+                logits, states, _ = model.forward_device(tok[:, None], states, attn_cache=cache)
+                out.append(logits[:, -1].clone())
+    return torch.stack(out)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("how", ["replaced", "written"])
+def test_captured_step_follows_the_frequencies(dtype, how):
+    """Frequencies that change between two calls are the ones of the next call, captured or not."""
+    from neuratensor_b200 import NeuraTensorModel, rotary_frequencies
+    torch.manual_seed(21)
+    model = NeuraTensorModel(config()).to(DEV).to(dtype).eval()
+    ids, tokens = torch.randint(0, 1000, (2, 25), device=DEV), torch.randint(0, 1000, (6, 2), device=DEV)
+    before = steps(model, ids, tokens, True)
+    assert torch.equal(before, steps(model, ids, tokens, False))
+    for factor in (4.0, 16.0):
+        f, _ = rotary_frequencies(64, scaling="linear", factor=factor, device=DEV)
+        for a in model.attn_layers.values():
+            if how == "replaced":
+                a.rope.inv_freq = f.clone()
+            else:
+                a.rope.inv_freq.copy_(f)
+        torch.cuda.empty_cache()
+        held = [torch.full((32,), 1e3, device=DEV) for _ in range(64)]          # whatever was freed is someone else's now
+        after = steps(model, ids, tokens, True)
+        assert torch.equal(after, steps(model, ids, tokens, False))
+        assert not torch.equal(after[1:], before[1:])
+        before = after
+        del held
+
+
+def test_a_longer_prompt_finds_the_same_captured_step():
+    """On a model without tables, too: the step that is captured for the first call serves the next ones."""
+    from neuratensor_b200 import NeuraTensorModel
+    torch.manual_seed(22)
+    model = NeuraTensorModel(config()).to(DEV).to(BF16).eval()
+    graphs = []
+    with torch.no_grad():
+        for prompt in (5, 130, 60):
+            ids = torch.randint(0, 1000, (2, prompt), device=DEV)
+            out = model.generate(ids, max_new_tokens=20, top_k=1, attn_cache=True)[0]
+            graphs.append(model.decode_graph(2, ids.device, BF16, 1024))
+            cold, _ = model.generate(ids, max_new_tokens=20, top_k=1, attn_cache=True, use_graph=False)
+            assert torch.equal(out, cold)
+    assert graphs[0] is graphs[1] is graphs[2]
