@@ -17,6 +17,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor
+from torch.autograd.graph import increment_version
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libneuratensor_native.so")
 
@@ -502,6 +503,13 @@ def _refuse_grad(fn: str, t: Tensor, u: Optional[Tensor] = None) -> None:
         raise RuntimeError(f"{fn} has no backward; detach the inputs or run under torch.no_grad()")
 
 
+def _refuse_out(fn: str, *ts: Tensor) -> None:
+    """What is written must not be part of a graph, as for torch's own out= and in-place operations."""
+    for t in ts:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{fn} writes a tensor that requires grad; detach it or run under torch.no_grad()")
+
+
 def _ints(t: Tensor, dtype: torch.dtype, what: str) -> Tensor:
     if t.dtype == dtype:
         return t
@@ -571,16 +579,21 @@ def _rotary(x, positions, inv_freq, layout, mscale, inverse, out):
     if unit != 1 and D > 1:
         x = x.contiguous()
         x_sb, x_st, x_sh, _ = x.stride()
-    if out is None:
+    given = out is not None
+    if not given:
         out = _like(x)
     elif out.shape != x.shape or out.dtype != x.dtype or out.stride(3) != 1:
         raise ValueError("out must have x's shape and dtype and unit stride in D")
     elif any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
         raise ValueError("out must not overlap itself")
+    else:
+        _refuse_out("rotary", out)
     y_sb, y_st, y_sh, _ = out.stride()
     inv_freq = inv_freq.contiguous()
     _launch(index, "nt_rotary", code, B, T, H, D, R, layout == "interleaved", inverse, mscale, x.data_ptr(), x_sb, x_st, x_sh,
             positions.data_ptr(), p_sb, inv_freq.data_ptr(), out.data_ptr(), y_sb, y_st, y_sh)
+    if given:
+        increment_version(out)          # so that a backward pass that saved it before knows
     return out
 
 
@@ -597,20 +610,22 @@ def _row_ints(fn: str, what: str, t: Optional[Tensor], B: int) -> Optional[Tenso
 
 def _cache_args(fn, B, D, k_codes, k_scale, v_codes, v_scale, table, lengths, counts):
     """Checks the tensors of a cache; returns (heads, page, pages, blocks, table, lengths, counts)."""
-    if k_codes.dim() != 4 or k_codes.shape != v_codes.shape or k_codes.shape[3] != D:
-        raise ValueError(f"{fn}: codes must be [pages, heads, page, {D}], got {tuple(k_codes.shape)} and "
-                         f"{tuple(v_codes.shape)}")
+    shape = k_codes.shape
+    if len(shape) != 4 or v_codes.shape != shape or shape[3] != D:
+        raise ValueError(f"{fn}: codes must be [pages, heads, page, {D}], got {tuple(shape)} and {tuple(v_codes.shape)}")
     for t in (k_codes, v_codes):
-        if t.dtype not in (torch.float8_e4m3fn, torch.uint8) or not t.is_contiguous():
+        dtype = t.dtype
+        if dtype != torch.float8_e4m3fn and dtype != torch.uint8 or not t.is_contiguous():
             raise ValueError(f"{fn}: codes must be contiguous float8_e4m3fn (or its bytes as uint8)")
-    n, H, P, _ = k_codes.shape
+    n, H, P, _ = shape
+    per_head = (n, H)
     for t in (k_scale, v_scale):
-        if t.dtype != torch.float32 or t.shape != (n, H) or not t.is_contiguous():
-            raise ValueError(f"{fn}: scales must be contiguous float32 [pages, heads] = {(n, H)}")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != B or (table.stride(1) != 1 and
-                                                                               table.shape[1] > 1):
+        if t.dtype != torch.float32 or t.shape != per_head or not t.is_contiguous():
+            raise ValueError(f"{fn}: scales must be contiguous float32 [pages, heads] = {per_head}")
+    entries = table.shape
+    if table.dtype != torch.int32 or len(entries) != 2 or entries[0] != B or (entries[1] > 1 and table.stride(1) != 1):
         raise ValueError(f"{fn}: table must be int32 [{B}, blocks] with unit stride")
-    return H, P, n, table.shape[1], _row_ints(fn, "lengths", lengths, B), _row_ints(fn, "counts", counts, B)
+    return H, P, n, entries[1], _row_ints(fn, "lengths", lengths, B), _row_ints(fn, "counts", counts, B)
 
 
 def kv_append(k: Tensor, v: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: Tensor, v_scale: Tensor, table: Tensor,
@@ -627,27 +642,32 @@ def kv_append(k: Tensor, v: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: T
     sequence and stand once among its blocks; a bad length, count or page is skipped and
     flagged (device_error_flags)."""
     _refuse_grad("kv_append", k, v)
+    _refuse_out("kv_append", k_codes, k_scale, v_codes, v_scale)
     index = _device_index(k, v, k_codes, k_scale, v_codes, v_scale, table, lengths, counts)
     code = _dtype_code(k)
-    if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype:
-        raise ValueError(f"k and v must be [B, T, H, D] of one dtype, got {tuple(k.shape)} {k.dtype} and "
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or v.dtype != k.dtype:
+        raise ValueError(f"k and v must be [B, T, H, D] of one dtype, got {tuple(shape)} {k.dtype} and "
                          f"{tuple(v.shape)} {v.dtype}")
-    B, T, H, D = k.shape
+    B, T, H, D = shape
     heads, P, n, blocks, lengths, counts = _cache_args("kv_append", B, D, k_codes, k_scale, v_codes, v_scale, table,
                                                        lengths, counts)
     if heads != H:
         raise ValueError(f"kv_append: the cache has {heads} heads, k and v have {H}")
     if k_codes.data_ptr() == v_codes.data_ptr() and n:
         raise ValueError("kv_append: keys and values need a cache each")
-    if k.stride(3) != 1:
+    k_sb, k_st, k_sh, unit = k.stride()
+    if unit != 1:
         k = k.contiguous()
-    if v.stride(3) != 1:
+        k_sb, k_st, k_sh, _ = k.stride()
+    v_sb, v_st, v_sh, unit = v.stride()
+    if unit != 1:
         v = v.contiguous()
-    k_sb, k_st, k_sh, _ = k.stride()
-    v_sb, v_st, v_sh, _ = v.stride()
+        v_sb, v_st, v_sh, _ = v.stride()
     _launch(index, "nt_kv_append", code, B, T, H, D, P, n, blocks, k.data_ptr(), k_sb, k_st, k_sh, v.data_ptr(), v_sb, v_st,
             v_sh, k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
             table.stride(0), lengths.data_ptr(), _ptr(counts))
+    increment_version((k_codes, k_scale, v_codes, v_scale))
 
 
 @functools.lru_cache(maxsize=256)
@@ -770,14 +790,19 @@ def logits_process(logits: Tensor, tokens: Optional[Tensor] = None, lengths: Opt
         if allowed.shape[1] > 1 and allowed.stride(1) != 1:
             allowed = allowed.contiguous()
         allowed_ld = allowed.stride(0) if allowed.shape[0] == B else 0
-    if out is None:
+    given = out is not None
+    if not given:
         out = _like(logits)
     elif out.shape != logits.shape or out.dtype != logits.dtype or (V > 1 and out.stride(1) != 1) or \
             (B > 1 and out.stride(0) < V):
         raise ValueError("out must be [B, V] in the logits' dtype with unit column stride")
+    else:
+        _refuse_out("logits_process", out)
     _launch(index, "nt_logits_process", code, B, V, logits.data_ptr(), logits.stride(0), _ptr(tokens), tok_ld, L,
             _ptr(lengths), _ptr(prompt_lengths), each, _ptr(rep), rep_all, _ptr(fq), fq_all, _ptr(ps), ps_all,
             _ptr(bias_ids), ids_ld, _ptr(bias), bias_ld, NB, _ptr(allowed), allowed_ld, out.data_ptr(), out.stride(0))
+    if given:
+        increment_version(out)
     return out
 
 
