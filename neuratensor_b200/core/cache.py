@@ -70,11 +70,19 @@ class AttentionCache:
         self.lengths.zero_()
         self.filled = 0
 
-    def move(self, tokens: int) -> None:
-        """Counts `tokens` more on the host (a replayed graph counts on the device itself)."""
+    def require_batch(self, batch: int) -> None:
+        if self.batch != batch:
+            raise ValueError(f"the attention cache is for {self.batch} sequences, got {batch}")
+
+    def require(self, tokens: int) -> None:
+        """Refuses `tokens` more where they do not fit."""
         if self.filled + tokens > self.max_tokens:
             raise ValueError(f"the attention cache holds {self.max_tokens} tokens a sequence; "
                              f"{self.filled} + {tokens} do not fit")
+
+    def move(self, tokens: int) -> None:
+        """Counts `tokens` more on the host (a replayed graph counts on the device itself)."""
+        self.require(tokens)
         self.filled += tokens
 
     def advance(self, tokens: int) -> None:

@@ -316,8 +316,7 @@ class NeuraTensorModel(nn.Module):
             input_ids = input_ids[:, : self.config.max_seq_len]
         B, T = input_ids.shape
         if attn_cache is not None:
-            if attn_cache.batch != B:
-                raise ValueError(f"the attention cache is for {attn_cache.batch} sequences, got {B}")
+            attn_cache.require_batch(B)
             attn_cache.advance(T)
         g = self.group_size(T)
         if B <= g:
@@ -428,7 +427,8 @@ class NeuraTensorModel(nn.Module):
 
         Beyond the reference: ``attn_cache`` lets the attention layers see their window
         of earlier tokens instead of the new one alone (True: for this call; an
-        ``AttentionCache`` carries on and is left behind the last token that was run);
+        ``AttentionCache`` carries on and is left behind the last token that was run; one
+        without room for the call is refused);
         ``frequency_penalty`` and ``presence_penalty`` are taken off per occurrence of a
         generated token and for any; ``logit_bias`` maps token ids to what is added;
         ``allowed`` is a mask of the tokens that may come next, boolean [B or 1, vocab] or
@@ -454,6 +454,10 @@ class NeuraTensorModel(nn.Module):
                 raise ValueError(f"logit_bias must be at most {MAX_BIAS:g} in size, got {v} for token {i}")
         fixed = None if callable(allowed) else allowed_words(allowed, B, self.config.vocab_size)
         stop = set(stop_tokens or [])
+        if isinstance(attn_cache, AttentionCache):
+            # a stop token may end the call at once, without one all tokens are run
+            attn_cache.require_batch(B)
+            attn_cache.require(min(prompt, self.config.max_seq_len) + (0 if stop else max_new_tokens))
         want_graph = use_graph and out.is_cuda and max_new_tokens > 1
         graph = cache = None
         if isinstance(attn_cache, AttentionCache):

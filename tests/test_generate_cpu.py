@@ -60,3 +60,23 @@ def test_a_captured_step_is_told_of_new_frequencies():
         change()
         assert sig(1024) != with_cache and sig(0) != without
         del kept
+
+
+def test_generate_refuses_a_cache_without_room():
+    """Before anything runs, and the cache stays where it was."""
+    from neuratensor_b200 import AttentionCache, NeuraTensorModel
+    model = NeuraTensorModel(config())
+    cache = AttentionCache(model.config, 2, 32, "cpu", page=16)
+    cache.filled = 20
+    ids = torch.zeros(2, 3, dtype=torch.int64)
+    for kw in (dict(max_new_tokens=10), dict(max_new_tokens=1000), dict(input_ids=torch.zeros(2, 13, dtype=torch.int64), stop_tokens=[1])):
+        with pytest.raises(ValueError, match="do not fit"):
+            model.generate(**{**dict(input_ids=ids, attn_cache=cache), **kw})
+    with pytest.raises(ValueError, match="for 2 sequences"):
+        model.generate(ids[:1], max_new_tokens=1, attn_cache=cache)
+    for kw in (dict(max_new_tokens=9), dict(max_new_tokens=1000, stop_tokens=[1]),        # 20 + 3 + 9 = 32; ends where it stops
+               dict(input_ids=torch.zeros(2, 100, dtype=torch.int64), max_new_tokens=1)):
+        with pytest.raises((RuntimeError, ValueError)) as e:                              # no GPU here, or 64 of 100 tokens that do not fit
+            model.generate(**{**dict(input_ids=ids, attn_cache=cache), **kw})
+        assert ("CUDA" in str(e.value)) == ("input_ids" not in kw)
+        cache.filled, cache.lengths = 20, cache.lengths * 0

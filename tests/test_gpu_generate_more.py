@@ -72,3 +72,29 @@ def test_a_longer_prompt_finds_the_same_captured_step():
             cold, _ = model.generate(ids, max_new_tokens=20, top_k=1, attn_cache=True, use_graph=False)
             assert torch.equal(out, cold)
     assert graphs[0] is graphs[1] is graphs[2]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_carried_cache_holds_what_one_sequence_would(dtype):
+    """Two calls on one cache against the same tokens run one after the other on a fresh one: codes, scales and
+    lengths are equal, and every greedy token has its row's largest logit."""
+    from neuratensor_b200 import AttentionCache, NeuraTensorModel
+    torch.manual_seed(23)
+    model = NeuraTensorModel(config()).to(DEV).to(dtype).eval()
+    ids, more = torch.randint(0, 1000, (2, 50), device=DEV), torch.randint(0, 1000, (2, 20), device=DEV)
+    carried, fresh = (AttentionCache(model.config, 2, 200, DEV, page=16) for _ in range(2))
+    with torch.no_grad():
+        first, states = model.generate(ids, max_new_tokens=30, top_k=1, attn_cache=carried)
+        second, _ = model.generate(more, max_new_tokens=7, top_k=1, attn_cache=carried, states=states)
+        assert first.shape == (2, 80) and second.shape == (2, 27)
+        states = None
+        for whole, prompt in ((first, 50), (second, 20)):
+            logits, states, _ = model.forward_device(whole[:, :prompt], states, last_only=True, attn_cache=fresh)
+            for t in range(prompt, whole.shape[1]):
+                row, tok = logits[:, -1], whole[:, t:t + 1]
+                assert torch.equal(row.gather(1, tok)[:, 0], row.amax(-1))
+                logits, states, _ = model.forward_device(tok, states, attn_cache=fresh)
+    assert carried.filled == fresh.filled == 107 and torch.equal(carried.lengths, fresh.lengths)
+    for a, b in zip(carried.layers.values(), fresh.layers.values()):
+        for p, q in zip(a, b):
+            assert torch.equal(p.view(torch.uint8), q.view(torch.uint8)) and (p.dtype == E4M3 or p.abs().max() > 0)
