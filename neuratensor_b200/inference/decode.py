@@ -51,7 +51,8 @@ class StepGraph:
         self.mem, self.st = self._split(self.flat)
         nbytes = native.block_workspace_bytes(dtype, batch, seq, cfg.d_model, di, cfg.d_state)
         self.ws = torch.empty(nbytes, dtype=torch.uint8, device=device)   # owned: the graph keeps its address
-        self.attn_cache = AttentionCache(cfg, batch, cache_tokens, device, max_step=max(seq, 1)) if cache_tokens else None
+        # a token more than asked for: what is captured stands behind one
+        self.attn_cache = AttentionCache(cfg, batch, cache_tokens + 1, device, max_step=max(seq, 1)) if cache_tokens else None
         self.logits: Optional[Tensor] = None
         self.counts: Optional[Tensor] = None
         self.graph = torch.cuda.CUDAGraph()
@@ -73,17 +74,22 @@ class StepGraph:
 
     def _capture(self) -> None:
         dev = self.tok.device
-        seq = self.tok.shape[1]
-        if self.attn_cache is not None:
-            # a step: tokens are ahead of it (zeros here, which reset() forgets)
-            self.attn_cache.advance(seq)
+
+        def stand():
+            # a token is ahead of the step (zeros here, forgotten below), so that it attends over the cache
+            if self.attn_cache is not None:
+                self.attn_cache.reset()
+                self.attn_cache.advance(1)
+
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(side), torch.no_grad():
             # warm-up outside the capture: weight caches, RoPE tables and each
             # kernel's one-time attributes are set up here
             for _ in range(2):
+                stand()
                 self._forward()
+            stand()
         torch.cuda.current_stream(dev).wait_stream(side)
         with torch.no_grad(), torch.cuda.graph(self.graph):
             self.logits, self.counts = self._forward()

@@ -98,3 +98,27 @@ def test_a_carried_cache_holds_what_one_sequence_would(dtype):
     for a, b in zip(carried.layers.values(), fresh.layers.values()):
         for p, q in zip(a, b):
             assert torch.equal(p.view(torch.uint8), q.view(torch.uint8)) and (p.dtype == E4M3 or p.abs().max() > 0)
+
+
+@pytest.mark.parametrize("prompt,seq,capacity", [(12, 20, 32), (16, 16, 32), (300, 200, 500)])
+def test_a_captured_chunk_may_fill_its_cache(prompt, seq, capacity):
+    """step_graph for chunks of several tokens: the capture itself takes no room, and a replay up to the last token
+    of the cache is the chunk launched kernel by kernel."""
+    from neuratensor_b200 import AttentionCache, NeuraTensorModel
+    torch.manual_seed(24)
+    model = NeuraTensorModel(config()).to(DEV).to(BF16).eval()
+    ids = torch.randint(0, 1000, (2, prompt + seq), device=DEV)
+    with torch.no_grad():
+        g = model.step_graph(2, seq, ids.device, BF16, cache_tokens=capacity)
+        cache = AttentionCache(model.config, 2, capacity + 1, DEV, max_step=seq)
+        out = []
+        for c in (g.attn_cache, cache):
+            _, states, _ = model.forward_device(ids[:, :prompt], attn_cache=c)
+            if c is cache:
+                out.append(model.forward_device(ids[:, prompt:], states, attn_cache=c)[0])
+            else:
+                g.load_states(states)
+                out.append(g.replay(ids[:, prompt:]).clone())
+        assert g.attn_cache.filled == prompt + seq
+    assert torch.equal(*out)
+    assert g.attn_cache.lengths.tolist() == [prompt + seq] * 2
