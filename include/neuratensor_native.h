@@ -27,6 +27,7 @@
  *   nt_block_forward       FusedSpikeBlock.forward     neuratensor/core/fused.py:101-147
  *   nt_window_attention    SlidingWindowAttention RoPE + SDPA neuratensor/core/model.py:148-178
  *   nt_attention_forward   SlidingWindowAttention.forward neuratensor/core/model.py:148-181
+ *   nt_attention_output    SlidingWindowAttention o_proj + residual neuratensor/core/model.py:180-181
  *   nt_embedding           NeuraTensorModel.embedding  neuratensor/core/model.py:258
  *   nt_lm_head             NeuraTensorModel.norm + lm_head neuratensor/core/model.py:283-284
  *   nt_greedy_tokens       top-k = 1 sampling in NeuraTensorModel.generate model.py:344-359
@@ -184,6 +185,12 @@ NT_API int nt_attention_forward(int dtype, int64_t B, int64_t T, int64_t dm, int
                                 const void* x, const void* norm_w, const void* W_qkv, const void* W_o,
                                 const void* cos_t, const void* sin_t, void* out,
                                 void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The end of nt_attention_forward for attention that was taken elsewhere
+ * (model.py:180-181): out = rnd(rnd(o W_o^T) + x).  o, x, out: [M, dm] in `dtype`;
+ * W_o: [dm, dm].  out may be x. */
+NT_API int nt_attention_output(int dtype, int64_t M, int64_t dm, const void* o, const void* W_o, const void* x,
+                               void* out, void* stream);
 
 /* Embedding gather -- NeuraTensorModel.embedding (model.py:258, nn.Embedding):
  * out[r, :] = W[ids[r], :] for r < M.  ids: [M] int64; W: [vocab, dm]; out:

@@ -195,7 +195,7 @@ class SlidingWindowAttention(nn.Module):
             cache.append(layer, qkv[:, :, H:2 * H], qkv[:, :, 2 * H:], lengths)
             out.append(cache.attend(layer, qkv[:, :, :H], lengths).view(B, b - a, dm))
         o = out[0] if len(out) == 1 else torch.cat(out, dim=1)
-        return F.linear(o, self.o_proj.weight.to(x.dtype)) + x
+        return native.attention_output(o, self.o_proj.weight, x)
 
     def forward_torch(self, x: Tensor) -> Tensor:
         """The reference's op sequence (fp32, CPU tensors, head dims other than 64 and 128)."""

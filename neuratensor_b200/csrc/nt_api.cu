@@ -545,11 +545,22 @@ int nt_attention_forward(int dtype, int64_t B, int64_t T, int64_t dm, int64_t n_
     // RoPE + windowed causal softmax attention (model.py:159-179)
     NT_TRY(nt_window_attention(dtype, B, T, n_heads, hd, window, qkv, 3 * dm, cos_t, sin_t, o, dm, stream));
     // o_proj + residual (model.py:180-181)
+    return nt_attention_output(dtype, M, dm, o, W_o, x, out, stream);
+}
+
+int nt_attention_output(int dtype, int64_t M, int64_t dm, const void* o, const void* W_o, const void* x, void* out,
+                        void* stream) {
+    if (!act_dtype_ok(dtype)) return fail(NT_ERR_DTYPE, "nt_attention_output: dtype %d", dtype);
+    if (M < 0 || dm < 1) return fail(NT_ERR_ARG, "nt_attention_output: bad sizes");
+    if (M == 0) return NT_OK;
+    if (!o || !W_o || !x || !out) return fail(NT_ERR_ARG, "nt_attention_output: null pointer");
+    NT_TRY(check_gemm_operand(o, dm, dtype, "nt_attention_output(o)"));
+    NT_TRY(check_gemm_operand(W_o, dm, dtype, "nt_attention_output(W_o)"));
     GemmArgs g{};
     g.M = M; g.N = dm; g.K = dm;
     g.A = o; g.lda = dm; g.Bw = W_o; g.ldb = dm;
     g.epi.kind = EPI_RESID; g.epi.out = out; g.epi.ldo = dm; g.epi.resid = x; g.epi.ldr = dm;
-    return launch_gemm(dtype, g, st);
+    return launch_gemm(dtype, g, as_stream(stream));
 }
 
 int nt_lif_ssm_fused(int64_t B, int64_t L, int64_t d, int64_t N, const void* x, const void* delta, const void* Bm,

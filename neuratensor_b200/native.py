@@ -65,6 +65,7 @@ _SIGS = {
     "nt_greedy_tokens": ([_I32, _I64, _I64, _P, _I64, _P, _P, _P], _I32),
     "nt_attention_workspace_bytes": ([_I32, _I64, _I64, _I64], _I64),
     "nt_attention_forward": ([_I32, _I64, _I64, _I64, _I64, _I64] + [_P] * 8 + [_I64, _P], _I32),
+    "nt_attention_output": ([_I32, _I64, _I64] + [_P] * 5, _I32),
     "nt_lm_head_workspace_bytes": ([_I32, _I64, _I64, _I64], _I64),
     "nt_lm_head": ([_I32, _I64, _I64, _I64, _P, _P, _P, _P, _P, _I64, _P], _I32),
     "nt_rotary": ([_I32, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _F32, _P, _I64, _I64, _I64, _P, _I64, _P, _P, _I64,
@@ -406,6 +407,21 @@ def attention_forward(x: Tensor, norm_w: Tensor, W_qkv: Tensor, W_o: Tensor, n_h
     rc = L.nt_attention_forward(_DT[x.dtype], B, T, dm, n_heads, int(window), _p(x), _p(nw), _p(Wq), _p(Wo),
                                 _p(cos), _p(sin), _p(out), _p(ws), ws.numel(), _stream(dev))
     _check("nt_attention_forward", rc)
+    return out
+
+
+def attention_output(o: Tensor, W_o: Tensor, x: Tensor) -> Tensor:
+    """o_proj + residual (model.py:180-181), the end of attention_forward for attention that
+    was taken elsewhere: o [..., d_model] @ W_o^T, rounded, + x in x.dtype."""
+    dev = _require_cuda(o, W_o, x)
+    if o.shape != x.shape or o.dtype != x.dtype or W_o.shape != (x.shape[-1], x.shape[-1]):
+        raise ValueError(f"o and x must be [..., d_model] of one dtype and W_o [d_model, d_model], got {tuple(o.shape)} "
+                         f"{o.dtype}, {tuple(x.shape)} {x.dtype} and {tuple(W_o.shape)}")
+    dm = x.shape[-1]
+    o, W, x = _c(o), _c(W_o, x.dtype), _c(x)
+    out = torch.empty_like(x)
+    rc = load().nt_attention_output(_dtype_code(x), x.numel() // dm, dm, _p(o), _p(W), _p(x), _p(out), _stream(dev))
+    _check("nt_attention_output", rc)
     return out
 
 

@@ -80,3 +80,25 @@ def test_generate_refuses_a_cache_without_room():
             model.generate(**{**dict(input_ids=ids, attn_cache=cache), **kw})
         assert ("CUDA" in str(e.value)) == ("input_ids" not in kw)
         cache.filled, cache.lengths = 20, cache.lengths * 0
+
+
+def test_attention_output_status():
+    """Statuses and messages of the entry point that need no GPU."""
+    import ctypes
+
+    from neuratensor_b200 import build, native
+    build.build()
+    L, X = native.load(), ctypes.c_void_p(4096)
+
+    def call(dtype=1, M=2, dm=64, o=X, W=X, x=X, out=X):
+        return L.nt_attention_output(dtype, M, dm, o, W, x, out, None), L.nt_last_error().decode()
+
+    assert call(M=0, o=None)[0] == 0
+    for bad, status, text in ((dict(dtype=2), 2, "dtype"), (dict(M=-1), 1, "sizes"), (dict(dm=0), 1, "sizes"),
+                              (dict(o=None), 1, "null"), (dict(W=None), 1, "null"), (dict(x=None), 1, "null"),
+                              (dict(out=None), 1, "null"), (dict(dm=60), 1, "multiple of 8"),
+                              (dict(o=ctypes.c_void_p(4104)), 1, "alignment")):
+        rc, said = call(**bad)
+        assert rc == status and text in said
+    with pytest.raises(RuntimeError, match="CUDA"):
+        native.attention_output(*[torch.zeros(64, 64)] * 3)

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from test_gpu_generate_memory import config
-from test_gpu_step_ops import BF16, DEV, E4M3, F32
+from test_gpu_step_ops import BF16, DEV, E4M3, F32, close
 
 pytestmark = pytest.mark.gpu
 
@@ -122,3 +122,41 @@ def test_a_captured_chunk_may_fill_its_cache(prompt, seq, capacity):
         assert g.attn_cache.filled == prompt + seq
     assert torch.equal(*out)
     assert g.attn_cache.lengths.tolist() == [prompt + seq] * 2
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,dm", [(1, 128), (8, 640), (64, 2048), (37, 256)])
+def test_attention_output_against_definition(dtype, M, dm):
+    from neuratensor_b200 import native
+    torch.manual_seed(25)
+    o, x = (torch.randn(M, dm, device=DEV).to(dtype) for _ in range(2))
+    W = (torch.randn(dm, dm, device=DEV) / dm ** 0.5).to(dtype)
+    acc = o.double() @ W.double().t()
+    terms = o.double().abs() @ W.double().abs().t()
+    y = native.attention_output(o, W, x)
+    # dm products summed in float32, one rounding to the type, the residual's sum rounded once more
+    u = torch.finfo(dtype).eps / 2
+    tol = dm * 2.0 ** -24 * terms + u * (acc.abs() + dm * 2.0 ** -24 * terms)
+    close(y, acc + x.double(), u, (1 + u) * tol)
+    part = native.attention_output(o.view(1, M, dm)[:, :1], W, x.view(1, M, dm)[:, :1])
+    assert part.shape == (1, 1, dm)
+    for bad in (dict(o=o[:, :64]), dict(x=x.double()), dict(W_o=W[:64])):
+        with pytest.raises(ValueError):
+            native.attention_output(**{**dict(o=o, W_o=W, x=x), **bad})
+
+
+def test_a_step_with_memory_calls_no_library_product():
+    """Eager and on the device: no matrix product of torch's runs in a layer with a memory."""
+    from neuratensor_b200 import AttentionCache
+    from neuratensor_b200.core.model import SlidingWindowAttention
+    attn = SlidingWindowAttention(128, 2, 40).to(DEV).to(BF16)
+    cache = AttentionCache(config(), 2, 60, DEV)
+    layer = next(iter(cache.layers))
+    with torch.no_grad():
+        cache.advance(9)
+        attn.forward_cached(torch.randn(2, 9, 128, device=DEV).to(BF16), cache, layer)
+        cache.advance(1)
+        x = torch.randn(2, 1, 128, device=DEV).to(BF16)
+        with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+            attn.forward_cached(x, cache, layer)
+    assert not {e.key for e in prof.key_averages()} & {"aten::linear", "aten::matmul", "aten::mm", "aten::addmm", "aten::bmm"}
