@@ -36,7 +36,7 @@
 // 8 tokens of 4 heads on each of 8 x 8 cached heads over up to 16384 keys: 107 to
 // 116 and 124.
 //
-// The kernel alone, caches flushed, for 64 streams of 16 bf16 heads of 128 with
+// The kernel alone with weights of one f16, caches flushed, for 64 streams of 16 bf16 heads of 128 with
 // window 512 (134 MB of codes) / 8 ragged caches of up to 65536 tokens, 32 heads
 // over 8: 34.9 / 101.7 us with a ring of two tiles, 36.0 / 104.7 with three,
 // 43.5 / 125.5 with four (two ahead; 32 KB a CTA).
@@ -677,8 +677,11 @@ Plan plan_of(int64_t B, int64_t T, int64_t G, int64_t H, int64_t D, int64_t page
     if (window >= 0) span = std::min(span, window + std::min<int64_t>(T, kRows) + kTile);
     const int64_t tiles = span / kTile + 1, base = B * H * pl.row_tiles;
     if (base <= 2 * 148 && tiles <= 72) {
-        // few short sequences: all warps of an SM on two of them, and no second launch
-        // (one sequence, 10 heads of 64, 257 keys: 6.1 us against 8.8 in chunks)
+        // few short sequences: all warps of an SM on two of them, and no second launch (kernels of
+        // one sequence, 10 heads of 64, 257 keys: 6.1 us against 8.8 in chunks).  The limit of 72
+        // tiles lies between few heads and many (us between events, eight warps : chunks, windows of
+        // 512, 1024, 1500 and 2048): 10 heads of 64 10.3 : 12.3, 14.3 : 12.3, 16.4 : 13.2, 18.4 : 14.4;
+        // 256 of 128 18.4 : 21.4, 24.6 : 28.7, 30.7 : 32.9, 36.9 : 41.0.
         pl.warps = 8;
         pl.chunk = (int)tiles;
         pl.splits = 1;
@@ -694,8 +697,12 @@ Plan plan_of(int64_t B, int64_t T, int64_t G, int64_t H, int64_t D, int64_t page
         return pl;
     } else {
         // CTAs of two warps: one wave of eight per SM where a window makes the sequences
-        // alike, half as many again, for a table's capacity, where they are ragged
-        // (24 drafts, window 1001: 8 14.5 us, 12 17.4 us)
+        // alike, half as many again, for a table's capacity, where they may be ragged.  Between
+        // events, us, 8 : 12.  Windows: 300 heads, 1000 30.8 : 34.8; 512 ragged, 1000 38.8 : 43.0;
+        // 64 ragged, 2048 20.5 : 23.5; drafts of 4 float32 tokens, 400 heads, 1000 28.7 : 32.9.
+        // None: 600 ragged of up to 4000 115.9 : 96.3; drafts of 8 tokens of 2 heads, 64 cached heads,
+        // ragged of up to 8192 47.1 : 44.9, all of 8192 59.4 : 67.7; 16 heads on each of 16, ragged of
+        // up to 16384 36.9 : 45.0.
         pl.warps = 2;
         const int64_t want = std::max<int64_t>(1, (window >= 0 ? 8 : 12) * 148 / std::max<int64_t>(1, base));
         pl.chunk = (int)std::max<int64_t>(2 * pl.warps, (tiles + want - 1) / want);

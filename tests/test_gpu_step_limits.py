@@ -89,3 +89,26 @@ def test_attention_of_subnormal_queries(nat, dtype):  # noqa: F811
     n = torch.tensor(lengths, device=DEV, dtype=torch.int32)
     want, tol = attention64(q, cache, table, lengths, [T], None, P, scale=2.0 ** 124)
     close(nat.kv_attention(q, *cache, table, n, scale=2.0 ** 124), want, half(dtype), tol)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,T,H,G,D,P,low,high,window", [
+    (3, 1, 2, 16, 64, 16, 100, 1500, None), (520, 1, 1, 1, 64, 16, 1, 1500, None), (150, 1, 2, 1, 64, 32, 900, 1500, 1000),
+    (2, 1, 3, 1, 128, 64, 1200, 1500, 1300), (3, 9, 2, 2, 64, 32, 60, 1500, None)])
+def test_attention_in_chunks_of_every_sequence_and_head(nat, dtype, B, T, H, G, D, P, low, high, window):  # noqa: F811
+    """Spans over several chunks, whose partial rows lie apart by sequence, head and row tile
+    (test_step_chunks_cpu.py checks that these sizes are split)."""
+    g = gen(90)
+    lengths = torch.randint(low, high + 1, (B,), device=DEV, generator=g)
+    lengths[-1] = high
+    cache, table = large_cache(B, -(-high // P), H, P, D, 91, 1)
+    scale = 2.0 ** torch.randint(-2, 3, cache[1].shape, device=DEV, generator=g).float()
+    cache[1].copy_(scale / 4)
+    cache[3].copy_(scale)
+    q = torch.randn(B, T, H * G, D, device=DEV, generator=g).to(dtype)
+    o = nat.kv_attention(q, *cache, table, lengths, window=window)
+    n = lengths.tolist()
+    want, tol = attention64(q, cache, table, n, [min(T, x) for x in n], window, P)
+    close(o, want, half(dtype), tol)
+    again = nat.kv_attention(q, *cache, table, lengths, window=window)
+    assert torch.equal(o, again)
