@@ -32,6 +32,7 @@ from torch import Tensor
 
 from .cache import AttentionCache
 from .fused import BlockState, FusedSpikeBlock, rate_like_reference
+from .rotary import Seen
 
 
 @dataclass
@@ -65,11 +66,6 @@ class ModelConfig:
         return self.vocab_size * self.d_model + self.n_layers * block + self.n_attn_layers * attn + head
 
 
-def _stamp(t: Tensor) -> Tuple[int, int]:
-    """Tells a buffer's contents from later ones, for whoever holds the tensor as well (so that its id stays its own)."""
-    return id(t), 0 if t.is_inference() else t._version
-
-
 class RotaryEmbedding(nn.Module):
     """Rotary position embedding tables (model.py:88-116), rebuilt when ``inv_freq`` is replaced or written."""
 
@@ -80,21 +76,21 @@ class RotaryEmbedding(nn.Module):
         self._max_cached = 0
         self.register_buffer("cos_cached", torch.empty(0), persistent=False)
         self.register_buffer("sin_cached", torch.empty(0), persistent=False)
-        self._made_from = (inv_freq, _stamp(inv_freq))      # what the tables hold the angles of
+        self._made_from = Seen(inv_freq)                   # what the tables hold the angles of
 
     def _apply(self, fn, *args, **kw):
-        current = self._made_from[1] == _stamp(self.inv_freq)
+        current = self._made_from.still(self.inv_freq)
         super()._apply(fn, *args, **kw)
         if current:                                         # moved or cast, the tables with it
-            self._made_from = (self.inv_freq, _stamp(self.inv_freq))
+            self._made_from = Seen(self.inv_freq)
         return self
 
     def _build_cache(self, seq_len: int, device, dtype) -> None:
         if seq_len <= self._max_cached and self.cos_cached.dtype == dtype and self.cos_cached.device == device \
-                and self._made_from[1] == _stamp(self.inv_freq):
+                and self._made_from.still(self.inv_freq):
             return
         self._max_cached = seq_len
-        self._made_from = (self.inv_freq, _stamp(self.inv_freq))
+        self._made_from = Seen(self.inv_freq)
         pos = torch.arange(seq_len, device=device, dtype=torch.float32)
         ang = torch.outer(pos, self.inv_freq.to(device))
         ang = torch.cat([ang, ang], dim=-1)
@@ -169,9 +165,9 @@ class SlidingWindowAttention(nn.Module):
         H, hd = self.n_heads, self.head_dim
         held = getattr(self, "_rope_freq", None)
         src = self.rope.inv_freq
-        if held is None or held[0] != (_stamp(src), x.device):
-            held = self._rope_freq = ((_stamp(src), x.device), src, src.to(x.device, torch.float32))
-        freq = held[2]
+        if held is None or not held[0].still(src) or held[1].device != x.device:
+            held = self._rope_freq = (Seen(src), src.to(x.device, torch.float32))
+        freq = held[1]
         before = cache.filled - T                       # tokens of the sequences ahead of x
 
         def heads(a: int, b: int) -> Tensor:            # q | k | v heads [B, b - a, 3H, hd] of tokens a..b-1 of x
@@ -378,11 +374,10 @@ class NeuraTensorModel(nn.Module):
         return sum(p.numel() for p in self.parameters() if p.requires_grad)
 
     def _graph_signature(self, cache_tokens: int):
-        """What a captured forward reads besides its own buffers.  With an attention cache the layers rotate
-        by their frequencies (``forward_cached``), without one by their tables of them."""
+        """What a captured forward reads besides its own buffers and its layers' frequencies.  With an attention
+        cache the layers rotate by those alone (``forward_cached``), without one by their tables of them."""
         layers = self.attn_layers.values()
         return (tuple((p.data_ptr(), p._version) for p in self.parameters()),
-                tuple(_stamp(a.rope.inv_freq) for a in layers),
                 () if cache_tokens else tuple((a.rope.cos_cached.data_ptr(), a.rope.sin_cached.data_ptr()) for a in layers))
 
     @torch.no_grad()
@@ -398,7 +393,7 @@ class NeuraTensorModel(nn.Module):
         key = (batch, seq, str(device), dtype, cache_tokens)
         cache = self.__dict__.setdefault("_step_graphs", {})
         hit = cache.pop(key, None)
-        if hit is None or hit[0] != sig:
+        if hit is None or hit[0] != sig or not hit[1].frequencies_hold():
             hit = None
             while len(cache) >= 4:
                 cache.pop(next(iter(cache)))

@@ -13,6 +13,21 @@ import torch
 from torch import Tensor
 
 
+class Seen:
+    """A buffer as it was: held, so that no other tensor can take its place unnoticed, with its version."""
+
+    def __init__(self, t: Tensor) -> None:
+        self.tensor, self.version = t, self._version(t)
+
+    @staticmethod
+    def _version(t: Tensor) -> int:
+        return 0 if t.is_inference() else t._version
+
+    def still(self, t: Tensor) -> bool:
+        """Whether `t` is the buffer, unwritten since."""
+        return t is self.tensor and self._version(t) == self.version
+
+
 def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
                        trained_len: int = 2048, fast: float = 32.0, slow: float = 1.0,
                        device=None) -> Tuple[Tensor, float]:

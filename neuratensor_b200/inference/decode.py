@@ -28,6 +28,7 @@ from torch import Tensor
 
 from ..core.cache import AttentionCache
 from ..core.fused import BlockState
+from ..core.rotary import Seen
 
 
 class StepGraph:
@@ -57,9 +58,14 @@ class StepGraph:
         self.counts: Optional[Tensor] = None
         self.graph = torch.cuda.CUDAGraph()
         self._capture()
-        # the captured addresses outlive a rebuild of what they belong to
-        self.rotations = [(a.rope.inv_freq, a.rope.cos_cached, a.rope.sin_cached, getattr(a, "_rope_freq", None))
-                          for a in model.attn_layers.values()]
+        # the frequencies as captured; and the captured addresses outlive a rebuild of what they belong to
+        layers = model.attn_layers.values()
+        self.frequencies = [Seen(a.rope.inv_freq) for a in layers]
+        self.held = [(a.rope.cos_cached, a.rope.sin_cached, getattr(a, "_rope_freq", None)) for a in layers]
+
+    def frequencies_hold(self) -> bool:
+        """Whether every attention layer still has the frequencies that were captured."""
+        return all(f.still(a.rope.inv_freq) for f, a in zip(self.frequencies, self.model.attn_layers.values()))
 
     def _states(self) -> List[BlockState]:
         return [BlockState(membrane=m, ssm_state=s) for m, s in zip(self.mem, self.st)]

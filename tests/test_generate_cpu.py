@@ -35,7 +35,7 @@ def test_moved_and_copied_tables_stay():
     rope, x = RotaryEmbedding(64), torch.zeros(1, 9, 64, dtype=torch.bfloat16)
     table = rope(x.float())[0]
     other = copy.deepcopy(rope)
-    assert torch.equal(other(x.float())[0], table) and other._made_from[0] is other.inv_freq
+    assert torch.equal(other(x.float())[0], table)
     rope = rope.to(torch.bfloat16)
     assert torch.equal(rope(x)[0], table.to(torch.bfloat16))
     rope.inv_freq.mul_(0.5)
@@ -43,23 +43,36 @@ def test_moved_and_copied_tables_stay():
 
 
 def test_a_captured_step_is_told_of_new_frequencies():
-    """A captured step with an attention cache reads the frequencies, one without reads the tables."""
+    """A captured step holds the frequencies that it was captured with; only one without a cache reads the tables."""
     from neuratensor_b200 import NeuraTensorModel
+    from neuratensor_b200.core.rotary import Seen
+    from neuratensor_b200.inference.decode import StepGraph
     model = NeuraTensorModel(config()).to(torch.bfloat16)
-    rope = next(iter(model.attn_layers.values())).rope
-    sig = model._graph_signature
-    x = torch.zeros(1, 9, 64, dtype=torch.bfloat16)
-    with_cache, without = sig(1024), sig(0)
-    rope(x)                                                         # tables, and longer ones
-    assert sig(1024) == with_cache and sig(0) != without
-    with_cache, without = sig(1024), sig(0)
-    rope(torch.zeros(1, 20, 64, dtype=torch.bfloat16))
-    assert sig(1024) == with_cache and sig(0) != without
+    step = object.__new__(StepGraph)                                # as one is behind its capture
+    step.model, step.frequencies = model, [Seen(a.rope.inv_freq) for a in model.attn_layers.values()]
+    rope = list(model.attn_layers.values())[-1].rope
+    for T in (9, 20):                                               # tables, and longer ones
+        with_cache, without = model._graph_signature(1024), model._graph_signature(0)
+        rope(torch.zeros(1, T, 64, dtype=torch.bfloat16))
+        assert model._graph_signature(1024) == with_cache and model._graph_signature(0) != without
+        assert step.frequencies_hold()
     for change in (lambda: rope.inv_freq.mul_(0.5), lambda: setattr(rope, "inv_freq", rope.inv_freq.clone())):
-        with_cache, without, kept = sig(1024), sig(0), rope.inv_freq
         change()
-        assert sig(1024) != with_cache and sig(0) != without
-        del kept
+        assert not step.frequencies_hold()
+        step.frequencies = [Seen(a.rope.inv_freq) for a in model.attn_layers.values()]
+        assert step.frequencies_hold()
+
+
+def test_a_copied_model_does_not_go_by_the_original_buffers():
+    """What a copy keeps of its frequencies is its own: no later tensor can pass for the original's."""
+    from neuratensor_b200 import RotaryEmbedding
+    rope, x = RotaryEmbedding(64), torch.zeros(1, 9, 64)
+    rope(x)
+    other = copy.deepcopy(rope)
+    assert other._made_from.tensor is other.inv_freq and other._made_from.tensor is not rope.inv_freq
+    f = rope.inv_freq / 3
+    other.inv_freq = f
+    assert torch.equal(other(x)[0][1], torch.cat([f, f]).cos())
 
 
 def test_generate_refuses_a_cache_without_room():
