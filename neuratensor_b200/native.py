@@ -751,7 +751,6 @@ def _per_row(name: str, v, B: int, none: float, index: int) -> Tuple[Optional[Te
     if isinstance(v, Tensor):
         if v.shape != (B,):
             raise ValueError(f"{name} must be a number or [{B}], got {tuple(v.shape)}")
-        _refuse_grad(f"logits_process ({name})", v)
         if v.get_device() != index:
             raise RuntimeError(f"{name} must be on CUDA device {index}, got {v.device}")
         return _c(v, torch.float32), none
@@ -775,7 +774,6 @@ def logits_process(logits: Tensor, tokens: Optional[Tensor] = None, lengths: Opt
     word v // 32 makes the logit -inf (pack_allowed), all of a row without a bit: it has no
     probabilities, so ask for them only where a token is left.  float32 arithmetic, one
     rounding; out may be logits."""
-    _refuse_grad("logits_process", logits, bias)
     index = _device_index(logits, tokens, lengths, prompt_lengths, bias_ids, bias, allowed, out)
     code = _dtype_code(logits)
     if logits.dim() != 2:
@@ -801,6 +799,7 @@ def logits_process(logits: Tensor, tokens: Optional[Tensor] = None, lengths: Opt
     rep, rep_all = _per_row("repetition", repetition, B, 1.0, index)
     fq, fq_all = _per_row("frequency", frequency, B, 0.0, index)
     ps, ps_all = _per_row("presence", presence, B, 0.0, index)
+    _refuse_grad("logits_process", logits, bias, rep, fq, ps)
     if rep is None and not (math.isfinite(rep_all) and (rep_all > 0.0 or each and rep_all != 0.0)):
         raise ValueError(f"repetition must be {'finite and not' if each else 'above'} 0, got {rep_all}")
     NB = ids_ld = bias_ld = 0
