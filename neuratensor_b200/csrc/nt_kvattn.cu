@@ -30,13 +30,14 @@
 // memory, and the CTAs that share a head in a second kernel, in a fixed order.
 // Probabilities are 2^14 p as a pair of f16, the second what the first leaves, for
 // bf16 outputs too, so that these are a float32 result rounded once (one f16, off
-// by 2^-12, changes one bf16 output in ten).  The second product hides behind the
-// codes' loads while a cached head has few query rows: between events, 39.0 us with
-// one f16 and with two for the 64 streams below, 138 and 140 for the ragged caches;
-// 8 tokens of 4 heads on each of 8 x 8 cached heads over up to 16384 keys: 107 to
-// 116 and 124.
+// by 2^-12, changes one bf16 output in ten).  With four query rows of a cached head
+// or fewer (HALF) the first halves take columns 0..3 of the product and the second
+// ones columns 4..7, whose queries repeat the rows: the pair costs one select, and the
+// kernels below take what they took with one f16 (34.9 us, 103.2 against 103.0).
+// With more rows it is a second product (drafts of 5 rows 14.1 against 13.9 us; 107 to
+// 116 against 124 for 8 tokens of 4 heads on 8 x 8 cached heads of up to 16384 keys).
 //
-// The kernel alone with weights of one f16, caches flushed, for 64 streams of 16 bf16 heads of 128 with
+// The kernel alone, caches flushed, for 64 streams of 16 bf16 heads of 128 with
 // window 512 (134 MB of codes) / 8 ragged caches of up to 65536 tokens, 32 heads
 // over 8: 34.9 / 101.7 us with a ring of two tiles, 36.0 / 104.7 with three,
 // 43.5 / 125.5 with four (two ahead; 32 KB a CTA).
@@ -142,8 +143,9 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
 }
 // Tiles [first, last) of one row tile of head h, sequence b, by the W warps of a
 // CTA: the rows themselves when these are all of its tiles, else their means over
-// the tiles with their maxima and totals in `part`.
-template <int DT, int D, int W>
+// the tiles with their maxima and totals in `part`.  HALF: there are four rows or
+// fewer; columns 4..7 repeat them and take the weights' second halves.
+template <int DT, int D, int W, bool HALF>
 __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, int row_tile, const Span& s, int first,
                                        int last, float* part, unsigned char* smem) {
     using El = Elem<DT>;
@@ -152,10 +154,11 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
     constexpr int MT = D / 16;                 // 16-dimension tiles of the second
     constexpr bool kPair = DT == NT_F32;       // a second product with what f16 leaves of q
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int row = row_tile * kRows + g, t = row / a.G;
+    constexpr int kMask = HALF ? 3 : 7;
+    const int row = row_tile * kRows + (g & kMask), t = row / a.G;
     const bool live = t < s.cnt;
     // in the products a lane holds rows 2c and 2c + 1: their positions
-    const int t0 = (row_tile * kRows + 2 * c) / a.G, t1 = (row_tile * kRows + 2 * c + 1) / a.G;
+    const int t0 = (row_tile * kRows + ((2 * c) & kMask)) / a.G, t1 = (row_tile * kRows + ((2 * c + 1) & kMask)) / a.G;
     const int p0 = t0 < s.cnt ? s.start + t0 : -1, p1 = t1 < s.cnt ? s.start + t1 : -1;
     // every row of the CTA sees all of a tile when it lies in [all_lo, all_hi)
     const int all_hi = s.start + row_tile * kRows / a.G + 1, all_lo = a.window >= 0 ? s.hi - 1 - a.window : 0;
@@ -342,8 +345,17 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
             const float w10 = ex2(sc[1][0] - b0f) * fold, w11 = ex2(sc[1][1] - b1f) * fold;
             uint32_t pk0 = pack_h2(w00, w01), pk1 = pack_h2(w10, w11);
             const float2 rest0 = unpack_h2(pk0), rest1 = unpack_h2(pk1);
-            uint32_t bl0 = transpose(pack_h2(w00 - rest0.x, w01 - rest0.y));
-            uint32_t bl1 = transpose(pack_h2(w10 - rest1.x, w11 - rest1.y));
+            const uint32_t lo0 = pack_h2(w00 - rest0.x, w01 - rest0.y), lo1 = pack_h2(w10 - rest1.x, w11 - rest1.y);
+            uint32_t bl0 = 0u, bl1 = 0u;
+            if constexpr (HALF) {
+                if (c >= 2) {
+                    pk0 = lo0;
+                    pk1 = lo1;
+                }
+            } else {
+                bl0 = transpose(lo0);
+                bl1 = transpose(lo1);
+            }
             l0 = fmaf(w00 + w10, unfold, l0);
             l1 = fmaf(w01 + w11, unfold, l1);
             uint32_t bh0 = transpose(pk0), bh1 = transpose(pk1);  // row g, keys 2c, 2c+1 and 2c+8, 2c+9
@@ -400,7 +412,7 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
                     uint32_t f[4];
                     v_tile(j, f);
                     mma_f16(o[j], f[0], f[1], f[2], f[3], bh0, bh1, o[j][0], o[j][1], o[j][2], o[j][3]);
-                    mma_f16(o[j], f[0], f[1], f[2], f[3], bl0, bl1, o[j][0], o[j][1], o[j][2], o[j][3]);
+                    if constexpr (!HALF) mma_f16(o[j], f[0], f[1], f[2], f[3], bl0, bl1, o[j][0], o[j][1], o[j][2], o[j][3]);
                 }
             } else {
                 float f_out = plain ? 1.f : rel;
@@ -417,7 +429,7 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
                         float e[4];
                         v_tile(j, f);
                         mma_f16(e, f[0], f[1], f[2], f[3], bh0, bh1, 0.f, 0.f, 0.f, 0.f);
-                        mma_f16(e, f[0], f[1], f[2], f[3], bl0, bl1, e[0], e[1], e[2], e[3]);
+                        if constexpr (!HALF) mma_f16(e, f[0], f[1], f[2], f[3], bl0, bl1, e[0], e[1], e[2], e[3]);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             o[j][k] = fmaf(f_out, e[k], o[j][k]);
@@ -452,6 +464,12 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
         l1 += __shfl_xor_sync(0xffffffffu, l1, k);
     }
 
+    if constexpr (HALF) {
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[j][k] += __shfl_xor_sync(0xffffffffu, o[j][k], 2);
+    }
     // Join the warps.  A warp leaves the mean of the values that it saw, beside its
     // maximum and total: a mean is no larger than the largest value, where a sum of
     // cached values of 1e36 and more would pass float32's range.
@@ -462,6 +480,7 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
     float (*sl)[kRows] = sm + W;
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
+        if (HALF && c >= 2) break;
         const int d = g * (D / 8) + 2 * j;
         *reinterpret_cast<float2*>(&so[warp][2 * c][d]) = make_float2(o[j][0] * r0 * v_unit, o[j][2] * r0 * v_unit);
         *reinterpret_cast<float2*>(&so[warp][2 * c + 1][d]) = make_float2(o[j][1] * r1 * v_unit, o[j][3] * r1 * v_unit);
@@ -506,7 +525,7 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
 
 // W warps per CTA, 16 to an SM (128 registers a thread).  A CTA takes `chunk`
 // tiles of one row tile.
-template <int DT, int D, int W>
+template <int DT, int D, int W, bool HALF>
 __global__ void __launch_bounds__(W * 32, 16 / W) kv_attention_kernel(const __grid_constant__ KvAttnArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     const int split = blockIdx.x, h = blockIdx.y / a.row_tiles, row_tile = blockIdx.y % a.row_tiles;
@@ -516,7 +535,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) kv_attention_kernel(const __gr
     const int first = split * a.chunk, last = min(first + a.chunk, s.tiles);
     if (split > 0 && first >= s.tiles) return;
     float* part = a.part + ((b * gridDim.y + blockIdx.y) * a.splits + split) * (kRows * (D + 2));
-    attend<DT, D, W>(a, b, h, row_tile, s, first, last, part, smem);
+    attend<DT, D, W, HALF>(a, b, h, row_tile, s, first, last, part, smem);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
@@ -557,7 +576,7 @@ __device__ __forceinline__ int64_t share_of(int64_t total, int ctas) {
     return n > kEvenLeast ? n : kEvenLeast;
 }
 
-template <int DT, int D, int W>
+template <int DT, int D, int W, bool HALF>
 __global__ void __launch_bounds__(W * 32, 16 / W) kv_attention_even_kernel(const __grid_constant__ KvAttnArgs a, int B) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int before[kEvenBatch + 1];
@@ -571,7 +590,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) kv_attention_even_kernel(const
         const int64_t rel = at - (int64_t)before[b] * a.H;
         const int h = (int)(rel / s.tiles), first = (int)(rel - (int64_t)h * s.tiles);
         const int last = (int)(end - at < s.tiles - first ? first + (end - at) : s.tiles);
-        attend<DT, D, W>(a, b, h, 0, s, first, last, a.part + (2 * (int64_t)blockIdx.x + (at != begin)) * (kRows * (D + 2)), smem);
+        attend<DT, D, W, HALF>(a, b, h, 0, s, first, last, a.part + (2 * (int64_t)blockIdx.x + (at != begin)) * (kRows * (D + 2)), smem);
         at += last - first;
         __syncthreads();                                // the sums are read before the next ring is filled
     }
@@ -731,29 +750,36 @@ int launch_join(const KvAttnArgs& a, int64_t B, int ctas, cudaStream_t stream) {
     return check_launch("kv_attention_join_kernel");
 }
 
-template <int DT, int D, int W>
+template <int DT, int D, int W, bool HALF>
 int launch_kv_attention(const KvAttnArgs& a, int64_t B, int even, cudaStream_t stream) {
     const size_t smem = std::max(kRingBytes<D, W>, sizeof(float) * W * kRows * (D + 2));
     if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kv_attention_kernel<DT, D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const cudaError_t e = cudaFuncSetAttribute(kv_attention_kernel<DT, D, W, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return fail(NT_ERR_CUDA, "nt_kv_attention: %s", cudaGetErrorString(e));
     }
     if constexpr (W == 2) {
         if (even) {
-            kv_attention_even_kernel<DT, D, W><<<even, W * 32, smem, stream>>>(a, (int)B);
+            kv_attention_even_kernel<DT, D, W, HALF><<<even, W * 32, smem, stream>>>(a, (int)B);
             const int rc = check_launch("kv_attention_even_kernel");
             return rc != NT_OK ? rc : launch_join<DT, D, true>(a, B, even, stream);
         }
     }
     const dim3 grid((unsigned)a.splits, (unsigned)(a.H * a.row_tiles), (unsigned)B);
-    kv_attention_kernel<DT, D, W><<<grid, W * 32, smem, stream>>>(a);
+    kv_attention_kernel<DT, D, W, HALF><<<grid, W * 32, smem, stream>>>(a);
     const int rc = check_launch("kv_attention_kernel");
     return rc != NT_OK || a.splits == 1 ? rc : launch_join<DT, D, false>(a, B, 0, stream);
 }
 
+template <int DT, int D, bool HALF>
+int launch_warps(const KvAttnArgs& a, int64_t B, const Plan& pl, cudaStream_t stream) {
+    return pl.warps == 8 ? launch_kv_attention<DT, D, 8, HALF>(a, B, 0, stream)
+                         : launch_kv_attention<DT, D, 2, HALF>(a, B, pl.even, stream);
+}
+// HALF wherever it can be: us a call of the 8 ragged caches above 109 against 113, of the 64 streams
+// 30.7 against 31.4.
 template <int DT, int D>
 int launch_planned(const KvAttnArgs& a, int64_t B, const Plan& pl, cudaStream_t stream) {
-    return pl.warps == 8 ? launch_kv_attention<DT, D, 8>(a, B, 0, stream) : launch_kv_attention<DT, D, 2>(a, B, pl.even, stream);
+    return 2 * a.T * a.G <= kRows ? launch_warps<DT, D, true>(a, B, pl, stream) : launch_warps<DT, D, false>(a, B, pl, stream);
 }
 
 }  // namespace
