@@ -112,3 +112,36 @@ def test_attention_in_chunks_of_every_sequence_and_head(nat, dtype, B, T, H, G, 
     close(o, want, half(dtype), tol)
     again = nat.kv_attention(q, *cache, table, lengths, window=window)
     assert torch.equal(o, again)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,G", [(3, 1), (2, 2), (1, 4), (6, 1), (3, 2), (5, 3)])
+@pytest.mark.parametrize("window", [20, None])
+def test_a_nan_reaches_the_rows_that_see_it(nat, dtype, T, G, window):  # noqa: F811
+    """With the second halves of the weights in columns of their own (four rows or fewer) and as a second product;
+    over pages whose scales are 2^60 apart, which take a product of their own, too."""
+    P, D, H, n = 16, 64, 2, 100
+    for spread in (0, 60):
+        cache, table = large_cache(1, 7, H, P, D, 95, 1)
+        q = torch.randn(1, T, H * G, D, device=DEV, generator=gen(96)).to(dtype)
+        if spread:
+            cache[3][table[0, ::2].long()] = 2.0 ** -spread
+        lengths = torch.tensor([n], device=DEV, dtype=torch.int32)
+        want, tol = attention64(q, cache, table, [n], [T], window, P)
+        close(nat.kv_attention(q, *cache, table, lengths, window=window), want, half(dtype), tol)
+        for key in (99, 98, 97, 96, 81, 79, 78, 77, 40):
+            page, slot = int(table[0, key // P]), key % P
+            for side in (0, 2):
+                codes = cache[side].view(torch.uint8)
+                kept = codes[page, 0, slot].clone()
+                codes[page, 0, slot, 7] = 0x7f                       # one NaN, of head 0
+                o = nat.kv_attention(q, *cache, table, lengths, window=window)
+                codes[page, 0, slot] = kept
+                for t in range(T):
+                    p = n - T + t
+                    sees = key <= p and (window is None or key >= p - window)
+                    bad = torch.zeros(H * G, D, dtype=torch.bool, device=DEV)
+                    if sees:
+                        bad[:G, 7 if side else slice(None)] = True
+                    assert torch.equal(o[0, t].isnan(), bad)
+                    close(o[0, t][~bad], want[0, t][~bad], half(dtype), tol[0, t][~bad])
