@@ -188,7 +188,7 @@ NT_API int nt_attention_forward(int dtype, int64_t B, int64_t T, int64_t dm, int
 
 /* The end of nt_attention_forward for attention that was taken elsewhere
  * (model.py:180-181): out = rnd(rnd(o W_o^T) + x).  o, x, out: [M, dm] in `dtype`;
- * W_o: [dm, dm].  out may be x. */
+ * W_o: [dm, dm].  out must not overlap the inputs. */
 NT_API int nt_attention_output(int dtype, int64_t M, int64_t dm, const void* o, const void* W_o, const void* x,
                                void* out, void* stream);
 
