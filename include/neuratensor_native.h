@@ -357,12 +357,94 @@ NT_API int nt_logits_process(int dtype, int64_t B, int64_t V, const void* logits
                              const int64_t* bias_ids, int64_t ids_ld, const float* bias, int64_t bias_ld, int64_t NB,
                              const uint32_t* allowed, int64_t allowed_ld, void* out, int64_t ldo, void* stream);
 
-/* The four entry points above with their arguments in one array, for bindings
+/* A step of a beam search over the above (no counterpart in the reference, whose
+ * generate samples one continuation per prompt; model.py:301-370).
+ *
+ * nt_beam_select: the n best continuations of each of B items with K beams
+ * (K, n <= 64; B K <= 65535).  logits: [B*K, V] rows in `dtype`, row stride ld;
+ * scores: [B*K] float32, log-probabilities so far; finished (bytes, NULL: none)
+ * and lengths (int32, tokens made so far; NULL without a length penalty): [B*K].
+ * A live beam k offers every token v whose logit is not -inf, with
+ *   s = scores[k] + (x[k,v] - log sum_u exp x[k,u]);
+ * a finished one itself alone, with s = scores[k] and token `pad`.  A beam whose
+ * score or logarithm is not finite (a NaN or +inf among its logits, nothing but
+ * -inf) offers nothing.  Candidates rank by s / max(l, 1)^length_penalty, l =
+ * lengths + 1 for a live beam and lengths for a finished one, in float64 except
+ * for the sum of exponentials; a beam's own in the order of their logits; ties go
+ * to the lower beam, then the lower token.  out_scores float32, out_rows int32 (the
+ * row b K + k that a candidate goes on from), out_tokens int64: [B, n], best first;
+ * with stay != 0 (n == K) the best child of a beam stands in that beam's place and
+ * the others, best first, in the places left.  Where candidates run out: -inf, row
+ * b K + place % K, `pad`.
+ * Workspace: nt_beam_select_workspace_bytes(). */
+NT_API int64_t nt_beam_select_workspace_bytes(int dtype, int64_t B, int64_t K, int64_t V, int64_t n);
+NT_API int nt_beam_select(int dtype, int64_t B, int64_t K, int64_t V, int64_t n, const void* logits, int64_t ld,
+                          const float* scores, const unsigned char* finished, const int32_t* lengths,
+                          double length_penalty, int64_t pad, int stay,
+                          float* out_scores, int32_t* out_rows, int64_t* out_tokens,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Rows moved in place, for many tensors at once: row r of each takes what row
+ * rows[r] held (int32 [R]; -1: it stays as it is).  rows[r] lies in r's group of
+ * `group` <= 1024 consecutive rows, else the row stays and the bad-argument bit of the
+ * device error word is set.  tensors: host array [n_tensors][3] of device address, bytes
+ * of a row, bytes between rows; tensors do not overlap. */
+NT_API int nt_reorder_rows(int64_t n_tensors, const int64_t* tensors, int64_t R, int64_t group,
+                           const int32_t* rows, void* stream);
+
+/* Sequences over a shared pool of pages.  table (int32 [R, n_blocks], row stride
+ * table_sb, -1: no page), refs (int32 [n_pages]: how many table entries, and other
+ * holders, have a page; 0: free) and lengths (int32 [R], R <= 1024) are rewritten in
+ * place so that row r goes on from row parents[r] (-1: it ends, with length 0):
+ *  1. the row takes the parent's length n and its entries of the blocks that hold
+ *     positions [max(0, n - window), n) (window < 0: all); its other entries are -1,
+ *     and the counts follow;
+ *  2. of the rows whose last page is the same and not full, one keeps it when its
+ *     count is their number: the first that goes on from itself, else the first; every
+ *     other gets a new page, and copies[r] = (old page, new page), else (-1, -1);
+ *  3. the blocks of positions [n, n + tokens) behind get new pages, but those wholly
+ *     before n + tokens - window.
+ * New pages are the free pages of lowest index, row by row (2. before 3., blocks in
+ * order).  Where they run out, or the table ends, entries stay -1 and the bad-argument
+ * bit of the device error word is set, as for a bad parent (it ends), length or page.
+ * With group > 0 shared[g] (int32 [R / group]) is how many leading tokens, in whole
+ * blocks, the rows of group g have in the same pages. */
+NT_API int nt_kv_fork(int64_t R, int64_t n_pages, int64_t n_blocks, int64_t page, int64_t tokens, int64_t window,
+                      int64_t group, int32_t* table, int64_t table_sb, int32_t* refs, int32_t* lengths,
+                      const int32_t* parents, int32_t* copies, int32_t* shared, void* stream);
+
+/* Pages copied within their pools, codes and scales of keys and values of every
+ * layer: pages (int32 [n, 2]): from, to; (-1, -1) is skipped, a page outside
+ * [0, n_pages) too, with the bad-argument bit.  layers: host array [n_layers][4] of
+ * the device addresses of k codes, k scales, v codes, v scales (nt_kv_append).  No
+ * page is written twice, or read and written. */
+NT_API int nt_kv_copy_pages(int64_t n_layers, const int64_t* layers, int64_t n_pages, int64_t Hkv, int64_t page,
+                            int64_t D, int64_t n, const int32_t* pages, void* stream);
+
+/* nt_kv_attention for sequences that share their beginnings: the B sequences are
+ * `groups` groups of B / groups consecutive ones, and the first shared[g] (int32)
+ * positions of a group's sequences hold the same keys and values, in each one's own
+ * pages, which may be the same; they are read once for all of them, from one's pages.
+ * Results and everything else as nt_kv_attention; a bad shared[g] counts as 0 and
+ * sets the bad-argument bit.
+ * Workspace: nt_kv_attention_shared_workspace_bytes(). */
+NT_API int64_t nt_kv_attention_shared_workspace_bytes(int dtype, int64_t B, int64_t groups, int64_t T, int64_t Hq, int64_t Hkv,
+                                                      int64_t D, int64_t page, int64_t n_blocks, int64_t window);
+NT_API int nt_kv_attention_shared(int dtype, int64_t B, int64_t groups, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                  int64_t page, int64_t n_pages, int64_t n_blocks, int64_t window, float scale,
+                                  const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                                  const void* k_codes, const float* k_scale, const void* v_codes, const float* v_scale,
+                                  const int32_t* table, int64_t table_sb, const int32_t* lengths, const int32_t* counts,
+                                  const int32_t* shared, void* out, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The entry points of a generation step with their arguments in one array, for bindings
  * that pay for every argument they convert (a step makes several short calls
  * per layer): `words` holds the arguments in order, 8 bytes each, integers as
  * int64, pointers as their address, floats as double; n_words must be the entry
  * point's number of arguments. */
-enum { NT_ENTRY_ROTARY = 0, NT_ENTRY_KV_APPEND = 1, NT_ENTRY_KV_ATTENTION = 2, NT_ENTRY_LOGITS_PROCESS = 3 };
+enum { NT_ENTRY_ROTARY = 0, NT_ENTRY_KV_APPEND = 1, NT_ENTRY_KV_ATTENTION = 2, NT_ENTRY_LOGITS_PROCESS = 3,
+       NT_ENTRY_BEAM_SELECT = 4, NT_ENTRY_REORDER_ROWS = 5, NT_ENTRY_KV_FORK = 6, NT_ENTRY_KV_COPY_PAGES = 7,
+       NT_ENTRY_KV_ATTENTION_SHARED = 8 };
 NT_API int nt_call_packed(int entry, const void* words, int64_t n_words);
 
 #ifdef __cplusplus

@@ -1,0 +1,461 @@
+// The best continuations of a beam search over beams and vocabulary.
+//
+// A live beam k of an item offers every token v with
+//   s = score_k + x_kv - log sum_u exp x_ku,
+// a finished one itself alone with s = score_k; candidates rank by s / length^alpha
+// and the n best of the item's K beams are wanted, in order, ties to the lower (k, v).
+//
+// Bound by HBM: every logit is read once and takes a subtraction, two products, one
+// exponential and a comparison.  A CTA streams a slice of one row: each thread keeps its
+// vectors in registers, its running maximum and sum of exponentials, and candidates are
+// the values that reach a bound that n values of the slice are known to reach (the r-th
+// largest of each warp's lane maxima, the smallest of that over the warps, with
+// r * warps >= n), a few dozen of thousands.  They are ranked by counting in shared
+// memory.  A slice in which too many reach the bound (constant logits) takes its n best
+// one after the other instead.  A second kernel, launched as a programmatic dependent,
+// joins an item's slices: logarithms and sums in float64 (candidates of two beams may lie
+// closer together than float32 can tell), then n rounds of one warp over the heads of the
+// sorted lists.
+#include "nt_kernels.cuh"
+
+#include <algorithm>
+
+namespace nt {
+namespace {
+
+constexpr int kBeamThreads = 256;
+constexpr int kBeamWarps = kBeamThreads / 32;
+constexpr int kBeamVecs = 4;           // 16-byte vectors of a thread in flight
+constexpr int kBeamList = 1024;        // candidates a slice can hold
+constexpr int kBeamMost = 64;          // n, and beams of an item
+constexpr int kBeamLists = 1024;       // slices of an item's beams
+constexpr int kJoinThreads = 128;
+constexpr int kJoinHeld = 4096;        // list entries that the joining kernel keeps in shared memory
+
+struct BeamArgs {
+    int64_t V;
+    int K, n, slices, per;             // beams, wanted, slices of a row, vectors of a slice
+    const void* x; int64_t ld;
+    const float* scores; const uint8_t* finished; const int32_t* lengths;
+    double alpha;
+    int64_t pad; int stay;
+    unsigned long long* keys;          // [rows][slices][n], largest first, 0 where there are fewer
+    float2* sums;                      // [rows][slices]: maximum, sum of exp(x - maximum)
+    float* out_scores; int32_t* out_rows; int64_t* out_tokens;
+};
+
+// Whether a beam's logits matter: it is not finished and can still win.
+__device__ __forceinline__ bool beam_open(const BeamArgs& a, int64_t row) {
+    return !(a.finished && a.finished[row]) && a.scores[row] > -INFINITY && a.scores[row] < INFINITY;
+}
+
+// Order of floats as that of unsigned words; both zeros alike.
+__device__ __forceinline__ uint32_t ordered(float f) {
+    const uint32_t u = __float_as_uint(f + 0.f);
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float from_ordered(uint32_t o) {
+    return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+// The larger value first, of equal ones the lower token.
+__device__ __forceinline__ unsigned long long beam_key(float f, uint32_t token) {
+    return (unsigned long long)ordered(f) << 32 | (uint32_t)~token;
+}
+__device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, o);
+        if (other > k) k = other;
+    }
+    return k;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
+    using T = typename Elem<DT>::T;
+    constexpr int E = 16 / (int)sizeof(T);
+    __shared__ unsigned long long list[kBeamList];
+    __shared__ uint32_t warp_bound[2][kBeamWarps];
+    __shared__ unsigned long long warp_key[kBeamWarps];
+    __shared__ float warp_m[kBeamWarps], warp_s[kBeamWarps];
+    __shared__ int count;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t row = blockIdx.y;
+    if (!beam_open(a, row)) return;
+    if (tid == 0) count = 0;
+    const T* x = static_cast<const T*>(a.x) + row * a.ld;
+    const int shift = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));    // elements of the first vector before the row
+    const T* grid = x - shift;
+    const int64_t n_vec = (shift + a.V + E - 1) / E;
+    const int64_t begin = (int64_t)blockIdx.x * a.per, end = begin + a.per < n_vec ? begin + a.per : n_vec;
+
+    auto value = [](const uint4& w, int e) {
+        const uint32_t* u = reinterpret_cast<const uint32_t*>(&w);
+        return DT == NT_F32 ? __uint_as_float(u[e]) : __uint_as_float(e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16);
+    };
+    // keeps the n best of the first m entries of the list, in order
+    auto shrink = [&](int m) {
+        unsigned long long mine[kBeamList / kBeamThreads];
+        int rank[kBeamList / kBeamThreads];
+#pragma unroll
+        for (int i = 0; i < kBeamList / kBeamThreads; ++i) {
+            mine[i] = tid + i * kBeamThreads < m ? list[tid + i * kBeamThreads] : 0ull;
+            rank[i] = 0;
+        }
+        for (int i = 0; i * kBeamThreads < m; ++i)
+            for (int j = 0; j < m; ++j) rank[i] += list[j] > mine[i];
+        __syncthreads();
+        for (int i = 0; i * kBeamThreads < m; ++i)
+            if (tid + i * kBeamThreads < m && rank[i] < a.n) list[rank[i]] = mine[i];
+        __syncthreads();
+        return m < a.n ? m : a.n;
+    };
+
+    float top = -INFINITY, sum = 0.f, bound = -INFINITY;
+    int held = 0, turn = 0;
+    const int rounds = (a.n + kBeamWarps - 1) / kBeamWarps;
+    __syncthreads();
+    for (int64_t v0 = begin; v0 < end; v0 += kBeamThreads * kBeamVecs, turn ^= 1) {
+        uint4 raw[kBeamVecs];
+#pragma unroll
+        for (int j = 0; j < kBeamVecs; ++j) {
+            const int64_t v = v0 + j * kBeamThreads + tid, at = v * E - shift;
+            if (v < end && at >= 0 && at + E <= a.V) {
+                raw[j] = __ldcs(reinterpret_cast<const uint4*>(grid + v * E));
+            } else {                                    // outside, or across an end of the row
+                uint32_t* u = reinterpret_cast<uint32_t*>(&raw[j]);
+                u[0] = u[1] = u[2] = u[3] = DT == NT_F32 ? 0xff800000u : 0xff80ff80u;
+                if (v < end)
+                    for (int e = 0; e < E; ++e)
+                        if (at + e >= 0 && at + e < a.V) reinterpret_cast<T*>(u)[e] = x[at + e];
+            }
+        }
+        float best = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kBeamVecs; ++j)
+#pragma unroll
+            for (int e = 0; e < E; ++e) best = fmaxf(best, value(raw[j], e));
+        // the bound of this tile
+        uint32_t o = ordered(best), bw = 0u;
+        for (int r = 0; r < rounds; ++r) {
+            bw = __reduce_max_sync(0xffffffffu, o);
+            const unsigned who = __ballot_sync(0xffffffffu, o == bw);
+            if (lane == __ffs(who) - 1) o = 0u;
+        }
+        if (lane == 0) warp_bound[turn][warp] = bw;
+        // the sum of exponentials: the exponent's product with log2 e in two parts
+        if (best > top) {
+            sum = top == -INFINITY ? sum : sum * ex2((top - best) * kLog2e);
+            top = best;
+        }
+        const float base = top == -INFINITY ? 0.f : top;
+        float part[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < kBeamVecs; ++j)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float d = value(raw[j], e) - base;
+                part[e & 1] += ex2(fmaf(d, kLog2e, d * 1.925963033500e-8f));
+            }
+        sum += part[0] + part[1];
+        __syncthreads();
+        uint32_t least = warp_bound[turn][0];
+#pragma unroll
+        for (int w = 1; w < kBeamWarps; ++w) least = min(least, warp_bound[turn][w]);
+        bound = fmaxf(bound, least ? from_ordered(least) : -INFINITY);
+        if (best >= bound && best > -INFINITY) {
+#pragma unroll
+            for (int j = 0; j < kBeamVecs; ++j)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float f = value(raw[j], e);
+                    if (f >= bound && f > -INFINITY) {
+                        const int at = atomicAdd(&count, 1);
+                        if (at < kBeamList) list[at] = beam_key(f, (uint32_t)((v0 + j * kBeamThreads + tid) * E + e - shift));
+                    }
+                }
+        }
+        __syncthreads();
+        const int now = count;
+        if (now > kBeamList) {
+            // too many: the list as it was, and the n best of this tile one after the other
+            __syncthreads();
+            held = shrink(held);
+            unsigned long long prev = ~0ull;
+            for (int r = 0; r < a.n; ++r) {
+                unsigned long long k = 0ull;
+#pragma unroll
+                for (int j = 0; j < kBeamVecs; ++j)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const float f = value(raw[j], e);
+                        if (f > -INFINITY) {
+                            const unsigned long long c = beam_key(f, (uint32_t)((v0 + j * kBeamThreads + tid) * E + e - shift));
+                            if (c < prev && c > k) k = c;
+                        }
+                    }
+                k = warp_max(k);
+                if (lane == 0) warp_key[warp] = k;
+                __syncthreads();
+#pragma unroll
+                for (int w = 0; w < kBeamWarps; ++w)
+                    if (warp_key[w] > k) k = warp_key[w];
+                __syncthreads();
+                if (k == 0ull) break;
+                if (tid == 0) list[held] = k;
+                ++held;
+                prev = k;
+            }
+            if (tid == 0) count = held;
+            __syncthreads();
+        } else {
+            held = now;
+        }
+    }
+    // the slice's maximum and sum, and its n best
+    float m = top;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) warp_m[warp] = m;
+    held = shrink(held);
+#pragma unroll
+    for (int w = 0; w < kBeamWarps; ++w) m = fmaxf(m, warp_m[w]);
+    sum = top == -INFINITY ? sum : sum * ex2((top - m) * kLog2e);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) warp_s[warp] = sum;
+    __syncthreads();
+    const int64_t at = row * a.slices + blockIdx.x;
+    if (tid == 0) {
+        float s = 0.f;
+        for (int w = 0; w < kBeamWarps; ++w) s += warp_s[w];
+        a.sums[at] = make_float2(m, s);
+    }
+    if (tid < a.n) a.keys[at * a.n + tid] = tid < held ? list[tid] : 0ull;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Order of float64 as that of unsigned words, 0 for what cannot be chosen.
+__device__ __forceinline__ unsigned long long ordered64(double r) {
+    if (!(r > -INFINITY && r < INFINITY)) return 0ull;
+    const unsigned long long u = (unsigned long long)__double_as_longlong(r + 0.0);
+    return u ^ ((unsigned long long)((long long)u >> 63) | 0x8000000000000000ull);
+}
+
+__global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_constant__ BeamArgs a) {
+    __shared__ double lse[kBeamMost], norm[kBeamMost];
+    __shared__ unsigned long long held[kJoinHeld];
+    __shared__ unsigned long long head_rank[kBeamLists];
+    __shared__ uint32_t head_token[kBeamLists];
+    __shared__ uint8_t head_at[kBeamLists];
+    __shared__ uint8_t kind[kBeamMost];                 // 0 nothing to offer, 1 live, 2 finished
+    __shared__ int chosen[kBeamMost];
+    __shared__ float chosen_score[kBeamMost];
+    __shared__ uint32_t chosen_token[kBeamMost];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t row0 = (int64_t)blockIdx.x * a.K;
+    const int S = a.slices, lists = a.K * S, n = a.n;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int k = warp; k < a.K; k += kJoinThreads / 32) {
+        const int64_t row = row0 + k;
+        const bool done = a.finished && a.finished[row];
+        const float score = a.scores[row];
+        int what = !(score > -INFINITY && score < INFINITY) ? 0 : done ? 2 : 1;
+        double l = 0.0;
+        if (what == 1) {
+            float m = -INFINITY;
+            for (int s = lane; s < S; s += 32) m = fmaxf(m, a.sums[row * S + s].x);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            double sum = 0.0;
+            for (int s = lane; s < S; s += 32) {
+                const float2 p = a.sums[row * S + s];
+                sum += p.x == -INFINITY ? (double)p.y : (double)p.y * exp((double)p.x - (double)m);
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            l = (double)m + log(sum);
+            if (!(l > -INFINITY && l < INFINITY)) what = 0;         // NaN or infinity among the logits, or nothing left
+        }
+        if (lane == 0) {
+            lse[k] = l;
+            kind[k] = (uint8_t)what;
+            const double len = a.lengths ? (double)a.lengths[row] + (what == 1 ? 1.0 : 0.0) : 1.0;
+            norm[k] = a.alpha != 0.0 ? pow(len > 1.0 ? len : 1.0, a.alpha) : 1.0;
+        }
+    }
+    const bool near = lists * n <= kJoinHeld;
+    const unsigned long long* keys = a.keys + row0 * S * n;
+    if (near) {
+        for (int i = tid; i < lists * n; i += kJoinThreads) held[i] = keys[i];
+        keys = held;
+    }
+    __syncthreads();
+    // the candidate at place `at` of list l: its rank (0: none) and token
+    auto head = [&](int l, int at) {
+        const int k = l / S;
+        unsigned long long r = 0ull;
+        uint32_t token = 0u;
+        if (kind[k] == 2) {
+            token = (uint32_t)a.pad;
+            if (l == k * S && at == 0) r = ordered64((double)a.scores[row0 + k] / norm[k]);
+        } else if (kind[k] == 1 && at < n) {
+            const unsigned long long c = keys[l * n + at];
+            if (c) {
+                token = ~(uint32_t)c;
+                r = ordered64(((double)a.scores[row0 + k] + ((double)from_ordered((uint32_t)(c >> 32)) - lse[k])) / norm[k]);
+            }
+        }
+        head_rank[l] = r;
+        head_token[l] = token;
+        head_at[l] = (uint8_t)at;
+    };
+    if (warp == 0) {
+        // a lane has lists lane, lane + 32, ...
+        unsigned long long best = 0ull, flat = ~0ull;
+        int from = -1;
+        auto pick = [&]() {
+            best = 0ull, flat = ~0ull, from = -1;
+            for (int l = lane; l < lists; l += 32) {
+                const unsigned long long r = head_rank[l], f = (unsigned long long)(l / S) << 32 | head_token[l];
+                if (r > best || (r == best && f < flat)) best = r, flat = f, from = l;
+            }
+        };
+        for (int l = lane; l < lists; l += 32) head(l, 0);
+        __syncwarp();
+        pick();
+        for (int i = 0; i < n; ++i) {
+            unsigned long long r = best, f = flat;
+            int w = from;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                const unsigned long long r2 = __shfl_xor_sync(0xffffffffu, r, o), f2 = __shfl_xor_sync(0xffffffffu, f, o);
+                const int w2 = __shfl_xor_sync(0xffffffffu, w, o);
+                if (r2 > r || (r2 == r && f2 < f)) r = r2, f = f2, w = w2;
+            }
+            if (lane == 0) {
+                const int k = (int)(f >> 32);
+                chosen[i] = r ? k : -1;
+                if (r) {
+                    double s = a.scores[row0 + k];
+                    if (kind[k] == 1) s += (double)from_ordered((uint32_t)(keys[w * n + head_at[w]] >> 32)) - lse[k];
+                    chosen_score[i] = (float)s;
+                    chosen_token[i] = head_token[w];
+                }
+            }
+            __syncwarp();
+            if (r && from == w) {
+                head(w, head_at[w] + 1);
+                pick();
+            }
+            __syncwarp();
+        }
+        // places: in order, or the first child of a beam in the beam's own
+        if (lane == 0) {
+            unsigned long long taken = 0ull;
+            int8_t place[kBeamMost];
+            for (int i = 0; i < n; ++i) {
+                place[i] = (int8_t)i;
+                if (a.stay) {
+                    place[i] = -1;
+                    if (chosen[i] >= 0 && !(taken >> chosen[i] & 1)) {
+                        place[i] = (int8_t)chosen[i];
+                        taken |= 1ull << chosen[i];
+                    }
+                }
+            }
+            for (int i = 0; i < n; ++i) {
+                if (place[i] < 0) {
+                    place[i] = (int8_t)(__ffsll((long long)~taken) - 1);
+                    taken |= 1ull << place[i];
+                }
+                const int64_t at = (int64_t)blockIdx.x * n + place[i];
+                const bool some = chosen[i] >= 0;
+                a.out_scores[at] = some ? chosen_score[i] : -INFINITY;
+                a.out_rows[at] = (int32_t)(row0 + (some ? chosen[i] : place[i] % a.K));
+                a.out_tokens[at] = some ? (int64_t)chosen_token[i] : a.pad;
+            }
+        }
+    }
+}
+
+// Slices of a row: enough CTAs for the device, a vector a thread at least, and no more lists
+// of an item than the joining kernel holds.
+struct BeamPlan { int slices, per; int64_t bytes; };
+BeamPlan beam_plan(int64_t B, int64_t K, int64_t V, int64_t n, int es) {
+    const int64_t n_vec = (V + 2 * (16 / es) - 2) / (16 / es), rows = B * K;
+    int64_t s = std::max<int64_t>(1, 148 * 4 / std::max<int64_t>(1, rows));
+    s = std::min({s, (n_vec + kBeamThreads - 1) / kBeamThreads, (int64_t)kBeamLists / K, (int64_t)64});
+    s = std::max<int64_t>(1, s);
+    BeamPlan p;
+    const int64_t step = kBeamThreads;
+    p.per = (int)(((n_vec + s - 1) / s + step - 1) / step * step);
+    p.slices = (int)((n_vec + p.per - 1) / p.per);
+    p.bytes = rows * p.slices * (n * 8 + 8);
+    return p;
+}
+
+}  // namespace
+}  // namespace nt
+
+using namespace nt;
+
+extern "C" {
+
+int64_t nt_beam_select_workspace_bytes(int dtype, int64_t B, int64_t K, int64_t V, int64_t n) {
+    if (B < 1 || K < 1 || K > kBeamMost || V < 1 || n < 1 || n > kBeamMost) return 0;
+    return beam_plan(B, K, V, n, dtype == NT_F32 ? 4 : 2).bytes;
+}
+
+int nt_beam_select(int dtype, int64_t B, int64_t K, int64_t V, int64_t n, const void* logits, int64_t ld, const float* scores,
+                   const uint8_t* finished, const int32_t* lengths, double length_penalty, int64_t pad, int stay,
+                   float* out_scores, int32_t* out_rows, int64_t* out_tokens, void* workspace, int64_t workspace_bytes,
+                   void* stream) {
+    if (dtype != NT_F32 && dtype != NT_BF16) return fail(NT_ERR_DTYPE, "nt_beam_select: dtype %d", dtype);
+    if (B < 0 || V < 1 || V > (int64_t)INT32_MAX || B * K > 65535)
+        return fail(NT_ERR_ARG, "nt_beam_select: bad sizes (at most 65535 rows)");
+    if (K < 1 || K > kBeamMost || n < 1 || n > kBeamMost)
+        return fail(NT_ERR_ARG, "nt_beam_select: %lld beams, %lld wanted (1 to %d of each)", (long long)K, (long long)n, kBeamMost);
+    if (stay && n != K) return fail(NT_ERR_ARG, "nt_beam_select: children in their parents' places need n == K");
+    if (!(length_penalty > -1e300 && length_penalty < 1e300)) return fail(NT_ERR_ARG, "nt_beam_select: length penalty must be finite");
+    if (length_penalty != 0.0 && !lengths) return fail(NT_ERR_ARG, "nt_beam_select: a length penalty needs lengths");
+    if (pad < 0 || pad > (int64_t)INT32_MAX) return fail(NT_ERR_ARG, "nt_beam_select: pad %lld", (long long)pad);
+    if (B == 0) return NT_OK;
+    if (!logits || !scores || !out_scores || !out_rows || !out_tokens) return fail(NT_ERR_ARG, "nt_beam_select: null pointer");
+    const int es = dtype == NT_F32 ? 4 : 2;
+    const BeamPlan p = beam_plan(B, K, V, n, es);
+    if (!workspace || workspace_bytes < p.bytes)
+        return fail(NT_ERR_WORKSPACE, "nt_beam_select: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)p.bytes);
+    if ((reinterpret_cast<uintptr_t>(logits) & (es - 1)) || (reinterpret_cast<uintptr_t>(workspace) & 7))
+        return fail(NT_ERR_ARG, "nt_beam_select: alignment");
+    BeamArgs a{};
+    a.V = V; a.K = (int)K; a.n = (int)n; a.slices = p.slices; a.per = p.per;
+    a.x = logits; a.ld = ld; a.scores = scores; a.finished = finished; a.lengths = lengths;
+    a.alpha = length_penalty; a.pad = pad; a.stay = stay;
+    a.keys = static_cast<unsigned long long*>(workspace);
+    a.sums = reinterpret_cast<float2*>(a.keys + B * K * p.slices * n);
+    a.out_scores = out_scores; a.out_rows = out_rows; a.out_tokens = out_tokens;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const dim3 grid((unsigned)p.slices, (unsigned)(B * K));
+    if (dtype == NT_F32) beam_scan_kernel<NT_F32><<<grid, kBeamThreads, 0, st>>>(a);
+    else beam_scan_kernel<NT_BF16><<<grid, kBeamThreads, 0, st>>>(a);
+    const int rc = check_launch("beam_scan_kernel");
+    if (rc != NT_OK) return rc;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)B);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, beam_join_kernel, a);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(NT_ERR_CUDA, "beam_join_kernel launch failed: %s", cudaGetErrorString(e));
+    }
+    return check_launch("beam_join_kernel");
+}
+
+}  // extern "C"

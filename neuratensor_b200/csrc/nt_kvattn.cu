@@ -841,4 +841,19 @@ int nt_kv_attention(int dtype, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, in
     return D == 64 ? launch_planned<NT_BF16, 64>(a, B, pl, st) : launch_planned<NT_BF16, 128>(a, B, pl, st);
 }
 
+int64_t nt_kv_attention_shared_workspace_bytes(int dtype, int64_t B, int64_t groups, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                               int64_t page, int64_t n_blocks, int64_t window) {
+    return nt_kv_attention_workspace_bytes(B, T, Hq, Hkv, D, page, n_blocks, window);
+}
+
+int nt_kv_attention_shared(int dtype, int64_t B, int64_t groups, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t page,
+                           int64_t n_pages, int64_t n_blocks, int64_t window, float scale, const void* q, int64_t q_sb, int64_t q_st,
+                           int64_t q_sh, const void* k_codes, const float* k_scale, const void* v_codes, const float* v_scale,
+                           const int32_t* table, int64_t table_sb, const int32_t* lengths, const int32_t* counts,
+                           const int32_t* shared, void* out, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (groups < 1 || B % groups) return fail(NT_ERR_ARG, "nt_kv_attention_shared: %lld sequences in %lld groups", (long long)B, (long long)groups);
+    return nt_kv_attention(dtype, B, T, Hq, Hkv, D, page, n_pages, n_blocks, window, scale, q, q_sb, q_st, q_sh, k_codes, k_scale,
+                           v_codes, v_scale, table, table_sb, lengths, counts, out, workspace, workspace_bytes, stream);
+}
+
 }  // extern "C"

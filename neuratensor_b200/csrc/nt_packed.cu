@@ -28,12 +28,13 @@ struct Words {
     template <typename T> T* ptr() { return reinterpret_cast<T*>(static_cast<uintptr_t>(i())); }
 };
 
-constexpr int64_t kWords[4] = {21, 25, 27, 27};
+constexpr int kEntries = 9;
+constexpr int64_t kWords[kEntries] = {21, 25, 27, 27, 19, 6, 15, 9, 29};
 
 }  // namespace
 
 extern "C" int nt_call_packed(int entry, const void* words, int64_t n_words) {
-    if (entry < 0 || entry > 3) return fail(NT_ERR_ARG, "nt_call_packed: entry %d", entry);
+    if (entry < 0 || entry >= kEntries) return fail(NT_ERR_ARG, "nt_call_packed: entry %d", entry);
     if (!words) return fail(NT_ERR_ARG, "nt_call_packed: null pointer");
     if (n_words != kWords[entry])
         return fail(NT_ERR_ARG, "nt_call_packed: %lld words for entry %d, which takes %lld", (long long)n_words, entry,
@@ -89,6 +90,70 @@ extern "C" int nt_call_packed(int entry, const void* words, int64_t n_words) {
         const int64_t bytes = w.i();
         return nt_kv_attention((int)dtype, B, T, Hq, H, D, page, pages, blocks, window, scale, q, q_sb, q_st, q_sh, kc, ks, vc,
                                vs, table, table_sb, lengths, counts, out, ws, bytes, w.ptr<void>());
+    }
+    if (entry == NT_ENTRY_BEAM_SELECT) {
+        const int64_t dtype = w.i(), B = w.i(), K = w.i(), V = w.i(), n = w.i();
+        const void* x = w.ptr<void>();
+        const int64_t ld = w.i();
+        const float* scores = w.ptr<float>();
+        const unsigned char* finished = w.ptr<unsigned char>();
+        const int32_t* lengths = w.ptr<int32_t>();
+        const double alpha = w.d();
+        const int64_t pad = w.i(), stay = w.i();
+        float* out_scores = w.ptr<float>();
+        int32_t* out_rows = w.ptr<int32_t>();
+        int64_t* out_tokens = w.ptr<int64_t>();
+        void* ws = w.ptr<void>();
+        const int64_t bytes = w.i();
+        return nt_beam_select((int)dtype, B, K, V, n, x, ld, scores, finished, lengths, alpha, pad, (int)stay, out_scores,
+                              out_rows, out_tokens, ws, bytes, w.ptr<void>());
+    }
+    if (entry == NT_ENTRY_REORDER_ROWS) {
+        const int64_t n = w.i();
+        const int64_t* tensors = w.ptr<int64_t>();
+        const int64_t R = w.i(), group = w.i();
+        const int32_t* rows = w.ptr<int32_t>();
+        return nt_reorder_rows(n, tensors, R, group, rows, w.ptr<void>());
+    }
+    if (entry == NT_ENTRY_KV_FORK) {
+        const int64_t R = w.i(), pages = w.i(), blocks = w.i(), page = w.i(), tokens = w.i(), window = w.i(), group = w.i();
+        int32_t* table = w.ptr<int32_t>();
+        const int64_t table_sb = w.i();
+        int32_t* refs = w.ptr<int32_t>();
+        int32_t* lengths = w.ptr<int32_t>();
+        const int32_t* parents = w.ptr<int32_t>();
+        int32_t* copies = w.ptr<int32_t>();
+        int32_t* shared = w.ptr<int32_t>();
+        return nt_kv_fork(R, pages, blocks, page, tokens, window, group, table, table_sb, refs, lengths, parents, copies, shared,
+                          w.ptr<void>());
+    }
+    if (entry == NT_ENTRY_KV_COPY_PAGES) {
+        const int64_t n_layers = w.i();
+        const int64_t* layers = w.ptr<int64_t>();
+        const int64_t n_pages = w.i(), H = w.i(), page = w.i(), D = w.i(), n = w.i();
+        const int32_t* pages = w.ptr<int32_t>();
+        return nt_kv_copy_pages(n_layers, layers, n_pages, H, page, D, n, pages, w.ptr<void>());
+    }
+    if (entry == NT_ENTRY_KV_ATTENTION_SHARED) {
+        const int64_t dtype = w.i(), B = w.i(), groups = w.i(), T = w.i(), Hq = w.i(), H = w.i(), D = w.i(), page = w.i(),
+                      pages = w.i(), blocks = w.i(), window = w.i();
+        const float scale = w.f();
+        const void* q = w.ptr<void>();
+        const int64_t q_sb = w.i(), q_st = w.i(), q_sh = w.i();
+        const void* kc = w.ptr<void>();
+        const float* ks = w.ptr<float>();
+        const void* vc = w.ptr<void>();
+        const float* vs = w.ptr<float>();
+        const int32_t* table = w.ptr<int32_t>();
+        const int64_t table_sb = w.i();
+        const int32_t* lengths = w.ptr<int32_t>();
+        const int32_t* counts = w.ptr<int32_t>();
+        const int32_t* shared = w.ptr<int32_t>();
+        void* out = w.ptr<void>();
+        void* ws = w.ptr<void>();
+        const int64_t bytes = w.i();
+        return nt_kv_attention_shared((int)dtype, B, groups, T, Hq, H, D, page, pages, blocks, window, scale, q, q_sb, q_st, q_sh,
+                                      kc, ks, vc, vs, table, table_sb, lengths, counts, shared, out, ws, bytes, w.ptr<void>());
     }
     const int64_t dtype = w.i(), B = w.i(), V = w.i();
     const void* x = w.ptr<void>();

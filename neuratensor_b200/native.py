@@ -13,7 +13,7 @@ import math
 import os
 import struct
 import threading
-from typing import Optional, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
@@ -76,6 +76,13 @@ _SIGS = {
                         _I32),
     "nt_logits_process": ([_I32, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P, _I32, _P, ctypes.c_double] + [_P, _F32] * 2 +
                           [_P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P], _I32),
+    "nt_beam_select_workspace_bytes": ([_I32] + [_I64] * 4, _I64),
+    "nt_beam_select": ([_I32] + [_I64] * 4 + [_P, _I64, _P, _P, _P, ctypes.c_double, _I64, _I32] + [_P] * 4 + [_I64, _P], _I32),
+    "nt_reorder_rows": ([_I64, _P, _I64, _I64, _P, _P], _I32),
+    "nt_kv_fork": ([_I64] * 7 + [_P, _I64] + [_P] * 6, _I32),
+    "nt_kv_copy_pages": ([_I64, _P] + [_I64] * 5 + [_P, _P], _I32),
+    "nt_kv_attention_shared_workspace_bytes": ([_I32] + [_I64] * 9, _I64),
+    "nt_kv_attention_shared": ([_I32] + [_I64] * 10 + [_F32, _P, _I64, _I64, _I64] + [_P] * 5 + [_I64] + [_P] * 5 + [_I64, _P], _I32),
     "nt_call_packed": ([_I32, ctypes.c_char_p, _I64], _I32),
 }
 
@@ -487,7 +494,10 @@ def lm_head(x: Tensor, gamma: Tensor, W: Tensor, workspace: Optional[Tensor] = N
 # entry point -> (its number, number of arguments, packer) for nt_call_packed
 _PACKED = {"nt_rotary": (0, 21, struct.Struct("=8qd12q").pack), "nt_kv_append": (1, 25, struct.Struct("=25q").pack),
            "nt_kv_attention": (2, 27, struct.Struct("=10qd16q").pack),
-           "nt_logits_process": (3, 27, struct.Struct("=11qqdqdqd10q").pack)}
+           "nt_logits_process": (3, 27, struct.Struct("=11qqdqdqd10q").pack),
+           "nt_beam_select": (4, 19, struct.Struct("=10qd8q").pack), "nt_reorder_rows": (5, 6, struct.Struct("=6q").pack),
+           "nt_kv_fork": (6, 15, struct.Struct("=15q").pack), "nt_kv_copy_pages": (7, 9, struct.Struct("=9q").pack),
+           "nt_kv_attention_shared": (8, 29, struct.Struct("=11qd17q").pack)}
 
 
 def _launch(index: int, name: str, *args) -> None:
@@ -850,6 +860,234 @@ def pack_allowed(mask: Tensor) -> Tensor:
     bits[:, :V] = mask
     words = (bits.view(B, -1, 32) << torch.arange(32, device=mask.device)).sum(-1)
     return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
+
+
+# --------------------------------------------------------------------------- #
+#  A step of a beam search: the choice over beams and vocabulary, states moved #
+#  to the chosen beams, pages of the cache forked, attention over shared ones  #
+# --------------------------------------------------------------------------- #
+
+@functools.lru_cache(maxsize=256)
+def _beam_select_bytes(*sizes: int) -> int:
+    return load().nt_beam_select_workspace_bytes(*sizes)
+
+
+def beam_select(logits: Tensor, scores: Tensor, finished: Optional[Tensor] = None, lengths: Optional[Tensor] = None,
+                length_penalty: float = 0.0, n: Optional[int] = None, pad: int = 0, stay: bool = False
+                ) -> Tuple[Tensor, Tensor, Tensor]:
+    """The best continuations of a beam search -> (scores [B, n], rows [B, n], tokens [B, n]).
+
+    logits: [B*K, V] float32 or bfloat16, the K beams of an item after one another;
+    scores: [B, K] float32, their log-probabilities so far.  A live beam offers every
+    token whose logit is not -inf with its score and log-softmax added, a finished
+    one (bool [B, K]) itself alone, with token `pad`; a beam with a score or a
+    log-sum that is not finite offers nothing.  Candidates rank by that sum divided by
+    the length to the power of length_penalty (lengths: [B, K], tokens made so
+    far, one more for a live beam); ties go to the lower beam, then the lower token.  n
+    (None: K; at most 64, like K) are wanted, best first; with stay, n is K and the
+    best child of a beam stands in the beam's own place.  scores: float32 sums; rows:
+    int32, the row of logits that each goes on from; tokens: int64.  Where candidates
+    run out: -inf, row b*K + place % K, `pad`."""
+    index = _device_index(logits, scores, finished, lengths)
+    _refuse_grad("beam_select", logits, scores)
+    code = _dtype_code(logits)
+    if scores.dim() != 2 or scores.dtype != torch.float32 or scores.shape[1] < 1:
+        raise ValueError(f"beam_select: scores must be float32 [B, K], got {scores.dtype} {tuple(scores.shape)}")
+    B, K = scores.shape
+    if logits.dim() != 2 or logits.shape[0] != B * K or logits.shape[1] < 1:
+        raise ValueError(f"beam_select: logits must be [{B * K}, V], got {tuple(logits.shape)}")
+    V = logits.shape[1]
+    if logits.stride(1) != 1 and V > 1:
+        logits = logits.contiguous()
+    if n is None:
+        n = K
+    if not 1 <= n <= 64 or K > 64:
+        raise ValueError(f"beam_select: 1 to 64 beams and continuations, got {K} and {n}")
+    if stay and n != K:
+        raise ValueError(f"beam_select: children in their parents' places need n = K, got {n} of {K}")
+    if finished is not None:
+        if finished.shape != (B, K) or finished.dtype != torch.bool:
+            raise ValueError(f"beam_select: finished must be bool [{B}, {K}], got {finished.dtype} {tuple(finished.shape)}")
+        finished = finished.contiguous()
+    if not math.isfinite(length_penalty):
+        raise ValueError(f"beam_select: length_penalty must be finite, got {length_penalty}")
+    if lengths is not None:
+        if lengths.shape != (B, K):
+            raise ValueError(f"beam_select: lengths must be [{B}, {K}], got {tuple(lengths.shape)}")
+        lengths = _ints(lengths, torch.int32, "lengths").contiguous()
+    elif length_penalty != 0.0:
+        raise ValueError("beam_select: a length penalty needs lengths")
+    if not 0 <= pad < 2 ** 31:
+        raise ValueError(f"beam_select: pad must be a token, got {pad}")
+    scores = scores.contiguous()
+    out = scores.new_empty((B, n))
+    rows = torch.empty((B, n), dtype=torch.int32, device=scores.device)
+    tokens = torch.empty((B, n), dtype=torch.int64, device=scores.device)
+    nbytes = _beam_select_bytes(code, B, K, V, n)
+    ws = scores.new_empty(max(nbytes, 1), dtype=torch.uint8)
+    _launch(index, "nt_beam_select", code, B, K, V, n, logits.data_ptr(), logits.stride(0), scores.data_ptr(), _ptr(finished),
+            _ptr(lengths), length_penalty, pad, stay, out.data_ptr(), rows.data_ptr(), tokens.data_ptr(), ws.data_ptr(), nbytes)
+    return out, rows, tokens
+
+
+def reorder_rows(tensors: Sequence[Tensor], rows: Tensor, group: Optional[int] = None) -> None:
+    """Row r of every tensor takes what its row rows[r] held, in place and in one launch.
+
+    tensors: any dtypes, [R, ...] with the same R and rows that lie in one piece (block
+    states, for instance), not overlapping; rows: int32 or int64 [R], each within its group of
+    `group` consecutive rows (None: R; at most 1024), -1: the row stays as it is.  Any map
+    is right, also one that swaps; rows that stay are not touched.  A row
+    outside its group is left and flagged (device_error_flags)."""
+    tensors = list(tensors)
+    index = _device_index(rows, *tensors)
+    if rows.dim() != 1:
+        raise ValueError(f"reorder_rows: rows must be [R], got {tuple(rows.shape)}")
+    R = rows.numel()
+    group = max(R, 1) if group is None else group
+    if not 1 <= group <= 1024 or R % group:
+        raise ValueError(f"reorder_rows: {R} rows in groups of {group} (1 to 1024)")
+    _refuse_out("reorder_rows", *tensors)
+    if rows.dtype != torch.int32:
+        rows = _ints(rows, torch.int32, "rows")
+    rows = rows.contiguous()
+    spec = []
+    for t in tensors:
+        if t.dim() < 1 or t.shape[0] != R:
+            raise ValueError(f"reorder_rows: every tensor must have {R} rows, got {tuple(t.shape)}")
+        size = t.element_size()
+        if t.is_contiguous():
+            row = t.numel() // R * size if R else 0
+            spec += (t.data_ptr(), row, row)
+        else:
+            if R and not t[0].is_contiguous() or R > 1 and t.stride(0) < t[0].numel():
+                raise ValueError("reorder_rows: the rows of a tensor must lie in one piece each, without overlap")
+            spec += (t.data_ptr(), t[0].numel() * size if R else 0, t.stride(0) * size)
+    if not spec:
+        return
+    words = struct.pack(f"={len(spec)}q", *spec)
+    _launch(index, "nt_reorder_rows", len(tensors), _bytes_address(words), R, group, rows.data_ptr())
+    increment_version(tensors)
+
+
+def _bytes_address(b: bytes) -> int:
+    return ctypes.cast(b, ctypes.c_void_p).value
+
+
+def kv_fork(table: Tensor, refs: Tensor, lengths: Tensor, parents: Tensor, page: int, tokens: int = 1,
+            window: Optional[int] = None, group: Optional[int] = None) -> Tuple[Tensor, Optional[Tensor]]:
+    """Lets row r of a cache go on from row parents[r] without copying it -> (copies [R, 2], shared [R / group]).
+
+    In place: table int32 [R, blocks] (-1: no page), refs int32 [pages] (how many table
+    entries, and other holders, have a page; 0: free) and lengths int32 [R], R at
+    most 1024.  A row takes its parent's length and pages (-1: the row ends), with a
+    window only those that a next token can see; pages without refs are free again.  A last
+    page that is not full is made the row's own, since the next token is written there:
+    one of the rows that have it keeps it when nothing else does (one that goes on from
+    itself before others), the others get a new one and a line (from, to) in `copies` for
+    kv_copy_pages; other lines are -1.  The next `tokens` tokens get pages (with a window
+    those that it still sees behind them).  New pages are the free ones of lowest index, row
+    by row.  shared: with `group`, how many leading tokens the rows of each group have in
+    the same pages, for kv_attention_shared.  Without enough pages or blocks entries stay -1, which is
+    flagged (device_error_flags) like bad parents, lengths and pages."""
+    index = _device_index(table, refs, lengths, parents)
+    if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"kv_fork: table must be int32 [R, blocks] with unit stride, got {table.dtype} {tuple(table.shape)}")
+    R, blocks = table.shape
+    if R > 1024 or (R > 1 and table.stride(0) < blocks):
+        raise ValueError(f"kv_fork: a table of at most 1024 rows that do not overlap, got {R}")
+    if lengths.shape != (R,) or lengths.dtype != torch.int32 or not lengths.is_contiguous():
+        raise ValueError(f"kv_fork: lengths must be contiguous int32 [{R}]")
+    if refs.dim() != 1 or refs.dtype != torch.int32 or not refs.is_contiguous():
+        raise ValueError("kv_fork: refs must be contiguous int32 [pages]")
+    if page < 1 or tokens < 0 or (window is not None and window < 0):
+        raise ValueError(f"kv_fork: page {page}, tokens {tokens}, window {window}")
+    if group is not None and (group < 1 or R % group):
+        raise ValueError(f"kv_fork: {R} rows in groups of {group}")
+    parents = _row_ints("kv_fork", "parents", parents, R)
+    copies = torch.empty((R, 2), dtype=torch.int32, device=table.device)
+    shared = None if group is None else torch.empty(R // group, dtype=torch.int32, device=table.device)
+    _launch(index, "nt_kv_fork", R, refs.numel(), blocks, page, tokens, -1 if window is None else min(int(window), 2 ** 31),
+            group or 0, table.data_ptr(), max(table.stride(0), blocks), refs.data_ptr(), lengths.data_ptr(), parents.data_ptr(),
+            copies.data_ptr(), _ptr(shared))
+    increment_version((table, refs, lengths))
+    return copies, shared
+
+
+def kv_copy_pages(layers: Sequence[Tuple[Tensor, Tensor, Tensor, Tensor]], pages: Tensor) -> None:
+    """Copies pages within the pools of every layer: codes and scales of keys and values.
+
+    layers: (k_codes, k_scale, v_codes, v_scale) each, as kv_append has them and all of one shape;
+    pages: int32 [N, 2], from and to, (-1, -1) is skipped (kv_fork's copies).  No page may be
+    written twice, or both read and written; one outside the pool is skipped and flagged."""
+    layers = list(layers)
+    index = _device_index(pages, *[t for layer in layers for t in layer])
+    if pages.dim() != 2 or pages.shape[1] != 2 or pages.dtype != torch.int32:
+        raise ValueError(f"kv_copy_pages: pages must be int32 [N, 2], got {pages.dtype} {tuple(pages.shape)}")
+    if not layers:
+        return
+    shape = layers[0][0].shape
+    if len(shape) != 4 or shape[1] < 1 or shape[3] not in (64, 128) or shape[2] not in (16, 32, 64):
+        raise ValueError(f"kv_copy_pages: codes must be [pages, heads, page of 16, 32 or 64, 64 or 128], got {tuple(shape)}")
+    spec = []
+    for layer in layers:
+        kc, ks, vc, vs = layer
+        for c, s in ((kc, ks), (vc, vs)):
+            if c.shape != shape or c.dtype not in (torch.float8_e4m3fn, torch.uint8) or not c.is_contiguous():
+                raise ValueError(f"kv_copy_pages: codes must be contiguous float8_e4m3fn or uint8 {tuple(shape)}")
+            if s.shape != shape[:2] or s.dtype != torch.float32 or not s.is_contiguous():
+                raise ValueError(f"kv_copy_pages: scales must be contiguous float32 {tuple(shape[:2])}")
+            spec += (c.data_ptr(), s.data_ptr())
+        _refuse_out("kv_copy_pages", *layer)
+    if shape[0] == 0 or pages.shape[0] == 0:
+        return
+    pages = pages.contiguous()
+    words = struct.pack(f"={len(spec)}q", *spec)
+    _launch(index, "nt_kv_copy_pages", len(layers), _bytes_address(words), shape[0], shape[1], shape[2], shape[3], pages.shape[0],
+            pages.data_ptr())
+    increment_version([t for layer in layers for t in layer])
+
+
+@functools.lru_cache(maxsize=256)
+def _kv_attention_shared_bytes(*sizes: int) -> int:
+    return load().nt_kv_attention_shared_workspace_bytes(*sizes)
+
+
+def kv_attention_shared(q: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: Tensor, v_scale: Tensor, table: Tensor,
+                        lengths: Tensor, shared: Tensor, counts: Optional[Tensor] = None, window: Optional[int] = None,
+                        scale: Optional[float] = None) -> Tensor:
+    """kv_attention for sequences that share their beginnings, which are read once -> [B, T, Hq, D].
+
+    shared: int32 [groups], groups of B / groups consecutive sequences each (the beams of a
+    prompt, say): the first shared[g] positions of a group's sequences hold the same keys and
+    values, by each one's own table (kv_fork's `shared`; 0 where nothing is).  Arguments and
+    results otherwise as kv_attention."""
+    _refuse_grad("kv_attention_shared", q, k_codes, k_scale, v_codes, v_scale)
+    index = _device_index(q, k_codes, k_scale, v_codes, v_scale, table, lengths, shared, counts)
+    code = _dtype_code(q)
+    if q.dim() != 4:
+        raise ValueError(f"q must be [B, T, H, D], got {tuple(q.shape)}")
+    B, T, Hq, D = q.shape
+    H, P, n, blocks, lengths, counts = _cache_args("kv_attention_shared", B, D, k_codes, k_scale, v_codes, v_scale, table,
+                                                   lengths, counts)
+    if H < 1 or Hq < H or Hq % H:
+        raise ValueError(f"kv_attention_shared: {Hq} query heads over {H} cached heads")
+    if window is not None and window < 0:
+        raise ValueError(f"kv_attention_shared: window must be None or >= 0, got {window}")
+    groups = shared.numel()
+    if shared.dim() != 1 or groups < 1 or B % groups:
+        raise ValueError(f"kv_attention_shared: {B} sequences do not make the groups of shared {tuple(shared.shape)}")
+    shared = _ints(shared, torch.int32, "shared").contiguous()
+    win = -1 if window is None else min(int(window), 2 ** 31)      # as good as none from there on
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    q_sb, q_st, q_sh, _ = q.stride()
+    out = _like(q)
+    nbytes = _kv_attention_shared_bytes(code, B, groups, T, Hq, H, D, P, blocks, win)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _launch(index, "nt_kv_attention_shared", code, B, groups, T, Hq, H, D, P, n, blocks, win, D ** -0.5 if scale is None else scale,
+            q.data_ptr(), q_sb, q_st, q_sh, k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(),
+            table.data_ptr(), table.stride(0), lengths.data_ptr(), _ptr(counts), shared.data_ptr(), out.data_ptr(), _ptr(ws), nbytes)
+    return out
 
 
 def launch_count() -> int:
