@@ -70,6 +70,37 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
     return k;
 }
 
+// Elements at .. at + 15 / sizeof(T) of a row of V, -inf behind its end.  What a thread takes does
+// not depend on the row's alignment, so that equal rows have equal sums: a row off 16-byte
+// alignment takes two aligned vectors and picks.
+template <typename T>
+__device__ __forceinline__ uint4 beam_load(const T* x, int off, int64_t at, int64_t V) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const int before = off / (int)sizeof(T);            // elements of the first aligned vector that come before `at`
+    uint4 out;
+    uint32_t* o = reinterpret_cast<uint32_t*>(&out);
+    if (off == 0 && at + E <= V) {
+        out = __ldcs(reinterpret_cast<const uint4*>(x + at));
+    } else if (off != 0 && at >= before && at - before + 2 * E <= V) {
+        const uint4* p = reinterpret_cast<const uint4*>(x + at - before);
+        uint32_t w[9];
+        *reinterpret_cast<uint4*>(w) = __ldg(p);
+        *reinterpret_cast<uint4*>(w + 4) = __ldg(p + 1);
+        w[8] = 0u;
+        const int odd = (off & 2) * 8;                  // bits
+#pragma unroll
+        for (int k = 0; k < 4; ++k)                     // one of the four, the same for the row
+            if (off >> 2 == k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = __funnelshift_r(w[i + k], w[i + k + 1], odd);
+    } else {
+        o[0] = o[1] = o[2] = o[3] = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+        for (int e = 0; e < E; ++e)
+            if (at + e < V) reinterpret_cast<T*>(o)[e] = x[at + e];
+    }
+    return out;
+}
+
 template <int DT>
 __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
     using T = typename Elem<DT>::T;
@@ -84,11 +115,12 @@ __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_co
     if (!beam_open(a, row)) return;
     if (tid == 0) count = 0;
     const T* x = static_cast<const T*>(a.x) + row * a.ld;
-    const int shift = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));    // elements of the first vector before the row
-    const T* grid = x - shift;
-    const int64_t n_vec = (shift + a.V + E - 1) / E;
+    const int off = (int)(reinterpret_cast<uintptr_t>(x) & 15);       // bytes by which the row is off 16-byte alignment
+    const int64_t n_vec = (a.V + E - 1) / E;
     const int64_t begin = (int64_t)blockIdx.x * a.per, end = begin + a.per < n_vec ? begin + a.per : n_vec;
 
+    const uint4 none = DT == NT_F32 ? make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u)
+                                    : make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
     auto value = [](const uint4& w, int e) {
         const uint32_t* u = reinterpret_cast<const uint32_t*>(&w);
         return DT == NT_F32 ? __uint_as_float(u[e]) : __uint_as_float(e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16);
@@ -119,16 +151,8 @@ __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_co
         uint4 raw[kBeamVecs];
 #pragma unroll
         for (int j = 0; j < kBeamVecs; ++j) {
-            const int64_t v = v0 + j * kBeamThreads + tid, at = v * E - shift;
-            if (v < end && at >= 0 && at + E <= a.V) {
-                raw[j] = __ldcs(reinterpret_cast<const uint4*>(grid + v * E));
-            } else {                                    // outside, or across an end of the row
-                uint32_t* u = reinterpret_cast<uint32_t*>(&raw[j]);
-                u[0] = u[1] = u[2] = u[3] = DT == NT_F32 ? 0xff800000u : 0xff80ff80u;
-                if (v < end)
-                    for (int e = 0; e < E; ++e)
-                        if (at + e >= 0 && at + e < a.V) reinterpret_cast<T*>(u)[e] = x[at + e];
-            }
+            const int64_t v = v0 + j * kBeamThreads + tid;
+            raw[j] = v < end ? beam_load<T>(x, off, v * E, a.V) : none;
         }
         float best = -INFINITY;
 #pragma unroll
@@ -171,7 +195,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_co
                     const float f = value(raw[j], e);
                     if (f >= bound && f > -INFINITY) {
                         const int at = atomicAdd(&count, 1);
-                        if (at < kBeamList) list[at] = beam_key(f, (uint32_t)((v0 + j * kBeamThreads + tid) * E + e - shift));
+                        if (at < kBeamList) list[at] = beam_key(f, (uint32_t)((v0 + j * kBeamThreads + tid) * E + e));
                     }
                 }
         }
@@ -190,7 +214,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_co
                     for (int e = 0; e < E; ++e) {
                         const float f = value(raw[j], e);
                         if (f > -INFINITY) {
-                            const unsigned long long c = beam_key(f, (uint32_t)((v0 + j * kBeamThreads + tid) * E + e - shift));
+                            const unsigned long long c = beam_key(f, (uint32_t)((v0 + j * kBeamThreads + tid) * E + e));
                             if (c < prev && c > k) k = c;
                         }
                     }
@@ -383,7 +407,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
 // of an item than the joining kernel holds.
 struct BeamPlan { int slices, per; int64_t bytes; };
 BeamPlan beam_plan(int64_t B, int64_t K, int64_t V, int64_t n, int es) {
-    const int64_t n_vec = (V + 2 * (16 / es) - 2) / (16 / es), rows = B * K;
+    const int64_t n_vec = (V + 16 / es - 1) / (16 / es), rows = B * K;
     int64_t s = std::max<int64_t>(1, 148 * 4 / std::max<int64_t>(1, rows));
     s = std::min({s, (n_vec + kBeamThreads - 1) / kBeamThreads, (int64_t)kBeamLists / K, (int64_t)64});
     s = std::max<int64_t>(1, s);
