@@ -425,8 +425,7 @@ NT_API int nt_kv_copy_pages(int64_t n_layers, const int64_t* layers, int64_t n_p
  * `groups` groups of B / groups consecutive ones, and the first shared[g] (int32)
  * positions of a group's sequences hold the same keys and values, in each one's own
  * pages, which may be the same; they are read once for all of them, from one's pages.
- * Results and everything else as nt_kv_attention; a bad shared[g] counts as 0 and
- * sets the bad-argument bit.
+ * Results and everything else as nt_kv_attention (shared[g] < 0 counts as 0).
  * Workspace: nt_kv_attention_shared_workspace_bytes(). */
 NT_API int64_t nt_kv_attention_shared_workspace_bytes(int dtype, int64_t B, int64_t groups, int64_t T, int64_t Hq, int64_t Hkv,
                                                       int64_t D, int64_t page, int64_t n_blocks, int64_t window);
