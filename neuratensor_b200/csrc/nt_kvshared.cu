@@ -15,14 +15,15 @@
 // two; a float32 query is a pair of f16 (22 bits) and takes its product twice.  The block
 // scales of K multiply scores, in the softmax.  V becomes bf16 with its block's scale, exactly
 // (four significant bits), and the weights, which lie in any range, two bf16 (16 bits, for
-// bf16 outputs) or three (24 bits).  Weights are 1 at the row's reference, which follows
-// its maximum when that is 2^8 larger, and values are divided by 2^32, so that sums of finite
-// ones stay finite; values below 2^-94 lose bits by it, 2^-102 at most.
+// bf16 outputs) or three (24 bits).  Weights are 1 at the row's reference, which moves to
+// a block's maximum when the block's weights come to more than 2^10, and values are divided by
+// 2^32, so that sums of finite ones stay finite; values below 2^-94 lose bits by it, 2^-102 at most.
 //
 // A CTA: four warps of softmax (a thread a row), of which one thread issues the products, and
-// four that load codes one tile ahead, convert them and write the operands (K as it lies, V
+// eight that load codes one tile ahead, convert them and write the operands (K as it lies, V
 // transposed by stmatrix, its dimensions in an order of their own that the join undoes).  Two
-// CTAs share an SM where they fit, so that one's products run under the other's softmax.  The
+// CTAs share an SM where they fit, so that one's products run under the other's softmax; the
+// softmax warps take registers from the others.  The
 // tiles of all groups and heads in a row are cut into even shares, one a CTA.
 #include "nt_kvattn.cuh"
 
@@ -36,20 +37,22 @@ using namespace kva;
 constexpr int kSRows = 128;            // query rows of a tile
 constexpr int kSKeys = 128;            // keys of a tile
 constexpr int kSGroups = 512;          // groups of a call
-constexpr int kSoftWarps = 4, kLoadWarps = 4;
+constexpr int kSoftWarps = 4, kLoadWarps = 8;
 constexpr int kSThreads = 32 * (kSoftWarps + kLoadWarps);
 constexpr float kSUp = 4294967296.f;   // 2^32: values are held divided by it
-constexpr float kSLag = 8.f;           // a maximum this much (log2) above the reference moves it
+constexpr float kSMost = 1024.f;       // a block's weights that come to more move the reference to their maximum
 
 struct SharedArgs {
     KvAttnArgs a;                      // a.part: the rest's partial rows
     int B, groups, K;                  // sequences, groups, sequences of a group
-    int rows, row_tiles, rows_cap;     // query rows of a cached head of a group, tiles of them, rows of a partial tile
+    int rows, row_tiles, rows_cap;     // query rows of a cached head of a group, tiles of them, rows of a tile at most
+    int copies;                        // of a tile's rows among the 128: each takes its part of a tile's keys
     int64_t stride;                    // floats of a partial tile
     int ctas;
     const int32_t* shared;
     int64_t* info;                     // [groups][2]: tiles per head before the group, lo | hi << 32; then the total
-    float* part;                       // partial tiles: [rows_cap][D] means, [rows_cap] references, [rows_cap] totals
+    int32_t* rest_info;                // in even shares: tiles per head of the rest before each sequence, and the total
+    float* part;                       // partial tiles: [copies * rows_cap][D] means, as many references and totals
 };
 
 // The keys [lo, hi) that the rows of a group have in common and all see, in whole tiles of 16.
@@ -127,26 +130,49 @@ __device__ __forceinline__ uint64_t s_desc(uint32_t addr) {
 __host__ __device__ constexpr uint32_t s_idesc(uint32_t type, int N) {
     return 1u << 4 | type << 7 | type << 10 | (uint32_t)(N >> 3) << 17 | (uint32_t)(kSRows >> 4) << 24;
 }
-// 32 lanes x 32 columns, a thread a lane
-__device__ __forceinline__ void s_ld32(uint32_t at, float (&v)[32]) {
-    uint32_t r[32];
+// 32 lanes x 16 columns, a thread a lane: asked for, and waited for
+__device__ __forceinline__ void s_ld16(uint32_t at, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(at));
+}
+// the registers pass through, so that nothing reads them before
+__device__ __forceinline__ void s_ld_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :: "memory");
+}
+// the same, 32 columns
+__device__ __forceinline__ void s_ld32(uint32_t at, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(at));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void s_ld_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :: "memory");
 }
 __device__ __forceinline__ void s_st16(uint32_t at, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
         ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
           "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(at) : "memory");
+}
+__device__ __forceinline__ void s_ld8(uint32_t at, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(at));
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]) :: "memory");
+}
+__device__ __forceinline__ void s_st8(uint32_t at, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(at) : "memory");
 }
 __device__ __forceinline__ uint32_t pack_b2(float lo, float hi) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
@@ -160,7 +186,10 @@ __device__ __forceinline__ void s_stmatrix_t(uint32_t at, uint32_t m0, uint32_t 
 // Where a dimension's sum stands among the columns: the order in which stmatrix leaves V's dimensions.
 __host__ __device__ constexpr int column_of(int d) { return (d & ~63) + (d % 16 / 2) * 8 + (d % 64 / 16) * 2 + (d & 1); }
 
-struct SharedBars { uint64_t k_full, v_full, s_full, p_full, o_done, q_full; };
+constexpr int kSBlocks = kSKeys / kTile;               // blocks of 16 keys of a tile
+struct SharedBars { uint64_t k_full, v_full, s_full, p_full, o_done, q_full, found[4]; };
+// Where a tile's blocks lie (in elements of the codes, < 0: not to be seen) and their scales (of K < 0 then).
+struct SharedBlocks { int64_t off[kSBlocks]; float ks[kSBlocks], vs[kSBlocks]; };
 
 template <int DT, int D>
 __global__ void __launch_bounds__(kSThreads, SharedCfg<DT, D>::kPerSm) kv_shared_kernel(const __grid_constant__ SharedArgs s) {
@@ -170,7 +199,8 @@ __global__ void __launch_bounds__(kSThreads, SharedCfg<DT, D>::kPerSm) kv_shared
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ SharedBars bars;
     __shared__ uint32_t tmem_base;
-    __shared__ float k_scale[2][kSKeys / kTile];        // of a tile's blocks of 16 keys; < 0: not to be seen
+    __shared__ SharedBlocks blocks[4];                  // of tiles t, t + 1, ...
+    __shared__ float row_scale[kSRows];                 // what a row's scores are multiplied by, besides their block's scale
     __shared__ int64_t before[kSGroups + 1];            // tiles per head ahead of a group
     __shared__ int c_lo[kSGroups], c_hi[kSGroups], c_lead[kSGroups];
     const KvAttnArgs& a = s.a;
@@ -236,6 +266,7 @@ __global__ void __launch_bounds__(kSThreads, SharedCfg<DT, D>::kPerSm) kv_shared
         mbar_init(smem_u32(&bars.p_full), kSoftWarps);
         mbar_init(smem_u32(&bars.o_done), 1);
         mbar_init(smem_u32(&bars.q_full), kSoftWarps);
+        for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&bars.found[i]), 2 * kSBlocks);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kSoftWarps) {
@@ -263,6 +294,7 @@ __global__ void __launch_bounds__(kSThreads, SharedCfg<DT, D>::kPerSm) kv_shared
     };
 
     if (warp < kSoftWarps) {
+        if constexpr (Cfg::kPerSm == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
         // ---------------- queries, softmax, results: a thread a row ----------------
         const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
         const uint32_t qs = smem_u32(q_smem), ks_smem = smem_u32(k_smem), vs_smem = smem_u32(v_smem);
@@ -271,70 +303,87 @@ __global__ void __launch_bounds__(kSThreads, SharedCfg<DT, D>::kPerSm) kv_shared
         for (int64_t at = begin; at < end && ok; ++seg) {
             const Segment e = segment(at, g);
             g = e.g;
-            const int row = e.rt * kSRows + tid, rows = min(kSRows, s.rows - e.rt * kSRows);
-            const bool busy = warp * 32 < rows;          // this warp has rows
-            float f_row = 0.f;
+            const int rows = min(kSRows, s.rows - e.rt * kSRows);
+            // a tile of 32 rows or fewer stands four times among the lanes, one of 64 twice: each copy takes a part of
+            // the keys' columns, and has a reference, a total and sums of its own
+            const int copy = warp / (4 / s.copies), row0 = warp % (4 / s.copies) * 32;
+            const bool busy = row0 < rows;               // this warp has rows
+            const int first_block = copy * (8 / s.copies), last_block = first_block + 8 / s.copies;
+            // Queries, a row by the lanes that hold eight of its elements each, in f16, scaled by a power of two so
+            // that the largest is in [2^13, 2^14); the scores' scale is positive, its sign the query's.
             {
-                const int beam = row / (a.T * a.G), t = row / a.G % a.T;
+                constexpr int LR = D / 8, RW = 32 / LR;  // lanes of a row, rows at a time
+                const int row = e.rt * kSRows + row0 + lane, beam = row / (a.T * a.G), t = row / a.G % a.T;
                 const int64_t b = (int64_t)e.g * s.K + beam;
                 int lo, hi;
-                const bool live = row < s.rows && common_of(s, (int)b, &lo, &hi) && t < (a.counts ? a.counts[b] : a.T);
-                const T* q = static_cast<const T*>(a.q) + (live ? b * a.q_sb + (int64_t)t * a.q_st + (int64_t)(e.h * a.G + row % a.G) * a.q_sh : 0);
-                auto read8 = [&](int d, float (&v)[8]) {
-                    if (!live) {
+                const bool live = row0 + lane < rows && common_of(s, (int)b, &lo, &hi) && t < (a.counts ? a.counts[b] : a.T);
+                // where lane's row lies, in elements; -1: no such row
+                const int64_t mine = live ? b * a.q_sb + (int64_t)t * a.q_st + (int64_t)(e.h * a.G + row % a.G) * a.q_sh : -1;
+                const int d = lane % LR * 8;
+#pragma unroll 1
+                for (int r0 = 0; r0 < 32; r0 += 4 * RW) {
+                    uint4 raw[4][sizeof(T) / 2];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-                    } else if (a.q_vec) {
-                        constexpr int E = 16 / (int)sizeof(T);
+                    for (int j = 0; j < 4; ++j) {
+                        const int64_t off = __shfl_sync(0xffffffffu, mine, r0 + j * RW + lane / LR);
+                        const T* q = static_cast<const T*>(a.q) + off + d;
 #pragma unroll
-                        for (int i = 0; i < 8; i += E) {
-                            const uint4 w = __ldg(reinterpret_cast<const uint4*>(q + d + i));
-                            const T* x = reinterpret_cast<const T*>(&w);
-#pragma unroll
-                            for (int j = 0; j < E; ++j) v[i + j] = El::to_f(x[j]);
+                        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+                            raw[j][i] = make_uint4(0, 0, 0, 0);
+                            if (off >= 0) {
+                                if (a.q_vec) raw[j][i] = __ldg(reinterpret_cast<const uint4*>(q) + i);
+                                else
+#pragma unroll 1
+                                    for (int x = 0; x < 16 / (int)sizeof(T); ++x) {
+                                        const uint32_t bits = sizeof(T) == 4 ? reinterpret_cast<const uint32_t*>(q)[4 * i + x]
+                                                                             : (uint32_t)reinterpret_cast<const uint16_t*>(q)[x];
+                                        const int word = sizeof(T) == 4 ? x : x / 2, at = sizeof(T) == 4 ? 0 : x % 2 * 16;
+                                        raw[j][i].x |= word == 0 ? bits << at : 0u;
+                                        raw[j][i].y |= word == 1 ? bits << at : 0u;
+                                        raw[j][i].z |= word == 2 ? bits << at : 0u;
+                                        raw[j][i].w |= word == 3 ? bits << at : 0u;
+                                    }
+                            }
                         }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = El::load(q + d + i);
                     }
-                };
-                float amax = 0.f;
-#pragma unroll 4
-                for (int d = 0; d < D; d += 8) {
-                    float v[8];
-                    read8(d, v);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float m = fabsf(v[i]);
-                        if (m <= 3.402823466e38f) amax = fmaxf(amax, m);
-                    }
-                }
-                // a power of two that brings the largest to [2^13, 2^14); the scores' scale is positive, its sign the query's
-                int x = 127 + 13 - (int)(__float_as_uint(amax) >> 23);
-                x = amax > 0.f ? (x > 126 ? 126 : x) : 0;
-                float up = __uint_as_float((uint32_t)(127 + x) << 23);
-                f_row = __uint_as_float((uint32_t)(127 - x) << 23) * fabsf(a.scale_log2);
-                if (a.scale_log2 < 0.f) up = -up;
-#pragma unroll 2
-                for (int d = 0; d < D; d += 8) {
-                    float v[8];
-                    read8(d, v);
-                    uint32_t hi[4], lo4[4];
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = warp * 32 + r0 + j * RW + lane / LR;
+                        float v[8], amax = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x0 = v[2 * i] * up, x1 = v[2 * i + 1] * up;
-                        hi[i] = pack_h2(x0, x1);
-                        const float2 r = unpack_h2(hi[i]);
-                        lo4[i] = pack_h2(x0 - r.x, x1 - r.y);
+                        for (int i = 0; i < 8; ++i) {
+                            const uint4 w4 = raw[j][DT == NT_F32 ? i / 4 : 0];
+                            const int k = DT == NT_F32 ? i % 4 : i / 2;
+                            const uint32_t u = k == 0 ? w4.x : k == 1 ? w4.y : k == 2 ? w4.z : w4.w;
+                            v[i] = __uint_as_float(DT == NT_F32 ? u : i & 1 ? u & 0xffff0000u : u << 16);
+                            const float m = fabsf(v[i]);
+                            if (m <= 3.402823466e38f) amax = fmaxf(amax, m);
+                        }
+#pragma unroll
+                        for (int o = 1; o < LR; o *= 2) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                        int x = 127 + 13 - (int)(__float_as_uint(amax) >> 23);
+                        x = amax > 0.f ? (x > 126 ? 126 : x) : 0;
+                        float up = __uint_as_float((uint32_t)(127 + x) << 23);
+                        if (lane % LR == 0) row_scale[r] = __uint_as_float((uint32_t)(127 - x) << 23) * fabsf(a.scale_log2);
+                        if (a.scale_log2 < 0.f) up = -up;
+                        uint32_t hi4[4], lo4[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x0 = v[2 * i] * up, x1 = v[2 * i + 1] * up;
+                            hi4[i] = pack_h2(x0, x1);
+                            const float2 rest = unpack_h2(hi4[i]);
+                            lo4[i] = pack_h2(x0 - rest.x, x1 - rest.y);
+                        }
+                        const int at8 = (d / 64) * (kSRows * 128) + r * 128 + (((d % 64 / 8) ^ (r & 7)) << 4);
+                        *reinterpret_cast<uint4*>(q_smem + at8) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
+                        if constexpr (Cfg::NQ == 2) *reinterpret_cast<uint4*>(q_smem + Cfg::kQ + at8) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
                     }
-                    const int at8 = (d / 64) * (kSRows * 128) + tid * 128 + (((d % 64 / 8) ^ (tid & 7)) << 4);
-                    *reinterpret_cast<uint4*>(q_smem + at8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if constexpr (Cfg::NQ == 2) *reinterpret_cast<uint4*>(q_smem + Cfg::kQ + at8) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&bars.q_full));
+            const float f_row = row_scale[tid];
 
             float m = -INFINITY, l = 0.f;               // reference (log2) and total
             for (int tile = e.first; tile < e.last; ++tile, ++it) {
@@ -363,71 +412,94 @@ __global__ void __launch_bounds__(kSThreads, SharedCfg<DT, D>::kPerSm) kv_shared
                 }
                 s_fence_after();
                 if (busy) {
-                    const float* ks = k_scale[it & 1];
-                    float mx = -INFINITY;
+                    const float* ks = blocks[it & 3].ks;
+                    // Two blocks of 16 keys at a time, the next ones' scores on their way: a block's weights go where its
+                    // scores lie, 8 columns a piece.  The other copies' keys have none here.
+                    uint32_t v[32];
+                    s_ld32(lanes + first_block * 16, v);
+                    if (s.copies > 1) {
+                        uint32_t zero[16];
 #pragma unroll
-                    for (int c = 0; c < kSKeys / 32; ++c) {
-                        float v[32];
-                        s_ld32(lanes + c * 32, v);
-#pragma unroll
-                        for (int n = 0; n < 2; ++n) {
-                            const float k = ks[2 * c + n];
-                            if (k >= 0.f) {
-                                float x = v[16 * n];
-#pragma unroll
-                                for (int i = 1; i < 16; ++i) x = fmaxf(x, v[16 * n + i]);
-                                mx = fmaxf(mx, x * (f_row * k));
-                            }
+                        for (int i = 0; i < 16; ++i) zero[i] = 0u;
+#pragma unroll 1
+                        for (int c = 0; c < kSBlocks; ++c) {
+                            if (c >= first_block && c < last_block) continue;
+                            s_st16(lanes + c * 16, zero);
+                            if constexpr (Cfg::NP == 3) s_st8(lanes + Cfg::kCol3 + c * 8, *reinterpret_cast<uint32_t (*)[8]>(zero));
                         }
                     }
-                    const bool move = mx > m + kSLag;
-                    if (__any_sync(0xffffffffu, move)) {
-                        const float next = move ? mx : m, f = m == -INFINITY ? 0.f : ex2(m - next);
-                        const float by = move ? f : 1.f;
-                        if (tile > e.first) {
+#pragma unroll 1
+                    for (int c = first_block; c < last_block; c += 2) {
+                        const float k0 = ks[c], k1 = ks[c + 1];
+                        // a block that is not seen has no weight
+                        const float f[2] = {k0 >= 0.f ? f_row * k0 : 0.f, k1 >= 0.f ? f_row * k1 : 0.f};
+                        const bool seen = k0 >= 0.f || k1 >= 0.f;
+                        float p[32], sum;
+                        auto weigh = [&]() {
+                            const float at = m == -INFINITY ? 0.f : m, base[2] = {k0 < 0.f ? INFINITY : at, k1 < 0.f ? INFINITY : at};
+                            float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                            for (int c = 0; c < D / 32; ++c) {
-                                float v[32];
-                                s_ld32(lanes + Cfg::kColO + c * 32, v);
-                                uint32_t w[16];
+                            for (int i = 0; i < 32; ++i) {
+                                p[i] = ex2(fmaf(__uint_as_float(v[i]), f[i / 16], -base[i / 16]));
+                                part[i & 3] += p[i];
+                            }
+                            sum = (part[0] + part[1]) + (part[2] + part[3]);
+                        };
+                        s_ld_wait(v);
+                        weigh();
+                        // the reference is far below the blocks' maximum (or there is none yet, or a NaN)
+                        if (__any_sync(0xffffffffu, seen && (!(sum <= kSMost) || m == -INFINITY))) {
+                            float x[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                                for (int n = 0; n < 2; ++n) {
+                            for (int i = 0; i < 32; ++i) x[i / 16] = fmaxf(x[i / 16], __uint_as_float(v[i]));
+                            const float mx = fmaxf(k0 >= 0.f ? x[0] * f[0] : -INFINITY, k1 >= 0.f ? x[1] * f[1] : -INFINITY);
+                            // to a whole number, so that what is there already is multiplied by a power of two
+                            const bool move = mx > m;
+                            const float next = move ? ceilf(mx) : m;
+                            const float by = !move ? 1.f : next - m < 126.f ? __uint_as_float((uint32_t)(127 - (int)(next - m)) << 23) : 0.f;
+                            m = next;
+                            l *= by;
+                            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                            const __nv_bfloat162 by2 = __floats2bfloat162_rn(by, by);
+                            auto scale = [&](int col, bool packed) {        // 8 columns
+                                uint32_t w[8];
+                                s_ld8(lanes + col, w);
 #pragma unroll
-                                    for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[16 * n + i] * by);
-                                    s_st16(lanes + Cfg::kColO + c * 32 + 16 * n, w);
+                                for (int i = 0; i < 8; ++i) {
+                                    const __nv_bfloat162 y = __hmul2_rn(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), by2);
+                                    w[i] = packed ? *reinterpret_cast<const uint32_t*>(&y) : __float_as_uint(__uint_as_float(w[i]) * by);
                                 }
-                            }
+                                s_st8(lanes + col, w);
+                            };
+                            if (tile > e.first)
+#pragma unroll 1
+                                for (int d = 0; d < D; d += 8) scale(Cfg::kColO + d, false);
+#pragma unroll 1
+                            for (int col = first_block * 2; col < c * 2; ++col) scale(col * 8, true);
+                            if constexpr (Cfg::NP == 3)
+#pragma unroll 1
+                                for (int col = first_block; col < c; ++col) scale(Cfg::kCol3 + col * 8, true);
+                            weigh();
                         }
-                        l *= by;
-                        m = next;
-                    }
-                    const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-                    for (int c = 0; c < kSKeys / 32; ++c) {
-                        float v[32];
-                        s_ld32(lanes + c * 32, v);
-                        uint32_t w0[16], w1[16], w2[16];
+                        l += sum;
+                        if (c + 2 < last_block) s_ld32(lanes + (c + 2) * 16, v);
 #pragma unroll
                         for (int n = 0; n < 2; ++n) {
-                            const float k = ks[2 * c + n], f = f_row * k;
-                            const bool seen = k >= 0.f;
+                            uint32_t w[16], w2[8];
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
-                                const float p0 = seen ? ex2(fmaf(v[16 * n + 2 * i], f, -base)) : 0.f;
-                                const float p1 = seen ? ex2(fmaf(v[16 * n + 2 * i + 1], f, -base)) : 0.f;
-                                l += p0 + p1;
+                                const float p0 = p[16 * n + 2 * i], p1 = p[16 * n + 2 * i + 1];
                                 const uint32_t h = pack_b2(p0, p1);
                                 const float r0 = p0 - __uint_as_float(h << 16), r1 = p1 - __uint_as_float(h & 0xffff0000u);
                                 const uint32_t h2 = pack_b2(r0, r1);
-                                w0[8 * n + i] = h;
-                                w1[8 * n + i] = h2;
+                                w[i] = h;
+                                w[8 + i] = h2;
                                 if constexpr (Cfg::NP == 3)
-                                    w2[8 * n + i] = pack_b2(r0 - __uint_as_float(h2 << 16), r1 - __uint_as_float(h2 & 0xffff0000u));
+                                    w2[i] = pack_b2(r0 - __uint_as_float(h2 << 16), r1 - __uint_as_float(h2 & 0xffff0000u));
                             }
+                            s_st16(lanes + (c + n) * 16, w);
+                            if constexpr (Cfg::NP == 3) s_st8(lanes + Cfg::kCol3 + (c + n) * 8, w2);
                         }
-                        s_st16(lanes + c * 32, w0);
-                        s_st16(lanes + c * 32 + 16, w1);
-                        if constexpr (Cfg::NP == 3) s_st16(lanes + Cfg::kCol3 + c * 16, w2);
                     }
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
@@ -441,7 +513,7 @@ __global__ void __launch_bounds__(kSThreads, SharedCfg<DT, D>::kPerSm) kv_shared
                         for (int p = 0; p < Cfg::NP; ++p)
 #pragma unroll
                             for (int k = 0; k < kSKeys / 16; ++k)
-                                s_mma_ts(tmem + Cfg::kColO, tmem + (p == 2 ? Cfg::kCol3 + k * 8 : k / 2 * 32 + k % 2 * 8 + p * 16),
+                                s_mma_ts(tmem + Cfg::kColO, tmem + (p == 2 ? Cfg::kCol3 + k * 8 : k * 16 + p * 8),
                                          s_desc(vs_smem + k / 4 * (D * 128) + k % 4 * 32), s_idesc(1, D), tile > e.first || p || k);
                         s_commit(smem_u32(&bars.o_done));
                     } else {
@@ -457,121 +529,131 @@ __global__ void __launch_bounds__(kSThreads, SharedCfg<DT, D>::kPerSm) kv_shared
                 const int64_t slot = ((int64_t)e.g * a.H + e.h) * s.row_tiles + e.rt + blockIdx.x;
                 float* part = s.part + slot * s.stride;
                 const float inv = l != 0.f ? kSUp / l : 0.f;
+                const int r = copy * s.rows_cap + row0 + lane, n = s.copies * s.rows_cap;
+                const bool mine = row0 + lane < rows;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 16) {
+                    uint32_t w[16];
+                    s_ld16(lanes + Cfg::kColO + c, w);
+                    s_ld_wait(w);
+                    if (mine) {
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    float v[32];
-                    s_ld32(lanes + Cfg::kColO + c * 32, v);
-                    if (tid < rows) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<float4*>(part + tid * D + c * 32 + i) =
-                                make_float4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
+                        for (int i = 0; i < 16; i += 4)
+                            *reinterpret_cast<float4*>(part + r * D + c + i) =
+                                make_float4(__uint_as_float(w[i]) * inv, __uint_as_float(w[i + 1]) * inv, __uint_as_float(w[i + 2]) * inv,
+                                            __uint_as_float(w[i + 3]) * inv);
                     }
                 }
-                if (tid < rows) {
-                    part[s.rows_cap * D + tid] = m;
-                    part[s.rows_cap * D + s.rows_cap + tid] = l * (float)(1 << (int)kPShift);      // as attend() leaves it
+                if (mine) {
+                    part[n * D + r] = m;
+                    part[n * D + n + r] = l * (float)(1 << (int)kPShift);      // as attend() leaves it
                 }
             }
             s_fence_before();
             at += e.last - e.first;
         }
     } else {
+        // the launch's 384 threads have 80 registers each (30720): 128 x 112 and 256 x 64 of them
+        if constexpr (Cfg::kPerSm == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         // ---------------- codes: global memory -> registers -> operands ----------------
         constexpr int CH = D / 16;                      // 16-code pieces of a key
         constexpr int N = kSKeys * CH / (32 * kLoadWarps);      // of a thread, K and V each
         const int w = warp - kSoftWarps, lt = w * 32 + lane;
-        // the tile whose codes are in registers, and what lane j < 8 knows of its j-th block of 16 keys
-        struct Pages { int page; float ks, vs; };
-        uint4 kr[N], vr[N];
+        const int n_tiles = (int)(end - begin);
+        // The first of these warps looks up where blocks lie, a lane a block, for the tile three ahead of the one in
+        // work: its scales are on their way into shared memory while the next one's table entries are asked for.
+        Segment e = segment(begin, 0);
         int64_t at = begin;
-        Segment e = segment(at, 0);
-        auto advance = [&]() {                          // to the next tile; false behind the last
-            ++at;
-            if (at >= end) return false;
-            if (++e.first >= e.last) e = segment(at, e.g);
-            return true;
-        };
+        int entry = -2, slot = 0, head = 0;
         bool bad_page = false;
-        auto look_up = [&]() {
-            Pages p{-1, -1.f, 0.f};
+        auto ask_entry = [&]() {                        // -1: no page, -2: not wanted
+            entry = -2;
+            if (at >= end) return;
             const int key = c_lo[e.g] + e.first * kSKeys + lane * kTile;
-            if (lane < kSKeys / kTile && key < c_hi[e.g]) {
-                const int pg = a.table[(int64_t)c_lead[e.g] * a.table_sb + (key >> a.page_shift)];
-                if (pg < 0 || pg >= a.n_pages) {
-                    bad_page = true;
+            if (lane < kSBlocks && key < c_hi[e.g]) entry = max(__ldg(a.table + (int64_t)c_lead[e.g] * a.table_sb + (key >> a.page_shift)), -1);
+            slot = key & ((1 << a.page_shift) - 1);
+            head = e.h;
+            if (++at < end && ++e.first >= e.last) e = segment(at, e.g);
+        };
+        auto ask_scales = [&](int tile) {
+            if (lane < kSBlocks) {
+                SharedBlocks& to = blocks[tile & 3];
+                const bool there = entry >= 0 && entry < a.n_pages;
+                const int64_t row = (int64_t)entry * a.H + head;
+                to.off[lane] = there ? ((row << a.page_shift) + slot) * D : -1;
+                if (there) {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&to.ks[lane])), "l"(a.ks + row) : "memory");
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&to.vs[lane])), "l"(a.vs + row) : "memory");
                 } else {
-                    p.page = pg;
-                    p.ks = __ldg(a.ks + (int64_t)pg * a.H + e.h);
-                    p.vs = __ldg(a.vs + (int64_t)pg * a.H + e.h);
+                    to.ks[lane] = -1.f;
+                    to.vs[lane] = 0.f;
+                    if (entry != -2) bad_page = true;
                 }
+                // arrives when the lane's copies have landed, and for what it has written itself
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&bars.found[tile & 3])) : "memory");
+                mbar_arrive(smem_u32(&bars.found[tile & 3]));
             }
-            return p;
+            __syncwarp();
         };
+        if (w == 0)
+            for (int i = 0; i < 3; ++i) {
+                ask_entry();
+                ask_scales(i);
+            }
+        if (w == 0) ask_entry();
         // K piece j of a thread: key (j * threads + lt) / CH; V piece j of a warp: 8 keys x 64 dimensions, key of the lane's quarter
-        auto k_key = [&](int j) { return (j * 32 * kLoadWarps + lt) / CH; };
-        auto v_unit = [&](int j) { return j * kLoadWarps + w; };
-        auto code_at = [&](const uint8_t* codes, int pg, int key, int dim) {
-            const int slot = (c_lo[e.g] + e.first * kSKeys + key) & ((1 << a.page_shift) - 1);
-            return __ldg(reinterpret_cast<const uint4*>(codes + ((((int64_t)pg * a.H + e.h) << a.page_shift) + slot) * D + dim));
+        uint4 kr[N], vr[N];
+        auto fetch = [&](const uint8_t* codes, int tile, int key, int dim) {
+            const int64_t o = blocks[tile & 3].off[key / kTile];
+            uint4 r = make_uint4(0, 0, 0, 0);
+            if (o >= 0)
+                asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(codes + o + key % kTile * D + dim));
+            return r;
         };
-        auto load_k = [&](const Pages& p) {
+        auto load_k = [&](int tile) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) kr[j] = fetch(a.kc, tile, (j * 32 * kLoadWarps + lt) / CH, lt % CH * 16);
+        };
+        auto load_v = [&](int tile) {
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const int key = k_key(j), pg = __shfl_sync(0xffffffffu, p.page, key / kTile);
-                kr[j] = pg >= 0 ? code_at(a.kc, pg, key, lt % CH * 16) : make_uint4(0, 0, 0, 0);
+                const int u = j * kLoadWarps + w;
+                vr[j] = fetch(a.vc, tile, u / (D / 64) * 8 + lane / 4, u % (D / 64) * 64 + lane % 4 * 16);
             }
         };
-        auto load_v = [&](const Pages& p) {
+        bool ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.found[0]), 0));
+        if (ok) {
+            load_k(0);
+            load_v(0);
+        }
+        for (int it = 0; it < n_tiles && ok; ++it) {
+            const bool more = it + 1 < n_tiles;
+            ok = (it == 0 || __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.s_full), (it - 1) & 1))) &&
+                 (!more || __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.found[(it + 1) & 3]), ((it + 1) >> 2) & 1)));
+            if (!ok) break;
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const int u = v_unit(j), key = u / (D / 64) * 8 + lane / 4;
-                const int pg = __shfl_sync(0xffffffffu, p.page, key / kTile);
-                vr[j] = pg >= 0 ? code_at(a.vc, pg, key, u % (D / 64) * 64 + lane % 4 * 16) : make_uint4(0, 0, 0, 0);
-            }
-        };
-        Pages now = look_up(), next{};
-        load_k(now);
-        load_v(now);
-        bool more = true;
-        for (int it = 0; more; ++it) {
-            bool ok = it == 0 || __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.s_full), (it - 1) & 1));
-            if (!ok) {
-                if (lane == 0) atomicOr(a.err, ERRF_TIMEOUT_PRODUCER);
-                break;
-            }
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int key = k_key(j), c = lt % CH, panel = c / 4;
-                const uint32_t words[4] = {kr[j].x, kr[j].y, kr[j].z, kr[j].w};
+                const int key = (j * 32 * kLoadWarps + lt) / CH, c = lt % CH, panel = c / 4;
                 uint4 h[2];
-                h[0] = make_uint4(cvt_lo(words[0]), cvt_hi(words[0]), cvt_lo(words[1]), cvt_hi(words[1]));
-                h[1] = make_uint4(cvt_lo(words[2]), cvt_hi(words[2]), cvt_lo(words[3]), cvt_hi(words[3]));
+                h[0] = make_uint4(cvt_lo(kr[j].x), cvt_hi(kr[j].x), cvt_lo(kr[j].y), cvt_hi(kr[j].y));
+                h[1] = make_uint4(cvt_lo(kr[j].z), cvt_hi(kr[j].z), cvt_lo(kr[j].w), cvt_hi(kr[j].w));
                 unsigned char* base = k_smem + panel * (kSKeys * 128) + key * 128;
                 // panel 1 writes its odd chunk first, so that eight lanes meet eight banks
                 const int o = panel & 1, ch = c % 4 * 2;
                 *reinterpret_cast<uint4*>(base + (((ch + o) ^ (key & 7)) << 4)) = o ? h[1] : h[0];
                 *reinterpret_cast<uint4*>(base + (((ch + 1 - o) ^ (key & 7)) << 4)) = o ? h[0] : h[1];
             }
-            if (w == 0 && lane < kSKeys / kTile) k_scale[it & 1][lane] = now.ks;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&bars.k_full));
-            const float vs = now.vs * (1.f / kSUp);
-            more = advance();
-            if (more) {
-                next = look_up();
-                load_k(next);
-            }
+            if (more) load_k(it + 1);
             ok = it == 0 || __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars.o_done), (it - 1) & 1));
-            if (!ok) {
-                if (lane == 0) atomicOr(a.err, ERRF_TIMEOUT_PRODUCER);
-                break;
-            }
+            if (!ok) break;
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const int u = v_unit(j), ko = u / (D / 64), half = u % (D / 64);
-                const float f = __shfl_sync(0xffffffffu, vs, ko / 2);
+                const int u = j * kLoadWarps + w, ko = u / (D / 64), half = u % (D / 64);
+                const float f = blocks[it & 3].vs[ko / 2] * (1.f / kSUp);
                 const uint32_t words[4] = {vr[j].x, vr[j].y, vr[j].z, vr[j].w};
                 uint32_t b[8];
 #pragma unroll
@@ -588,11 +670,13 @@ __global__ void __launch_bounds__(kSThreads, SharedCfg<DT, D>::kPerSm) kv_shared
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&bars.v_full));
-            if (more) {
-                now = next;
-                load_v(now);
+            if (more) load_v(it + 1);
+            if (w == 0) {                               // what stood in these places was read for tile it - 1
+                ask_scales(it + 3);
+                ask_entry();
             }
         }
+        if (!ok && lane == 0) atomicOr(a.err, ERRF_TIMEOUT_PRODUCER);
         if (bad_page) atomicOr(a.err, ERRF_BAD_ARG);
     }
     s_fence_before();
@@ -637,7 +721,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) kv_rest_kernel(const __grid_co
 }
 
 // Tiles per head of the sequences before i, for i <= B, by all threads of a CTA, with the groups' common keys.
-__device__ __forceinline__ void rest_before(const SharedArgs& s, int* before, int* c_lo, int* c_hi, bool flag) {
+__device__ __forceinline__ void rest_before(const SharedArgs& s, int* before, int* c_lo, int* c_hi) {
     for (int g = threadIdx.x; g < s.groups; g += blockDim.x) {
         c_lo[g] = 0;
         c_hi[g] = 0x7fffffff;
@@ -666,7 +750,7 @@ __device__ __forceinline__ void rest_before(const SharedArgs& s, int* before, in
                 const int g = (i0 + lane) / s.K;
                 const Span e = rest_of(s, i0 + lane, 0, Common{c_lo[g], c_hi[g]});
                 n = e.tiles;
-                if (e.bad && flag) atomicOr(s.a.err, ERRF_BAD_ARG);
+                if (e.bad && blockIdx.x == 0) atomicOr(s.a.err, ERRF_BAD_ARG);
             }
 #pragma unroll
             for (int k = 1; k < 32; k *= 2) {
@@ -679,6 +763,8 @@ __device__ __forceinline__ void rest_before(const SharedArgs& s, int* before, in
         if (lane == 0) before[0] = 0;
     }
     __syncthreads();
+    if (blockIdx.x == 0)                                // for the join
+        for (int i = threadIdx.x; i <= s.B; i += blockDim.x) s.rest_info[i] = before[i];
 }
 
 // In even shares, for ragged sequences (see kv_attention_even_kernel): two partial rows a CTA.
@@ -688,7 +774,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) kv_rest_even_kernel(const __gr
     __shared__ int before[kEvenBatch + 1], c_lo[kEvenBatch], c_hi[kEvenBatch];
     const KvAttnArgs& a = s.a;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    rest_before(s, before, c_lo, c_hi, blockIdx.x == 0);
+    rest_before(s, before, c_lo, c_hi);
     const int64_t total = (int64_t)before[s.B] * a.H, share = share_of(total, gridDim.x);
     const int64_t begin = blockIdx.x * share, end = begin + share < total ? begin + share : total;
     // a share can hold many short heads, so each has a slot of its own: head and CTA counted together
@@ -710,58 +796,57 @@ __global__ void __launch_bounds__(W * 32, 16 / W) kv_rest_even_kernel(const __gr
 // Joins a query row's parts: those of the shared tiles, then those of the rest.
 // ---------------------------------------------------------------------------
 constexpr int kSJoinWarps = 8;
-template <int DT, int D, bool EVEN>
+// W warps a row: one where there are rows enough, which needs no barrier, else all of a CTA.
+template <int DT, int D, bool EVEN, int W>
 __global__ void __launch_bounds__(kSJoinWarps * 32) kv_shared_join_kernel(const __grid_constant__ SharedArgs s, int rest_ctas) {
     using El = Elem<DT>;
     using T = typename El::T;
     constexpr int E = D / 32;
     const KvAttnArgs& a = s.a;
-    const int heads = a.H * a.G, t = blockIdx.x / heads, hq = blockIdx.x % heads, h = hq / a.G;
-    const int64_t b = blockIdx.z;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = a.H * a.G;
+    const int64_t at = (int64_t)blockIdx.x * (kSJoinWarps / W) + warp / W;      // row (b, t, head)
+    if (at >= (int64_t)s.B * a.T * heads) return;       // a whole CTA when W is all its warps
+    const int hq = (int)(at % heads), t = (int)(at / heads % a.T), h = hq / a.G;
+    const int64_t b = at / heads / a.T;
     const int g = (int)b / s.K, beam = (int)b % s.K;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kPart = kRows * (D + 2);
+    const int len = a.lengths[b], cnt = a.counts ? a.counts[b] : a.T;
+    const bool live = cnt > 0 && t < cnt && cnt <= a.T && len >= cnt && len <= (a.n_blocks << a.page_shift);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t info0 = s.info[2 * g], info1 = s.info[2 * g + 1], info2 = s.info[2 * g + 2];
-    const Common c{(int)(uint32_t)info1, (int)(info1 >> 32)};
-    const int cnt = a.counts ? a.counts[b] : a.T;
     // the shared tiles
-    const int srow = (beam * a.T + t) * a.G + hq % a.G, rt = srow / kSRows;
+    const int srow = (beam * a.T + t) * a.G + hq % a.G, rt = srow / kSRows, r1 = srow % kSRows;
     const int64_t per_head = (int64_t)a.H * s.row_tiles, share = (s.info[2 * s.groups] * per_head + s.ctas - 1) / s.ctas;
     const int64_t tiles = info2 - info0, item = (int64_t)g * per_head + (int64_t)h * s.row_tiles + rt;
-    int n1 = 0;
-    const int64_t step1 = s.stride;
+    int n1 = 0, n2 = 0;
     const float* part1 = s.part;
     if (tiles > 0) {
         const int64_t g0 = info0 * per_head + ((int64_t)h * s.row_tiles + rt) * tiles, c0 = g0 / share;
-        n1 = (int)((g0 + tiles - 1) / share - c0 + 1);
-        part1 += (item + c0) * step1;
+        n1 = (int)((g0 + tiles - 1) / share - c0 + 1) * s.copies;
+        part1 += (item + c0) * s.stride;
     }
-    const int r1 = srow % kSRows;
     // the rest
     const int row = t * a.G + hq % a.G, row_tile = row / kRows, r2 = row % kRows;
-    int n2 = 0;
     const float* part2 = a.part;
     if constexpr (EVEN) {
-        __shared__ int before[kEvenBatch + 1], c_lo[kEvenBatch], c_hi[kEvenBatch];
-        rest_before(s, before, c_lo, c_hi, false);
-        const int64_t sh = share_of((int64_t)before[s.B] * a.H, rest_ctas);
-        const int n = before[b + 1] - before[b];
+        const int first = s.rest_info[b], n = s.rest_info[b + 1] - first;
+        const int64_t sh = share_of((int64_t)s.rest_info[s.B] * a.H, rest_ctas);
         if (n > 0) {
-            const int64_t g0 = (int64_t)before[b] * a.H + (int64_t)h * n, c0 = g0 / sh;
+            const int64_t g0 = (int64_t)first * a.H + (int64_t)h * n, c0 = g0 / sh;
             n2 = (int)((g0 + n - 1) / sh - c0 + 1);
             part2 += (b * a.H + h + c0) * kPart;
         }
     } else {
-        const Span e = rest_of(s, b, row_tile, c);
+        const Span e = rest_of(s, b, row_tile, Common{(int)(uint32_t)info1, (int)(info1 >> 32)});
         n2 = (e.tiles + a.chunk - 1) / a.chunk;
         part2 += (b * (int64_t)(a.H * a.row_tiles) + h * a.row_tiles + row_tile) * a.splits * kPart;
     }
-    const bool live = cnt > 0 && t < cnt && cnt <= a.T && a.lengths[b] >= cnt && a.lengths[b] <= (a.n_blocks << a.page_shift);
     const int n = live ? n1 + n2 : 0;
+    const int held = s.copies * s.rows_cap;              // rows of a partial tile
+    auto row_of = [&](int i) { return i % s.copies * s.rows_cap + r1; };
     auto ref_of = [&](int i, float* l) {
-        const float* p = i < n1 ? part1 + i * step1 + (int64_t)s.rows_cap * D + r1 : part2 + (int64_t)(i - n1) * kPart + kRows * D + r2;
-        *l = p[i < n1 ? s.rows_cap : kRows];
+        const float* p = i < n1 ? part1 + i / s.copies * s.stride + held * D + row_of(i) : part2 + (int64_t)(i - n1) * kPart + kRows * D + r2;
+        *l = p[i < n1 ? held : kRows];
         return *p;
     };
     // the row's reference and total: every warp takes them from all parts
@@ -784,46 +869,41 @@ __global__ void __launch_bounds__(kSJoinWarps * 32) kv_shared_join_kernel(const 
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = 0.f;
 #pragma unroll 4
-    for (int i = warp; i < n; i += kSJoinWarps) {
+    for (int i = warp % W; i < n; i += W) {
         float li;
         const float mi = ref_of(i, &li), f = ex2(mi - base) * li * inv;
-        float v[E];
-        if (i < n1) {
-            const float* p = part1 + i * step1 + (int64_t)r1 * D;
+        const bool shared = i < n1;
+        const float* p = shared ? part1 + i / s.copies * s.stride + row_of(i) * D : part2 + (int64_t)(i - n1) * kPart + r2 * D;
 #pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                const float2 x = *reinterpret_cast<const float2*>(p + column_of(lane * E + e));
-                v[e] = x.x;
-                v[e + 1] = x.y;
-            }
-        } else {
-            const float* p = part2 + (int64_t)(i - n1) * kPart + r2 * D + lane * E;
-#pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                const float2 x = *reinterpret_cast<const float2*>(p + e);
-                v[e] = x.x;
-                v[e + 1] = x.y;
-            }
+        for (int e = 0; e < E; e += 2) {
+            const float2 x = *reinterpret_cast<const float2*>(p + (shared ? column_of(lane * E + e) : lane * E + e));
+            sum[e] = fmaf(f, x.x, sum[e]);
+            sum[e + 1] = fmaf(f, x.y, sum[e + 1]);
         }
-#pragma unroll
-        for (int e = 0; e < E; ++e) sum[e] = fmaf(f, v[e], sum[e]);
     }
-    __shared__ float ws[kSJoinWarps][D];
+    if constexpr (W > 1) {
+        __shared__ float ws[kSJoinWarps][D];
 #pragma unroll
-    for (int e = 0; e < E; ++e) ws[warp][lane * E + e] = sum[e];
-    __syncthreads();
-    for (int d = threadIdx.x; d < D; d += kSJoinWarps * 32) {
-        float x = 0.f;
+        for (int e = 0; e < E; ++e) ws[warp][lane * E + e] = sum[e];
+        __syncthreads();
+        if (warp) return;
 #pragma unroll
-        for (int w = 0; w < kSJoinWarps; ++w) x += ws[w][d];
-        static_cast<T*>(a.out)[((b * a.T + t) * (int64_t)heads + hq) * D + d] = El::from_f(live && tot != 0.f ? x : 0.f);
+        for (int e = 0; e < E; ++e) {
+            sum[e] = 0.f;
+#pragma unroll
+            for (int w = 0; w < kSJoinWarps; ++w) sum[e] += ws[w][lane * E + e];
+        }
     }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        static_cast<T*>(a.out)[at * D + lane * E + e] = El::from_f(live && tot != 0.f ? sum[e] : 0.f);
 }
 
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-struct SharedPlan { bool use; Plan rest; int rows, row_tiles, rows_cap, ctas; int64_t stride, info, part, rest_part, bytes; };
+constexpr int64_t kSJoinRows = 1024;    // rows from which on a warp joins one alone
+struct SharedPlan { bool use; Plan rest; int rows, row_tiles, rows_cap, copies, ctas; int64_t stride, info, rest_info, part, rest_part, bytes; };
 
 SharedPlan shared_plan(int dtype, int64_t B, int64_t groups, int64_t T, int64_t G, int64_t H, int64_t D, int64_t page, int64_t n_blocks,
                        int64_t window) {
@@ -841,11 +921,13 @@ SharedPlan shared_plan(int dtype, int64_t B, int64_t groups, int64_t T, int64_t 
     const int64_t align = 256;
     auto up = [&](int64_t x) { return (x + align - 1) / align * align; };
     p.info = up((2 * groups + 2) * 8);
-    p.stride = (p.rows_cap * (D + 2) + 3) / 4 * 4;      // written 16 bytes at a time
+    p.rest_info = p.rest.even ? up((B + 1) * 4) : 0;
+    p.copies = p.rows_cap <= 32 ? 4 : p.rows_cap <= 64 ? 2 : 1;
+    p.stride = (p.copies * p.rows_cap * (D + 2) + 3) / 4 * 4;      // written 16 bytes at a time
     p.part = up((groups * H * p.row_tiles + p.ctas) * p.stride * 4);
     const int64_t slots = p.rest.even ? B * H + p.rest.even : B * H * p.rest.row_tiles * p.rest.splits;
     p.rest_part = up(slots * kRows * (D + 2) * 4);
-    p.bytes = p.info + p.part + p.rest_part;
+    p.bytes = p.info + p.rest_info + p.part + p.rest_part;
     return p;
 }
 
@@ -875,11 +957,19 @@ int launch_rest(const SharedArgs& s, const SharedPlan& p, cudaStream_t stream) {
     int ctas = p.rest.even;
     void* one[] = {&args};
     void* two[] = {&args, &ctas};
-    const dim3 join((unsigned)(s.a.T * s.a.H * s.a.G), 1, (unsigned)s.B);
+    const int64_t rows = (int64_t)s.B * s.a.T * s.a.H * s.a.G;
+    const bool one_warp = rows >= kSJoinRows;
+    const dim3 join((unsigned)(one_warp ? (rows + kSJoinWarps - 1) / kSJoinWarps : rows));
+    auto launch_join = [&](bool even) {
+        const void* f = one_warp ? (even ? (const void*)kv_shared_join_kernel<DT, D, true, 1> : (const void*)kv_shared_join_kernel<DT, D, false, 1>)
+                                 : (even ? (const void*)kv_shared_join_kernel<DT, D, true, kSJoinWarps>
+                                         : (const void*)kv_shared_join_kernel<DT, D, false, kSJoinWarps>);
+        return launch_after(f, "kv_shared_join_kernel", join, dim3(kSJoinWarps * 32), 0, two, stream);
+    };
     if constexpr (W == 2) {
         if (p.rest.even) {
             const int rc = launch_after((const void*)kv_rest_even_kernel<DT, D, W, HALF>, "kv_rest_even_kernel", dim3(ctas), dim3(W * 32), smem, one, stream);
-            return rc != NT_OK ? rc : launch_after((const void*)kv_shared_join_kernel<DT, D, true>, "kv_shared_join_kernel", join, dim3(kSJoinWarps * 32), 0, two, stream);
+            return rc != NT_OK ? rc : launch_join(true);
         }
     }
     if (smem > 48 * 1024) {
@@ -888,7 +978,7 @@ int launch_rest(const SharedArgs& s, const SharedPlan& p, cudaStream_t stream) {
     }
     const dim3 grid((unsigned)s.a.splits, (unsigned)(s.a.H * s.a.row_tiles), (unsigned)s.B);
     const int rc = launch_after((const void*)kv_rest_kernel<DT, D, W, HALF>, "kv_rest_kernel", grid, dim3(W * 32), smem, one, stream);
-    return rc != NT_OK ? rc : launch_after((const void*)kv_shared_join_kernel<DT, D, false>, "kv_shared_join_kernel", join, dim3(kSJoinWarps * 32), 0, two, stream);
+    return rc != NT_OK ? rc : launch_join(false);
 }
 
 template <int DT, int D>
@@ -941,7 +1031,7 @@ int nt_kv_attention_shared(int dtype, int64_t B, int64_t groups, int64_t T, int6
     if (!p.use)
         return nt_kv_attention(dtype, B, T, Hq, Hkv, D, page, n_pages, n_blocks, window, scale, q, q_sb, q_st, q_sh, k_codes, k_scale,
                                v_codes, v_scale, table, table_sb, lengths, counts, out, workspace, workspace_bytes, stream);
-    if (Hkv * p.rest.row_tiles > 65535 || T * Hq > INT32_MAX)
+    if (Hkv * p.rest.row_tiles > 65535 || B * T * Hq > INT32_MAX)
         return fail(NT_ERR_ARG, "nt_kv_attention_shared: %lld query rows in one call", (long long)(T * Hq));
     if (!workspace || workspace_bytes < p.bytes)
         return fail(NT_ERR_WORKSPACE, "nt_kv_attention_shared: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)p.bytes);
@@ -966,12 +1056,13 @@ int nt_kv_attention_shared(int dtype, int64_t B, int64_t groups, int64_t T, int6
     a.err = device_error_word(dev);
     if (!a.err) return fail(NT_ERR_CUDA, "nt_kv_attention_shared: error word unavailable");
     s.B = (int)B; s.groups = (int)groups; s.K = (int)(B / groups);
-    s.rows = p.rows; s.row_tiles = p.row_tiles; s.rows_cap = p.rows_cap; s.stride = p.stride; s.ctas = p.ctas;
+    s.rows = p.rows; s.row_tiles = p.row_tiles; s.rows_cap = p.rows_cap; s.copies = p.copies; s.stride = p.stride; s.ctas = p.ctas;
     s.shared = shared;
     char* ws = static_cast<char*>(workspace);
     s.info = reinterpret_cast<int64_t*>(ws);
-    s.part = reinterpret_cast<float*>(ws + p.info);
-    a.part = reinterpret_cast<float*>(ws + p.info + p.part);
+    s.rest_info = reinterpret_cast<int32_t*>(ws + p.info);
+    s.part = reinterpret_cast<float*>(ws + p.info + p.rest_info);
+    a.part = reinterpret_cast<float*>(ws + p.info + p.rest_info + p.part);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (dtype == NT_F32) return D == 64 ? launch_shared<NT_F32, 64>(s, p, st) : launch_shared<NT_F32, 128>(s, p, st);
     return D == 64 ? launch_shared<NT_BF16, 64>(s, p, st) : launch_shared<NT_BF16, 128>(s, p, st);
