@@ -849,11 +849,12 @@ __global__ void __launch_bounds__(kSJoinWarps * 32) kv_shared_join_kernel(const 
         *l = p[i < n1 ? held : kRows];
         return *p;
     };
-    // the row's reference and total: every warp takes them from all parts
-    float m = -INFINITY, tot = 0.f;
+    // the row's reference and total: every warp takes them from all parts, a lane a part
+    float m = -INFINITY, tot = 0.f, m_own = -INFINITY, l_own = 0.f;      // of part `lane`
     for (int i = lane; i < n; i += 32) {
         float li;
         const float mi = ref_of(i, &li), up = fmaxf(m, mi), base = up == -INFINITY ? 0.f : up;
+        if (i == lane) m_own = mi, l_own = li;
         tot = fmaf(ex2(mi - base), li, tot * ex2(m - base));
         m = up;
     }
@@ -868,17 +869,33 @@ __global__ void __launch_bounds__(kSJoinWarps * 32) kv_shared_join_kernel(const 
     float sum[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = 0.f;
-#pragma unroll 4
-    for (int i = warp % W; i < n; i += W) {
-        float li;
-        const float mi = ref_of(i, &li), f = ex2(mi - base) * li * inv;
-        const bool shared = i < n1;
-        const float* p = shared ? part1 + i / s.copies * s.stride + row_of(i) * D : part2 + (int64_t)(i - n1) * kPart + r2 * D;
+    // 32 parts at a time: their weights a lane each, then their rows, eight on their way
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        if (i0 && i0 + lane < n) m_own = ref_of(i0 + lane, &l_own);
+        const float f_own = i0 + lane < n ? ex2(m_own - base) * l_own * inv : 0.f;
+        const int upto = min(32, n - i0);
+        for (int j0 = warp % W; j0 < upto; j0 += 8 * W) {
+            float2 x[8][E / 2];
 #pragma unroll
-        for (int e = 0; e < E; e += 2) {
-            const float2 x = *reinterpret_cast<const float2*>(p + (shared ? column_of(lane * E + e) : lane * E + e));
-            sum[e] = fmaf(f, x.x, sum[e]);
-            sum[e + 1] = fmaf(f, x.y, sum[e + 1]);
+            for (int j = 0; j < 8; ++j) {
+                const int i = i0 + j0 + j * W;
+                const bool shared = i < n1;
+                const float* p = shared ? part1 + i / s.copies * s.stride + row_of(i) * D : part2 + (int64_t)(i - n1) * kPart + r2 * D;
+#pragma unroll
+                for (int e = 0; e < E; e += 2)
+                    x[j][e / 2] = j0 + j * W < upto ? *reinterpret_cast<const float2*>(p + (shared ? column_of(lane * E + e) : lane * E + e))
+                                                    : make_float2(0.f, 0.f);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float f = __shfl_sync(0xffffffffu, f_own, (j0 + j * W) & 31);
+                if (j0 + j * W < upto)
+#pragma unroll
+                    for (int e = 0; e < E; e += 2) {
+                        sum[e] = fmaf(f, x[j][e / 2].x, sum[e]);
+                        sum[e + 1] = fmaf(f, x[j][e / 2].y, sum[e + 1]);
+                    }
+            }
         }
     }
     if constexpr (W > 1) {
