@@ -29,13 +29,25 @@ struct KvAttnArgs {
     void* out;
     float* part;                       // partial rows: [kRows][D] means, [kRows] maxima, [kRows] totals
     unsigned* err;
+    int beams;                         // sequences whose rows are taken together (ROWS_TOGETHER)
 };
 
+// What attend() takes: the rows of one sequence; those, with keys left out and always to partial rows; or
+// the rows of several sequences over keys that all of them see, always to partial rows.
+enum { ROWS_OF_ONE = 0, ROWS_WITH_GAP = 1, ROWS_TOGETHER = 2 };
+
 // What the rows of one row tile see of their sequence: keys [lo, hi), in tiles from lo16.
-// skip, gap: `gap` keys behind the first `skip` tiles are left out (only where attend is told so).
-struct Span { int cnt, start, lo, hi, lo16, tiles; bool bad; int skip, gap; };
-template <bool GAP> __device__ __forceinline__ int key_of(const Span& s, int tile) {
-    return s.lo16 + tile * kTile + (GAP && tile >= s.skip ? s.gap : 0);
+// skip, gap: `gap` keys behind the first `skip` tiles are left out (ROWS_WITH_GAP); lead: the sequence whose
+// pages are read (ROWS_TOGETHER).
+struct Span { int cnt, start, lo, hi, lo16, tiles; bool bad; int skip, gap, lead; };
+template <int MODE> __device__ __forceinline__ int key_of(const Span& s, int tile) {
+    return s.lo16 + tile * kTile + (MODE == ROWS_WITH_GAP && tile >= s.skip ? s.gap : 0);
+}
+
+// New tokens of a sequence, 0 where its counts cannot be.
+__device__ __forceinline__ int tokens_of(const KvAttnArgs& a, int64_t b) {
+    const int len = a.lengths[b], cnt = a.counts ? a.counts[b] : a.T;
+    return cnt < 0 || cnt > a.T || len < cnt || len > (a.n_blocks << a.page_shift) ? 0 : cnt;
 }
 
 __device__ __forceinline__ Span span_of(const KvAttnArgs& a, int64_t b, int row_tile) {
@@ -108,9 +120,8 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
 // Tiles [first, last) of one row tile of head h, sequence b, by the W warps of a
 // CTA: the rows themselves when these are all of its tiles, else their means over
 // the tiles with their maxima and totals in `part`.  HALF: there are four rows or
-// fewer; columns 4..7 repeat them and take the weights' second halves.  GAP: the span
-// leaves keys out, and the rows always go to `part`.
-template <int DT, int D, int W, bool HALF, bool GAP = false>
+// fewer; columns 4..7 repeat them and take the weights' second halves.
+template <int DT, int D, int W, bool HALF, int MODE = ROWS_OF_ONE>
 __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, int row_tile, const Span& s, int first,
                                        int last, float* part, unsigned char* smem) {
     using El = Elem<DT>;
@@ -120,13 +131,14 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
     constexpr bool kPair = DT == NT_F32;       // a second product with what f16 leaves of q
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     constexpr int kMask = HALF ? 3 : 7;
-    const int row = row_tile * kRows + (g & kMask), t = row / a.G;
-    const bool live = t < s.cnt;
+    constexpr bool kTogether = MODE == ROWS_TOGETHER;
+    const int row = row_tile * kRows + (g & kMask), beam = kTogether ? row / a.G / a.T : 0, t = kTogether ? row / a.G % a.T : row / a.G;
+    const bool live = kTogether ? beam < a.beams && t < tokens_of(a, b + beam) : t < s.cnt;
     // in the products a lane holds rows 2c and 2c + 1: their positions
     const int t0 = (row_tile * kRows + ((2 * c) & kMask)) / a.G, t1 = (row_tile * kRows + ((2 * c + 1) & kMask)) / a.G;
-    const int p0 = t0 < s.cnt ? s.start + t0 : -1, p1 = t1 < s.cnt ? s.start + t1 : -1;
+    const int p0 = kTogether ? s.hi : t0 < s.cnt ? s.start + t0 : -1, p1 = kTogether ? s.hi : t1 < s.cnt ? s.start + t1 : -1;
     // every row of the CTA sees all of a tile when it lies in [all_lo, all_hi)
-    const int all_hi = s.start + row_tile * kRows / a.G + 1, all_lo = a.window >= 0 ? s.hi - 1 - a.window : 0;
+    const int all_hi = kTogether ? s.hi : s.start + row_tile * kRows / a.G + 1, all_lo = !kTogether && a.window >= 0 ? s.hi - 1 - a.window : 0;
 
     // o[j]: dimensions g*D/8 + 2j (rows 2c, 2c+1) and g*D/8 + 2j + 1 (the same rows), in units of v_unit
     float o[MT][4];
@@ -138,7 +150,7 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
     // page and the scales of the j-th of 32 tiles: f_* for the tiles being
     // fetched, c_* for those being computed, one behind.
     const int mine = last - first > warp ? (last - first - warp + W - 1) / W : 0;
-    const int32_t* table = a.table + b * a.table_sb;
+    const int32_t* table = a.table + (kTogether ? s.lead : b) * a.table_sb;
     int f_page = -1, c_page = -1;
     float f_ks = 0.f, f_vs = 0.f, c_ks = 0.f, c_vs = 0.f;
     bool bad_page = false;
@@ -148,7 +160,7 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
         if ((i & 31) == 0) {
             f_page = -1;
             if (i + lane < mine) {
-                const int pg = table[key_of<GAP>(s, first + warp + W * (i + lane)) >> a.page_shift];
+                const int pg = table[key_of<MODE>(s, first + warp + W * (i + lane)) >> a.page_shift];
                 if (pg < 0 || pg >= a.n_pages) {
                     bad_page = true;
                 } else {
@@ -160,7 +172,7 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
         }
         const int pg = __shfl_sync(0xffffffffu, f_page, i & 31);
         if (pg >= 0 && i < mine) {
-            const int slot = key_of<GAP>(s, first + warp + W * i) & ((1 << a.page_shift) - 1);
+            const int slot = key_of<MODE>(s, first + warp + W * i) & ((1 << a.page_shift) - 1);
             const int64_t off = ((((int64_t)pg * a.H + h) << a.page_shift) + slot) * D + lane * 16;
             const uint32_t dst = ring_u32 + (i % kStages) * (2 * kTileBytes<D>);
             constexpr int CH = D / 16;                  // chunks of a row
@@ -181,7 +193,7 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
     {
         float v[D / 64][16];
         float amax = 0.f;
-        const T* q = static_cast<const T*>(a.q) + b * a.q_sb + (int64_t)t * a.q_st + (int64_t)(h * a.G + row % a.G) * a.q_sh;
+        const T* q = static_cast<const T*>(a.q) + (b + beam) * a.q_sb + (int64_t)t * a.q_st + (int64_t)(h * a.G + row % a.G) * a.q_sh;
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
             if (!live) {
@@ -242,7 +254,7 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncwarp();                                   // every lane's part of tile i has landed
         if (__shfl_sync(0xffffffffu, c_page, i & 31) >= 0) {
-            const int key0 = key_of<GAP>(s, first + warp + W * i);
+            const int key0 = key_of<MODE>(s, first + warp + W * i);
             const unsigned char* kt = ring + (i % kStages) * (2 * kTileBytes<D>);
             const unsigned char* vt = kt + kTileBytes<D>;
             const float ks = __shfl_sync(0xffffffffu, c_ks, i & 31), vs = __shfl_sync(0xffffffffu, c_vs, i & 31);
@@ -457,8 +469,8 @@ __device__ __forceinline__ void attend(const KvAttnArgs& a, int64_t b, int h, in
         sl[warp][2 * c + 1] = l1;
     }
     __syncthreads();
-    const int rows = min(kRows, a.T * a.G - row_tile * kRows);
-    const bool alone = !GAP && last - first == s.tiles; // this CTA has seen all keys
+    const int rows = min(kRows, (kTogether ? a.beams : 1) * a.T * a.G - row_tile * kRows);
+    const bool alone = MODE == ROWS_OF_ONE && last - first == s.tiles;      // this CTA has seen all keys
     for (int i = threadIdx.x; i < rows * D; i += (W * 32)) {
         const int r = i / D, d = i % D;
         float mm = -INFINITY;

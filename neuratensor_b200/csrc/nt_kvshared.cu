@@ -59,8 +59,9 @@ struct SharedArgs {
 struct Common { int lo, hi; };
 // One sequence's part in it; a sequence without new tokens has none.
 __device__ __forceinline__ bool common_of(const SharedArgs& s, int b, int* lo, int* hi) {
-    const int len = s.a.lengths[b], cnt = s.a.counts ? s.a.counts[b] : s.a.T;
-    if (cnt <= 0 || cnt > s.a.T || len < cnt || len > (s.a.n_blocks << s.a.page_shift)) return false;
+    const int cnt = tokens_of(s.a, b);
+    if (cnt == 0) return false;
+    const int len = s.a.lengths[b];
     *lo = s.a.window >= 0 && len - 1 > s.a.window ? len - 1 - s.a.window : 0;
     *hi = len - cnt + 1;
     return true;
@@ -715,13 +716,14 @@ __global__ void __launch_bounds__(W * 32, 16 / W) kv_rest_kernel(const __grid_co
     const int first = split * a.chunk, last = min(first + a.chunk, e.tiles);
     if (first < e.tiles) {
         float* part = a.part + ((b * gridDim.y + blockIdx.y) * a.splits + split) * (kRows * (D + 2));
-        attend<DT, D, W, HALF, true>(a, b, h, row_tile, e, first, last, part, smem);
+        attend<DT, D, W, HALF, ROWS_WITH_GAP>(a, b, h, row_tile, e, first, last, part, smem);
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the join follows this kernel alone, and needs the one before too
 }
 
-// Tiles per head of the sequences before i, for i <= B, by all threads of a CTA, with the groups' common keys.
-__device__ __forceinline__ void rest_before(const SharedArgs& s, int* before, int* c_lo, int* c_hi) {
+// Tiles per head (and `more` for each) of the sequences before i, for i <= B, by all threads of a CTA, with the
+// groups' common keys.
+__device__ __forceinline__ void rest_before(const SharedArgs& s, int* before, int* c_lo, int* c_hi, int more = 0) {
     for (int g = threadIdx.x; g < s.groups; g += blockDim.x) {
         c_lo[g] = 0;
         c_hi[g] = 0x7fffffff;
@@ -749,7 +751,7 @@ __device__ __forceinline__ void rest_before(const SharedArgs& s, int* before, in
             if (i0 + lane < s.B) {
                 const int g = (i0 + lane) / s.K;
                 const Span e = rest_of(s, i0 + lane, 0, Common{c_lo[g], c_hi[g]});
-                n = e.tiles;
+                n = e.tiles ? e.tiles + more : 0;
                 if (e.bad && blockIdx.x == 0) atomicOr(s.a.err, ERRF_BAD_ARG);
             }
 #pragma unroll
@@ -785,7 +787,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W) kv_rest_even_kernel(const __gr
         const int64_t rel = at - (int64_t)before[b] * a.H;
         const int h = (int)(rel / e.tiles), first = (int)(rel - (int64_t)h * e.tiles);
         const int last = (int)(end - at < e.tiles - first ? first + (end - at) : e.tiles);
-        attend<DT, D, W, HALF, true>(a, b, h, 0, e, first, last, a.part + ((int64_t)b * a.H + h + blockIdx.x) * (kRows * (D + 2)), smem);
+        attend<DT, D, W, HALF, ROWS_WITH_GAP>(a, b, h, 0, e, first, last, a.part + ((int64_t)b * a.H + h + blockIdx.x) * (kRows * (D + 2)), smem);
         at += last - first;
         __syncthreads();                                // the sums are read before the next ring is filled
     }
@@ -793,11 +795,90 @@ __global__ void __launch_bounds__(W * 32, 16 / W) kv_rest_even_kernel(const __gr
 }
 
 // ---------------------------------------------------------------------------
+// Few rows a group: the shared part and the rest by attend(), in one kernel.  The shared
+// part takes the group's rows, eight at a time, as the columns of one product; all tiles
+// of both parts lie in a row (the groups' shared ones, then the sequences' rests) and are cut
+// into even shares of CTAs of two warps; a head, which takes as long to begin and to end as
+// kFewBegin tiles, counts as so many more.  Every head of either has a slot of its own for
+// each CTA that it reaches: its number and the CTA's, added up.
+// ---------------------------------------------------------------------------
+constexpr int kFewBegin = 12;
+template <int DT, int D, bool HALF_C, bool HALF_R>
+__global__ void __launch_bounds__(64, 8) kv_few_kernel(const __grid_constant__ SharedArgs s) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int before[kEvenBatch + 1], c_lo[kEvenBatch], c_hi[kEvenBatch], c_before[kEvenBatch + 1], c_lead[kEvenBatch];
+    const KvAttnArgs& a = s.a;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    for (int g = threadIdx.x; g < s.groups; g += 64) c_lead[g] = 0x7fffffff;
+    rest_before(s, before, c_lo, c_hi, kFewBegin);
+    for (int b = threadIdx.x; b < s.B; b += 64)
+        if (tokens_of(a, b)) atomicMin(&c_lead[b / s.K], b);
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x < 32) {
+        int sum = 0;
+        for (int i0 = 0; i0 < s.groups; i0 += 32) {
+            int n = i0 + lane < s.groups ? (c_hi[i0 + lane] - c_lo[i0 + lane]) / kTile : 0;
+            if (n) n += kFewBegin;
+#pragma unroll
+            for (int k = 1; k < 32; k *= 2) {
+                const int up = __shfl_up_sync(0xffffffffu, n, k);
+                if (lane >= k) n += up;
+            }
+            if (i0 + lane < s.groups) c_before[i0 + lane + 1] = sum + n;
+            sum += __shfl_sync(0xffffffffu, n, 31);
+        }
+        if (lane == 0) c_before[0] = 0;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0)
+        for (int g = threadIdx.x; g <= s.groups; g += 64) {
+            s.info[2 * g] = c_before[g];
+            if (g < s.groups) s.info[2 * g + 1] = (int64_t)c_hi[g] << 32 | (uint32_t)c_lo[g];
+        }
+    const int64_t per_head = (int64_t)a.H * s.row_tiles, common = c_before[s.groups] * per_head, total = common + (int64_t)before[s.B] * a.H;
+    const int64_t share = share_of(total, gridDim.x);
+    const int64_t begin = blockIdx.x * share, end = begin + share < total ? begin + share : total;
+    int g = 0, b = 0;
+    for (int64_t at = begin; at < end;) {
+        int64_t rel, item;
+        int units;                                      // of the head: its tiles and kFewBegin
+        const bool together = at < common;
+        Span e;
+        if (together) {
+            while (c_before[g + 1] * per_head <= at) ++g;
+            e.lo = e.lo16 = c_lo[g];
+            e.hi = c_hi[g];
+            e.lead = c_lead[g];
+            e.tiles = (e.hi - e.lo) / kTile;
+            units = c_before[g + 1] - c_before[g];
+            rel = at - c_before[g] * per_head;
+            item = g * per_head;
+        } else {
+            while (common + (int64_t)before[b + 1] * a.H <= at) ++b;
+            e = rest_of(s, b, 0, Common{c_lo[b / s.K], c_hi[b / s.K]});
+            units = before[b + 1] - before[b];
+            rel = at - common - (int64_t)before[b] * a.H;
+            item = s.groups * per_head + (int64_t)b * a.H;
+        }
+        const int n = (int)(rel / units), from = (int)(rel - (int64_t)n * units), to = (int)(end - at < units - from ? from + (end - at) : units);
+        const int first = max(from - kFewBegin, 0), last = to - kFewBegin;
+        if (last > 0) {
+            float* part = a.part + (item + n + blockIdx.x) * (kRows * (D + 2));
+            if (together) attend<DT, D, 2, HALF_C, ROWS_TOGETHER>(a, (int64_t)g * s.K, n / s.row_tiles, n % s.row_tiles, e, first, last, part, smem);
+            else attend<DT, D, 2, HALF_R, ROWS_WITH_GAP>(a, b, n, 0, e, first, last, part, smem);
+        }
+        at += to - from;
+        __syncthreads();                                // the sums are read before the next ring is filled
+    }
+}
+
+// ---------------------------------------------------------------------------
 // Joins a query row's parts: those of the shared tiles, then those of the rest.
 // ---------------------------------------------------------------------------
 constexpr int kSJoinWarps = 8;
 // W warps a row: one where there are rows enough, which needs no barrier, else all of a CTA.
-template <int DT, int D, bool EVEN, int W>
+enum { REST_IN_CHUNKS = 0, REST_IN_SHARES = 1, ALL_IN_SHARES = 2 };
+template <int DT, int D, int HOW, int W>
 __global__ void __launch_bounds__(kSJoinWarps * 32) kv_shared_join_kernel(const __grid_constant__ SharedArgs s, int rest_ctas) {
     using El = Elem<DT>;
     using T = typename El::T;
@@ -810,31 +891,39 @@ __global__ void __launch_bounds__(kSJoinWarps * 32) kv_shared_join_kernel(const 
     const int64_t b = at / heads / a.T;
     const int g = (int)b / s.K, beam = (int)b % s.K;
     constexpr int kPart = kRows * (D + 2);
-    const int len = a.lengths[b], cnt = a.counts ? a.counts[b] : a.T;
-    const bool live = cnt > 0 && t < cnt && cnt <= a.T && len >= cnt && len <= (a.n_blocks << a.page_shift);
+    const bool live = t < tokens_of(a, b);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t info0 = s.info[2 * g], info1 = s.info[2 * g + 1], info2 = s.info[2 * g + 2];
+    constexpr bool kFew = HOW == ALL_IN_SHARES;          // both parts in rows of eight
     // the shared tiles
-    const int srow = (beam * a.T + t) * a.G + hq % a.G, rt = srow / kSRows, r1 = srow % kSRows;
-    const int64_t per_head = (int64_t)a.H * s.row_tiles, share = (s.info[2 * s.groups] * per_head + s.ctas - 1) / s.ctas;
+    constexpr int kTileRows = kFew ? kRows : kSRows;
+    const int srow = (beam * a.T + t) * a.G + hq % a.G, rt = srow / kTileRows, r1 = srow % kTileRows;
+    const int64_t per_head = (int64_t)a.H * s.row_tiles, common = s.info[2 * s.groups] * per_head;
     const int64_t tiles = info2 - info0, item = (int64_t)g * per_head + (int64_t)h * s.row_tiles + rt;
+    int rest_first = 0, rest_n = 0, rest_all = 0;
+    if constexpr (HOW != REST_IN_CHUNKS) {
+        rest_first = s.rest_info[b];
+        rest_n = s.rest_info[b + 1] - rest_first;
+        rest_all = s.rest_info[s.B];
+    }
+    const int64_t share = kFew ? share_of(common + (int64_t)rest_all * a.H, rest_ctas) : (common + s.ctas - 1) / s.ctas;
+    constexpr int begin = kFew ? kFewBegin : 0;          // units of a head ahead of its tiles
     int n1 = 0, n2 = 0;
-    const float* part1 = s.part;
+    const float* part1 = kFew ? a.part : s.part;
     if (tiles > 0) {
-        const int64_t g0 = info0 * per_head + ((int64_t)h * s.row_tiles + rt) * tiles, c0 = g0 / share;
-        n1 = (int)((g0 + tiles - 1) / share - c0 + 1) * s.copies;
-        part1 += (item + c0) * s.stride;
+        const int64_t g0 = info0 * per_head + ((int64_t)h * s.row_tiles + rt) * tiles, c0 = (g0 + begin) / share;
+        n1 = (int)((g0 + tiles - 1) / share - c0 + 1) * (kFew ? 1 : s.copies);
+        part1 += (item + c0) * (kFew ? kPart : s.stride);
     }
     // the rest
     const int row = t * a.G + hq % a.G, row_tile = row / kRows, r2 = row % kRows;
     const float* part2 = a.part;
-    if constexpr (EVEN) {
-        const int first = s.rest_info[b], n = s.rest_info[b + 1] - first;
-        const int64_t sh = share_of((int64_t)s.rest_info[s.B] * a.H, rest_ctas);
-        if (n > 0) {
-            const int64_t g0 = (int64_t)first * a.H + (int64_t)h * n, c0 = g0 / sh;
-            n2 = (int)((g0 + n - 1) / sh - c0 + 1);
-            part2 += (b * a.H + h + c0) * kPart;
+    if constexpr (HOW != REST_IN_CHUNKS) {
+        if (rest_n > 0) {
+            const int64_t sh = kFew ? share : share_of((int64_t)rest_all * a.H, rest_ctas);
+            const int64_t g0 = (kFew ? common : 0) + (int64_t)rest_first * a.H + (int64_t)h * rest_n, c0 = (g0 + begin) / sh;
+            n2 = (int)((g0 + rest_n - 1) / sh - c0 + 1);
+            part2 += ((kFew ? s.groups * per_head : 0) + b * a.H + h + c0) * kPart;
         }
     } else {
         const Span e = rest_of(s, b, row_tile, Common{(int)(uint32_t)info1, (int)(info1 >> 32)});
@@ -842,11 +931,14 @@ __global__ void __launch_bounds__(kSJoinWarps * 32) kv_shared_join_kernel(const 
         part2 += (b * (int64_t)(a.H * a.row_tiles) + h * a.row_tiles + row_tile) * a.splits * kPart;
     }
     const int n = live ? n1 + n2 : 0;
-    const int held = s.copies * s.rows_cap;              // rows of a partial tile
-    auto row_of = [&](int i) { return i % s.copies * s.rows_cap + r1; };
+    const int copies = kFew ? 1 : s.copies, cap = kFew ? kRows : s.rows_cap, held = copies * cap;      // rows of a partial tile
+    // part i's row: its means; its reference lies `refs` floats behind the tile's begin, its total as many rows on
+    auto tile_of = [&](int i) { return i < n1 ? part1 + i / copies * (kFew ? (int64_t)kPart : s.stride) : part2 + (int64_t)(i - n1) * kPart; };
+    auto row_of = [&](int i) { return i < n1 ? i % copies * cap + r1 : r2; };
     auto ref_of = [&](int i, float* l) {
-        const float* p = i < n1 ? part1 + i / s.copies * s.stride + held * D + row_of(i) : part2 + (int64_t)(i - n1) * kPart + kRows * D + r2;
-        *l = p[i < n1 ? held : kRows];
+        const int rows = i < n1 ? held : kRows;
+        const float* p = tile_of(i) + rows * D + row_of(i);
+        *l = p[rows];
         return *p;
     };
     // the row's reference and total: every warp takes them from all parts, a lane a part
@@ -879,8 +971,8 @@ __global__ void __launch_bounds__(kSJoinWarps * 32) kv_shared_join_kernel(const 
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int i = i0 + j0 + j * W;
-                const bool shared = i < n1;
-                const float* p = shared ? part1 + i / s.copies * s.stride + row_of(i) * D : part2 + (int64_t)(i - n1) * kPart + r2 * D;
+                const bool shared = !kFew && i < n1;
+                const float* p = tile_of(i) + row_of(i) * D;
 #pragma unroll
                 for (int e = 0; e < E; e += 2)
                     x[j][e / 2] = j0 + j * W < upto ? *reinterpret_cast<const float2*>(p + (shared ? column_of(lane * E + e) : lane * E + e))
@@ -919,25 +1011,34 @@ __global__ void __launch_bounds__(kSJoinWarps * 32) kv_shared_join_kernel(const 
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
+constexpr int64_t kFewRows = 16;        // query rows of a cached head of a group up to which attend() takes them
 constexpr int64_t kSJoinRows = 1024;    // rows from which on a warp joins one alone
-struct SharedPlan { bool use; Plan rest; int rows, row_tiles, rows_cap, copies, ctas; int64_t stride, info, rest_info, part, rest_part, bytes; };
+struct SharedPlan { bool use, few; Plan rest; int rows, row_tiles, rows_cap, copies, ctas; int64_t stride, info, rest_info, part, rest_part, bytes; };
 
 SharedPlan shared_plan(int dtype, int64_t B, int64_t groups, int64_t T, int64_t G, int64_t H, int64_t D, int64_t page, int64_t n_blocks,
                        int64_t window) {
     SharedPlan p{};
     const int64_t K = B / groups, rows = K * T * G;
-    p.use = K > 1 && groups <= kSGroups && rows <= (1 << 20);
+    const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
+    p.rows = (int)std::min<int64_t>(rows, 1 << 20);
+    p.few = rows <= kFewRows;
+    p.use = K > 1 && (p.few ? B <= kEvenBatch : groups <= kSGroups && rows <= (1 << 20));
     if (!p.use) return p;
+    p.info = up((2 * groups + 2) * 8);
+    if (p.few) {
+        p.row_tiles = (int)((rows + kRows - 1) / kRows);
+        p.rest_info = up((B + 1) * 4);
+        p.ctas = 8 * 148;
+        p.rest_part = up((groups * H * p.row_tiles + B * H + p.ctas) * kRows * (D + 2) * 4);
+        p.bytes = p.info + p.rest_info + p.rest_part;
+        return p;
+    }
     p.rest = plan_of(B, T, G, H, D, page, n_blocks, window);
     if (!p.rest.even && p.rest.warps == 8) p.rest.splits = 1;
-    p.rows = (int)rows;
     p.row_tiles = (int)((rows + kSRows - 1) / kSRows);
     p.rows_cap = (int)std::min<int64_t>(rows, kSRows);
     const bool two = dtype == NT_BF16 ? true : D == 64;
     p.ctas = 148 * (two ? 2 : 1);
-    const int64_t align = 256;
-    auto up = [&](int64_t x) { return (x + align - 1) / align * align; };
-    p.info = up((2 * groups + 2) * 8);
     p.rest_info = p.rest.even ? up((B + 1) * 4) : 0;
     p.copies = p.rows_cap <= 32 ? 4 : p.rows_cap <= 64 ? 2 : 1;
     p.stride = (p.copies * p.rows_cap * (D + 2) + 3) / 4 * 4;      // written 16 bytes at a time
@@ -967,26 +1068,34 @@ int launch_after(const void* kernel, const char* name, dim3 grid, dim3 block, si
     return check_launch(name);
 }
 
+template <int DT, int D, int HOW>
+int launch_shared_join(const SharedArgs& s, int ctas, cudaStream_t stream) {
+    SharedArgs args = s;
+    void* two[] = {&args, &ctas};
+    const int64_t rows = (int64_t)s.B * s.a.T * s.a.H * s.a.G;
+    const bool one_warp = rows >= kSJoinRows;
+    const void* f = one_warp ? (const void*)kv_shared_join_kernel<DT, D, HOW, 1> : (const void*)kv_shared_join_kernel<DT, D, HOW, kSJoinWarps>;
+    return launch_after(f, "kv_shared_join_kernel", dim3((unsigned)(one_warp ? (rows + kSJoinWarps - 1) / kSJoinWarps : rows)),
+                        dim3(kSJoinWarps * 32), 0, two, stream);
+}
+
+template <int DT, int D, bool HALF_C, bool HALF_R>
+int launch_few(const SharedArgs& s, cudaStream_t stream) {
+    const size_t smem = std::max(kRingBytes<D, 2>, sizeof(float) * 2 * kRows * (D + 2));
+    kv_few_kernel<DT, D, HALF_C, HALF_R><<<s.ctas, 64, smem, stream>>>(s);
+    const int rc = check_launch("kv_few_kernel");
+    return rc != NT_OK ? rc : launch_shared_join<DT, D, ALL_IN_SHARES>(s, s.ctas, stream);
+}
+
 template <int DT, int D, int W, bool HALF>
 int launch_rest(const SharedArgs& s, const SharedPlan& p, cudaStream_t stream) {
     const size_t smem = std::max(kRingBytes<D, W>, sizeof(float) * W * kRows * (D + 2));
     SharedArgs args = s;
-    int ctas = p.rest.even;
     void* one[] = {&args};
-    void* two[] = {&args, &ctas};
-    const int64_t rows = (int64_t)s.B * s.a.T * s.a.H * s.a.G;
-    const bool one_warp = rows >= kSJoinRows;
-    const dim3 join((unsigned)(one_warp ? (rows + kSJoinWarps - 1) / kSJoinWarps : rows));
-    auto launch_join = [&](bool even) {
-        const void* f = one_warp ? (even ? (const void*)kv_shared_join_kernel<DT, D, true, 1> : (const void*)kv_shared_join_kernel<DT, D, false, 1>)
-                                 : (even ? (const void*)kv_shared_join_kernel<DT, D, true, kSJoinWarps>
-                                         : (const void*)kv_shared_join_kernel<DT, D, false, kSJoinWarps>);
-        return launch_after(f, "kv_shared_join_kernel", join, dim3(kSJoinWarps * 32), 0, two, stream);
-    };
     if constexpr (W == 2) {
         if (p.rest.even) {
-            const int rc = launch_after((const void*)kv_rest_even_kernel<DT, D, W, HALF>, "kv_rest_even_kernel", dim3(ctas), dim3(W * 32), smem, one, stream);
-            return rc != NT_OK ? rc : launch_join(true);
+            const int rc = launch_after((const void*)kv_rest_even_kernel<DT, D, W, HALF>, "kv_rest_even_kernel", dim3(p.rest.even), dim3(W * 32), smem, one, stream);
+            return rc != NT_OK ? rc : launch_shared_join<DT, D, REST_IN_SHARES>(s, p.rest.even, stream);
         }
     }
     if (smem > 48 * 1024) {
@@ -995,11 +1104,15 @@ int launch_rest(const SharedArgs& s, const SharedPlan& p, cudaStream_t stream) {
     }
     const dim3 grid((unsigned)s.a.splits, (unsigned)(s.a.H * s.a.row_tiles), (unsigned)s.B);
     const int rc = launch_after((const void*)kv_rest_kernel<DT, D, W, HALF>, "kv_rest_kernel", grid, dim3(W * 32), smem, one, stream);
-    return rc != NT_OK ? rc : launch_join(false);
+    return rc != NT_OK ? rc : launch_shared_join<DT, D, REST_IN_CHUNKS>(s, 0, stream);
 }
 
 template <int DT, int D>
 int launch_shared(const SharedArgs& s, const SharedPlan& p, cudaStream_t stream) {
+    if (p.few) {
+        if (p.rows <= kRows / 2) return launch_few<DT, D, true, true>(s, stream);
+        return 2 * s.a.T * s.a.G <= kRows ? launch_few<DT, D, false, true>(s, stream) : launch_few<DT, D, false, false>(s, stream);
+    }
     using Cfg = SharedCfg<DT, D>;
     const cudaError_t e = cudaFuncSetAttribute(kv_shared_kernel<DT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kBytes);
     if (e != cudaSuccess) return fail(NT_ERR_CUDA, "nt_kv_attention_shared: %s", cudaGetErrorString(e));
@@ -1048,7 +1161,7 @@ int nt_kv_attention_shared(int dtype, int64_t B, int64_t groups, int64_t T, int6
     if (!p.use)
         return nt_kv_attention(dtype, B, T, Hq, Hkv, D, page, n_pages, n_blocks, window, scale, q, q_sb, q_st, q_sh, k_codes, k_scale,
                                v_codes, v_scale, table, table_sb, lengths, counts, out, workspace, workspace_bytes, stream);
-    if (Hkv * p.rest.row_tiles > 65535 || B * T * Hq > INT32_MAX)
+    if ((!p.few && Hkv * p.rest.row_tiles > 65535) || B * T * Hq > INT32_MAX)
         return fail(NT_ERR_ARG, "nt_kv_attention_shared: %lld query rows in one call", (long long)(T * Hq));
     if (!workspace || workspace_bytes < p.bytes)
         return fail(NT_ERR_WORKSPACE, "nt_kv_attention_shared: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)p.bytes);
@@ -1072,7 +1185,7 @@ int nt_kv_attention_shared(int dtype, int64_t B, int64_t groups, int64_t T, int6
     a.out = out;
     a.err = device_error_word(dev);
     if (!a.err) return fail(NT_ERR_CUDA, "nt_kv_attention_shared: error word unavailable");
-    s.B = (int)B; s.groups = (int)groups; s.K = (int)(B / groups);
+    s.B = (int)B; s.groups = (int)groups; s.K = a.beams = (int)(B / groups);
     s.rows = p.rows; s.row_tiles = p.row_tiles; s.rows_cap = p.rows_cap; s.copies = p.copies; s.stride = p.stride; s.ctas = p.ctas;
     s.shared = shared;
     char* ws = static_cast<char*>(workspace);
