@@ -1011,7 +1011,15 @@ __global__ void __launch_bounds__(kSJoinWarps * 32) kv_shared_join_kernel(const 
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-constexpr int64_t kFewRows = 16;        // query rows of a cached head of a group up to which attend() takes them
+// Query rows of a cached head of a group up to which attend() takes them.  us a call, attend() : tcgen05, 16
+// heads of 128: 8 rows over 65536 keys 64 : 146; 32 rows over 4096 31 : 44, over 65536 171 : 159; 64 rows over
+// 4096 46 : 60, over 16384 104 : 82, over 65536 317 : 168.
+constexpr int64_t kFewRows = 32;
+// What a call must be able to reach for the sharing to pay: keys a sequence, and bytes of codes of all of them.
+// us a call, without sharing : with it, 4 beams of 16 heads of 128: 512 keys 8.7 : 14.8, 2048 keys 17.8 : 15.4; 16 such
+// groups in a window of 512 keys 27 : 31, over 2048 keys 89 : 45; 8 beams of 10 heads of 64 over 1024 keys 13.4 : 14.5,
+// over 2048 15.6 : 14.8.
+constexpr int64_t kSReach = 1024, kSBytes = 16 << 20;
 constexpr int64_t kSJoinRows = 1024;    // rows from which on a warp joins one alone
 struct SharedPlan { bool use, few; Plan rest; int rows, row_tiles, rows_cap, copies, ctas; int64_t stride, info, rest_info, part, rest_part, bytes; };
 
@@ -1021,8 +1029,10 @@ SharedPlan shared_plan(int dtype, int64_t B, int64_t groups, int64_t T, int64_t 
     const int64_t K = B / groups, rows = K * T * G;
     const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
     p.rows = (int)std::min<int64_t>(rows, 1 << 20);
-    p.few = rows <= kFewRows;
-    p.use = K > 1 && (p.few ? B <= kEvenBatch : groups <= kSGroups && rows <= (1 << 20));
+    int64_t reach = n_blocks * page;
+    if (window >= 0) reach = std::min(reach, window + T);
+    p.few = rows <= kFewRows && T * G <= kRows;
+    p.use = K > 1 && reach >= kSReach && B * H * reach * 2 * D >= kSBytes && (p.few ? B <= kEvenBatch : groups <= kSGroups && rows <= (1 << 20));
     if (!p.use) return p;
     p.info = up((2 * groups + 2) * 8);
     if (p.few) {

@@ -47,6 +47,13 @@ def setup(groups, K, H, P, D, shared, lengths, seed, spread=0.7, own=0.3, spare_
     return cache, table
 
 
+def wide(table, P, tokens=1 << 18):
+    """The table with room for `tokens`, as one has that is made for the longest sequence: from a thousand keys and
+    some megabytes on that a call can reach, what is shared is read once, below that by every row."""
+    more = torch.full((table.shape[0], tokens // P), -1, device=DEV, dtype=torch.int32)
+    return torch.cat([table, more], 1)
+
+
 def ints(v):
     return torch.tensor(v, device=DEV, dtype=torch.int32)
 
@@ -64,11 +71,18 @@ def ints(v):
     (64, 1, 1, 4, [700], [1 + 3 * i for i in range(64)], None, None),
     (3, 1, 2, 1, [128, 127, 15], [1] * 9, None, 0),
     (7, 4, 1, 11, [130], [4] * 7, None, 129),
-    (1, 1, 1, 16, [600, 90], [1, 2], None, None)])
-def test_against_definition(nat, dtype, P, D, K, T, H, G, shared, behind, counts, window):
+    (1, 1, 1, 16, [600, 90], [1, 2], None, None),
+    (2, 1, 2, 1, [1500, 2200], [1, 90, 33, 700], None, 1024),
+    (4, 2, 1, 4, [1400], [2, 300, 5, 47], [2, 1, 0, 2], 1100),
+    (8, 5, 1, 7, [1600], [5, 6, 7, 8, 9, 10, 64, 65], [5, 5, 0, 4, 5, 1, 2, 5], 1030),
+    (3, 12, 1, 1, [1700], [12, 40, 20], None, 1200)])
+@pytest.mark.parametrize("roomy", [False, True])
+def test_against_definition(nat, dtype, P, D, K, T, H, G, shared, behind, counts, window, roomy):
     groups = len(shared)
     lengths = [shared[b // K] + n for b, n in enumerate(behind)]
     cache, table = setup(groups, K, H, P, D, shared, lengths, 50 + K)
+    if roomy:
+        table = wide(table, P)
     B = groups * K
     cnt = counts if counts else [T] * B
     q = (1.5 * torch.randn(B, T, H * G, D, device=DEV, generator=gen(60))).to(dtype)
@@ -89,7 +103,8 @@ def test_against_definition(nat, dtype, P, D, K, T, H, G, shared, behind, counts
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("groups,K,H,G,longest,tail,window", [
     (40, 3, 2, 1, 900, 50, None), (3, 20, 4, 1, 5000, 300, None), (1, 33, 1, 4, 20000, 30, None), (100, 2, 1, 1, 300, 400, 64),
-    (2, 5, 16, 1, 2000, 64, 512), (1, 300, 1, 1, 700, 20, None)])
+    (2, 5, 16, 1, 2000, 64, 512), (1, 300, 1, 1, 700, 20, None), (30, 4, 1, 1, 3000, 700, 1024), (2, 60, 1, 4, 2500, 400, 1500),
+    (260, 2, 1, 1, 200, 30, None), (520, 33, 1, 1, 40, 9, None)])
 def test_many_ragged_groups(nat, dtype, groups, K, H, G, longest, tail, window):
     """Shares of the work that begin and end inside groups, groups without keys, idle and bad sequences."""
     P, D = 32, 64
@@ -99,6 +114,7 @@ def test_many_ragged_groups(nat, dtype, groups, K, H, G, longest, tail, window):
     lengths = [shared[b // K] + rng.randint(0, tail) for b in range(groups * K)]
     counts = [0 if rng.random() < 0.1 or n == 0 else 1 for n in lengths]
     cache, table = setup(groups, K, H, P, D, shared, lengths, 70 + groups, spare_blocks=5)
+    table = wide(table, P)
     q = torch.randn(groups * K, 1, H * G, D, device=DEV, generator=gen(71)).to(dtype)
     n, c = ints(lengths), ints(counts)
     o = nat.kv_attention_shared(q, *cache, table, n, ints(shared), counts=c, window=window)
@@ -120,6 +136,7 @@ def test_shared_counts_and_bad_pages(nat, dtype):
     P, D, H, K = 16, 64, 2, 3
     lengths, shared = [200, 210, 190, 64, 64, 64], [180, 48]
     cache, table = setup(2, K, H, P, D, shared, lengths, 80)
+    table = wide(table, P)
     q = torch.randn(6, 1, H, D, device=DEV, generator=gen(81)).to(dtype)
     want, tol = attention64(q, cache, table, lengths, [1] * 6, None, P)
     for fewer in ([-1, 48], [180, -5], [17, 15]):
@@ -138,12 +155,13 @@ def test_shared_counts_and_bad_pages(nat, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("D", [64, 128])
-def test_extreme_scales_and_scores(nat, dtype, D):
+@pytest.mark.parametrize("D,K", [(64, 4), (128, 4), (64, 40), (128, 40)])
+def test_extreme_scales_and_scores(nat, dtype, D, K):
     """Pages whose scales are far apart, sharp and flat rows, tiny and large queries, a scale of its own, values near the largest."""
-    P, H, K, shared = 16, 2, 4, [700]
-    lengths = [700 + 9 * b for b in range(1, 5)]
+    P, H, shared = 16, 2, [700]
+    lengths = [700 + 9 * b for b in range(1, K + 1)]
     cache, table = setup(1, K, H, P, D, shared, lengths, 82)
+    table = wide(table, P)
     first = table[max(range(K), key=lambda r: lengths[r])].long()
     for j, f in ((3, 2.0 ** -60), (5, 2.0 ** 30), (20, 2.0 ** -30), (41, 2.0 ** 12)):
         for b in range(K):
@@ -168,12 +186,14 @@ def test_extreme_scales_and_scores(nat, dtype, D):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-def test_not_finite(nat, dtype):
+@pytest.mark.parametrize("K", [3, 20])
+def test_not_finite(nat, dtype, K):
     """A NaN reaches exactly the rows that see it; a query that is not finite only its own row."""
-    P, D, H, K, T, shared, window = 16, 64, 1, 3, 2, [300], 200
-    lengths = [310, 330, 302]
-    for where, key in (("v", 150), ("k", 150), ("v", 299), ("v", 108), ("k", 120), ("v", 101), ("k", 129), ("v", 5)):
+    P, D, H, T, shared, window = 16, 64, 1, 2, [1300], 1200
+    lengths = ([1310, 1330, 1302] * K)[:K]
+    for where, key in (("v", 150), ("k", 150), ("v", 1299), ("v", 108), ("k", 120), ("v", 101), ("k", 129), ("v", 5), ("k", 700)):
         cache, table = setup(1, K, H, P, D, shared, lengths, 85, own=0.0)
+        table = wide(table, P)
         q = torch.randn(K, T, H, D, device=DEV, generator=gen(86)).to(dtype)
         clean, tol = attention64(q, cache, table, lengths, [T] * K, window, P)
         for b in range(K):
@@ -189,6 +209,7 @@ def test_not_finite(nat, dtype):
                 d = ((o[b, t, 0].double() - clean[b, t, 0]).abs() - half(dtype) * clean[b, t, 0].abs() - tol[b, t, 0])[~bad]
                 assert d.numel() == 0 or d.max() <= 0
     cache, table = setup(1, K, H, P, D, shared, lengths, 87)
+    table = wide(table, P)
     for v in (float("nan"), float("inf"), -float("inf")):
         q = torch.randn(K, T, H, D, device=DEV, generator=gen(88)).to(dtype)
         want, tol = attention64(q, cache, table, lengths, [T] * K, window, P)
@@ -199,10 +220,12 @@ def test_not_finite(nat, dtype):
         close(o, want, half(dtype), tol)
 
 
-def test_layouts_streams_and_graphs(nat):
-    groups, K, T, H, D, P = 2, 4, 1, 4, 64, 16
-    shared, lengths = [300, 150], [301, 333, 340, 309, 151, 152, 153, 160]
+@pytest.mark.parametrize("K", [4, 36])
+def test_layouts_streams_and_graphs(nat, K):
+    groups, T, H, D, P = 2, 1, 4, 64, 16
+    shared, lengths = [300, 150], ([301, 333, 340, 309] * K)[:K] + ([151, 152, 153, 160] * K)[:K]
     cache, table = setup(groups, K, H, P, D, shared, lengths, 89)
+    table = wide(table, P)
     B = groups * K
     qkv = torch.randn(B, T, 3 * H, D, device=DEV, generator=gen(90)).to(BF16)
     q = qkv[:, :, :H]
@@ -229,7 +252,7 @@ def test_layouts_streams_and_graphs(nat):
     for g in graphs:
         g.replay()
     assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
-    n -= ints([1, 20, 0, 9, 0, 0, 1, 3])
+    n -= ints(([1, 20, 0, 9] * K)[:K] + ([0, 0, 1, 3] * K)[:K])
     s.copy_(ints([288, 0]))
     want = nat.kv_attention_shared(q, *cache, table, n, s)
     for _ in range(3):
