@@ -408,10 +408,13 @@ NT_API int nt_reorder_rows(int64_t n_tensors, const int64_t* tensors, int64_t R,
  * order).  Where they run out, or the table ends, entries stay -1 and the bad-argument
  * bit of the device error word is set, as for a bad parent (it ends), length or page.
  * With group > 0 shared[g] (int32 [R / group]) is how many leading tokens, in whole
- * blocks, the rows of group g have in the same pages. */
+ * blocks, the rows of group g have in the same pages.
+ * Workspace: nt_kv_fork_workspace_bytes() (0 without groups). */
+NT_API int64_t nt_kv_fork_workspace_bytes(int64_t R, int64_t n_blocks, int64_t group);
 NT_API int nt_kv_fork(int64_t R, int64_t n_pages, int64_t n_blocks, int64_t page, int64_t tokens, int64_t window,
                       int64_t group, int32_t* table, int64_t table_sb, int32_t* refs, int32_t* lengths,
-                      const int32_t* parents, int32_t* copies, int32_t* shared, void* stream);
+                      const int32_t* parents, int32_t* copies, int32_t* shared,
+                      void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Pages copied within their pools, codes and scales of keys and values of every
  * layer: pages (int32 [n, 2]): from, to; (-1, -1) is skipped, a page outside

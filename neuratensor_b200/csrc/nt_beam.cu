@@ -8,10 +8,10 @@
 // Bound by HBM: every logit is read once and takes a subtraction, two products, one
 // exponential and a comparison.  A CTA streams a slice of one row: each thread keeps its
 // vectors in registers, its running maximum and sum of exponentials, and candidates are
-// the values that reach a bound that n values of the slice are known to reach (the r-th
+// the values that reach a bound that n values of the slice are known to reach: first the r-th
 // largest of each warp's lane maxima, the smallest of that over the warps, with
-// r * warps >= n), a few dozen of thousands.  They are ranked by counting in shared
-// memory.  A slice in which too many reach the bound (constant logits) takes its n best
+// r * warps >= n, which a few dozen of thousands reach, then the n-th best so far.  They are
+// ranked by counting in shared memory.  A slice in which too many reach the bound (constant logits) takes its n best
 // one after the other instead.  A second kernel, launched as a programmatic dependent,
 // joins an item's slices: logarithms and sums in float64 (candidates of two beams may lie
 // closer together than float32 can tell), then n rounds of one warp over the heads of the
@@ -29,8 +29,8 @@ constexpr int kBeamVecs = 4;           // 16-byte vectors of a thread in flight
 constexpr int kBeamList = 1024;        // candidates a slice can hold
 constexpr int kBeamMost = 64;          // n, and beams of an item
 constexpr int kBeamLists = 1024;       // slices of an item's beams
-constexpr int kJoinThreads = 128;
-constexpr int kJoinHeld = 4096;        // list entries that the joining kernel keeps in shared memory
+constexpr int kJoinThreads = 256;
+constexpr int kJoinHeld = 2048;        // list entries whose ranks the joining kernel keeps in shared memory
 
 struct BeamArgs {
     int64_t V;
@@ -94,9 +94,16 @@ __device__ __forceinline__ uint4 beam_load(const T* x, int off, int64_t at, int6
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[i] = __funnelshift_r(w[i + k], w[i + k + 1], odd);
     } else {
-        o[0] = o[1] = o[2] = o[3] = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
-        for (int e = 0; e < E; ++e)
-            if (at + e < V) reinterpret_cast<T*>(o)[e] = x[at + e];
+        // element by element, across the row's end too
+        auto bits = [&](int e) -> uint32_t {
+            if constexpr (sizeof(T) == 4) return at + e < V ? reinterpret_cast<const uint32_t*>(x)[at + e] : 0xff800000u;
+            else return at + e < V ? (uint32_t)reinterpret_cast<const uint16_t*>(x)[at + e] : 0xff80u;
+        };
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) o[i] = bits(i);
+            else o[i] = bits(2 * i) | bits(2 * i + 1) << 16;
+        }
     }
     return out;
 }
@@ -106,7 +113,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_co
     using T = typename Elem<DT>::T;
     constexpr int E = 16 / (int)sizeof(T);
     __shared__ unsigned long long list[kBeamList];
-    __shared__ uint32_t warp_bound[2][kBeamWarps];
+    __shared__ uint32_t warp_bound[kBeamWarps];
     __shared__ unsigned long long warp_key[kBeamWarps];
     __shared__ float warp_m[kBeamWarps], warp_s[kBeamWarps];
     __shared__ int count;
@@ -134,40 +141,60 @@ __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_co
             mine[i] = tid + i * kBeamThreads < m ? list[tid + i * kBeamThreads] : 0ull;
             rank[i] = 0;
         }
-        for (int i = 0; i * kBeamThreads < m; ++i)
-            for (int j = 0; j < m; ++j) rank[i] += list[j] > mine[i];
+        for (int j = 0; j < m; ++j) {
+            const unsigned long long k = list[j];
+#pragma unroll
+            for (int i = 0; i < kBeamList / kBeamThreads; ++i) rank[i] += k > mine[i];
+        }
         __syncthreads();
-        for (int i = 0; i * kBeamThreads < m; ++i)
+#pragma unroll
+        for (int i = 0; i < kBeamList / kBeamThreads; ++i)
             if (tid + i * kBeamThreads < m && rank[i] < a.n) list[rank[i]] = mine[i];
         __syncthreads();
         return m < a.n ? m : a.n;
     };
 
     float top = -INFINITY, sum = 0.f, bound = -INFINITY;
-    int held = 0, turn = 0;
+    int held = 0, bound_of = 0;                         // entries when the bound was taken
     const int rounds = (a.n + kBeamWarps - 1) / kBeamWarps;
-    __syncthreads();
-    for (int64_t v0 = begin; v0 < end; v0 += kBeamThreads * kBeamVecs, turn ^= 1) {
-        uint4 raw[kBeamVecs];
+    uint4 raw[kBeamVecs], next[kBeamVecs];
+    auto load = [&](int64_t v0, uint4 (&to)[kBeamVecs]) {
 #pragma unroll
         for (int j = 0; j < kBeamVecs; ++j) {
             const int64_t v = v0 + j * kBeamThreads + tid;
-            raw[j] = v < end ? beam_load<T>(x, off, v * E, a.V) : none;
+            to[j] = v < end ? beam_load<T>(x, off, v * E, a.V) : none;
         }
+    };
+    load(begin, next);
+    __syncthreads();
+    for (int64_t v0 = begin; v0 < end; v0 += kBeamThreads * kBeamVecs) {
+#pragma unroll
+        for (int j = 0; j < kBeamVecs; ++j) raw[j] = next[j];
+        if (v0 + kBeamThreads * kBeamVecs < end) load(v0 + kBeamThreads * kBeamVecs, next);
         float best = -INFINITY;
+        if constexpr (DT == NT_F32) {
 #pragma unroll
-        for (int j = 0; j < kBeamVecs; ++j)
+            for (int j = 0; j < kBeamVecs; ++j)
 #pragma unroll
-            for (int e = 0; e < E; ++e) best = fmaxf(best, value(raw[j], e));
-        // the bound of this tile
-        uint32_t o = ordered(best), bw = 0u;
-        for (int r = 0; r < rounds; ++r) {
-            bw = __reduce_max_sync(0xffffffffu, o);
-            const unsigned who = __ballot_sync(0xffffffffu, o == bw);
-            if (lane == __ffs(who) - 1) o = 0u;
+                for (int e = 0; e < E; ++e) best = fmaxf(best, value(raw[j], e));
+        } else {
+            __nv_bfloat162 two = *reinterpret_cast<const __nv_bfloat162*>(&none.x);
+#pragma unroll
+            for (int j = 0; j < kBeamVecs; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) two = __hmax2(two, reinterpret_cast<const __nv_bfloat162*>(&raw[j])[e]);
+            best = fmaxf(__low2float(two), __high2float(two));
         }
-        if (lane == 0) warp_bound[turn][warp] = bw;
-        // the sum of exponentials: the exponent's product with log2 e in two parts
+        if (held < a.n) {
+            // no bound yet: the r-th largest of each warp's lane maxima, the smallest of that over the warps
+            uint32_t o = ordered(best), bw = 0u;
+            for (int r = 0; r < rounds; ++r) {
+                bw = __reduce_max_sync(0xffffffffu, o);
+                const unsigned who = __ballot_sync(0xffffffffu, o == bw);
+                if (lane == __ffs(who) - 1) o = 0u;
+            }
+            if (lane == 0) warp_bound[warp] = bw;
+        }
         if (best > top) {
             sum = top == -INFINITY ? sum : sum * ex2((top - best) * kLog2e);
             top = best;
@@ -177,16 +204,15 @@ __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_co
 #pragma unroll
         for (int j = 0; j < kBeamVecs; ++j)
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float d = value(raw[j], e) - base;
-                part[e & 1] += ex2(fmaf(d, kLog2e, d * 1.925963033500e-8f));
-            }
+            for (int e = 0; e < E; ++e) part[e & 1] += ex2((value(raw[j], e) - base) * kLog2e);
         sum += part[0] + part[1];
-        __syncthreads();
-        uint32_t least = warp_bound[turn][0];
+        if (held < a.n) {
+            __syncthreads();
+            uint32_t least = warp_bound[0];
 #pragma unroll
-        for (int w = 1; w < kBeamWarps; ++w) least = min(least, warp_bound[turn][w]);
-        bound = fmaxf(bound, least ? from_ordered(least) : -INFINITY);
+            for (int w = 1; w < kBeamWarps; ++w) least = min(least, warp_bound[w]);
+            bound = least ? from_ordered(least) : -INFINITY;
+        }
         if (best >= bound && best > -INFINITY) {
 #pragma unroll
             for (int j = 0; j < kBeamVecs; ++j)
@@ -235,6 +261,14 @@ __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_co
         } else {
             held = now;
         }
+        // the n-th best so far is the bound of what follows
+        if (held >= a.n && (bound_of == 0 || held >= bound_of + 64) && v0 + kBeamThreads * kBeamVecs < end) {
+            held = shrink(held);
+            bound_of = held;
+            bound = from_ordered((uint32_t)(list[a.n - 1] >> 32));
+            if (tid == 0) count = held;
+            __syncthreads();
+        }
     }
     // the slice's maximum and sum, and its n best
     float m = top;
@@ -268,13 +302,11 @@ __device__ __forceinline__ unsigned long long ordered64(double r) {
 
 __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_constant__ BeamArgs a) {
     __shared__ double lse[kBeamMost], norm[kBeamMost];
-    __shared__ unsigned long long held[kJoinHeld];
-    __shared__ unsigned long long head_rank[kBeamLists];
-    __shared__ uint32_t head_token[kBeamLists];
-    __shared__ uint8_t head_at[kBeamLists];
+    __shared__ unsigned long long ranks[kJoinHeld];
+    __shared__ uint32_t tokens[kJoinHeld];
+    __shared__ uint16_t head_at[kBeamLists];
     __shared__ uint8_t kind[kBeamMost];                 // 0 nothing to offer, 1 live, 2 finished
-    __shared__ int chosen[kBeamMost];
-    __shared__ float chosen_score[kBeamMost];
+    __shared__ int chosen[kBeamMost], chosen_from[kBeamMost];
     __shared__ uint32_t chosen_token[kBeamMost];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row0 = (int64_t)blockIdx.x * a.K;
@@ -294,7 +326,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
             double sum = 0.0;
             for (int s = lane; s < S; s += 32) {
                 const float2 p = a.sums[row * S + s];
-                sum += p.x == -INFINITY ? (double)p.y : (double)p.y * exp((double)p.x - (double)m);
+                sum += p.x == m || p.x == -INFINITY ? (double)p.y : (double)p.y * exp((double)p.x - (double)m);
             }
 #pragma unroll
             for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -310,95 +342,103 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     }
     const bool near = lists * n <= kJoinHeld;
     const unsigned long long* keys = a.keys + row0 * S * n;
-    if (near) {
-        for (int i = tid; i < lists * n; i += kJoinThreads) held[i] = keys[i];
-        keys = held;
-    }
     __syncthreads();
-    // the candidate at place `at` of list l: its rank (0: none) and token
-    auto head = [&](int l, int at) {
+    // the sum of the candidate at place i of list l, which is there
+    auto sum_of = [&](int l, int i) {
         const int k = l / S;
-        unsigned long long r = 0ull;
-        uint32_t token = 0u;
-        if (kind[k] == 2) {
-            token = (uint32_t)a.pad;
-            if (l == k * S && at == 0) r = ordered64((double)a.scores[row0 + k] / norm[k]);
-        } else if (kind[k] == 1 && at < n) {
-            const unsigned long long c = keys[l * n + at];
-            if (c) {
-                token = ~(uint32_t)c;
-                r = ordered64(((double)a.scores[row0 + k] + ((double)from_ordered((uint32_t)(c >> 32)) - lse[k])) / norm[k]);
-            }
-        }
-        head_rank[l] = r;
-        head_token[l] = token;
-        head_at[l] = (uint8_t)at;
+        const double s = a.scores[row0 + k];
+        return kind[k] == 2 ? s : s + ((double)from_ordered((uint32_t)(keys[l * n + i] >> 32)) - lse[k]);
     };
+    // its rank (0: it is not) and token
+    auto look = [&](int l, int i, uint32_t* token) -> unsigned long long {
+        const int k = l / S;
+        *token = (uint32_t)a.pad;
+        if (kind[k] == 2 ? l != k * S || i > 0 : kind[k] != 1 || i >= n) return 0ull;
+        if (kind[k] == 1) {
+            const unsigned long long c = keys[l * n + i];
+            if (!c) return 0ull;
+            *token = ~(uint32_t)c;
+        }
+        return ordered64(a.alpha != 0.0 ? sum_of(l, i) / norm[k] : sum_of(l, i));
+    };
+    if (near)
+        for (int i = tid; i < lists * n; i += kJoinThreads) {
+            uint32_t token;
+            ranks[i] = look(i / n, i % n, &token);
+            tokens[i] = token;
+        }
+    __syncthreads();
     if (warp == 0) {
-        // a lane has lists lane, lane + 32, ...
-        unsigned long long best = 0ull, flat = ~0ull;
+        // a lane has lists lane, lane + 32, ...; its best head
+        unsigned long long best = 0ull;
+        uint32_t beam = ~0u, token = ~0u;
         int from = -1;
         auto pick = [&]() {
-            best = 0ull, flat = ~0ull, from = -1;
+            best = 0ull, beam = token = ~0u, from = -1;
             for (int l = lane; l < lists; l += 32) {
-                const unsigned long long r = head_rank[l], f = (unsigned long long)(l / S) << 32 | head_token[l];
-                if (r > best || (r == best && f < flat)) best = r, flat = f, from = l;
+                const int i = head_at[l];
+                uint32_t t = 0u;
+                unsigned long long r = 0ull;
+                if (i < n) {
+                    if (near) r = ranks[l * n + i], t = tokens[l * n + i];
+                    else r = look(l, i, &t);
+                }
+                const uint32_t k = l / S;
+                if (r > best || (r && r == best && (k < beam || (k == beam && t < token)))) best = r, beam = k, token = t, from = l;
             }
         };
-        for (int l = lane; l < lists; l += 32) head(l, 0);
-        __syncwarp();
+        for (int l = lane; l < lists; l += 32) head_at[l] = 0;
         pick();
         for (int i = 0; i < n; ++i) {
-            unsigned long long r = best, f = flat;
-            int w = from;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                const unsigned long long r2 = __shfl_xor_sync(0xffffffffu, r, o), f2 = __shfl_xor_sync(0xffffffffu, f, o);
-                const int w2 = __shfl_xor_sync(0xffffffffu, w, o);
-                if (r2 > r || (r2 == r && f2 < f)) r = r2, f = f2, w = w2;
+            // the largest rank, of equal ones the lowest beam and token
+            const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
+            bool mine = (uint32_t)(best >> 32) == hi;
+            const uint32_t lo = __reduce_max_sync(0xffffffffu, mine ? (uint32_t)best : 0u);
+            mine = mine && (uint32_t)best == lo;
+            if (__popc(__ballot_sync(0xffffffffu, mine)) > 1) {
+                const uint32_t k = __reduce_min_sync(0xffffffffu, mine ? beam : ~0u);
+                mine = mine && beam == k;
+                const uint32_t t = __reduce_min_sync(0xffffffffu, mine ? token : ~0u);
+                mine = mine && token == t;
             }
-            if (lane == 0) {
-                const int k = (int)(f >> 32);
-                chosen[i] = r ? k : -1;
-                if (r) {
-                    double s = a.scores[row0 + k];
-                    if (kind[k] == 1) s += (double)from_ordered((uint32_t)(keys[w * n + head_at[w]] >> 32)) - lse[k];
-                    chosen_score[i] = (float)s;
-                    chosen_token[i] = head_token[w];
-                }
+            if (!(hi | lo)) {                           // nothing left
+                if (lane == 0) chosen[i] = -1;
+                continue;
             }
-            __syncwarp();
-            if (r && from == w) {
-                head(w, head_at[w] + 1);
+            if (mine) {
+                chosen[i] = (int)beam;
+                chosen_from[i] = from * n + head_at[from];
+                chosen_token[i] = token;
+                ++head_at[from];
                 pick();
             }
             __syncwarp();
         }
+        __syncwarp();
         // places: in order, or the first child of a beam in the beam's own
+        __shared__ int8_t place[kBeamMost];
         if (lane == 0) {
             unsigned long long taken = 0ull;
-            int8_t place[kBeamMost];
             for (int i = 0; i < n; ++i) {
-                place[i] = (int8_t)i;
-                if (a.stay) {
-                    place[i] = -1;
-                    if (chosen[i] >= 0 && !(taken >> chosen[i] & 1)) {
-                        place[i] = (int8_t)chosen[i];
-                        taken |= 1ull << chosen[i];
-                    }
+                place[i] = (int8_t)(a.stay ? -1 : i);
+                if (a.stay && chosen[i] >= 0 && !(taken >> chosen[i] & 1)) {
+                    place[i] = (int8_t)chosen[i];
+                    taken |= 1ull << chosen[i];
                 }
             }
-            for (int i = 0; i < n; ++i) {
+            for (int i = 0; i < n; ++i)
                 if (place[i] < 0) {
                     place[i] = (int8_t)(__ffsll((long long)~taken) - 1);
                     taken |= 1ull << place[i];
                 }
-                const int64_t at = (int64_t)blockIdx.x * n + place[i];
-                const bool some = chosen[i] >= 0;
-                a.out_scores[at] = some ? chosen_score[i] : -INFINITY;
-                a.out_rows[at] = (int32_t)(row0 + (some ? chosen[i] : place[i] % a.K));
-                a.out_tokens[at] = some ? (int64_t)chosen_token[i] : a.pad;
-            }
+        }
+        __syncwarp();
+        for (int i = lane; i < n; i += 32) {
+            const int64_t at = (int64_t)blockIdx.x * n + place[i];
+            const bool some = chosen[i] >= 0;
+            a.out_scores[at] = some ? (float)sum_of(chosen_from[i] / n, chosen_from[i] % n) : -INFINITY;
+            a.out_rows[at] = (int32_t)(row0 + (some ? chosen[i] : place[i] % a.K));
+            a.out_tokens[at] = some ? (int64_t)chosen_token[i] : a.pad;
         }
     }
 }

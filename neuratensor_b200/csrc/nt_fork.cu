@@ -22,8 +22,8 @@ namespace {
 
 constexpr int kForkRows = 1024;
 constexpr int kForkThreads = 1024;
-constexpr int kTableThreads = 256;
-constexpr int kTableWords = 10240;     // table entries of a CTA in shared memory
+constexpr int kTableThreads = 512;
+constexpr int kTableWords = 7680;      // table entries of a CTA in shared memory
 
 struct ForkArgs {
     int R, group; int64_t n_pages, n_blocks; int page, tokens; int64_t window;   // window < 0: none
@@ -52,28 +52,39 @@ __device__ __forceinline__ int fork_length(const ForkArgs& a, int r, bool* bad) 
 
 __global__ void __launch_bounds__(kTableThreads) fork_table_kernel(const __grid_constant__ ForkArgs a) {
     __shared__ int32_t old[kTableWords];
-    const int64_t j0 = (int64_t)blockIdx.x * a.columns;
-    const int m = (int)(a.n_blocks - j0 < a.columns ? a.n_blocks - j0 : a.columns);
-    for (int i = threadIdx.x; i < a.R * m; i += kTableThreads) old[i] = a.table[(i / m) * a.table_sb + j0 + i % m];
-    __syncthreads();
+    __shared__ int32_t from[kForkRows];                 // the row that a row goes on from; its live blocks [low, high)
+    __shared__ int32_t low[kForkRows], high[kForkRows];
+    __shared__ int32_t differ[kForkRows];               // first block of these columns that a group's rows do not share
+    const int j0 = blockIdx.x * a.columns, m = (int)(a.n_blocks - j0 < a.columns ? a.n_blocks - j0 : a.columns);
     bool bad = false;
-    for (int i = threadIdx.x; i < a.R * m; i += kTableThreads) {
-        const int r = i / m, c = i % m;
+    for (int i = threadIdx.x; i < a.R * m; i += kTableThreads) old[i] = a.table[i / m * a.table_sb + j0 + i % m];
+    for (int r = threadIdx.x; r < a.R; r += kTableThreads) {
         const int len = fork_length(a, r, &bad);
-        const int64_t j = j0 + c, low = a.window >= 0 && len > a.window ? (len - a.window) / a.page : 0;
-        const int before = old[i];
-        int now = j >= low && j * a.page < len ? old[a.parents[r] * m + c] : -1;
-        if (now < -1 || now >= a.n_pages) {
-            now = -1;
-            bad = true;
-        }
+        from[r] = len ? a.parents[r] : 0;
+        low[r] = a.window >= 0 && len > a.window ? (int)((len - a.window) / a.page) : 0;
+        high[r] = (len + a.page - 1) / a.page;
+        differ[r] = 0x7fffffff;
+    }
+    __syncthreads();
+    auto entry = [&](int r, int c, bool* wrong) {
+        const int j = j0 + c, now = j >= low[r] && j < high[r] ? old[from[r] * m + c] : -1;
+        if (now >= -1 && now < a.n_pages) return now;
+        *wrong = true;
+        return -1;
+    };
+    for (int i = threadIdx.x; i < a.R * m; i += kTableThreads) {
+        const int r = i / m, c = i % m, before = old[i], now = entry(r, c, &bad);
         if (now != before) {
-            a.table[r * a.table_sb + j] = now;
+            a.table[r * a.table_sb + j0 + c] = now;
             if (now >= 0) atomicAdd(a.refs + now, 1);
             if (before >= 0 && before < a.n_pages) atomicAdd(a.refs + before, -1);
         }
+        if (a.group > 0 && r % a.group && now != entry(r - r % a.group, c, &bad)) atomicMin(&differ[r / a.group], j0 + c);
     }
     if (bad) atomicOr(a.err, ERRF_BAD_ARG);
+    __syncthreads();
+    if (a.group > 0)
+        for (int g = threadIdx.x; g < a.R / a.group; g += kTableThreads) a.alike[g * a.column_ctas + blockIdx.x] = differ[g];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
@@ -166,27 +177,37 @@ __global__ void __launch_bounds__(kForkThreads) fork_pages_kernel(const __grid_c
     copied[r] = copy;
     __syncthreads();
     int found = 0;
-    for (int64_t p0 = 0; p0 < a.n_pages && found < want; p0 += kForkThreads) {
-        const int64_t p = p0 + r;
-        const bool free = p < a.n_pages && a.refs[p] == 0;
+    for (int64_t p0 = 0; p0 < a.n_pages && found < want; p0 += 4 * kForkThreads) {
+        const int64_t p = p0 + 4 * r;
+        int32_t held[4];
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) held[i] = p + i < a.n_pages ? a.refs[p + i] : 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine += held[i] == 0;
         int here;
-        const int nth = found + prefix(free, warps, &here);
-        if (free && nth < want) {
-            int lo = 0, hi = kForkRows;                 // the last row that starts at or before nth
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                if (starts[mid] <= nth) lo = mid; else hi = mid;
+        int nth = found + prefix(mine, warps, &here);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (held[i] != 0) continue;
+            if (nth < want) {
+                int lo = 0, hi = kForkRows;             // the last row that starts at or before nth
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) / 2;
+                    if (starts[mid] <= nth) lo = mid; else hi = mid;
+                }
+                const int k = nth - starts[lo];
+                int64_t j;
+                if (copied[lo] && k == 0) {
+                    j = lens[lo] / a.page;
+                    a.copies[2 * lo + 1] = (int)(p + i);
+                } else {
+                    j = froms[lo] + k - copied[lo];
+                }
+                a.table[lo * a.table_sb + j] = (int)(p + i);
+                a.refs[p + i] = 1;
             }
-            int k = nth - starts[lo];
-            int64_t j;
-            if (copied[lo] && k == 0) {
-                j = lens[lo] / a.page;
-                a.copies[2 * lo + 1] = (int)p;
-            } else {
-                j = froms[lo] + k - copied[lo];
-            }
-            a.table[lo * a.table_sb + j] = (int)p;
-            a.refs[p] = 1;
+            ++nth;
         }
         found += here;
         __syncthreads();
@@ -214,20 +235,10 @@ __global__ void __launch_bounds__(kForkThreads) fork_pages_kernel(const __grid_c
     const int lane = r & 31;
     for (int g = r >> 5; g < a.R / a.group; g += kForkThreads / 32) {
         int least = INT32_MAX;
-        for (int i = lane; i < a.group; i += 32) least = min(least, lens[g * a.group + i]);
-        least = __reduce_min_sync(0xffffffffu, least) / a.page;
-        int alike = least;
-        for (int j0 = 0; j0 < least && alike == least; j0 += 32) {
-            bool differ = false;
-            if (j0 + lane < least) {
-                const int32_t* col = a.table + (int64_t)g * a.group * a.table_sb + j0 + lane;
-                const int mine = col[0];
-                for (int i = 1; i < a.group; ++i) differ |= col[i * a.table_sb] != mine;
-            }
-            const unsigned any = __ballot_sync(0xffffffffu, differ);
-            if (any) alike = j0 + __ffs(any) - 1;
-        }
-        if (lane == 0) a.shared[g] = alike * a.page;
+        for (int i = lane; i < a.group; i += 32) least = min(least, lens[g * a.group + i] / a.page);
+        for (int i = lane; i < a.column_ctas; i += 32) least = min(least, a.alike[g * a.column_ctas + i]);
+        least = __reduce_min_sync(0xffffffffu, least);
+        if (lane == 0) a.shared[g] = least * a.page;
     }
 }
 
@@ -269,6 +280,13 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_c
     }
 }
 
+// Columns of a CTA: all of the device's SMs, but a few columns each, which lie next to each other in memory.
+void fork_columns(int64_t R, int64_t n_blocks, int* columns, int* ctas) {
+    const int64_t most = std::min<int64_t>(std::max<int64_t>(n_blocks, 1), kTableWords / std::max<int64_t>(R, 1));
+    *columns = (int)std::min<int64_t>(most, std::max<int64_t>(8, (n_blocks + 147) / 148));
+    *ctas = (int)((n_blocks + *columns - 1) / *columns);
+}
+
 }  // namespace
 }  // namespace nt
 
@@ -276,15 +294,25 @@ using namespace nt;
 
 extern "C" {
 
+int64_t nt_kv_fork_workspace_bytes(int64_t R, int64_t n_blocks, int64_t group) {
+    if (R < 1 || R > kForkRows || n_blocks < 0 || group < 1) return 0;
+    int columns, ctas;
+    fork_columns(R, n_blocks, &columns, &ctas);
+    return (R / group) * (int64_t)ctas * 4;
+}
+
 int nt_kv_fork(int64_t R, int64_t n_pages, int64_t n_blocks, int64_t page, int64_t tokens, int64_t window, int64_t group,
                int32_t* table, int64_t table_sb, int32_t* refs, int32_t* lengths, const int32_t* parents, int32_t* copies,
-               int32_t* shared, void* stream) {
+               int32_t* shared, void* workspace, int64_t workspace_bytes, void* stream) {
     if (R < 0 || R > kForkRows) return fail(NT_ERR_ARG, "nt_kv_fork: %lld rows (at most %d)", (long long)R, kForkRows);
     if (page < 1 || page > 65536 || tokens < 0 || tokens > INT32_MAX / 2 || n_pages < 0 || n_pages > INT32_MAX || n_blocks < 0 ||
         n_blocks * page > (int64_t)INT32_MAX - 4096 || group < 0 || (group > 0 && R % group) || (n_blocks > 0 && table_sb < n_blocks))
         return fail(NT_ERR_ARG, "nt_kv_fork: bad sizes");
     if (R == 0) return NT_OK;
     if (!table || !refs || !lengths || !parents || !copies || (group > 0 && !shared)) return fail(NT_ERR_ARG, "nt_kv_fork: null pointer");
+    const int64_t need = nt_kv_fork_workspace_bytes(R, n_blocks, group);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(NT_ERR_WORKSPACE, "nt_kv_fork: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
     int dev = 0;
     cudaGetDevice(&dev);
     ForkArgs a{};
@@ -296,8 +324,8 @@ int nt_kv_fork(int64_t R, int64_t n_pages, int64_t n_blocks, int64_t page, int64
     if (!a.err) return fail(NT_ERR_CUDA, "nt_kv_fork: error word unavailable");
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (n_blocks > 0) {
-        a.columns = (int)std::min<int64_t>(std::min<int64_t>(64, n_blocks), kTableWords / R);
-        a.column_ctas = (int)((n_blocks + a.columns - 1) / a.columns);
+        fork_columns(R, n_blocks, &a.columns, &a.column_ctas);
+        a.alike = static_cast<int32_t*>(workspace);
         fork_table_kernel<<<a.column_ctas, kTableThreads, 0, st>>>(a);
         const int rc = check_launch("fork_table_kernel");
         if (rc != NT_OK) return rc;

@@ -29,7 +29,7 @@ struct Words {
 };
 
 constexpr int kEntries = 9;
-constexpr int64_t kWords[kEntries] = {21, 25, 27, 27, 19, 6, 15, 9, 29};
+constexpr int64_t kWords[kEntries] = {21, 25, 27, 27, 19, 6, 17, 9, 29};
 
 }  // namespace
 
@@ -124,8 +124,10 @@ extern "C" int nt_call_packed(int entry, const void* words, int64_t n_words) {
         const int32_t* parents = w.ptr<int32_t>();
         int32_t* copies = w.ptr<int32_t>();
         int32_t* shared = w.ptr<int32_t>();
+        void* ws = w.ptr<void>();
+        const int64_t bytes = w.i();
         return nt_kv_fork(R, pages, blocks, page, tokens, window, group, table, table_sb, refs, lengths, parents, copies, shared,
-                          w.ptr<void>());
+                          ws, bytes, w.ptr<void>());
     }
     if (entry == NT_ENTRY_KV_COPY_PAGES) {
         const int64_t n_layers = w.i();

@@ -33,15 +33,17 @@ __device__ __forceinline__ void move_straight(const MoveArgs& a, char* base, int
         if (src == r) continue;
         const W* s = reinterpret_cast<const W*>(base + src * stride);
         W* d = reinterpret_cast<W*>(base + r * stride);
-        int64_t i = threadIdx.x;
-        for (; i + 3 * kMoveThreads < n_words; i += 4 * kMoveThreads) {
-            const W v0 = s[i], v1 = s[i + kMoveThreads], v2 = s[i + 2 * kMoveThreads], v3 = s[i + 3 * kMoveThreads];
-            d[i] = v0;
-            d[i + kMoveThreads] = v1;
-            d[i + 2 * kMoveThreads] = v2;
-            d[i + 3 * kMoveThreads] = v3;
+        // a chunk's words all on their way, up to 16 a thread
+        constexpr int N = kMoveChunk / (int)sizeof(W) / kMoveThreads < 16 ? kMoveChunk / (int)sizeof(W) / kMoveThreads : 16;
+        for (int64_t i = threadIdx.x; i < n_words; i += N * kMoveThreads) {
+            W v[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (i + j * kMoveThreads < n_words) v[j] = s[i + j * kMoveThreads];
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (i + j * kMoveThreads < n_words) d[i + j * kMoveThreads] = v[j];
         }
-        for (; i < n_words; i += kMoveThreads) d[i] = s[i];
     }
 }
 template <typename W>

@@ -79,7 +79,8 @@ _SIGS = {
     "nt_beam_select_workspace_bytes": ([_I32] + [_I64] * 4, _I64),
     "nt_beam_select": ([_I32] + [_I64] * 4 + [_P, _I64, _P, _P, _P, ctypes.c_double, _I64, _I32] + [_P] * 4 + [_I64, _P], _I32),
     "nt_reorder_rows": ([_I64, _P, _I64, _I64, _P, _P], _I32),
-    "nt_kv_fork": ([_I64] * 7 + [_P, _I64] + [_P] * 6, _I32),
+    "nt_kv_fork_workspace_bytes": ([_I64] * 3, _I64),
+    "nt_kv_fork": ([_I64] * 7 + [_P, _I64] + [_P] * 6 + [_I64, _P], _I32),
     "nt_kv_copy_pages": ([_I64, _P] + [_I64] * 5 + [_P, _P], _I32),
     "nt_kv_attention_shared_workspace_bytes": ([_I32] + [_I64] * 9, _I64),
     "nt_kv_attention_shared": ([_I32] + [_I64] * 10 + [_F32, _P, _I64, _I64, _I64] + [_P] * 5 + [_I64] + [_P] * 5 + [_I64, _P], _I32),
@@ -496,7 +497,7 @@ _PACKED = {"nt_rotary": (0, 21, struct.Struct("=8qd12q").pack), "nt_kv_append": 
            "nt_kv_attention": (2, 27, struct.Struct("=10qd16q").pack),
            "nt_logits_process": (3, 27, struct.Struct("=11qqdqdqd10q").pack),
            "nt_beam_select": (4, 19, struct.Struct("=10qd8q").pack), "nt_reorder_rows": (5, 6, struct.Struct("=6q").pack),
-           "nt_kv_fork": (6, 15, struct.Struct("=15q").pack), "nt_kv_copy_pages": (7, 9, struct.Struct("=9q").pack),
+           "nt_kv_fork": (6, 17, struct.Struct("=17q").pack), "nt_kv_copy_pages": (7, 9, struct.Struct("=9q").pack),
            "nt_kv_attention_shared": (8, 29, struct.Struct("=11qd17q").pack)}
 
 
@@ -973,6 +974,11 @@ def _bytes_address(b: bytes) -> int:
     return ctypes.cast(b, ctypes.c_void_p).value
 
 
+@functools.lru_cache(maxsize=256)
+def _kv_fork_bytes(*sizes: int) -> int:
+    return load().nt_kv_fork_workspace_bytes(*sizes)
+
+
 def kv_fork(table: Tensor, refs: Tensor, lengths: Tensor, parents: Tensor, page: int, tokens: int = 1,
             window: Optional[int] = None, group: Optional[int] = None) -> Tuple[Tensor, Optional[Tensor]]:
     """Lets row r of a cache go on from row parents[r] without copying it -> (copies [R, 2], shared [R / group]).
@@ -1005,10 +1011,15 @@ def kv_fork(table: Tensor, refs: Tensor, lengths: Tensor, parents: Tensor, page:
         raise ValueError(f"kv_fork: {R} rows in groups of {group}")
     parents = _row_ints("kv_fork", "parents", parents, R)
     copies = torch.empty((R, 2), dtype=torch.int32, device=table.device)
-    shared = None if group is None else torch.empty(R // group, dtype=torch.int32, device=table.device)
+    shared = ws = None
+    nbytes = 0
+    if group is not None:
+        nbytes = _kv_fork_bytes(R, blocks, group)
+        shared = torch.empty(R // group, dtype=torch.int32, device=table.device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=table.device)
     _launch(index, "nt_kv_fork", R, refs.numel(), blocks, page, tokens, -1 if window is None else min(int(window), 2 ** 31),
             group or 0, table.data_ptr(), max(table.stride(0), blocks), refs.data_ptr(), lengths.data_ptr(), parents.data_ptr(),
-            copies.data_ptr(), _ptr(shared))
+            copies.data_ptr(), _ptr(shared), _ptr(ws), nbytes)
     increment_version((table, refs, lengths))
     return copies, shared
 
