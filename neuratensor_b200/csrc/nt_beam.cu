@@ -134,22 +134,33 @@ __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_co
     };
     // keeps the n best of the first m entries of the list, in order
     auto shrink = [&](int m) {
-        unsigned long long mine[kBeamList / kBeamThreads];
-        int rank[kBeamList / kBeamThreads];
+        if (m <= kBeamThreads) {
+            // several lanes an entry, each against its part of the others
+            const int q = m <= 32 ? 8 : m <= 64 ? 4 : m <= 128 ? 2 : 1, c = tid / q;
+            const unsigned long long mine = c < m ? list[c] : 0ull;
+            int rank = 0;
+            for (int j = tid % q; j < m; j += q) rank += list[j] > mine;
+            for (int o = 1; o < q; o *= 2) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+            __syncthreads();
+            if (tid % q == 0 && c < m && rank < a.n) list[rank] = mine;
+        } else {
+            unsigned long long mine[kBeamList / kBeamThreads];
+            int rank[kBeamList / kBeamThreads];
 #pragma unroll
-        for (int i = 0; i < kBeamList / kBeamThreads; ++i) {
-            mine[i] = tid + i * kBeamThreads < m ? list[tid + i * kBeamThreads] : 0ull;
-            rank[i] = 0;
+            for (int i = 0; i < kBeamList / kBeamThreads; ++i) {
+                mine[i] = tid + i * kBeamThreads < m ? list[tid + i * kBeamThreads] : 0ull;
+                rank[i] = 0;
+            }
+            for (int j = 0; j < m; ++j) {
+                const unsigned long long k = list[j];
+#pragma unroll
+                for (int i = 0; i < kBeamList / kBeamThreads; ++i) rank[i] += k > mine[i];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kBeamList / kBeamThreads; ++i)
+                if (tid + i * kBeamThreads < m && rank[i] < a.n) list[rank[i]] = mine[i];
         }
-        for (int j = 0; j < m; ++j) {
-            const unsigned long long k = list[j];
-#pragma unroll
-            for (int i = 0; i < kBeamList / kBeamThreads; ++i) rank[i] += k > mine[i];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kBeamList / kBeamThreads; ++i)
-            if (tid + i * kBeamThreads < m && rank[i] < a.n) list[rank[i]] = mine[i];
         __syncthreads();
         return m < a.n ? m : a.n;
     };
@@ -158,11 +169,22 @@ __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_co
     int held = 0, bound_of = 0;                         // entries when the bound was taken
     const int rounds = (a.n + kBeamWarps - 1) / kBeamWarps;
     uint4 raw[kBeamVecs], next[kBeamVecs];
+    // whole vectors of an aligned row, all of a tile, need no checks
+    const int64_t plain = off == 0 ? (end * E <= a.V ? end : end - 1) - kBeamVecs * kBeamThreads : -1;
+    const uint4* mine = reinterpret_cast<const uint4*>(x) + tid;
     auto load = [&](int64_t v0, uint4 (&to)[kBeamVecs]) {
+        if (v0 <= plain) {
 #pragma unroll
-        for (int j = 0; j < kBeamVecs; ++j) {
-            const int64_t v = v0 + j * kBeamThreads + tid;
-            to[j] = v < end ? beam_load<T>(x, off, v * E, a.V) : none;
+            for (int j = 0; j < kBeamVecs; ++j) to[j] = __ldcs(mine + v0 + j * kBeamThreads);
+        } else {
+#pragma unroll 1
+            for (int j = 0; j < kBeamVecs; ++j) {
+                const int64_t v = v0 + j * kBeamThreads + tid;
+                const uint4 w = v < end ? beam_load<T>(x, off, v * E, a.V) : none;
+#pragma unroll
+                for (int i = 0; i < kBeamVecs; ++i)
+                    if (i == j) to[i] = w;
+            }
         }
     };
     load(begin, next);
@@ -171,19 +193,17 @@ __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_co
 #pragma unroll
         for (int j = 0; j < kBeamVecs; ++j) raw[j] = next[j];
         if (v0 + kBeamThreads * kBeamVecs < end) load(v0 + kBeamThreads * kBeamVecs, next);
-        float best = -INFINITY;
-        if constexpr (DT == NT_F32) {
+        float tops[kBeamVecs], best = -INFINITY;        // of each vector, and of all
 #pragma unroll
-            for (int j = 0; j < kBeamVecs; ++j)
-#pragma unroll
-                for (int e = 0; e < E; ++e) best = fmaxf(best, value(raw[j], e));
-        } else {
-            __nv_bfloat162 two = *reinterpret_cast<const __nv_bfloat162*>(&none.x);
-#pragma unroll
-            for (int j = 0; j < kBeamVecs; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) two = __hmax2(two, reinterpret_cast<const __nv_bfloat162*>(&raw[j])[e]);
-            best = fmaxf(__low2float(two), __high2float(two));
+        for (int j = 0; j < kBeamVecs; ++j) {
+            if constexpr (DT == NT_F32) {
+                tops[j] = fmaxf(fmaxf(value(raw[j], 0), value(raw[j], 1)), fmaxf(value(raw[j], 2), value(raw[j], 3)));
+            } else {
+                const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(&raw[j]);
+                const __nv_bfloat162 two = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+                tops[j] = fmaxf(__low2float(two), __high2float(two));
+            }
+            best = fmaxf(best, tops[j]);
         }
         if (held < a.n) {
             // no bound yet: the r-th largest of each warp's lane maxima, the smallest of that over the warps
@@ -213,9 +233,9 @@ __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_co
             for (int w = 1; w < kBeamWarps; ++w) least = min(least, warp_bound[w]);
             bound = least ? from_ordered(least) : -INFINITY;
         }
-        if (best >= bound && best > -INFINITY) {
 #pragma unroll
-            for (int j = 0; j < kBeamVecs; ++j)
+        for (int j = 0; j < kBeamVecs; ++j)
+            if (tops[j] >= bound && tops[j] > -INFINITY) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const float f = value(raw[j], e);
@@ -224,7 +244,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_co
                         if (at < kBeamList) list[at] = beam_key(f, (uint32_t)((v0 + j * kBeamThreads + tid) * E + e));
                     }
                 }
-        }
+            }
         __syncthreads();
         const int now = count;
         if (now > kBeamList) {
