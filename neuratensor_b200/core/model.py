@@ -406,14 +406,35 @@ class NeuraTensorModel(nn.Module):
         """The captured single-token step for this batch size."""
         return self.step_graph(batch, 1, device, dtype, cache_tokens)
 
+    @torch.no_grad()
+    def beam_step(self, prompts: int, beams: int, device, dtype, cache_tokens: int, length_penalty: float,
+                  stop: Tuple[int, ...], capture: bool = True):
+        """A beam search's step (``inference/beams.py``), captured ones kept like ``step_graph``'s (the last two);
+        ``cache_tokens`` 0: without an attention memory."""
+        from ..inference.beams import BeamStep
+        if not capture:
+            return BeamStep(self, prompts, beams, device, dtype, cache_tokens, length_penalty, stop, capture=False)
+        cache_tokens = -(-cache_tokens // 1024) * 1024      # so that calls of other lengths find the same graph
+        key = (prompts, beams, str(device), dtype, cache_tokens, length_penalty, stop)
+        cache = self.__dict__.setdefault("_beam_steps", {})
+        hit = cache.pop(key, None)
+        if hit is None or hit[0] != self._graph_signature(cache_tokens) or not hit[1].frequencies_hold():
+            hit = None
+            while len(cache) >= 2:
+                cache.pop(next(iter(cache)))
+            step = BeamStep(self, prompts, beams, torch.device(device), dtype, cache_tokens, length_penalty, stop)
+            hit = (self._graph_signature(cache_tokens), step)
+        cache[key] = hit
+        return hit[1]
+
     def generate(self, input_ids: Tensor, max_new_tokens: int = 50, temperature: float = 1.0, top_k: int = 50,
                  top_p: float = 1.0, repetition_penalty: float = 1.0, stop_tokens: Optional[List[int]] = None,
                  states: Optional[List[Optional[BlockState]]] = None,
                  use_graph: bool = True, attn_cache: Union[bool, AttentionCache] = False,
                  frequency_penalty: float = 0.0, presence_penalty: float = 0.0,
                  logit_bias: Optional[Dict[int, float]] = None,
-                 allowed: Union[None, Tensor, Callable[[Tensor], Optional[Tensor]]] = None
-                 ) -> Tuple[Tensor, List[BlockState]]:
+                 allowed: Union[None, Tensor, Callable[[Tensor], Optional[Tensor]]] = None,
+                 num_beams: int = 1, length_penalty: float = 0.0) -> Tuple[Tensor, List[BlockState]]:
         """Autoregressive sampling with carried block state (model.py:301-370).
 
         On CUDA the per-token steps replay one captured graph of the whole model
@@ -430,9 +451,37 @@ class NeuraTensorModel(nn.Module):
         the int32 words of ``native.pack_allowed``, or a function of the tokens so far
         that returns one (or None).  Penalties and biases are finite (at most 1e20), and a
         mask that leaves a sequence no token is refused; a function's is read for that at
-        every step."""
+        every step.
+
+        ``num_beams`` above 1 searches instead of sampling (``inference/beams.py``): the
+        continuation of largest log-probability among the beams, divided by its length to
+        the power of ``length_penalty``; a beam ends with a stop token (then the first of them
+        fills up) or with ``max_new_tokens``.  It takes ``stop_tokens``, ``states``,
+        ``use_graph`` and ``attn_cache=True``; what shapes a distribution to sample from is
+        refused.  The states are the best beams', which have not run their last token."""
         from .. import native
         self.eval()
+        if num_beams != 1:
+            for name, given in (("temperature", temperature != 1.0), ("top_p", top_p != 1.0), ("repetition_penalty", repetition_penalty != 1.0),
+                                ("frequency_penalty", bool(frequency_penalty)), ("presence_penalty", bool(presence_penalty)),
+                                ("logit_bias", bool(logit_bias)), ("allowed", allowed is not None),
+                                ("an AttentionCache", isinstance(attn_cache, AttentionCache))):
+                if given:
+                    raise ValueError(f"beam search takes no {name}")
+            if not 2 <= num_beams <= 64 or input_ids.shape[0] * num_beams > 1024:
+                raise ValueError(f"num_beams must be 1 to 64 and at most 1024 in all, got {num_beams} for {input_ids.shape[0]} prompts")
+            if not math.isfinite(length_penalty):
+                raise ValueError(f"length_penalty must be finite, got {length_penalty}")
+            if any(not 0 <= t < self.config.vocab_size for t in stop_tokens or []):
+                raise ValueError(f"stop_tokens outside the vocabulary of {self.config.vocab_size}")
+            if max_new_tokens < 1 or input_ids.shape[1] < 1:
+                raise ValueError("beam search needs a prompt and at least one new token")
+            from ..inference.beams import beam_search
+            with torch.no_grad():
+                return beam_search(self, input_ids, max_new_tokens, num_beams, float(length_penalty), list(stop_tokens or []), states,
+                                   use_graph, bool(attn_cache))
+        if length_penalty:
+            raise ValueError("length_penalty is for num_beams above 1")
         out = input_ids
         B, prompt = out.shape
         # what would leave a row without a finite largest logit is refused before anything runs:

@@ -152,7 +152,7 @@ class InferenceEngine:
         """Returns [B, T + generated] token ids (engine.py:180-208).
 
         ``more``: the model's own arguments beyond the reference (``attn_cache``,
-        ``frequency_penalty``, ``presence_penalty``, ``logit_bias``, ``allowed``)."""
+        ``frequency_penalty``, ``presence_penalty``, ``logit_bias``, ``allowed``, ``num_beams``, ``length_penalty``)."""
         if reset_state:
             self.reset_state()
         ids = input_ids.to(self.device)
