@@ -25,7 +25,7 @@ namespace {
 
 constexpr int kBeamThreads = 256;
 constexpr int kBeamWarps = kBeamThreads / 32;
-constexpr int kBeamVecs = 4;           // 16-byte vectors of a thread in flight
+constexpr int kBeamVecs = 2;           // 16-byte vectors of a thread in work, and as many on their way
 constexpr int kBeamList = 1024;        // candidates a slice can hold
 constexpr int kBeamMost = 64;          // n, and beams of an item
 constexpr int kBeamLists = 1024;       // slices of an item's beams
@@ -70,6 +70,18 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
     return k;
 }
 
+// The 16 bytes that lie `off` bytes into lo and hi.
+__device__ __forceinline__ uint4 beam_pick(const uint4& lo, const uint4& hi, int off) {
+    const uint32_t w[9] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w, 0u};
+    const int odd = (off & 2) * 8;                      // bits
+    uint32_t o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)                         // one of the four, the same for the row
+        if (off >> 2 == k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = __funnelshift_r(w[i + k], w[i + k + 1], odd);
+    return make_uint4(o[0], o[1], o[2], o[3]);
+}
 // Elements at .. at + 15 / sizeof(T) of a row of V, -inf behind its end.  What a thread takes does
 // not depend on the row's alignment, so that equal rows have equal sums: a row off 16-byte
 // alignment takes two aligned vectors and picks.
@@ -83,16 +95,7 @@ __device__ __forceinline__ uint4 beam_load(const T* x, int off, int64_t at, int6
         out = __ldcs(reinterpret_cast<const uint4*>(x + at));
     } else if (off != 0 && at >= before && at - before + 2 * E <= V) {
         const uint4* p = reinterpret_cast<const uint4*>(x + at - before);
-        uint32_t w[9];
-        *reinterpret_cast<uint4*>(w) = __ldg(p);
-        *reinterpret_cast<uint4*>(w + 4) = __ldg(p + 1);
-        w[8] = 0u;
-        const int odd = (off & 2) * 8;                  // bits
-#pragma unroll
-        for (int k = 0; k < 4; ++k)                     // one of the four, the same for the row
-            if (off >> 2 == k)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] = __funnelshift_r(w[i + k], w[i + k + 1], odd);
+        out = beam_pick(__ldg(p), __ldg(p + 1), off);
     } else {
         // element by element, across the row's end too
         auto bits = [&](int e) -> uint32_t {
@@ -109,7 +112,7 @@ __device__ __forceinline__ uint4 beam_load(const T* x, int off, int64_t at, int6
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
+__global__ void __launch_bounds__(kBeamThreads, 4) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
     using T = typename Elem<DT>::T;
     constexpr int E = 16 / (int)sizeof(T);
     __shared__ unsigned long long list[kBeamList];
@@ -169,13 +172,21 @@ __global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const __grid_co
     int held = 0, bound_of = 0;                         // entries when the bound was taken
     const int rounds = (a.n + kBeamWarps - 1) / kBeamWarps;
     uint4 raw[kBeamVecs], next[kBeamVecs];
-    // whole vectors of an aligned row, all of a tile, need no checks
-    const int64_t plain = off == 0 ? (end * E <= a.V ? end : end - 1) - kBeamVecs * kBeamThreads : -1;
-    const uint4* mine = reinterpret_cast<const uint4*>(x) + tid;
+    // tiles of whole vectors need no checks: of an aligned row up to `plain`, of another from vector 1 to `picked`
+    constexpr int kTileVecs = kBeamVecs * kBeamThreads;
+    const int64_t plain = off == 0 ? min(end, a.V / E) - kTileVecs : -1;
+    const int64_t picked = off != 0 ? min(end, (a.V + off / (int)sizeof(T)) / E - 1) - kTileVecs : -1;
+    const uint4* mine = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(x) - off) + tid;
     auto load = [&](int64_t v0, uint4 (&to)[kBeamVecs]) {
         if (v0 <= plain) {
 #pragma unroll
             for (int j = 0; j < kBeamVecs; ++j) to[j] = __ldcs(mine + v0 + j * kBeamThreads);
+        } else if (v0 > 0 && v0 <= picked) {
+#pragma unroll
+            for (int j = 0; j < kBeamVecs; ++j) {
+                const uint4 lo = __ldg(mine + v0 + j * kBeamThreads), hi = __ldg(mine + v0 + j * kBeamThreads + 1);
+                to[j] = beam_pick(lo, hi, off);
+            }
         } else {
 #pragma unroll 1
             for (int j = 0; j < kBeamVecs; ++j) {
@@ -407,8 +418,20 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
                 if (r > best || (r && r == best && (k < beam || (k == beam && t < token)))) best = r, beam = k, token = t, from = l;
             }
         };
-        for (int l = lane; l < lists; l += 32) head_at[l] = 0;
-        pick();
+        // with a list a lane or none, its next two candidates are in registers
+        const bool each = near && lists <= 32;
+        int at = 0;
+        unsigned long long then = 0ull;
+        uint32_t then_token = 0u;
+        if (each) {
+            if (lane < lists) {
+                best = ranks[lane * n], token = tokens[lane * n], beam = lane / S, from = lane;
+                if (n > 1) then = ranks[lane * n + 1], then_token = tokens[lane * n + 1];
+            }
+        } else {
+            for (int l = lane; l < lists; l += 32) head_at[l] = 0;
+            pick();
+        }
         for (int i = 0; i < n; ++i) {
             // the largest rank, of equal ones the lowest beam and token
             const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
@@ -427,10 +450,17 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
             }
             if (mine) {
                 chosen[i] = (int)beam;
-                chosen_from[i] = from * n + head_at[from];
                 chosen_token[i] = token;
-                ++head_at[from];
-                pick();
+                if (each) {
+                    chosen_from[i] = lane * n + at++;
+                    best = then, token = then_token;
+                    then = 0ull;
+                    if (at + 1 < n) then = ranks[lane * n + at + 1], then_token = tokens[lane * n + at + 1];
+                } else {
+                    chosen_from[i] = from * n + head_at[from];
+                    ++head_at[from];
+                    pick();
+                }
             }
             __syncwarp();
         }

@@ -940,7 +940,7 @@ def reorder_rows(tensors: Sequence[Tensor], rows: Tensor, group: Optional[int] =
     is right, also one that swaps; rows that stay are not touched.  A row
     outside its group is left and flagged (device_error_flags)."""
     tensors = list(tensors)
-    index = _device_index(rows, *tensors)
+    index = _device_index(rows)
     if rows.dim() != 1:
         raise ValueError(f"reorder_rows: rows must be [R], got {tuple(rows.shape)}")
     R = rows.numel()
@@ -952,17 +952,18 @@ def reorder_rows(tensors: Sequence[Tensor], rows: Tensor, group: Optional[int] =
         rows = _ints(rows, torch.int32, "rows")
     rows = rows.contiguous()
     spec = []
-    for t in tensors:
+    for t in tensors:                                   # dozens of them, so no more than needed for each
+        if t.get_device() != index:
+            _device_index(rows, t)                      # says what is wrong
         if t.dim() < 1 or t.shape[0] != R:
             raise ValueError(f"reorder_rows: every tensor must have {R} rows, got {tuple(t.shape)}")
-        size = t.element_size()
         if t.is_contiguous():
-            row = t.numel() // R * size if R else 0
-            spec += (t.data_ptr(), row, row)
+            row = apart = t.nbytes // R if R else 0
         else:
             if R and not t[0].is_contiguous() or R > 1 and t.stride(0) < t[0].numel():
                 raise ValueError("reorder_rows: the rows of a tensor must lie in one piece each, without overlap")
-            spec += (t.data_ptr(), t[0].numel() * size if R else 0, t.stride(0) * size)
+            row, apart = (t[0].nbytes if R else 0), t.stride(0) * t.element_size()
+        spec += (t.data_ptr(), row, apart)
     if not spec:
         return
     words = struct.pack(f"={len(spec)}q", *spec)
