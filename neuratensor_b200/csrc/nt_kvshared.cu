@@ -25,6 +25,18 @@
 // CTAs share an SM where they fit, so that one's products run under the other's softmax; the
 // softmax warps take registers from the others.  The
 // tiles of all groups and heads in a row are cut into even shares, one a CTA.
+//
+// 64 samples of 4 query heads on each of 8 cached heads of 128 over 65536 shared keys (69 GFLOP,
+// 42 us at the measured rate; half as much again is done for the weights' second halves), caches
+// flushed: this kernel 123 us, the rest of the rows until 150, the join until 164.  A tile of 128
+// keys takes a CTA 8400 clocks, two CTAs an SM: scores 1300, softmax 4500, sums 1300, the rest
+// hand-overs.  The tensor cores are busy a fifth of the time, a scheduler issues four clocks in
+// ten; exponentials (1024 clocks a tile and scheduler) and conversions share what is left.  On
+// the way: 177 us with four loading warps whose registers spilled (shared memory leaves no L1
+// to catch that), 147 with eight, 131 with the look-ups in shared memory, 123 with 32 columns a step.
+//
+// Few rows (kFewRows) take the attention of nt_kvattn.cu instead, over both parts in one kernel;
+// short reaches (kSReach, kSBytes) that without sharing.
 #include "nt_kvattn.cuh"
 
 #include <cuda_bf16.h>
@@ -679,6 +691,7 @@ __global__ void __launch_bounds__(kSThreads, SharedCfg<DT, D>::kPerSm) kv_shared
         }
         if (!ok && lane == 0) atomicOr(a.err, ERRF_TIMEOUT_PRODUCER);
         if (bad_page) atomicOr(a.err, ERRF_BAD_ARG);
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
     s_fence_before();
     __syncthreads();

@@ -276,7 +276,7 @@ def test_reorder_refusals(nat):
     t = torch.arange(12.0, device=DEV).view(6, 2)
     rows = torch.arange(6, device=DEV, dtype=torch.int32)
     for bad in (dict(rows=rows.view(2, 3)), dict(group=4), dict(group=0), dict(tensors=[t[:5]]), dict(tensors=[t.t().contiguous().t()]),
-                dict(tensors=[t[:1].expand(6, 2)]), dict(tensors=[t[0, 0]]), dict(rows=torch.zeros(1025, device=DEV, dtype=torch.int32),
+                dict(tensors=[t[:1].expand(6, 2)]), dict(tensors=[t[0, 0]]), dict(tensors=[t, t.clone(), t]), dict(rows=torch.zeros(1025, device=DEV, dtype=torch.int32),
                                                                                 tensors=[torch.zeros(1025, 1, device=DEV)])):
         with pytest.raises(ValueError):
             nat.reorder_rows(**{**dict(tensors=[t], rows=rows), **bad})
