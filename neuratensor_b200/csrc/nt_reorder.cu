@@ -5,9 +5,9 @@
 // for all); where no row that is read is written, as when surviving beams keep their
 // places, they are copied straight.  Rows that stay are neither read nor written.  Bound
 // by HBM: each row that is followed is read once, each that changes written once.  One row in
-// four of the large preset's 28 blocks and 64 rows (947 MB): 148 us, 98 % of the copy rate;
-// half of 40 float32 rows of an odd length (56 MB), by 4-byte words with 16 of a thread on their way, 16 us
-// (with four 18, without them all but one 34).
+// four of the large preset's 28 blocks and 64 rows (947 MB): 147 us, 99 % of the copy rate;
+// half of 40 float32 rows of an odd length (56 MB), by 4-byte words, 17 us (with four of a thread on their way
+// 18).
 #include "nt_kernels.cuh"
 
 #include <algorithm>
@@ -36,8 +36,8 @@ __device__ __forceinline__ void move_straight(const MoveArgs& a, char* base, int
         if (src == r) continue;
         const W* s = reinterpret_cast<const W*>(base + src * stride);
         W* d = reinterpret_cast<W*>(base + r * stride);
-        // a chunk's words all on their way, up to 16 a thread
-        constexpr int N = kMoveChunk / (int)sizeof(W) / kMoveThreads < 16 ? kMoveChunk / (int)sizeof(W) / kMoveThreads : 16;
+        // a chunk's words on their way, up to 8 a thread (more registers cost a CTA an SM: 157 and 174 us for 148)
+        constexpr int N = kMoveChunk / (int)sizeof(W) / kMoveThreads < 8 ? kMoveChunk / (int)sizeof(W) / kMoveThreads : 8;
         int64_t i = threadIdx.x;
         for (; i - threadIdx.x + N * kMoveThreads <= n_words; i += N * kMoveThreads) {
             W v[N];
@@ -46,13 +46,13 @@ __device__ __forceinline__ void move_straight(const MoveArgs& a, char* base, int
 #pragma unroll
             for (int j = 0; j < N; ++j) d[i + j * kMoveThreads] = v[j];
         }
-        if (i - threadIdx.x < n_words) {                // the row's last chunk
-            W v[N];
+        for (; i - threadIdx.x < n_words; i += N / 2 * kMoveThreads) {      // the row's last chunk
+            W v[N / 2];
 #pragma unroll
-            for (int j = 0; j < N; ++j)
+            for (int j = 0; j < N / 2; ++j)
                 if (i + j * kMoveThreads < n_words) v[j] = s[i + j * kMoveThreads];
 #pragma unroll
-            for (int j = 0; j < N; ++j)
+            for (int j = 0; j < N / 2; ++j)
                 if (i + j * kMoveThreads < n_words) d[i + j * kMoveThreads] = v[j];
         }
     }
@@ -77,7 +77,7 @@ __device__ __forceinline__ void move_staged(const MoveArgs& a, char* base, int64
     }
 }
 
-__global__ void __launch_bounds__(kMoveThreads) reorder_rows_kernel(const __grid_constant__ MoveArgs a) {
+__global__ void __launch_bounds__(kMoveThreads, 5) reorder_rows_kernel(const __grid_constant__ MoveArgs a) {
     __shared__ __align__(16) unsigned char smem[kMoveStage];
     __shared__ int16_t from[kMoveGroup];
     __shared__ uint8_t read[kMoveGroup];
