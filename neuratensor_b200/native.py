@@ -955,8 +955,9 @@ def reorder_rows(tensors: Sequence[Tensor], rows: Tensor, group: Optional[int] =
     for t in tensors:                                   # dozens of them, so no more than needed for each
         if t.get_device() != index:
             _device_index(rows, t)                      # says what is wrong
-        if t.dim() < 1 or t.shape[0] != R:
-            raise ValueError(f"reorder_rows: every tensor must have {R} rows, got {tuple(t.shape)}")
+        shape = t.shape
+        if not shape or shape[0] != R:
+            raise ValueError(f"reorder_rows: every tensor must have {R} rows, got {tuple(shape)}")
         if t.is_contiguous():
             row = apart = t.nbytes // R if R else 0
         else:
@@ -1034,7 +1035,8 @@ def kv_copy_pages(layers: Sequence[Tuple[Tensor, Tensor, Tensor, Tensor]], pages
     pages: int32 [N, 2], from and to, (-1, -1) is skipped (kv_fork's copies).  No page may be
     written twice, or both read and written; one outside the pool is skipped and flagged."""
     layers = list(layers)
-    index = _device_index(pages, *[t for layer in layers for t in layer])
+    flat = [t for layer in layers for t in layer]
+    index = _device_index(pages, *flat)
     if pages.dim() != 2 or pages.shape[1] != 2 or pages.dtype != torch.int32:
         raise ValueError(f"kv_copy_pages: pages must be int32 [N, 2], got {pages.dtype} {tuple(pages.shape)}")
     if not layers:
@@ -1042,23 +1044,24 @@ def kv_copy_pages(layers: Sequence[Tuple[Tensor, Tensor, Tensor, Tensor]], pages
     shape = layers[0][0].shape
     if len(shape) != 4 or shape[1] < 1 or shape[3] not in (64, 128) or shape[2] not in (16, 32, 64):
         raise ValueError(f"kv_copy_pages: codes must be [pages, heads, page of 16, 32 or 64, 64 or 128], got {tuple(shape)}")
-    spec = []
-    for layer in layers:
-        kc, ks, vc, vs = layer
-        for c, s in ((kc, ks), (vc, vs)):
-            if c.shape != shape or c.dtype not in (torch.float8_e4m3fn, torch.uint8) or not c.is_contiguous():
+    per_head, f8, u8, f32 = shape[:2], torch.float8_e4m3fn, torch.uint8, torch.float32
+    for kc, ks, vc, vs in layers:
+        for c in (kc, vc):
+            dtype = c.dtype
+            if c.shape != shape or dtype != f8 and dtype != u8 or not c.is_contiguous():
                 raise ValueError(f"kv_copy_pages: codes must be contiguous float8_e4m3fn or uint8 {tuple(shape)}")
-            if s.shape != shape[:2] or s.dtype != torch.float32 or not s.is_contiguous():
-                raise ValueError(f"kv_copy_pages: scales must be contiguous float32 {tuple(shape[:2])}")
-            spec += (c.data_ptr(), s.data_ptr())
-        _refuse_out("kv_copy_pages", *layer)
+        for x in (ks, vs):
+            if x.shape != per_head or x.dtype != f32 or not x.is_contiguous():
+                raise ValueError(f"kv_copy_pages: scales must be contiguous float32 {tuple(per_head)}")
+    _refuse_out("kv_copy_pages", *flat)
+    spec = [t.data_ptr() for t in flat]
     if shape[0] == 0 or pages.shape[0] == 0:
         return
     pages = pages.contiguous()
     words = struct.pack(f"={len(spec)}q", *spec)
     _launch(index, "nt_kv_copy_pages", len(layers), _bytes_address(words), shape[0], shape[1], shape[2], shape[3], pages.shape[0],
             pages.data_ptr())
-    increment_version([t for layer in layers for t in layer])
+    increment_version(flat)
 
 
 @functools.lru_cache(maxsize=256)
