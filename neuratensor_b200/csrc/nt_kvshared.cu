@@ -29,11 +29,12 @@
 // 64 samples of 4 query heads on each of 8 cached heads of 128 over 65536 shared keys (69 GFLOP,
 // 42 us at the measured rate; half as much again is done for the weights' second halves), caches
 // flushed: this kernel 123 us, the rest of the rows until 150, the join until 164.  A tile of 128
-// keys takes a CTA 8400 clocks, two CTAs an SM: scores 1300, softmax 4500, sums 1300, the rest
-// hand-overs.  The tensor cores are busy a fifth of the time, a scheduler issues four clocks in
-// ten; exponentials (1024 clocks a tile and scheduler) and conversions share what is left.  On
+// keys takes a CTA 8400 clocks, two CTAs an SM, of which its 24 products take 1600 (65 to 68 each,
+// measured alone): the softmax and the conversions beside it are the longer side (at 159 us the
+// tensor cores were busy 21 % of the time and a scheduler issued in 39 % of its clocks).  On
 // the way: 177 us with four loading warps whose registers spilled (shared memory leaves no L1
-// to catch that), 147 with eight, 131 with the look-ups in shared memory, 123 with 32 columns a step.
+// to catch that), 147 with eight, 131 with the look-ups in shared memory, 123 with 32 columns a step.  D = 128 in
+// bf16 still spills 152 bytes a thread and reads 308.
 //
 // Few rows (kFewRows) take the attention of nt_kvattn.cu instead, over both parts in one kernel;
 // short reaches (kSReach, kSBytes) that without sharing.
