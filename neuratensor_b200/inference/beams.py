@@ -10,6 +10,7 @@ the host: tokens and parents are read once at the end, where the best beam is fo
 """
 from __future__ import annotations
 
+import weakref
 from typing import List, Optional, Tuple
 
 import torch
@@ -19,6 +20,7 @@ from .. import native
 from ..core.cache import BeamCache
 from ..core.fused import BlockState
 from ..core.rotary import Seen
+from .decode import capturing
 
 
 class BeamStep:
@@ -28,7 +30,8 @@ class BeamStep:
                  stop: Tuple[int, ...], capture: bool = True) -> None:
         cfg = model.config
         R, di = prompts * beams, cfg.d_model * cfg.expand
-        self.model, self.prompts, self.beams, self.alpha = model, prompts, beams, length_penalty
+        self.model = model          # weakly: the model holds the step, which holds what it reads instead
+        self.prompts, self.beams, self.alpha = prompts, beams, length_penalty
         self.tok = torch.zeros((R, 1), dtype=torch.int64, device=device)
         self.rows = torch.arange(R, dtype=torch.int32, device=device)
         self.scores = torch.zeros((prompts, beams), dtype=torch.float32, device=device)
@@ -47,6 +50,15 @@ class BeamStep:
         layers = model.attn_layers.values()
         self.frequencies = [Seen(a.rope.inv_freq) for a in layers]
         self.held = [(a.rope.cos_cached, a.rope.sin_cached, getattr(a, "_rope_freq", None)) for a in layers]
+        self.held += [list(model.children()), [getattr(b, "_cache", None) for b in model.blocks]]
+
+    @property
+    def model(self):
+        return self._model()
+
+    @model.setter
+    def model(self, model) -> None:
+        self._model = weakref.ref(model)
 
     def frequencies_hold(self) -> bool:
         """Whether every attention layer still has the frequencies that were captured."""
@@ -95,7 +107,7 @@ class BeamStep:
             stand()
         torch.cuda.current_stream(device).wait_stream(side)
         self.graph = torch.cuda.CUDAGraph()
-        with torch.no_grad(), torch.cuda.graph(self.graph):
+        with torch.no_grad(), capturing(self.graph):
             self._step()
 
     def begin(self, ids: Tensor, states) -> None:

@@ -21,6 +21,9 @@ table that it reads is rebuilt (``NeuraTensorModel.step_graph``).  Sampling stay
 """
 from __future__ import annotations
 
+import contextlib
+import gc
+import weakref
 from typing import List, Optional
 
 import torch
@@ -31,6 +34,20 @@ from ..core.fused import BlockState
 from ..core.rotary import Seen
 
 
+@contextlib.contextmanager
+def capturing(graph: "torch.cuda.CUDAGraph"):
+    """``torch.cuda.graph`` without the garbage collector: a collection in the middle of a capture may
+    destroy another graph (that of a model no longer used, say), which is not allowed then and ends the capture."""
+    on = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph):
+            yield
+    finally:
+        if on:
+            gc.enable()
+
+
 class StepGraph:
     """A captured forward for one (batch, length), device and dtype."""
 
@@ -39,16 +56,17 @@ class StepGraph:
         from .. import native
         cfg = model.config
         di = cfg.d_model * cfg.expand
-        self.model = model
+        self.model = model          # weakly: the model holds the graph, which holds what it reads instead
+        self._state_cls = model.blocks[0]._state_cls
         self.tok = torch.zeros((batch, seq), dtype=torch.int64, device=device)
         # every block's membrane and SSM state as views of one flat buffer (one memset,
         # one copy for all of them)
         n_mem, n_st = batch * di, batch * di * cfg.d_state
         self.flat = torch.zeros(len(model.blocks) * (n_mem + n_st), dtype=dtype, device=device)
+        n = len(model.blocks)
         self._split = lambda buf: (
-            [buf[i * (n_mem + n_st):i * (n_mem + n_st) + n_mem].view(batch, di) for i in range(len(model.blocks))],
-            [buf[i * (n_mem + n_st) + n_mem:(i + 1) * (n_mem + n_st)].view(batch, di, cfg.d_state)
-             for i in range(len(model.blocks))])
+            [buf[i * (n_mem + n_st):i * (n_mem + n_st) + n_mem].view(batch, di) for i in range(n)],
+            [buf[i * (n_mem + n_st) + n_mem:(i + 1) * (n_mem + n_st)].view(batch, di, cfg.d_state) for i in range(n)])
         self.mem, self.st = self._split(self.flat)
         nbytes = native.block_workspace_bytes(dtype, batch, seq, cfg.d_model, di, cfg.d_state)
         self.ws = torch.empty(nbytes, dtype=torch.uint8, device=device)   # owned: the graph keeps its address
@@ -62,6 +80,15 @@ class StepGraph:
         layers = model.attn_layers.values()
         self.frequencies = [Seen(a.rope.inv_freq) for a in layers]
         self.held = [(a.rope.cos_cached, a.rope.sin_cached, getattr(a, "_rope_freq", None)) for a in layers]
+        self.held += [list(model.children()), [getattr(b, "_cache", None) for b in model.blocks]]
+
+    @property
+    def model(self):
+        return self._model()
+
+    @model.setter
+    def model(self, model) -> None:
+        self._model = weakref.ref(model)
 
     def frequencies_hold(self) -> bool:
         """Whether every attention layer still has the frequencies that were captured."""
@@ -97,7 +124,7 @@ class StepGraph:
                 self._forward()
             stand()
         torch.cuda.current_stream(dev).wait_stream(side)
-        with torch.no_grad(), torch.cuda.graph(self.graph):
+        with torch.no_grad(), capturing(self.graph):
             self.logits, self.counts = self._forward()
         if self.attn_cache is not None:
             self.attn_cache.reset()
@@ -131,5 +158,4 @@ class StepGraph:
     def states(self) -> List[BlockState]:
         """Copies of the carried states (the static buffers change on the next replay)."""
         mem, st = self._split(self.flat.clone())
-        state_cls = self.model.blocks[0]._state_cls
-        return [state_cls(membrane=m, ssm_state=s) for m, s in zip(mem, st)]
+        return [self._state_cls(membrane=m, ssm_state=s) for m, s in zip(mem, st)]

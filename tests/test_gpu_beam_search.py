@@ -1,4 +1,7 @@
 """Beam search through ``generate`` (B200): against a search written out here that runs every beam from scratch."""
+import gc
+import weakref
+
 import pytest
 import torch
 
@@ -165,3 +168,58 @@ def test_memory_of_a_search_counts_its_pages(T, window, steps):
     from neuratensor_b200 import native
     assert native.device_error_flags(0) == 0
     assert (cache.table >= 0).sum(1).max() <= window // 16 + 2 and cache.lengths.tolist() == [T + steps] * (P * K)
+
+
+def test_through_the_engine():
+    from neuratensor_b200 import InferenceEngine
+    model = make(torch.bfloat16)
+    engine = InferenceEngine(model, dtype=torch.bfloat16)
+    ids = torch.randint(0, 211, (2, 11), generator=torch.Generator().manual_seed(4))
+    out = engine.generate(ids, max_new_tokens=7, num_beams=4, length_penalty=0.6, stop_tokens=[3, 9], attn_cache=True)
+    want, _ = model.generate(ids.to(DEV), max_new_tokens=7, num_beams=4, length_penalty=0.6, stop_tokens=[3, 9], attn_cache=True)
+    assert torch.equal(out, want) and out.shape == (2, 18)
+    sampled = engine.generate(ids, max_new_tokens=7, top_k=1, attn_cache=True)          # and sampling goes on beside it
+    assert sampled.shape == (2, 18)
+    with pytest.raises(ValueError, match="AttentionCache"):
+        engine.generate(ids, max_new_tokens=3, num_beams=2, attn_cache=AttentionCache(model.config, 2, 64, DEV))
+
+
+def test_models_and_their_captured_steps_go_together_and_captures_bear_collections():
+    """A step does not keep its model, so both go without the garbage collector; and one that destroys another graph does
+    not come in a capture."""
+    ids = torch.zeros(1, 4, dtype=torch.int64, device=DEV)
+    for capture in (lambda m: m.generate(ids, max_new_tokens=3, num_beams=2, attn_cache=True),
+                    lambda m: m.generate(ids, max_new_tokens=3, top_k=1, attn_cache=True)):
+        old = gc.get_threshold()
+        gc.disable()
+        try:
+            dead = make(torch.bfloat16)
+            capture(dead)
+            gone = weakref.ref(dead)
+            cycle = [list(dead.__dict__.get("_beam_steps", {}).values()) + list(dead.__dict__.get("_step_graphs", {}).values())]
+            del dead
+            assert gone() is None
+            cycle.append(cycle)                         # its graphs are left to the collector
+            del cycle
+            live = make(torch.bfloat16)
+            gc.set_threshold(1, 1, 1)                   # from here on every allocation may collect
+            gc.enable()
+            capture(live)
+        finally:
+            gc.set_threshold(*old)
+            gc.enable()
+
+
+def test_a_captured_step_outlives_its_model():
+    """A step that is kept while its model goes reads the weights that it was captured with."""
+    model = make(torch.bfloat16)
+    tok = torch.full((2, 1), 7, dtype=torch.int64, device=DEV)
+    graph = model.decode_graph(2, torch.device(DEV), torch.bfloat16)
+    graph.load_states(None)                             # capturing leaves the states where its own steps took them
+    want = graph.step(tok).clone()
+    del model
+    gc.collect()
+    junk = [torch.full((1 << 16,), 1e4, device=DEV) for _ in range(64)]                 # what was freed is written over
+    graph.load_states(None)
+    assert torch.equal(graph.step(tok), want) and len(graph.states()) == 4
+    del junk
