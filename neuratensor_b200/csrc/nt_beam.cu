@@ -125,11 +125,11 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_scan_kernel(const __grid
     __shared__ uint32_t warp_bound[kBeamWarps];
     __shared__ unsigned long long warp_key[kBeamWarps];
     __shared__ float warp_m[kBeamWarps], warp_s[kBeamWarps];
-    __shared__ int count;
+    __shared__ int found[3];                            // candidates of the tiles t, t + 1 and t + 2 (mod 3)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row = blockIdx.y;
     if (!beam_open(a, row)) return;
-    if (tid == 0) count = 0;
+    if (tid < 3) found[tid] = 0;
     const T* x = static_cast<const T*>(a.x) + row * a.ld;
     const int off = (int)(reinterpret_cast<uintptr_t>(x) & 15);       // bytes by which the row is off 16-byte alignment
     const int64_t n_vec = (a.V + E - 1) / E;
@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_scan_kernel(const __grid
     };
     load(begin, next);
     __syncthreads();
+    int slot = 0;
     for (int64_t v0 = begin; v0 < end; v0 += kBeamThreads * kBeamVecs) {
 #pragma unroll
         for (int j = 0; j < kBeamVecs; ++j) raw[j] = next[j];
@@ -257,16 +258,20 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_scan_kernel(const __grid
                 for (int e = 0; e < E; ++e) {
                     const float f = value(raw[j], e);
                     if (f >= bound && f > -INFINITY) {
-                        const int at = atomicAdd(&count, 1);
+                        const int at = held + atomicAdd(&found[slot], 1);
                         if (at < kBeamList) list[at] = beam_key(f, (uint32_t)((v0 + j * kBeamThreads + tid) * E + e));
                     }
                 }
             }
         __syncthreads();
-        const int now = count;
+        // A warp may count the next tile's candidates before another has read this tile's: each tile has a
+        // count of its own.  The one that the tile before has used, which all have read ahead of the barrier
+        // above, is cleared for the tile after the next, whose warps have passed that one's barrier.
+        const int now = held + found[slot], last = slot == 0 ? 2 : slot - 1;
+        if (tid == 0) found[last] = 0;
+        slot = slot == 2 ? 0 : slot + 1;
         if (now > kBeamList) {
             // too many: the list as it was, and the n best of this tile one after the other
-            __syncthreads();
             held = shrink(held);
             unsigned long long prev = ~0ull;
             for (int r = 0; r < a.n; ++r) {
@@ -293,7 +298,6 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_scan_kernel(const __grid
                 ++held;
                 prev = k;
             }
-            if (tid == 0) count = held;
             __syncthreads();
         } else {
             held = now;
@@ -303,8 +307,6 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_scan_kernel(const __grid
             held = shrink(held);
             bound_of = held;
             bound = from_ordered((uint32_t)(list[a.n - 1] >> 32));
-            if (tid == 0) count = held;
-            __syncthreads();
         }
     }
     // the slice's maximum and sum, and its n best
