@@ -458,7 +458,8 @@ class NeuraTensorModel(nn.Module):
         the power of ``length_penalty``; a beam ends with a stop token (then the first of them
         fills up) or with ``max_new_tokens``.  It takes ``stop_tokens``, ``states``,
         ``use_graph`` and ``attn_cache=True``; what shapes a distribution to sample from is
-        refused (but for ``top_k``, which is not looked at).  The states are the best beams', which have not run their last token."""
+        refused (but for ``top_k``, which is not looked at).  The states are the best beams', which have not run their last
+        token, that is the stop token of a beam that ended: what fills up behind it does not reach them."""
         from .. import native
         self.eval()
         if num_beams != 1:

@@ -5,7 +5,7 @@ prompt go on at once.  A step lets the attention memory's pages and the block st
 follow the chosen beams (``native.kv_fork`` and ``kv_copy_pages``, ``native.reorder_rows``),
 runs one token of every beam through the model, and chooses the next ones
 (``native.beam_select``); beams keep their places where they go on (``stay``), so what
-survives is not moved.  The whole step is captured as one CUDA graph and replayed without
+survives is not moved.  A beam that has ended keeps the states ahead of its stop token.  The whole step is captured as one CUDA graph and replayed without
 the host: tokens and parents are read once at the end, where the best beam is followed back.
 """
 from __future__ import annotations
@@ -70,9 +70,14 @@ class BeamStep:
         native.reorder_rows(self.mem + self.st, self.rows, group=self.beams)
         states = [BlockState(membrane=m, ssm_state=s) for m, s in zip(self.mem, self.st)]
         logits, new, _ = self.model.forward_device(self.tok, states, workspace=self.ws, attn_cache=self.cache)
+        ended = self.finished.view(-1, 1)               # they wait with the states ahead of their stop token
         for m, s, ns in zip(self.mem, self.st, new):
-            m.copy_(ns.membrane)
-            s.copy_(ns.ssm_state)
+            if self.stop is None:                       # none ends
+                m.copy_(ns.membrane)
+                s.copy_(ns.ssm_state)
+            else:
+                torch.where(ended, m, ns.membrane, out=m)
+                torch.where(ended[..., None], s, ns.ssm_state, out=s)
         self._choose(logits[:, -1, :])
 
     def _choose(self, logits: Tensor) -> None:
