@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import contextlib
 import gc
+import threading
 import weakref
 from typing import List, Optional
 
@@ -34,18 +35,23 @@ from ..core.fused import BlockState
 from ..core.rotary import Seen
 
 
+_one_capture = threading.RLock()
+
+
 @contextlib.contextmanager
 def capturing(graph: "torch.cuda.CUDAGraph"):
     """``torch.cuda.graph`` without the garbage collector: a collection in the middle of a capture may
-    destroy another graph (that of a model no longer used, say), which is not allowed then and ends the capture."""
-    on = gc.isenabled()
-    gc.disable()
-    try:
-        with torch.cuda.graph(graph):
-            yield
-    finally:
-        if on:
-            gc.enable()
+    destroy another graph (that of a model no longer used, say), which is not allowed then and ends the capture.
+    The collector is the whole process's, so threads that capture take turns."""
+    with _one_capture:
+        on = gc.isenabled()
+        gc.disable()
+        try:
+            with torch.cuda.graph(graph):
+                yield
+        finally:
+            if on:
+                gc.enable()
 
 
 class StepGraph:
