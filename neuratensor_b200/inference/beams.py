@@ -152,7 +152,7 @@ def beam_search(model, ids: Tensor, max_new_tokens: int, beams: int, length_pena
     P, prompt = ids.shape
     tokens = min(prompt, model.config.max_seq_len) + max_new_tokens if attn_cache else 0
     step = model.beam_step(P, beams, ids.device, model.lm_head.weight.dtype, tokens, length_penalty, tuple(stop),
-                           use_graph and max_new_tokens > 1)
+                           use_graph and ids.is_cuda and max_new_tokens > 1)
     step.begin(ids, states)
     made, parents = [step.tok.view(P, beams).clone()], []
     for i in range(1, max_new_tokens):
