@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kForkThreads) fork_pages_kernel(const __grid_c
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (r < a.R) {
         len = fork_length(a, r, &bad);
-        bad = false;                                    // flagged by the kernel before
+        bad = bad && a.n_blocks == 0;                   // flagged by the kernel before, which a table of no blocks does not have
         if (len % a.page) before = a.table[r * a.table_sb + len / a.page];
     }
     tail[r] = before;
@@ -312,7 +312,7 @@ int nt_kv_fork(int64_t R, int64_t n_pages, int64_t n_blocks, int64_t page, int64
         n_blocks * page > (int64_t)INT32_MAX - 4096 || group < 0 || (group > 0 && R % group) || (n_blocks > 0 && table_sb < n_blocks))
         return fail(NT_ERR_ARG, "nt_kv_fork: bad sizes");
     if (R == 0) return NT_OK;
-    if (!table || !refs || !lengths || !parents || !copies || (group > 0 && !shared)) return fail(NT_ERR_ARG, "nt_kv_fork: null pointer");
+    if ((!table && n_blocks > 0) || (!refs && n_pages > 0) || !lengths || !parents || !copies || (group > 0 && !shared)) return fail(NT_ERR_ARG, "nt_kv_fork: null pointer");
     const int64_t need = nt_kv_fork_workspace_bytes(R, n_blocks, group);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(NT_ERR_WORKSPACE, "nt_kv_fork: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
