@@ -423,7 +423,8 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
                     else r = look(l, i, &t);
                 }
                 const uint32_t k = l / S;
-                if (r > best || (r && r == best && (k < beam || (k == beam && t < token)))) best = r, beam = k, token = t, from = l;
+                if (r > best || (r && r == best && (k < beam || (k == beam && keys[l * n + i] > keys[from * n + head_at[from]]))))
+                    best = r, beam = k, token = t, from = l;
             }
         };
         // with a list a lane or none, its next two candidates are in registers
@@ -441,20 +442,27 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
             pick();
         }
         for (int i = 0; i < n; ++i) {
-            // the largest rank, of equal ones the lowest beam and token
+            // the largest rank, of equal ones the lowest beam, of its own the largest logit, then the lowest token
             const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
             bool mine = (uint32_t)(best >> 32) == hi;
             const uint32_t lo = __reduce_max_sync(0xffffffffu, mine ? (uint32_t)best : 0u);
             mine = mine && (uint32_t)best == lo;
-            if (__popc(__ballot_sync(0xffffffffu, mine)) > 1) {
-                const uint32_t k = __reduce_min_sync(0xffffffffu, mine ? beam : ~0u);
-                mine = mine && beam == k;
-                const uint32_t t = __reduce_min_sync(0xffffffffu, mine ? token : ~0u);
-                mine = mine && token == t;
-            }
             if (!(hi | lo)) {                           // nothing left
                 if (lane == 0) chosen[i] = -1;
                 continue;
+            }
+            if (__popc(__ballot_sync(0xffffffffu, mine)) > 1) {
+                const uint32_t k = __reduce_min_sync(0xffffffffu, mine ? beam : ~0u);
+                mine = mine && beam == k;
+                if (__popc(__ballot_sync(0xffffffffu, mine)) > 1) {
+                    // a beam's own, from several slices: sums alike, but the logits need not be (float64 drops what tells them apart
+                    // beside scores of 1e10 and more), so by these, then by token, as the slices' lists are
+                    const unsigned long long key = mine ? keys[from * n + (each ? at : head_at[from])] : 0ull;
+                    const uint32_t x = __reduce_max_sync(0xffffffffu, (uint32_t)(key >> 32));
+                    mine = mine && (uint32_t)(key >> 32) == x;
+                    const uint32_t t = __reduce_max_sync(0xffffffffu, mine ? (uint32_t)key : 0u);
+                    mine = mine && (uint32_t)key == t;
+                }
             }
             if (mine) {
                 chosen[i] = (int)beam;
