@@ -554,6 +554,8 @@ def _ints(t: Tensor, dtype: torch.dtype, what: str) -> Tensor:
         return t
     if t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
+    if dtype == torch.int32:                # what does not fit stays out of range
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1)
     return t.to(dtype)
 
 

@@ -58,3 +58,37 @@ def test_a_beams_own_are_in_the_order_of_their_logits_where_sums_are_alike(nat, 
     m = max(n, 4)
     got, rows, tokens = nat.beam_select(y, scores, finished=finished, n=m, pad=9)
     assert rows[0].tolist() == [0, 0, 1] + [2] * (m - 3) and tokens[0, :3].tolist() == [3, 5, 9] and torch.equal(tokens[0, 3:], ids[:m - 3])
+
+
+@pytest.mark.parametrize("far", [2 ** 32, -(2 ** 32), 2 ** 31, 2 ** 62])
+def test_indexes_past_32_bits_are_out_of_range(nat, far):
+    """int64 indexes that would be others in int32."""
+    t = torch.arange(12.0, device=DEV).view(6, 2)
+    nat.reorder_rows([t], ints([0, 1, 2, far + 1, 5, far + 4], torch.int64), group=3)
+    assert nat.device_error_flags(0) == 8
+    assert t.tolist() == [[0, 1], [2, 3], [4, 5], [6, 7], [10, 11], [10, 11]]        # those rows stay
+    table, refs, lengths = torch.full((3, 4), -1, device=DEV, dtype=torch.int32), ints([1, 1, 1, 0, 0, 0, 0]), ints([16, 16, 16])
+    table[:, 0] = ints([0, 1, 2])
+    nat.kv_fork(table, refs, lengths, ints([0, far, far + 1], torch.int64), 16, tokens=0)
+    assert nat.device_error_flags(0) == 8
+    assert lengths.tolist() == [16, 0, 0] and refs.tolist() == [1, 0, 0, 0, 0, 0, 0] and (table[1:] == -1).all()
+
+
+def test_lengths_and_shared_counts_past_32_bits(nat):
+    x = torch.randn(2, 50, device=DEV, generator=gen(1))
+    x[1] = x[0]
+    scores = torch.tensor([[-2.0, -2.0]], device=DEV)
+    # the longer beam's sums are divided by more, so that it is ahead
+    _, rows, _ = nat.beam_select(x, scores, lengths=ints([[3, 2 ** 32 + 1]], torch.int64), length_penalty=1.0, n=2)
+    assert (rows == 1).all()
+    H, D, P = 1, 64, 16
+    q = torch.randn(2, 1, H, D, device=DEV, generator=gen(2))
+    codes = torch.randint(0, 0x70, (300, H, P, D), device=DEV, dtype=torch.uint8, generator=gen(3))
+    scale = torch.full((300, H), 2.0 ** -8, device=DEV)
+    table = torch.arange(256, device=DEV, dtype=torch.int32).expand(2, 256).contiguous()
+    table[1, 2:] = 256 + torch.arange(254, device=DEV, dtype=torch.int32) % 40
+    table = torch.cat([table, torch.full((2, 1 << 14), -1, device=DEV, dtype=torch.int32)], 1)
+    args = (q, codes, scale, codes.clone(), scale.clone(), table, ints([4096, 4096]))
+    want = nat.kv_attention_shared(*args, ints([0]))
+    # counted as negative, which is nothing
+    assert torch.equal(nat.kv_attention_shared(*args, ints([-(2 ** 32) + 4096], torch.int64)), want)
