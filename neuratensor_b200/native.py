@@ -971,6 +971,8 @@ def reorder_rows(tensors: Sequence[Tensor], rows: Tensor, group: Optional[int] =
         return
     if len(set(spec[::3])) < len(tensors) and len({p for p, row in zip(spec[::3], spec[1::3]) if row}) < sum(1 for row in spec[1::3] if row):
         raise ValueError("reorder_rows: a tensor is given twice")
+    if rows.data_ptr() in spec[::3]:                    # the map is among what moves: the kernel reads one that does not
+        rows = rows.clone()
     words = struct.pack(f"={len(spec)}q", *spec)
     _launch(index, "nt_reorder_rows", len(tensors), _bytes_address(words), R, group, rows.data_ptr())
     increment_version(tensors)

@@ -92,3 +92,16 @@ def test_lengths_and_shared_counts_past_32_bits(nat):
     want = nat.kv_attention_shared(*args, ints([0]))
     # counted as negative, which is nothing
     assert torch.equal(nat.kv_attention_shared(*args, ints([-(2 ** 32) + 4096], torch.int64)), want)
+
+
+@pytest.mark.parametrize("groups,group", [(1, 7), (300, 4), (2, 1000)])
+def test_a_map_that_moves_with_the_rows(nat, groups, group):
+    """The map may be one of the tensors: it is read as it was."""
+    g = gen(group)
+    R = groups * group
+    rows = (torch.randint(0, group, (groups, group), device=DEV, generator=g) + group * torch.arange(groups, device=DEV)[:, None]).view(-1).int()
+    x = torch.randn(R, 300, device=DEV, generator=g)
+    src = rows.long()
+    want = [rows[src], x[src]]
+    nat.reorder_rows([rows, x], rows, group=group)
+    assert torch.equal(rows, want[0]) and torch.equal(x, want[1])
