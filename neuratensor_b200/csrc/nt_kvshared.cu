@@ -1034,6 +1034,11 @@ constexpr int64_t kFewRows = 32;
 // groups in a window of 512 keys 27 : 31, over 2048 keys 89 : 45; 8 beams of 10 heads of 64 over 1024 keys 13.4 : 14.5,
 // over 2048 15.6 : 14.8.
 constexpr int64_t kSReach = 1024, kSBytes = 16 << 20;
+// attend() takes kEvenBatch sequences at most; of more, groups of few rows take tcgen05 where at least so many sequences
+// share. us a call, without sharing : on tcgen05, 600 to 640 sequences of 8 heads of 128, bf16: groups of 2 over 4096 keys 609 : 1236,
+// of 4 603 : 647, of 8 635 : 378 (over 1024 keys 181 : 153), of 16 635 : 225; 4 heads of 64, of 4 251 : 200, of 8 250 : 126 (72 : 63);
+// float32 within a few percent of that. One head of 128 in groups of 8: 114 : 82 over 4096 keys, 40 : 53 over 1024.
+constexpr int64_t kSMany = 8;
 constexpr int64_t kSJoinRows = 1024;    // rows from which on a warp joins one alone
 struct SharedPlan { bool use, few; Plan rest; int rows, row_tiles, rows_cap, copies, ctas; int64_t stride, info, rest_info, part, rest_part, bytes; };
 
@@ -1045,8 +1050,9 @@ SharedPlan shared_plan(int dtype, int64_t B, int64_t groups, int64_t T, int64_t 
     p.rows = (int)std::min<int64_t>(rows, 1 << 20);
     int64_t reach = n_blocks * page;
     if (window >= 0) reach = std::min(reach, window + T);
-    p.few = rows <= kFewRows && T * G <= kRows;
-    p.use = K > 1 && reach >= kSReach && B * H * reach * 2 * D >= kSBytes && (p.few ? B <= kEvenBatch : groups <= kSGroups && rows <= (1 << 20));
+    p.few = rows <= kFewRows && T * G <= kRows && B <= kEvenBatch;
+    const bool tiles = groups <= kSGroups && rows <= (1 << 20) && (rows > kFewRows || T * G > kRows || K >= kSMany);
+    p.use = K > 1 && reach >= kSReach && B * H * reach * 2 * D >= kSBytes && (p.few || tiles);
     if (!p.use) return p;
     p.info = up((2 * groups + 2) * 8);
     if (p.few) {
