@@ -375,7 +375,7 @@ NT_API int nt_logits_process(int dtype, int64_t B, int64_t V, const void* logits
  * row b K + k that a candidate goes on from), out_tokens int64: [B, n], best first;
  * with stay != 0 (n == K) the best child of a beam stands in that beam's place and
  * the others, best first, in the places left.  Where candidates run out: -inf, row
- * b K + place % K, `pad`.
+ * b K + place % K, `pad`.  The outputs overlap no input.
  * Workspace: nt_beam_select_workspace_bytes(). */
 NT_API int64_t nt_beam_select_workspace_bytes(int dtype, int64_t B, int64_t K, int64_t V, int64_t n);
 NT_API int nt_beam_select(int dtype, int64_t B, int64_t K, int64_t V, int64_t n, const void* logits, int64_t ld,
@@ -408,7 +408,7 @@ NT_API int nt_reorder_rows(int64_t n_tensors, const int64_t* tensors, int64_t R,
  * order).  Where they run out, or the table ends, entries stay -1 and the bad-argument
  * bit of the device error word is set, as for a bad parent (it ends), length or page.
  * With group > 0 shared[g] (int32 [R / group]) is how many leading tokens, in whole
- * blocks, the rows of group g have in the same pages.
+ * blocks, the rows of group g have in the same pages: 0 where one has ended.
  * Workspace: nt_kv_fork_workspace_bytes() (0 without groups). */
 NT_API int64_t nt_kv_fork_workspace_bytes(int64_t R, int64_t n_blocks, int64_t group);
 NT_API int nt_kv_fork(int64_t R, int64_t n_pages, int64_t n_blocks, int64_t page, int64_t tokens, int64_t window,

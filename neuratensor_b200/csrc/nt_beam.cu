@@ -17,9 +17,9 @@
 // closer together than float32 can tell), then n rounds of one warp over the heads of the
 // sorted lists.
 //
-// Both kernels, caches flushed: 256 rows of 131072 float32 logits, 32 wanted, 50 + 16 us (the
+// Both kernels, caches flushed: 256 rows of 131072 float32 logits, 32 wanted, 48.5 + 15 us (the
 // 134 MB take 20.5; the candidates, their ranking and the waves' ends the rest: without candidates 36);
-// 64 rows of 32000 bf16 7.5 + 6; four rows 7.7 + 7.3, which is launch, one trip to memory each and the
+// 64 rows of 32000 bf16 7.3 + 6; four rows 7.8 + 7.4, which is launch, one trip to memory each and the
 // ranking.  On the way, at the first size: every tile's own bound 182 us; four vectors a thread
 // and two CTAs an SM 57; a ranking in which each entry took one thread 122.
 #include "nt_kernels.cuh"

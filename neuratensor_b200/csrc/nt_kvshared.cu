@@ -15,7 +15,10 @@
 // two; a float32 query is a pair of f16 (22 bits) and takes its product twice.  The block
 // scales of K multiply scores, in the softmax.  V becomes bf16 with its block's scale, exactly
 // (four significant bits), and the weights, which lie in any range, two bf16 (16 bits, for
-// bf16 outputs) or three (24 bits).  Weights are 1 at the row's reference, which moves to
+// bf16 outputs) or three (24 bits, float32 outputs; with a third piece for bf16 and heads of 128 one CTA's
+// TMEM would leave no room for another on its SM).  attend(), which takes short reaches and the rest of each row, has pairs of f16
+// there, 22 bits: a bf16 output shows neither (64 samples over 65536 keys, error against 64 bits
+// 1.6855e-3 with sharing, without it and for float32 products of torch's, of which rounding the output is all).  Weights are 1 at the row's reference, which moves to
 // a block's maximum when the block's weights come to more than 2^10, and values are divided by
 // 2^32, so that sums of finite ones stay finite; values below 2^-94 lose bits by it, 2^-102 at most.
 //
@@ -28,10 +31,11 @@
 //
 // 64 samples of 4 query heads on each of 8 cached heads of 128 over 65536 shared keys (69 GFLOP,
 // 42 us at the measured rate; half as much again is done for the weights' second halves), caches
-// flushed: this kernel 123 us, the rest of the rows until 150, the join until 164.  A tile of 128
+// flushed: this kernel 124 us, the rest of the rows until 153, the join until 166.  A tile of 128
 // keys takes a CTA 8400 clocks, two CTAs an SM, of which its 24 products take 1600 (65 to 68 each,
-// measured alone): the softmax and the conversions beside it are the longer side (at 159 us the
-// tensor cores were busy 21 % of the time and a scheduler issued in 39 % of its clocks).  On
+// measured alone): the softmax and the conversions beside it are the longer side (the tensor cores
+// are busy 31 % of the time, a scheduler issues in 54 % of its clocks; of 10 warps an issue 4 wait for
+// memory).  float32: 178, 204 and 218 us.  On
 // the way: 177 us with four loading warps whose registers spilled (shared memory leaves no L1
 // to catch that), 147 with eight, 131 with the look-ups in shared memory, 123 with 32 columns a step.  D = 128 in
 // bf16 still spills 152 bytes a thread and reads 308.

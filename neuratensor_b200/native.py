@@ -1001,7 +1001,8 @@ def kv_fork(table: Tensor, refs: Tensor, lengths: Tensor, parents: Tensor, page:
     kv_copy_pages; other lines are -1.  The next `tokens` tokens get pages (with a window
     those that it still sees behind them).  New pages are the free ones of lowest index, row
     by row.  shared: with `group`, how many leading tokens the rows of each group have in
-    the same pages, for kv_attention_shared.  Without enough pages or blocks entries stay -1, which is
+    the same pages, for kv_attention_shared; a row that ends has none, so its group shares nothing
+    (a row of no more use may go on from another of its group instead, with no new tokens).  Without enough pages or blocks entries stay -1, which is
     flagged (device_error_flags) like bad parents, lengths and pages."""
     index = _device_index(table, refs, lengths, parents)
     if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
