@@ -554,9 +554,14 @@ def _ints(t: Tensor, dtype: torch.dtype, what: str) -> Tensor:
         return t
     if t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
-    if dtype == torch.int32:                # what does not fit stays out of range
-        t = t.clamp(-2 ** 31, 2 ** 31 - 1)
     return t.to(dtype)
+
+
+def _indexes(t: Tensor, what: str) -> Tensor:
+    """_ints as int32, in which what does not fit stays out of range (6 us more for int64, a launch)."""
+    if t.dtype == torch.int64:
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1)
+    return _ints(t, torch.int32, what)
 
 
 class _Rotary(torch.autograd.Function):
@@ -917,7 +922,7 @@ def beam_select(logits: Tensor, scores: Tensor, finished: Optional[Tensor] = Non
     if lengths is not None:
         if lengths.shape != (B, K):
             raise ValueError(f"beam_select: lengths must be [{B}, {K}], got {tuple(lengths.shape)}")
-        lengths = _ints(lengths, torch.int32, "lengths").contiguous()
+        lengths = _indexes(lengths, "lengths").contiguous()
     elif length_penalty != 0.0:
         raise ValueError("beam_select: a length penalty needs lengths")
     if not 0 <= pad < 2 ** 31:
@@ -951,7 +956,7 @@ def reorder_rows(tensors: Sequence[Tensor], rows: Tensor, group: Optional[int] =
         raise ValueError(f"reorder_rows: {R} rows in groups of {group} (1 to 1024)")
     _refuse_out("reorder_rows", *tensors)
     if rows.dtype != torch.int32:
-        rows = _ints(rows, torch.int32, "rows")
+        rows = _indexes(rows, "rows")
     rows = rows.contiguous()
     spec = []
     for t in tensors:                                   # dozens of them, so no more than needed for each
@@ -1018,7 +1023,7 @@ def kv_fork(table: Tensor, refs: Tensor, lengths: Tensor, parents: Tensor, page:
         raise ValueError(f"kv_fork: page {page}, tokens {tokens}, window {window}")
     if group is not None and (group < 1 or R % group):
         raise ValueError(f"kv_fork: {R} rows in groups of {group}")
-    parents = _row_ints("kv_fork", "parents", parents, R)
+    parents = _row_ints("kv_fork", "parents", _indexes(parents, "parents"), R)
     copies = torch.empty((R, 2), dtype=torch.int32, device=table.device)
     shared = ws = None
     nbytes = 0
@@ -1098,7 +1103,7 @@ def kv_attention_shared(q: Tensor, k_codes: Tensor, k_scale: Tensor, v_codes: Te
     groups = shared.numel()
     if shared.dim() != 1 or groups < 1 or B % groups:
         raise ValueError(f"kv_attention_shared: {B} sequences do not make the groups of shared {tuple(shared.shape)}")
-    shared = _ints(shared, torch.int32, "shared").contiguous()
+    shared = _indexes(shared, "shared").contiguous()
     win = -1 if window is None else min(int(window), 2 ** 31)      # as good as none from there on
     if q.stride(3) != 1:
         q = q.contiguous()
