@@ -397,7 +397,8 @@ class NeuraTensorModel(nn.Module):
             hit = None
             while len(cache) >= 4:
                 cache.pop(next(iter(cache)))
-            graph = StepGraph(self, batch, seq, torch.device(device), dtype, cache_tokens)
+            with torch.inference_mode(False), torch.no_grad():      # its buffers are written in later calls, which may be outside it
+                graph = StepGraph(self, batch, seq, torch.device(device), dtype, cache_tokens)
             hit = (self._graph_signature(cache_tokens), graph)      # its warm-up may have built the tables
         cache[key] = hit                          # most recently used last
         return hit[1]
@@ -422,7 +423,8 @@ class NeuraTensorModel(nn.Module):
             hit = None
             while len(cache) >= 2:
                 cache.pop(next(iter(cache)))
-            step = BeamStep(self, prompts, beams, torch.device(device), dtype, cache_tokens, length_penalty, stop)
+            with torch.inference_mode(False), torch.no_grad():
+                step = BeamStep(self, prompts, beams, torch.device(device), dtype, cache_tokens, length_penalty, stop)
             hit = (self._graph_signature(cache_tokens), step)
         cache[key] = hit
         return hit[1]
